@@ -339,6 +339,110 @@ ORTHO_B200_API int ortho_b200_sieve(const float *w, const float *h_inv_diag, int
                        float *w_base_out, float *w_ortho_out,
                        void *scratch, int64_t scratch_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The operators around the projections of a decoding step: page bookkeeping, rotary positions with the write into a paged
+ * key-value cache, attention of one new token over that cache, and low-rank adapters beside a projection.  They have no
+ * counterpart in the reference, whose operator ends with the projection.
+ *
+ * `type` is ORTHO_B200_TYPE_F16 or ORTHO_B200_TYPE_BF16 and holds for every void * tensor of a record.  Strides count
+ * elements; the innermost dimension has stride 1.  Records are read during the call only.  No call allocates, synchronises
+ * or keeps anything; all check their record before anything is launched (ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_WORKSPACE).
+ * Indices that come from device memory (page numbers, slots, positions, adapter numbers, lengths) are checked on the device:
+ * one that is out of range is left out as described, nothing is read or written through it.
+ *
+ * Paged cache: `pages` pages of `page_size` tokens; key (or value) head h of the token at place o of page p starts at
+ * p * page_stride + o * token_stride + h * head_stride.  A slot is p * page_size + o.  block_table [rows, width] lists the pages of a
+ * request in the order of its tokens; entries behind a request's length are never read.
+ * ------------------------------------------------------------------------------------------- */
+
+/* One step's pages, slots and positions from the requests' lengths.  With c = max(cached, 0) and f = max(fresh, 0) tokens of
+ * request b: the pages ceil(c / P) .. ceil((c + f) / P) - 1 of every request are new and are taken, request after request, from
+ * the end of the first n = clamp(*available, 0, free_count) entries of free_pages: free_pages[n - 1] first.  They are written to
+ * block_table; a page that the pool or the table has no place for is not, and its tokens get slot -1.
+ *   lengths   [requests]      c + f
+ *   starts    [requests + 1]  first token of each request in this step, and their number
+ *   slots     [tokens]        slot, or -1 where the token has no page; -1 behind the last token
+ *   positions [tokens]        position in the request (from c on, 2^31 - 1 at most); -1 behind the last token
+ *   request_of[tokens]        request; -1 behind the last token
+ *   counts    [3]             tokens and pages asked for, pages left (0 if too few)
+ * `tokens` is the size of the token arrays: more tokens than that get their pages, but no place in the arrays.  The free list
+ * is not changed: the next step passes counts + 2 as `available`. */
+typedef struct ortho_b200_page_step_desc {
+    const int32_t *cached, *fresh;      /* [requests] */
+    int32_t *block_table;               /* [requests, width], rows table_stride apart */
+    const int32_t *free_pages;          /* [free_count] */
+    const int32_t *available;           /* [1] */
+    int32_t *lengths, *starts;
+    int64_t *slots;
+    int32_t *positions, *request_of, *counts;
+    int64_t requests, width, table_stride, free_count, tokens, page_size;
+} ortho_b200_page_step_desc;
+ORTHO_B200_API int ortho_b200_page_step(const ortho_b200_page_step_desc *d, void *stream);
+
+/* Rotary positions of queries and keys, and keys and values written to the paged cache.  Of the first `rotary` elements of a head,
+ * pair i < rotary / 2 is (i, i + rotary / 2), or (2 i, 2 i + 1) when `interleaved`, and becomes
+ * (a c - b s, b c + a s) with c = table[p][i], s = table[p][rotary / 2 + i] and p = positions[axis][t]; the pairs below
+ * section_ends[0] turn with axis 0, those below section_ends[1] with axis 1, and so on (section_ends[axes - 1] = rotary / 2).  A
+ * position outside the table turns nothing.  Computed in FP32, rounded once; the other elements and the values are copied.
+ * q and q_out may be NULL together (keys and values alone); rotary = 0 turns nothing and then neither table nor positions are
+ * read.  q_out may be q.  A token whose slot lies outside the cache is not written to it.  Two tokens with one slot: either. */
+#define ORTHO_B200_MAX_AXES 4
+typedef struct ortho_b200_rotary_append_desc {
+    const void *q, *k, *v;              /* [tokens, q_heads, head_dim], [tokens, kv_heads, head_dim] twice */
+    void *q_out, *k_cache, *v_cache;
+    const int64_t *slots;               /* [tokens] */
+    const int32_t *positions;           /* [axes, tokens], axes position_stride apart */
+    const float *table;                 /* [table_rows, rotary], contiguous: cosines, then sines */
+    int64_t tokens, q_heads, kv_heads, head_dim, rotary, table_rows, position_stride;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_cache_head_stride, v_page_stride, v_slot_stride, v_cache_head_stride;
+    int64_t pages, page_size;
+    int32_t axes, section_ends[ORTHO_B200_MAX_AXES], interleaved, type;
+} ortho_b200_rotary_append_desc;
+ORTHO_B200_API int ortho_b200_rotary_append(const ortho_b200_rotary_append_desc *d, void *stream);
+
+/* Attention of one query token per row over the paged cache: row b attends to the keys max(0, n - window) .. n - 1 (window 0: from
+ * 0) of the request in row row_of[b] of block_table (NULL: row b), n = clamp(lengths[b], 0, width * page_size):
+ * s = scale * q . k, out = sum softmax(s) v, lse = log sum exp s (optional, FP32 [batch, q_heads], contiguous).  Several rows may read one request:
+ * the tokens of a prompt with their own lengths.  Query head h reads KV head h / (q_heads / kv_heads).  A row without
+ * keys (length 0, a table row out of range) gives 0 and -inf; a key on a page outside the cache is left out.  What lies behind a
+ * length, NaN too, has no effect.  Scores, softmax and sums are FP32; the probabilities enter the matrix products as two 16-bit
+ * parts.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned, strides of q and caches multiples of 8.
+ * workspace: ortho_b200_paged_attention_workspace_bytes(d) bytes, 256-byte aligned (partial sums of requests that are split over CTAs;
+ * what it holds before does not matter). */
+typedef struct ortho_b200_paged_attention_desc {
+    const void *q, *k_cache, *v_cache;
+    void *out;                          /* [batch, q_heads, head_dim] */
+    float *lse;
+    const int32_t *block_table, *lengths, *row_of;
+    int64_t batch, q_heads, kv_heads, head_dim, rows, width, table_stride, pages, page_size, window;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    float scale;
+    int32_t type;
+} ortho_b200_paged_attention_desc;
+ORTHO_B200_API int64_t ortho_b200_paged_attention_workspace_bytes(const ortho_b200_paged_attention_desc *d);
+ORTHO_B200_API int ortho_b200_paged_attention(const ortho_b200_paged_attention_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + scales[e] * up[e] (down[e] x[t]) with
+ * e = ids[t]; out[t] = y[t] where ids[t] is not in [0, adapters).  ranks[e] (NULL: all `rank`) is the number of rows of down[e] and
+ * columns of up[e] that are used, rounded up to a multiple of 8; scales NULL: 1.  The inner sums are FP32 and stay so (two 16-bit
+ * parts in the second product), out is rounded once.  out may be y.  down and up are constants of the layer in the sense stated
+ * at ortho_b200_forward.  K a multiple of 8, rank a multiple of 8 up to 256; x, down and up 16-byte aligned, x_stride a multiple of 8.
+ * workspace: ortho_b200_low_rank_add_workspace_bytes(d) bytes, 256-byte aligned; what it holds before does not matter. */
+typedef struct ortho_b200_low_rank_desc {
+    const void *x, *y;                  /* [tokens, K], [tokens, N] */
+    void *out;                          /* [tokens, N] */
+    const void *down, *up;              /* [adapters, rank, K], [adapters, N, rank], contiguous */
+    const float *scales;                /* [adapters] or NULL */
+    const int32_t *ranks;               /* [adapters] or NULL */
+    const int32_t *ids;                 /* [tokens] */
+    int64_t tokens, K, N, adapters, rank, x_stride, y_stride, out_stride;
+    int32_t type;
+} ortho_b200_low_rank_desc;
+ORTHO_B200_API int64_t ortho_b200_low_rank_add_workspace_bytes(const ortho_b200_low_rank_desc *d);
+ORTHO_B200_API int ortho_b200_low_rank_add(const ortho_b200_low_rank_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Synchronises the device and reports whether any kernel of this library gave up on a bounded
  * wait since the last query (ERR_KERNEL, and the flag is cleared) or not (OK).  Replaces the
  * cudaDeviceSynchronize + error check at the end of the reference dispatcher

@@ -10,7 +10,7 @@ stream, and any failure raises instead of being dropped.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -433,3 +433,70 @@ def hessian_sieve(weight: torch.Tensor, h_inv_diag: torch.Tensor, curvature_thre
                                         torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(st, "ortho_b200_sieve")
     return wb, wo
+
+
+# ---- the operators around the projections of a decoding step ------------------------------------------------------------------
+# No counterpart in the reference.  All are asynchronous on the current stream of the tensors' device, take float16 or bfloat16
+# (one type in a call), raise TypeError / ValueError / RuntimeError for arguments that do not fit, and have no gradient.
+
+class PageStep(NamedTuple):
+    """What ``page_step`` computes; all int32 but the slots (int64)."""
+    lengths: torch.Tensor              # [requests]      tokens in the cache after the step
+    starts: torch.Tensor               # [requests + 1]  first token of each request in the step, and their number
+    slots: torch.Tensor                # [tokens]        place in the cache, -1 for none
+    positions: torch.Tensor            # [tokens]        position in the request, -1 behind the last token
+    requests: torch.Tensor             # [tokens]        request, -1 behind the last token
+    counts: torch.Tensor               # [3]             tokens, pages asked for, pages left
+
+
+def page_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+              available: torch.Tensor, page_size: int, tokens: int, out: Optional[PageStep] = None) -> PageStep:
+    """Pages, slots and positions of a step in which request ``b`` has ``cached[b]`` tokens in the cache and gets ``fresh[b]``
+    more.  New pages are taken, request after request, from the end of the first ``available[0]`` entries of ``free_pages``
+    (the last one first) and written to ``block_table`` [requests, pages] in place; where the pool or the table has no
+    room the tokens get slot -1.  ``tokens`` is the size of the token arrays, which list the requests' new tokens one
+    request after the other.  The next step's ``available`` is ``counts[2:]``.  ``out``: a result (or its six tensors) to write into.
+    All inputs are int32 tensors on the GPU; nothing is read back by the host."""
+    got = _lib.fast().page_step(cached, fresh, block_table, free_pages, available, page_size, tokens, out)
+    return got if isinstance(got, PageStep) else PageStep(*got)
+
+
+def rotary_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor, positions: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                  sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                  out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Turns queries and keys by their positions, writes keys and values into the paged cache and returns the turned queries.
+
+    ``q`` [tokens, q_heads, head_dim], ``k`` and ``v`` [tokens, kv_heads, head_dim] may be views of a fused projection.
+    ``k_cache`` / ``v_cache`` [pages, page_size, kv_heads, head_dim] with any strides but the last; token ``t`` goes to
+    ``slots[t]`` (int64, page * page_size + place), nowhere if that lies outside.  ``table`` float32 [positions, rotary_dim] holds cosines and then sines
+    (``rotary_table``); pair ``i`` of the first ``rotary_dim`` elements is ``(i, i + rotary_dim / 2)``, or
+    ``(2 i, 2 i + 1)`` when ``interleaved``.  ``positions`` int32 [tokens], or [axes, tokens] with ``sections``: how many
+    pairs turn with each axis (time, height, width).  A position outside the table turns nothing.  Without ``positions``
+    and ``table`` keys are written as they are and ``q`` must be None.  ``out`` may be ``q``."""
+    return _lib.fast().rotary_append(q, k, v, k_cache, v_cache, slots, positions, table, sections, interleaved, out)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: Optional[float] = None, window: int = 0, rows: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one query token per row over a paged cache: ``q`` [batch, q_heads, head_dim] -> the same shape.
+
+    Row ``b`` attends to the last ``window`` (0: all) of the first ``lengths[b]`` tokens of the request in row ``b``
+    of ``block_table`` (int32 [requests, pages]), or in row ``rows[b]``: several tokens of one prompt, each with its own
+    length.  Query head ``h`` reads key-value head ``h // (q_heads // kv_heads)``.  ``scale`` defaults to
+    ``head_dim ** -0.5``.  A row without keys gives zeros.  ``lse`` (float32 [batch, q_heads], written): logarithm of the sum of the exponentials, by which
+    results over parts of a cache are joined.  head_dim: a multiple of 8 up to 256."""
+    return _lib.fast().paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window, rows, out, lse)
+
+
+def low_rank_add(x: torch.Tensor, y: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,
+                 scales: Optional[torch.Tensor] = None, ranks: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y + scales[e] * up[e] (down[e] x)`` for every token, ``e = ids[t]``: the adapters of many requests beside the
+    projection that made ``y`` [..., out_features] from ``x`` [..., in_features].
+
+    ``down`` [adapters, rank, in_features], ``up`` [adapters, out_features, rank], ``ids`` int32 (one per token; outside
+    [0, adapters): no adapter), ``scales`` float32, ``ranks`` int32 [adapters]: rows of ``down`` and columns of ``up`` that an
+    adapter uses, rounded up to a multiple of 8.  rank is a multiple of 8 up to 256.  ``out`` may be ``y``."""
+    return _lib.fast().low_rank_add(x, y, down, up, ids, scales, ranks, out)

@@ -27,6 +27,39 @@ class LayerDesc(ctypes.Structure):
                 ("N", ctypes.c_int64), ("ldy", ctypes.c_int64), ("alpha", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
+def _fields(*groups):
+    return [(name, kind) for kind, names in groups for name in names.split()]
+
+
+class PageStepDesc(ctypes.Structure):
+    """``ortho_b200_page_step_desc``."""
+    _fields_ = _fields((ctypes.c_void_p, "cached fresh block_table free_pages available lengths starts slots positions request_of counts"),
+                       (ctypes.c_int64, "requests width table_stride free_count tokens page_size"))
+
+
+class RotaryAppendDesc(ctypes.Structure):
+    """``ortho_b200_rotary_append_desc``."""
+    _fields_ = _fields((ctypes.c_void_p, "q k v q_out k_cache v_cache slots positions table"),
+                       (ctypes.c_int64, "tokens q_heads kv_heads head_dim rotary table_rows position_stride q_token_stride q_head_stride "
+                        "k_token_stride k_head_stride v_token_stride v_head_stride out_token_stride out_head_stride k_page_stride k_slot_stride "
+                        "k_cache_head_stride v_page_stride v_slot_stride v_cache_head_stride pages page_size"),
+                       (ctypes.c_int32, "axes"), (ctypes.c_int32 * 4, "section_ends"), (ctypes.c_int32, "interleaved type"))
+
+
+class PagedAttentionDesc(ctypes.Structure):
+    """``ortho_b200_paged_attention_desc``."""
+    _fields_ = _fields((ctypes.c_void_p, "q k_cache v_cache out lse block_table lengths row_of"),
+                       (ctypes.c_int64, "batch q_heads kv_heads head_dim rows width table_stride pages page_size window q_token_stride "
+                        "q_head_stride out_token_stride out_head_stride k_page_stride k_slot_stride k_head_stride v_page_stride v_slot_stride "
+                        "v_head_stride"), (ctypes.c_float, "scale"), (ctypes.c_int32, "type"))
+
+
+class LowRankDesc(ctypes.Structure):
+    """``ortho_b200_low_rank_desc``."""
+    _fields_ = _fields((ctypes.c_void_p, "x y out down up scales ranks ids"),
+                       (ctypes.c_int64, "tokens K N adapters rank x_stride y_stride out_stride"), (ctypes.c_int32, "type"))
+
+
 class OrthoB200Error(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -121,6 +154,15 @@ def _declare(l):
     l.ortho_b200_forward_gather.restype = c.c_int
     l.ortho_b200_forward_gather.argtypes = [vp, vp, vp, i32p, i32p, i64, vp, i64, i64, i64, c.c_float,
                                             vp, vp, i64, vp, i64, i64, i64, vp]
+    for name, desc, scratch in (("page_step", PageStepDesc, False), ("rotary_append", RotaryAppendDesc, False),
+                                ("paged_attention", PagedAttentionDesc, True), ("low_rank_add", LowRankDesc, True)):
+        fn = getattr(l, "ortho_b200_" + name)
+        fn.restype = c.c_int
+        fn.argtypes = [c.POINTER(desc), vp, i64, vp] if scratch else [c.POINTER(desc), vp]
+        if scratch:
+            fn = getattr(l, f"ortho_b200_{name}_workspace_bytes")
+            fn.restype = i64
+            fn.argtypes = [c.POINTER(desc)]
 
 
 # every symbol include/ortho_b200.h declares
@@ -137,6 +179,8 @@ EXPORTS = [
     "ortho_b200_csr_marks_bytes", "ortho_b200_csr_count_marks", "ortho_b200_csr_fill_marks",
     "ortho_b200_sieve_scratch_bytes", "ortho_b200_sieve_onepass_scratch_bytes", "ortho_b200_sieve",
     "ortho_b200_forward_multi", "ortho_b200_multi_workspace_bytes", "ortho_b200_forward_typed", "ortho_b200_typed_scratch_bytes",
+    "ortho_b200_page_step", "ortho_b200_rotary_append", "ortho_b200_paged_attention", "ortho_b200_paged_attention_workspace_bytes",
+    "ortho_b200_low_rank_add", "ortho_b200_low_rank_add_workspace_bytes",
 ]
 
 
@@ -158,7 +202,7 @@ _fast = None
 
 
 def fast():
-    """The native host path (``csrc/fastcall.cpp``), pointed at the loaded library."""
+    """The native host path (``csrc/fastcall.cpp``, ``csrc/fastops.cpp``), pointed at the loaded library."""
     global _fast
     if _fast is None:
         l = lib()
@@ -172,6 +216,10 @@ def fast():
             raise ImportError(advice)
         f.set_library(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in
                         (l.ortho_b200_forward_multi, l.ortho_b200_multi_workspace_bytes, l.ortho_b200_forward_typed)))
+        f.set_operators(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in
+                          (l.ortho_b200_page_step, l.ortho_b200_rotary_append, l.ortho_b200_paged_attention,
+                           l.ortho_b200_paged_attention_workspace_bytes, l.ortho_b200_low_rank_add, l.ortho_b200_low_rank_add_workspace_bytes,
+                           l.ortho_b200_strerror, l.ortho_b200_last_cuda_error)))
         _fast = f
     return _fast
 

@@ -17,14 +17,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB_PATH = os.path.join(HERE, "libortho_b200.so")
-SOURCES = ["api.cu", "plan.cu", "decode.cu", "decode_stream.cu", "mid.cu", "wide.cu", "prefill.cu", "transpose.cu", "longrows.cu", "static_scratch.cu", "comm.cu", "pack.cu", "sieve.cu"]
+SOURCES = ["api.cu", "plan.cu", "decode.cu", "decode_stream.cu", "mid.cu", "wide.cu", "prefill.cu", "transpose.cu", "longrows.cu", "static_scratch.cu", "comm.cu", "pack.cu", "sieve.cu",
+           "pages.cu", "rotary.cu", "attention.cu", "adapters.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--use_fast_math",
     "-cudart", "static",
 ]
-# the forward's host path as a CPython extension (csrc/fastcall.cpp), compiled against the installed torch
-FAST_SOURCE = os.path.join(CSRC, "fastcall.cpp")
+# the host path as a CPython extension (csrc/fastcall.cpp: the forward, csrc/fastops.cpp: the other operators), compiled against the installed torch
+FAST_SOURCES = [os.path.join(CSRC, f) for f in ("fastcall.cpp", "fastops.cpp")]
 FAST_PATH = os.path.join(HERE, "_fastcall.so")
 FAST_STAMP = os.path.join(HERE, "build", "fastcall.txt")       # what the extension was compiled against
 
@@ -51,7 +52,7 @@ def _fast_against() -> str:
 
 
 def needs_build_fast() -> bool:
-    deps = [FAST_SOURCE, os.path.join(INCLUDE, "ortho_b200.h")]
+    deps = [*FAST_SOURCES, os.path.join(INCLUDE, "ortho_b200.h")]
     if not os.path.exists(FAST_PATH) or any(os.path.getmtime(d) > os.path.getmtime(FAST_PATH) for d in deps):
         return True
     try:
@@ -71,13 +72,20 @@ def build_fast(force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else "/usr/local/cuda"
     inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DORTHO_TORCH_VERSION="{torch.__version__}"',
-           *[f"-I{d}" for d in inc], FAST_SOURCE, "-o", FAST_PATH, f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ltorch"]
-    out = subprocess.run(cmd, capture_output=True, text=True)
+    objdir = os.path.dirname(FAST_STAMP)
+    os.makedirs(objdir, exist_ok=True)
+    objs = [os.path.join(objdir, os.path.basename(f).replace(".cpp", ".o")) for f in FAST_SOURCES]
+    procs = [(f, subprocess.Popen(["g++", "-O2", "-std=c++17", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                                   f'-DORTHO_TORCH_VERSION="{torch.__version__}"', *[f"-I{d}" for d in inc], "-c", f, "-o", o],
+                                  stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)) for f, o in zip(FAST_SOURCES, objs)]
+    procs = [(f, p, p.communicate()[0]) for f, p in procs]
+    for f, p, out in procs:
+        if p.returncode != 0:
+            raise RuntimeError(f"g++ failed on {os.path.basename(f)}:\n" + out)
+    out = subprocess.run(["g++", "-shared", *objs, "-o", FAST_PATH, f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ltorch"],
+                         capture_output=True, text=True)
     if out.returncode != 0:
-        raise RuntimeError("g++ failed on fastcall.cpp:\n" + out.stdout + out.stderr)
-    os.makedirs(os.path.dirname(FAST_STAMP), exist_ok=True)
+        raise RuntimeError("g++ failed to link the host path:\n" + out.stdout + out.stderr)
     with open(FAST_STAMP, "w") as f:
         f.write(_fast_against())
     return FAST_PATH

@@ -66,7 +66,7 @@ unsigned long long next_launch_tag()
     return z ? z : 1ull;
 }
 
-static int check_device()
+int check_device()
 {
     static thread_local int checked_device = -1;
     int dev = 0;
@@ -88,10 +88,10 @@ extern "C" const char *ortho_b200_strerror(int status)
     switch (status) {
         case ORTHO_B200_OK: return "ok";
         case ORTHO_B200_ERR_NULL: return "a required pointer is NULL";
-        case ORTHO_B200_ERR_SHAPE: return "unsupported shape (need M,N >= 1, K a multiple of 32 and <= 65536)";
-        case ORTHO_B200_ERR_ALIGN: return "q_weight, x and y must be 16-byte aligned";
+        case ORTHO_B200_ERR_SHAPE: return "unsupported shape or size (the call's constraints are in ortho_b200.h; a forward needs M,N >= 1, K a multiple of 32 and <= 65536)";
+        case ORTHO_B200_ERR_ALIGN: return "a pointer or stride is not aligned as the call needs it (a forward: q_weight, x and y to 16 bytes)";
         case ORTHO_B200_ERR_PLAN: return "plan is invalid or was built for another layer";
-        case ORTHO_B200_ERR_WORKSPACE: return "workspace missing or smaller than ortho_b200_workspace_bytes()";
+        case ORTHO_B200_ERR_WORKSPACE: return "workspace missing or smaller than the call's workspace query says (a forward: ortho_b200_workspace_bytes())";
         case ORTHO_B200_ERR_CUDA: return "a CUDA call failed (see ortho_b200_last_cuda_error)";
         case ORTHO_B200_ERR_DEVICE: return "current device is not a compute capability 10.x GPU";
         case ORTHO_B200_ERR_KERNEL: return "a kernel gave up on a bounded wait";

@@ -342,6 +342,8 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, metho
 
 }  // namespace
 
+extern PyMethodDef ortho_operator_methods[];                // fastops.cpp
+
 PyMODINIT_FUNC PyInit__fastcall(void)
 {
     for (int i = 0; i < 5; i++) s_buffers[i] = PyUnicode_InternFromString(kBuffers[i]);
@@ -352,6 +354,7 @@ PyMODINIT_FUNC PyInit__fastcall(void)
     s_value = PyUnicode_InternFromString("value");
     s_fast = PyUnicode_InternFromString("fast");
     PyObject *m = PyModule_Create(&module_def);
+    if (m && PyModule_AddFunctions(m, ortho_operator_methods) < 0) { Py_DECREF(m); return nullptr; }
     // the torch it was compiled against: a module built for another one is not to be used
     if (m && PyModule_AddStringConstant(m, "torch_version", ORTHO_TORCH_VERSION) < 0) { Py_DECREF(m); return nullptr; }
     return m;

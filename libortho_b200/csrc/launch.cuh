@@ -1,0 +1,61 @@
+// Launches of the operators around the projections: every kernel is a programmatic dependent of what precedes it on the stream
+// (it starts beside that kernel's tail and calls griddep_wait() before it touches anything that is not a layer's constant) and lets its
+// own successor start early.
+#pragma once
+
+#include "common.cuh"
+
+namespace ob {
+
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    OB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    count_launch();
+    return ORTHO_B200_OK;
+}
+
+int check_device();                    // api.cu: ERR_DEVICE where the current device is no compute capability 10.x GPU
+
+// ---- 16-bit types ---------------------------------------------------------------------------------
+template <class T> struct Half;
+template <> struct Half<__half> {
+    static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_half2(a, b); }
+};
+template <> struct Half<__nv_bfloat16> {
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+
+// n / d for 0 <= n < 2^31 and a divisor known at the launch: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d) < 2^32, the error of
+// n m / 2^(31 + s) is below n / 2^31 / d < 1 / d, so its integer part is the quotient.
+struct FastDiv {
+    uint32_t d, m, s;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div), m(0), s(0)
+    {
+        while ((1ull << s) < div) s++;
+        m = (uint32_t)(((1ull << (31 + s)) + div - 1) / div);      // div = 1: 2^31, s = 0
+    }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> (31 + s)); }
+};
+
+}  // namespace ob
