@@ -1,0 +1,578 @@
+// Attention of one new token per row over a paged key-value cache (one source for both 16-bit types):
+//
+//     s_j = scale q . k_j,   out = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max),   lse = max + log sum_j exp(s_j - max)
+//
+// Keys and values are read once and dominate everything else: with G query heads per key-value head there are G multiplications a byte.
+// So the cache streams through shared memory by asynchronous 16-byte copies, a ring of its own per warp (no barrier per tile), and all
+// query heads of a key-value head meet every key as the 8-column operand of m16n8k16 products: S^T = K Q^T (16 keys x 8 queries), running
+// maximum and sum per query in FP32, then O^T += V^T P^T (16 elements x 8 queries).  Queries are the narrow operand because there are few of
+// them; P^T gets from accumulator to operand layout by an 8 x 8 transposition in registers.
+//
+// The work is cut evenly whatever the lengths are.  A unit is 64 keys of one request and key-value head (16 per warp).  The units of all requests
+// are numbered in a row, and CTA c of n takes the units [U c / n, U (c + 1) / n): every CTA finds its place by summing the lengths itself.
+// A request that lies within one CTA is finished there; of one that is cut each CTA leaves its sums in the workspace and
+// join_kernel, launched behind as a programmatic dependent, adds them in order.  No atomics: the same bits every time.
+#pragma once
+
+#include "launch.cuh"
+
+namespace ob {
+
+struct AttentionArgs {
+    ortho_b200_paged_attention_desc d;
+    FastDiv by_page;
+    float scale_log2;                            // scale log2 e: exponentials are powers of two
+    int per_group, groups;                       // query heads of a key-value head in one unit, units' groups of them
+    int ctas;
+    int4 *cut;                                   // [ctas] of a CTA's last request: {row, head group, last CTA, 1} if it goes on, {.., 0} if not
+    float2 *sums;                                // [2 ctas][rows] (max, sum) of cut requests: continued from the CTA before, going on behind
+    float *part;                                 // [2 ctas][rows][head_dim]
+};
+
+constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kWarpKeys = 16, kUnitKeys = kWarpKeys * kAttnWarps;
+
+// Probabilities are powers of two of s - max + kLift: in FP16 the largest is then 2^12 and what is 2^-36 of it still has a value
+template <class T> struct AttnType;
+template <> struct AttnType<__half> {
+    static constexpr float lift = 12.f, below = 1.f - 1.f / 1024.f;
+    static __device__ __forceinline__ uint32_t pack_rz(float lo, float hi)
+    {
+        uint32_t r;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_16816(d, a, b0, b1); }
+};
+template <> struct AttnType<__nv_bfloat16> {
+    static constexpr float lift = 0.f, below = 1.f - 1.f / 128.f;
+    static __device__ __forceinline__ uint32_t pack_rz(float lo, float hi)
+    {
+        uint32_t r;
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+    {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ uint32_t shared_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix2(uint32_t &r0, uint32_t &r1, uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// 16 bytes, or zeros
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void *src, bool on)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// Shared memory of one CTA.  Rows of DP elements: 16-byte chunks exchanged within groups of eight by the row's number where a row is a multiple of
+// 128 bytes, 16 bytes of padding elsewhere; both put the eight rows that one ldmatrix phase reads into different banks.
+template <int DP, int NT>
+struct AttnShape {
+    static constexpr bool kSwap = DP % 64 == 0;
+    static constexpr int kPitch = DP * 2 + (kSwap ? 0 : 16), kChunks = DP / 8;
+    static constexpr int kHalfTile = kWarpKeys * kPitch;                       // keys, then values
+    static constexpr int kStage = 2 * kHalfTile;
+    static constexpr int kQ = NT * 8 * kPitch;
+    static constexpr int kFold = kAttnWarps * 8 * 68 * 4;                      // 8 queries x 64 elements of every warp, rows apart by 4 banks
+    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kFold + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
+    static constexpr int kTwo = 115712, kOne = 232448;                         // room of a CTA with two or one on an SM
+    static constexpr int kStages = bytes(4) <= kTwo ? 4 : bytes(3) <= kTwo ? 3 : bytes(2) <= kTwo ? 2 : bytes(4) <= kOne ? 4 : bytes(3) <= kOne ? 3 : 2;
+    static constexpr int kBytes = bytes(kStages), kPerSm = kBytes <= kTwo ? 2 : 1;
+    static constexpr bool kKeepQ = NT <= 2;                                    // query operands stay in registers
+    static __device__ __forceinline__ uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((kSwap ? chunk ^ (row & 7) : chunk) << 4)); }
+};
+
+// One request as the units see it
+struct Span { int from, n, units; int64_t row; };
+__device__ __forceinline__ Span span_of(const ortho_b200_paged_attention_desc &d, int64_t b)
+{
+    Span s;
+    s.row = d.row_of ? (int64_t)d.row_of[b] : b;
+    const int most = (int)(d.width * d.page_size);
+    int n = s.row >= 0 && s.row < d.rows ? d.lengths[b] : 0;
+    n = n < 0 ? 0 : n < most ? n : most;
+    s.n = n;
+    s.from = d.window > 0 && n > d.window ? n - (int)d.window : 0;
+    s.units = (n - s.from + kUnitKeys - 1) / kUnitKeys;
+    return s;
+}
+
+// Place in the row of all units: request, head group, 64 keys
+struct Walk {
+    int64_t b;
+    int inner, unit;
+    Span s;
+    __device__ __forceinline__ void step(const ortho_b200_paged_attention_desc &d, int inners)
+    {
+        if (++unit < s.units) return;
+        unit = 0;
+        if (++inner < inners) return;
+        inner = 0;
+        do b++, s = b < d.batch ? span_of(d, b) : Span{0, 0, 1, 0}; while (s.units == 0);
+    }
+};
+
+template <class T, int DP, int NT>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<DP, NT>::kPerSm)
+paged_attention_kernel(const __grid_constant__ AttentionArgs a)
+{
+    using Shape = AttnShape<DP, NT>;
+    using Type = AttnType<T>;
+    constexpr int S = Shape::kStages, KS = DP / 16;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const auto &d = a.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = (int)d.head_dim;
+    unsigned char *const ring = smem + warp * (S * Shape::kStage);
+    unsigned char *const q_ring = smem + kAttnWarps * S * Shape::kStage;
+    float *const fold = reinterpret_cast<float *>(q_ring + S * Shape::kQ);
+    float2 *const sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(fold) + Shape::kFold);
+    uint32_t *const seen = reinterpret_cast<uint32_t *>(sums + kAttnWarps * NT * 8) + warp * S;
+    const int inners = (int)d.kv_heads * a.groups, cta = blockIdx.x;
+
+    griddep_wait();
+    griddep_launch();
+
+    // ---- this CTA's units -------------------------------------------------------------------------------------
+    __shared__ long long warp_units[kAttnWarps];
+    __shared__ long long first_b, first_rest;
+    const int64_t per = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * per, b1 = b0 + per < d.batch ? b0 + per : d.batch;
+    long long mine = 0;
+    for (int64_t b = b0; b < b1; b++) mine += span_of(d, b).units;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_units[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; w++) {
+        if (w == warp) upto += total;
+        total += warp_units[w];
+    }
+    total *= inners;
+    const long long n = total < a.ctas ? total : a.ctas;                       // (every CTA that works has a unit)
+    const long long u0 = cta < n ? total * cta / n : 0, u1 = cta < n ? total * (cta + 1) / n : 0;
+    if (cta >= n && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
+    if (u0 < u1) {
+        const long long before = (upto - mine) * inners;
+        if (u0 >= before && u0 < upto * inners) {
+            long long rest = u0 - before;
+            int64_t b = b0;
+            for (;; b++) {
+                const long long here = (long long)span_of(d, b).units * inners;
+                if (rest < here) break;
+                rest -= here;
+            }
+            first_b = b;
+            first_rest = rest;
+        }
+    }
+    __syncthreads();
+
+    if (u0 < u1) {
+        Walk now;                                // the unit that is computed
+        now.b = first_b;
+        now.s = span_of(d, now.b);
+        now.inner = (int)(first_rest / now.s.units);
+        now.unit = (int)(first_rest % now.s.units);
+        Walk next = now;                         // the unit whose copies are issued next
+        long long left = u1 - u0;                // units not issued yet
+        int fresh_q = 0;                         // (request, head group) pairs issued so far: place in the ring of queries
+        bool first_issue = true;
+        // a lane's key of the unit `next`: its page is looked up one unit ahead of the copies
+        int page, place;
+        auto look_up = [&]() {
+            const int key = next.s.from + next.unit * kUnitKeys + warp * kWarpKeys + (lane & 15);
+            page = -1;
+            place = 0;
+            if (key < next.s.n) {
+                const int col = (int)a.by_page.quotient((uint32_t)key);
+                place = key - col * (int)d.page_size;
+                page = d.block_table[next.s.row * d.table_stride + col];
+            }
+        };
+        look_up();
+        auto issue = [&](int stage) {
+            if (left > 0) {
+                left--;
+                const int head = next.inner / a.groups, group = next.inner - head * a.groups;
+                if (page >= d.pages) page = -1;
+                const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
+                if (lane == 0) seen[stage] = ok;
+                const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
+                const T *const k = (const T *)d.k_cache + head * d.k_head_stride, *const v = (const T *)d.v_cache + head * d.v_head_stride;
+#pragma unroll
+                for (int i = 0; i < Shape::kChunks / 2; i++) {
+                    const int at = i * 32 + lane, row = at / Shape::kChunks, chunk = at % Shape::kChunks;
+                    const int pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
+                    const bool on = pg >= 0 && chunk * 8 < D;
+                    const int64_t p = on ? pg : 0, o = on ? pl : 0, e = on ? chunk * 8 : 0;
+                    copy16_async(dst + Shape::at(row, chunk), k + p * d.k_page_stride + o * d.k_slot_stride + e, on);
+                    copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), v + p * d.v_page_stride + o * d.v_slot_stride + e, on);
+                }
+                if (next.unit == 0 || first_issue) {                           // its queries, a quarter per warp
+                    const uint32_t qdst = shared_addr(q_ring + fresh_q * Shape::kQ);
+                    const int h0 = head * (int)(d.q_heads / d.kv_heads) + group * a.per_group;
+                    const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+                    for (int at = tid; at < NT * 8 * Shape::kChunks; at += kAttnThreads) {
+                        const int row = at / Shape::kChunks, chunk = at % Shape::kChunks;
+                        const bool on = row < heads && chunk * 8 < D;
+                        copy16_async(qdst + Shape::at(row, chunk),
+                                     (const T *)d.q + next.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
+                    }
+                    if (++fresh_q == S) fresh_q = 0;
+                    first_issue = false;
+                }
+                if (left > 0) {
+                    next.step(d, inners);
+                    look_up();
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S - 1; s++) issue(s);
+
+        uint32_t q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? KS : 1][2];
+        float o[KS][NT][4], top[NT][2], sum[NT][2];
+        int stage = 0, q_at = -1;
+        bool started_here = true;                // the request's first unit is this CTA's
+        for (long long u = u0; u < u1; u++) {
+            copy_wait<S - 2>();
+            __syncwarp();
+            if (u == u0 || now.unit == 0) {
+                started_here = now.unit == 0;
+                if (++q_at == S) q_at = 0;
+                __syncthreads();                 // every warp's part of the queries is there
+                if constexpr (Shape::kKeepQ) {
+                    const uint32_t src = shared_addr(q_ring + q_at * Shape::kQ);
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int ks = 0; ks < KS; ks++) ldmatrix2(q[t][ks][0], q[t][ks][1], src + Shape::at(t * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    top[t][0] = top[t][1] = -INFINITY;
+                    sum[t][0] = sum[t][1] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < KS; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
+                }
+            }
+            const uint32_t ok = seen[stage];
+            const uint32_t keys = shared_addr(ring + stage * Shape::kStage), values = keys + Shape::kHalfTile;
+            issue(stage == 0 ? S - 1 : stage - 1);
+            if (ok) {
+                float s[NT][4];
+#pragma unroll
+                for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t k[4];
+                    ldmatrix4(k, keys + Shape::at((lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        if constexpr (Shape::kKeepQ) {
+                            Type::mma(s[t], k, q[t][ks][0], q[t][ks][1]);
+                        } else {
+                            uint32_t b0, b1;
+                            ldmatrix2(b0, b1, shared_addr(q_ring + q_at * Shape::kQ) + Shape::at(t * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+                            Type::mma(s[t], k, b0, b1);
+                        }
+                    }
+                }
+                // rows (keys) lane / 4 and lane / 4 + 8, columns (queries) 2 (lane % 4) and the next
+                const bool on0 = (ok >> (lane >> 2)) & 1, on1 = (ok >> ((lane >> 2) + 8)) & 1;
+                float now_top[NT][2];
+                bool grows = false;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        s[t][e] = on0 ? s[t][e] * a.scale_log2 : -INFINITY;
+                        s[t][e + 2] = on1 ? s[t][e + 2] * a.scale_log2 : -INFINITY;
+                        float m = fmaxf(s[t][e], s[t][e + 2]);
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        grows = grows || m > top[t][e];
+                        now_top[t][e] = fmaxf(top[t][e], m);
+                    }
+                if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        float keep[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            keep[e] = now_top[t][e] == -INFINITY ? 1.f : exp2_approx(top[t][e] - now_top[t][e]);
+                            top[t][e] = now_top[t][e];
+                            sum[t][e] *= keep[e];
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; i++) {
+                            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1]; o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
+                        }
+                    }
+                }
+                // Probabilities as two 16-bit parts, so that the product keeps what FP32 has of them (one part alone would add an error as large as
+                // the output's own rounding).  The upper part is kept strictly below the value and the lower above zero: an infinite
+                // value then meets two positive factors, as in the formula.
+                uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float base = (top[t][e] == -INFINITY ? 0.f : top[t][e]) - Type::lift;
+                        p[e] = exp2_approx(s[t][e] - base);
+                        p[e + 2] = exp2_approx(s[t][e + 2] - base);
+                        sum[t][e] += p[e] + p[e + 2];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const uint32_t h = Type::pack_rz(p[2 * r] * Type::below, p[2 * r + 1] * Type::below);
+                        const float2 f = Half<T>::unpack(h);
+                        hi[t][r] = transpose8x8(h);
+                        lo[t][r] = transpose8x8(Half<T>::pack(p[2 * r] - f.x, p[2 * r + 1] - f.y));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    uint32_t v[4];
+                    ldmatrix4_trans(v, values + Shape::at((lane & 7) + (lane >> 4) * 8, i * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        Type::mma(o[i][t], v, hi[t][0], hi[t][1]);
+                        Type::mma(o[i][t], v, lo[t][0], lo[t][1]);
+                    }
+                }
+            }
+            if (++stage == S) stage = 0;
+            const bool last = now.unit == now.s.units - 1;
+            if (last || u + 1 == u1) {
+                // ---- the four warps' sums over their keys of this request become one ---------------------------------------
+                const int head = now.inner / a.groups, group = now.inner - head * a.groups;
+                const int h0 = head * (int)(d.q_heads / d.kv_heads) + group * a.per_group;
+                const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+                const bool whole = started_here && last;
+                const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float l = sum[t][e];
+                        l += __shfl_xor_sync(0xffffffffu, l, 4);
+                        l += __shfl_xor_sync(0xffffffffu, l, 8);
+                        l += __shfl_xor_sync(0xffffffffu, l, 16);
+                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(top[t][e], l);
+                    }
+                __syncthreads();
+                float factor[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float m = -INFINITY;
+#pragma unroll
+                        for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, sums[w * NT * 8 + t * 8 + 2 * (lane & 3) + e].x);
+                        factor[t][e] = top[t][e] == -INFINITY ? 0.f : exp2_approx(top[t][e] - m);
+                    }
+                const int fq = tid >> 4, fd = (tid & 15) * 4;                  // the query and the four elements that a thread adds up
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float m = -INFINITY, l = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, sums[w * NT * 8 + t * 8 + fq].x);
+#pragma unroll
+                    for (int w = 0; w < kAttnWarps; w++) {
+                        const float2 x = sums[w * NT * 8 + t * 8 + fq];
+                        l += x.x == -INFINITY ? x.y : x.y * exp2_approx(x.x - m);       // (nothing, or NaN)
+                    }
+                    const int row = t * 8 + fq;
+                    if (fd == 0 && row < heads) {
+                        if (!whole) a.sums[slot * NT * 8 + row] = make_float2(m, l);
+                        else if (d.lse) d.lse[now.b * d.q_heads + h0 + row] = l == 0.f ? -INFINITY : (m - Type::lift + __log2f(l)) * 0.6931471805599453f;
+                    }
+                    const float inverse = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+#pragma unroll
+                    for (int i0 = 0; i0 < KS; i0 += 4) {
+                        float *const to = fold + warp * 8 * 68 + 2 * (lane & 3) * 68 + (lane >> 2);
+#pragma unroll
+                        for (int i = i0; i < i0 + 4 && i < KS; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) to[(e & 1) * 68 + (i - i0) * 16 + (e >> 1) * 8] = o[i][t][e] * factor[t][e & 1];
+                        __syncthreads();
+                        const int el = i0 * 16 + fd;
+                        if (row < heads && el < D) {
+                            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int w = 0; w < kAttnWarps; w++) {
+                                const float4 y = *reinterpret_cast<const float4 *>(fold + (w * 8 + fq) * 68 + fd);
+                                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                            }
+                            if (whole) {
+                                uint2 r;
+                                r.x = Half<T>::pack(x.x * inverse, x.y * inverse);
+                                r.y = Half<T>::pack(x.z * inverse, x.w * inverse);
+                                *reinterpret_cast<uint2 *>((T *)d.out + now.b * d.out_token_stride + (h0 + row) * d.out_head_stride + el) = r;
+                            } else {
+                                *reinterpret_cast<float4 *>(a.part + (slot * NT * 8 + row) * D + el) = x;
+                            }
+                        }
+                        __syncthreads();
+                    }
+                }
+                if (u + 1 == u1 && tid == 0) {
+                    const bool goes_on = started_here && !last;
+                    // the CTA of the request's last unit: the last one whose first unit is not behind it
+                    const long long end = u + (now.s.units - now.unit);
+                    a.cut[cta] = make_int4((int)now.b, now.inner, goes_on ? (int)((end * n - 1) / total) : 0, goes_on ? 1 : 0);
+                }
+            }
+            if (u + 1 < u1) now.step(d, inners);
+        }
+        copy_wait<0>();
+    }
+    // ---- rows without keys ---------------------------------------------------------------------------------------
+    for (int64_t b = cta; b < d.batch; b += gridDim.x) {
+        if (span_of(d, b).units) continue;
+        const int chunks = D / 8;
+        for (int i = tid; i < (int)d.q_heads * chunks; i += kAttnThreads) {
+            const int h = i / chunks, c = i - h * chunks;
+            *reinterpret_cast<uint4 *>((T *)d.out + b * d.out_token_stride + h * d.out_head_stride + c * 8) = make_uint4(0, 0, 0, 0);
+            if (d.lse && c == 0) d.lse[b * d.q_heads + h] = -INFINITY;
+        }
+    }
+}
+
+// Adds the parts of a request that was cut, in the order of its keys.  A CTA per CTA of the kernel above (the one where a cut request starts) and
+// query head; its warps take every fourth part, a lane four elements (eight: head dims above 128).
+template <class T>
+__global__ void __launch_bounds__(128)
+join_kernel(const __grid_constant__ AttentionArgs a, int rows)
+{
+    __shared__ float4 acc[3][64];
+    const auto &d = a.d;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y, D = (int)d.head_dim;
+    griddep_wait();
+    griddep_launch();
+    const int4 cut = a.cut[blockIdx.x];
+    if (!cut.w) return;
+    const int head = cut.y / a.groups, group = cut.y - head * a.groups, per_kv = (int)(d.q_heads / d.kv_heads);
+    if (row >= min(a.per_group, per_kv - group * a.per_group)) return;
+    const int first = blockIdx.x, parts = cut.z - first + 1;
+    auto slot = [&](int i) { return ((int64_t)2 * (first + i) + (i == 0 ? 1 : 0)) * rows + row; };
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.sums[slot(i)].x);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = lane; i < parts; i += 32) {
+        const float2 s = a.sums[slot(i)];
+        l += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - m);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 4) {
+        const float top = a.sums[slot(i)].x, f = top == -INFINITY ? 0.f : exp2_approx(top - m);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int el = (h * 32 + lane) * 4;
+            if (el < D) {
+                const float4 y = *reinterpret_cast<const float4 *>(a.part + slot(i) * D + el);
+                x[h].x += f * y.x; x[h].y += f * y.y; x[h].z += f * y.z; x[h].w += f * y.w;
+            }
+        }
+    }
+    if (warp) { acc[warp - 1][lane] = x[0]; acc[warp - 1][32 + lane] = x[1]; }
+    __syncthreads();
+    if (warp) return;
+    const float inverse = l == 0.f ? 0.f : 1.f / l;
+    const int64_t h0 = head * per_kv + group * a.per_group + row;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int el = (h * 32 + lane) * 4;
+        if (el >= D) continue;
+#pragma unroll
+        for (int w = 0; w < 3; w++) { const float4 y = acc[w][h * 32 + lane]; x[h].x += y.x; x[h].y += y.y; x[h].z += y.z; x[h].w += y.w; }
+        uint2 r;
+        r.x = Half<T>::pack(x[h].x * inverse, x[h].y * inverse);
+        r.y = Half<T>::pack(x[h].z * inverse, x[h].w * inverse);
+        *reinterpret_cast<uint2 *>((T *)d.out + cut.x * d.out_token_stride + h0 * d.out_head_stride + el) = r;
+    }
+    if (d.lse && lane == 0) d.lse[cut.x * d.q_heads + h0] = l == 0.f ? -INFINITY : (m - AttnType<T>::lift + __log2f(l)) * 0.6931471805599453f;
+}
+
+// ---- host: which variant, how much workspace -----------------------------------------------------------------
+struct AttnPlan { int dp, nt, per_group, groups, ctas; int64_t bytes; };
+AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d);             // attention.cu
+template <class T> int launch_attention(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream);
+
+template <class T, int DP, int NT>
+int launch_attention_as(const AttentionArgs &a, cudaStream_t stream)
+{
+    auto kern = paged_attention_kernel<T, DP, NT>;
+    static bool attr_set[kMaxDevices] = {};
+    const int dev = current_device_index();
+    if (dev < 0) return ORTHO_B200_ERR_CUDA;
+    if (!attr_set[dev]) {
+        OB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnShape<DP, NT>::kBytes));
+        attr_set[dev] = true;
+    }
+    const int st = launch_dependent(kern, dim3((unsigned)a.ctas), kAttnThreads, AttnShape<DP, NT>::kBytes, stream, a);
+    if (st) return st;
+    return launch_dependent(join_kernel<T>, dim3((unsigned)a.ctas, (unsigned)a.per_group), 128, 0, stream, a, NT * 8);
+}
+
+template <class T, int DP>
+int launch_attention_dim(const AttentionArgs &a, int nt, cudaStream_t stream)
+{
+    if (nt == 1) return launch_attention_as<T, DP, 1>(a, stream);
+    if (nt == 2) return launch_attention_as<T, DP, 2>(a, stream);
+    if constexpr (DP <= 128) return launch_attention_as<T, DP, 4>(a, stream);
+    return ORTHO_B200_ERR_SHAPE;
+}
+
+#define OB_ATTENTION_DIMS(X) X(64) X(80) X(96) X(112) X(128) X(192) X(256)
+
+template <class T>
+int launch_attention(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
+{
+#define OB_CASE(DP) if (p.dp == DP) return launch_attention_dim<T, DP>(a, p.nt, stream);
+    OB_ATTENTION_DIMS(OB_CASE)
+#undef OB_CASE
+    return ORTHO_B200_ERR_SHAPE;
+}
+
+}  // namespace ob
