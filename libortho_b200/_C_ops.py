@@ -498,5 +498,5 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, down: torch.Tensor, up: torch
 
     ``down`` [adapters, rank, in_features], ``up`` [adapters, out_features, rank], ``ids`` int32 (one per token; outside
     [0, adapters): no adapter), ``scales`` float32, ``ranks`` int32 [adapters]: rows of ``down`` and columns of ``up`` that an
-    adapter uses, rounded up to a multiple of 8.  rank is a multiple of 8 up to 256.  ``out`` may be ``y``."""
+    adapter uses, rounded up to a multiple of 8.  rank is a multiple of 8 up to 256; up to 8192 adapters.  ``out`` may be ``y``."""
     return _lib.fast().low_rank_add(x, y, down, up, ids, scales, ranks, out)

@@ -41,7 +41,6 @@ template <> struct AttnType<__half> {
         asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_16816(d, a, b0, b1); }
 };
 template <> struct AttnType<__nv_bfloat16> {
     static constexpr float lift = 0.f, below = 1.f - 1.f / 128.f;
@@ -51,29 +50,8 @@ template <> struct AttnType<__nv_bfloat16> {
         asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-    {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
 };
 
-__device__ __forceinline__ uint32_t shared_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix2(uint32_t &r0, uint32_t &r1, uint32_t addr)
-{
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
 {
     uint32_t r;
@@ -303,11 +281,11 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         if constexpr (Shape::kKeepQ) {
-                            Type::mma(s[t], k, q[t][ks][0], q[t][ks][1]);
+                            Half<T>::mma(s[t], k, q[t][ks][0], q[t][ks][1]);
                         } else {
                             uint32_t b0, b1;
                             ldmatrix2(b0, b1, shared_addr(q_ring + q_at * Shape::kQ) + Shape::at(t * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
-                            Type::mma(s[t], k, b0, b1);
+                            Half<T>::mma(s[t], k, b0, b1);
                         }
                     }
                 }
@@ -372,8 +350,8 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     ldmatrix4_trans(v, values + Shape::at((lane & 7) + (lane >> 4) * 8, i * 2 + ((lane >> 3) & 1)));
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        Type::mma(o[i][t], v, hi[t][0], hi[t][1]);
-                        Type::mma(o[i][t], v, lo[t][0], lo[t][1]);
+                        Half<T>::mma(o[i][t], v, hi[t][0], hi[t][1]);
+                        Half<T>::mma(o[i][t], v, lo[t][0], lo[t][1]);
                     }
                 }
             }

@@ -327,6 +327,7 @@ PyObject *low_rank_add(PyObject *, PyObject *const *a, Py_ssize_t n)
     TORCH_CHECK_VALUE(down.is_contiguous() && up.is_contiguous() && aligned(down) && aligned(up), "down and up must be contiguous and 16-byte aligned");
     const int64_t E = down.size(0), R = down.size(1), K = down.size(2), N = up.size(1);
     TORCH_CHECK_VALUE(R >= 8 && R % 8 == 0 && R <= 256 && K >= 8 && K % 8 == 0 && N >= 1, "rank must be a multiple of 8 up to 256 and in_features a multiple of 8");
+    TORCH_CHECK_VALUE(E <= 8192, "at most 8192 adapters");
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K && y.dim() == x.dim() && y.size(-1) == N, "x must be [..., in_features] and y [..., out_features]");
     for (int64_t i = 0; i + 1 < x.dim(); i++) TORCH_CHECK_VALUE(x.size(i) == y.size(i), "x and y must have the same tokens");
     const int64_t T = x.numel() / K;
