@@ -3,18 +3,19 @@
 //     v[t] = down_e x[t],   out[t] = y[t] + scale_e up_e v[t],   e = ids[t]
 //
 // Few tokens: bound by the weights of the adapters in use (2 rank (K + N) bytes each).  Many tokens: by the activations (2 (K + 2 N) bytes a
-// token).  The operations are a few per byte either way, so both products run on m16n8k16 tensor-core instructions with operands loaded
-// straight from global memory, 16 or 8 bytes a lane: the order of k (or of the rank) inside an instruction is free as long as both operands use
-// the same one.
+// token).  The operations are a few per byte either way, so both products run on m16n8k16 tensor-core instructions.
 //
 // Tokens are grouped first, so that an adapter's weights are read once for all its tokens: `order` lists them by adapter, a tile is up to
 // kTile of them with one adapter.  Up to kFewTokens tokens every CTA groups them for itself; more are grouped by a kernel in front.
 //
-// down_kernel: a cluster of CTAs per tile and 16 to 64 ranks, K split over its warps, their sums joined through distributed shared memory in a fixed
-// order.  up_kernel: a CTA per tile and some columns; it is launched as a programmatic dependent and loads its first weights (constants of
-// the layer) while down_kernel still runs.
+// down_kernel: a cluster of CTAs per tile and 16 or 32 ranks, K split over its warps, their sums joined through distributed shared memory in a fixed
+// order.  Operands come straight from global memory, 16 bytes a lane: the order of k inside an instruction is free as long as both use
+// the same one.  up_kernel is launched as a programmatic dependent and fetches its first weights (constants of the layer) while down_kernel
+// still runs.
 #include "launch.cuh"
 #include "tma.cuh"
+
+#include <type_traits>
 
 namespace ob {
 
@@ -24,9 +25,10 @@ struct LowRankArgs {
     ortho_b200_low_rank_desc d;
     int *heads;                                  // {tiles with an adapter, all tiles}; these three: more than kFewTokens tokens
     int *order;                                  // [tokens] grouped by adapter, those without one last
-    int4 *tiles;                                 // {adapter or -1, first place in order, tokens, 0}
+    int4 *tiles;                                 // {adapter or -1, first place in order, tokens, rank}
     float *v;                                    // [tokens][rank], by place in order
-    int rank_groups;
+    int rank_groups;                             // of down_kernel's ranks
+    int blocks, padded, up_groups;               // of up_kernel's columns; rank in whole 16; groups of 64 ranks
     bool vectors, copies;                        // rows of y and out in 16-byte pieces; out is not y
 };
 
@@ -36,27 +38,31 @@ __device__ __forceinline__ int rank_of(const ortho_b200_low_rank_desc &d, int e)
     const int64_t r = ((int64_t)max(__ldcg(d.ranks + e), 0) + 7) / 8 * 8;
     return (int)(r < d.rank ? r : d.rank);
 }
-// the adapter of a token, or d.adapters for none
-__device__ __forceinline__ int adapter_of(const ortho_b200_low_rank_desc &d, int64_t t)
+// the adapter of a token and its rank; d.adapters for none
+__device__ __forceinline__ int adapter_of(const ortho_b200_low_rank_desc &d, int64_t t, int &rank)
 {
     const int32_t e = __ldcg(d.ids + t);
-    return e >= 0 && e < d.adapters && rank_of(d, e) > 0 ? e : (int)d.adapters;
+    rank = e >= 0 && e < d.adapters ? rank_of(d, e) : 0;
+    return rank > 0 ? e : (int)d.adapters;
 }
 
 // ---- grouping ----------------------------------------------------------------------------------------------------
 struct FewTokens { int adapter[kFewTokens], order[kFewTokens]; int4 at[kFewTokens], tiles[kFewTokens]; int count[kFewTokens / 32]; };
 
-// by a CTA of kFewTokens threads; returns (tiles with an adapter, all tiles)
+// by a CTA of kFewTokens threads or more; returns (tiles with an adapter, all tiles)
 template <int TILE>
 __device__ __forceinline__ int2 group_few(FewTokens &g, const ortho_b200_low_rank_desc &d)
 {
     const int t = threadIdx.x, T = (int)d.tokens, lane = t & 31, warp = t >> 5;
-    const int e = t < T ? adapter_of(d, t) : 0x7FFFFFFF;
-    g.adapter[t] = e;
-    g.at[t] = make_int4(-2, 0, 0, 0);
+    int rank = 0;
+    const int e = t < T ? adapter_of(d, t, rank) : 0x7FFFFFFF;
+    if (t < kFewTokens) {
+        g.adapter[t] = e;
+        g.at[t] = make_int4(-2, 0, 0, 0);
+    }
     __syncthreads();
     int less = 0, before = 0, same = 0;
-    for (int i = 0; i < T; i += 4) {
+    for (int i = 0; i < T && t < T; i += 4) {
         const int4 o = *reinterpret_cast<const int4 *>(g.adapter + i);
         less += (o.x < e) + (o.y < e) + (o.z < e) + (o.w < e);
         same += (o.x == e) + (o.y == e) + (o.z == e) + (o.w == e);
@@ -65,15 +71,15 @@ __device__ __forceinline__ int2 group_few(FewTokens &g, const ortho_b200_low_ran
     const int place = less + before;
     if (t < T) {
         g.order[place] = t;
-        if (before % TILE == 0) g.at[place] = make_int4(e < d.adapters ? e : -1, place, min(TILE, same - before), 0);
+        if (before % TILE == 0) g.at[place] = make_int4(e < d.adapters ? e : -1, place, min(TILE, same - before), rank);
     }
     __syncthreads();
-    const int4 mine = g.at[t];
+    const int4 mine = t < kFewTokens ? g.at[t] : make_int4(-2, 0, 0, 0);
     const uint32_t leads = __ballot_sync(0xffffffffu, mine.x != -2);
-    if (lane == 0) g.count[warp] = __popc(leads);
+    if (lane == 0 && t < kFewTokens) g.count[warp] = __popc(leads);
     const int real = __syncthreads_count(mine.x >= 0), all = __syncthreads_count(mine.x != -2);
     int at = __popc(leads & ((1u << lane) - 1));
-    for (int w = 0; w < warp; w++) at += g.count[w];
+    for (int w = 0; w < warp && t < kFewTokens; w++) at += g.count[w];
     if (mine.x != -2) g.tiles[at] = mine;
     __syncthreads();
     return make_int2(real, all);
@@ -85,7 +91,8 @@ template <int TILE>
 __global__ void __launch_bounds__(kGroupThreads)
 group_kernel(const __grid_constant__ LowRankArgs a)
 {
-    extern __shared__ int counts[];              // [adapters + 1], then the next free place of each
+    constexpr int AHEAD = 4;                     // tokens of a thread that are loaded together
+    extern __shared__ int counts[];              // [adapters + 1]
     __shared__ int2 warp_sum[kGroupThreads / 32];
     const auto &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = (int)d.adapters + 1, T = (int)d.tokens;
@@ -94,14 +101,30 @@ group_kernel(const __grid_constant__ LowRankArgs a)
     griddep_launch();
     for (int e = tid; e < E; e += kGroupThreads) counts[e] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < T; t0 += kGroupThreads) {
-        const int t = t0 + tid, e = t < T ? adapter_of(d, t) : -1;
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && __ffs(peers) - 1 == lane) atomicAdd(counts + e, __popc(peers));
-    }
+    // the adapter of each token, its rank, and its number among its adapter's tokens
+    auto each = [&](auto &&use) {
+        for (int t0 = 0; t0 < T; t0 += AHEAD * kGroupThreads) {
+            int e[AHEAD], rank[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int t = t0 + i * kGroupThreads + tid;
+                rank[i] = 0;
+                e[i] = t < T ? adapter_of(d, t, rank[i]) : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                if (t0 + i * kGroupThreads >= T) break;
+                const uint32_t peers = __match_any_sync(0xffffffffu, e[i]);
+                const int leader = __ffs(peers) - 1;
+                int base = 0;
+                if (e[i] >= 0 && leader == lane) base = atomicAdd(counts + e[i], __popc(peers));
+                use(t0 + i * kGroupThreads + tid, e[i], rank[i], base, peers, leader);
+            }
+        }
+    };
+    each([](int, int, int, int, uint32_t, int) {});
     __syncthreads();
     int2 before = make_int2(0, 0);               // tokens and tiles of the adapters before
-    int real = 0;
     for (int e0 = 0; e0 < E; e0 += kGroupThreads) {
         const int e = e0 + tid, n = e < E ? counts[e] : 0, tiles = (n + TILE - 1) / TILE;
         int2 sum = make_int2(n, tiles);
@@ -112,53 +135,53 @@ group_kernel(const __grid_constant__ LowRankArgs a)
         }
         if (lane == 31) warp_sum[warp] = sum;
         __syncthreads();
-        int2 total = before;
-        for (int w = 0; w < kGroupThreads / 32; w++) {
-            if (w == warp) { sum.x += total.x; sum.y += total.y; }
-            total.x += warp_sum[w].x;
-            total.y += warp_sum[w].y;
+        // every warp adds up the warps' sums for itself
+        int2 w = warp_sum[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, w.x, o), y = __shfl_up_sync(0xffffffffu, w.y, o);
+            if (lane >= o) { w.x += x; w.y += y; }
         }
-        if (e < E) { start[e] = sum.x - n; first_tile[e] = sum.y - tiles; }
-        if (e == E - 1) real = sum.y - tiles;
-        before = total;
+        const int px = __shfl_sync(0xffffffffu, w.x, warp ? warp - 1 : 0), py = __shfl_sync(0xffffffffu, w.y, warp ? warp - 1 : 0);
+        sum.x += before.x + (warp ? px : 0);
+        sum.y += before.y + (warp ? py : 0);
+        if (e < E) { start[e] = sum.x - n; first_tile[e] = sum.y - tiles; counts[e] = 0; }
+        if (e == E - 1) { a.heads[0] = sum.y - tiles; a.heads[1] = sum.y; }
+        before.x += __shfl_sync(0xffffffffu, w.x, 31);
+        before.y += __shfl_sync(0xffffffffu, w.y, 31);
         __syncthreads();
     }
-    if ((E - 1) % kGroupThreads == tid) { a.heads[0] = real; a.heads[1] = before.y; }
-    int *const place = counts;                   // how many of an adapter have their place
-    // (the counts are needed for the tiles' sizes: the next adapter's start less one's own)
-    for (int e = tid; e < E; e += kGroupThreads) place[e] = 0;
-    __syncthreads();
-    for (int t0 = 0; t0 < T; t0 += kGroupThreads) {
-        const int t = t0 + tid, e = t < T ? adapter_of(d, t) : -1;
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        const int leader = __ffs(peers) - 1;
-        int base = 0;
-        if (e >= 0 && leader == lane) base = atomicAdd(place + e, __popc(peers));
+    each([&](int t, int e, int rank, int base, uint32_t peers, int leader) {
         base = __shfl_sync(0xffffffffu, base, leader);
-        if (e >= 0) {
-            const int among = base + __popc(peers & ((1u << lane) - 1)), at = start[e] + among;
-            a.order[at] = t;
-            if (among % TILE == 0) {
-                const int end = e + 1 < E ? start[e + 1] : T;
-                a.tiles[first_tile[e] + among / TILE] = make_int4(e + 1 < E ? e : -1, at, min(TILE, end - at), 0);
-            }
+        if (e < 0) return;
+        const int among = base + __popc(peers & ((1u << lane) - 1)), at = start[e] + among;
+        a.order[at] = t;
+        if (among % TILE == 0) {
+            const int end = e + 1 < E ? start[e + 1] : T;
+            a.tiles[first_tile[e] + among / TILE] = make_int4(e + 1 < E ? e : -1, at, min(TILE, end - at), rank);
         }
-    }
+    });
 }
 
 // ---- v = down x ------------------------------------------------------------------------------------------------------
-constexpr int kDownWarps = 4;
-
-// MB blocks of 16 ranks (the 16-row operand) by NT of 8 tokens
-template <class T, int MB, int NT, bool FEW>
-__global__ void __launch_bounds__(32 * kDownWarps)
+// MB blocks of 16 ranks (the 16-row operand) by NT of 8 tokens, by a cluster of CTAS.  Few tokens: 64 warps a cluster, so that the K of usual layers
+// is in flight all at once.
+template <class T, int MB, int NT, int CTAS, int WARPS, bool FEW>
+__global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
 down_kernel(const __grid_constant__ LowRankArgs a)
 {
-    constexpr int TOKENS = NT * 8, RANKS = MB * 16, PITCH = RANKS + 4, CHUNKS = MB * NT >= 8 ? 2 : 4;
-    __shared__ __align__(16) float sums[kDownWarps][TOKENS][PITCH];
+    // a step is 32 k; CHUNKS steps of a warp are loaded together, 64 to 128 registers
+    constexpr int TOKENS = NT * 8, RANKS = MB * 16, PITCH = RANKS + 4, CHUNKS = NT > 2 ? (MB == 1 ? 3 : 2) : 4;
+    constexpr int QUADS = TOKENS * RANKS / 4, SHARE = QUADS / CTAS, WARP_QUADS = TOKENS * PITCH / 4;
+    static_assert(QUADS % CTAS == 0, "every CTA adds up the same share");
+    __shared__ __align__(16) float sums[WARPS][TOKENS][PITCH];
+    // this CTA's share of the results, from every CTA of the cluster; twice where there is room
+    constexpr int TURNS = NT > 2 ? 1 : 2;
+    __shared__ __align__(16) float4 arrived[TURNS][CTAS][SHARE];
     __shared__ __align__(16) unsigned char few_smem[FEW ? sizeof(FewTokens) : 16];
     const auto &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = (int)cluster_ctarank();
+    cluster_arrive();                            // (waited for before the first store into another CTA: it has started then)
     griddep_wait();
     griddep_launch();
     FewTokens &few = *reinterpret_cast<FewTokens *>(few_smem);
@@ -174,11 +197,13 @@ down_kernel(const __grid_constant__ LowRankArgs a)
         order = a.order;
         tiles = a.tiles;
     }
-    const int K = (int)d.K, steps = (K + 31) / 32, clusters = gridDim.x / ctas;
+    const int K = (int)d.K, steps = (K + 31) / 32, clusters = gridDim.x / CTAS;
     const int quad = lane & 3, row = lane >> 2;
-    for (int64_t unit = blockIdx.x / ctas; unit < (int64_t)real * a.rank_groups; unit += clusters) {
+    int turn = 0;
+    cluster_wait();
+    for (int64_t unit = blockIdx.x / CTAS; unit < (int64_t)real * a.rank_groups; unit += clusters) {
         const int4 tile = tiles[unit / a.rank_groups];
-        const int r0 = (int)(unit % a.rank_groups) * RANKS, rank = rank_of(d, tile.x);
+        const int r0 = (int)(unit % a.rank_groups) * RANKS, rank = tile.w;
         if (r0 >= rank) continue;                // (the whole cluster)
         const T *x[NT];
 #pragma unroll
@@ -189,13 +214,13 @@ down_kernel(const __grid_constant__ LowRankArgs a)
         for (int m = 0; m < MB; m++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-        // 32 k a step, 8 of them (16 bytes of every row) a lane; steps are dealt to the cluster's warps in turn
-        const int stride = ctas * kDownWarps;
-        for (int s0 = cta * kDownWarps + warp; s0 < steps; s0 += CHUNKS * stride) {
+        // 8 of a step's k (16 bytes of every row) a lane; steps are dealt to the cluster's warps in turn
+        constexpr int STRIDE = CTAS * WARPS;
+        for (int s0 = cta * WARPS + warp; s0 < steps; s0 += CHUNKS * STRIDE) {
             uint4 wv[CHUNKS][MB][2], xv[CHUNKS][NT];
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++) {
-                const int k = (s0 + c * stride) * 32 + quad * 8;
+                const int k = (s0 + c * STRIDE) * 32 + quad * 8;
                 const bool on = k < K;
 #pragma unroll
                 for (int m = 0; m < MB; m++)
@@ -204,7 +229,7 @@ down_kernel(const __grid_constant__ LowRankArgs a)
                         wv[c][m][h] = on && r0 + m * 16 + h * 8 + row < rank ? ldg_stream(w + (int64_t)(m * 16 + h * 8) * d.K + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int j = 0; j < NT; j++)
-                    xv[c][j] = on && j * 8 < tile.z ? *reinterpret_cast<const uint4 *>(x[j] + k) : make_uint4(0, 0, 0, 0);
+                    xv[c][j] = on && j * 8 < tile.z ? load16(x[j] + k) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++)
@@ -220,6 +245,9 @@ down_kernel(const __grid_constant__ LowRankArgs a)
                     }
                 }
         }
+        // The warps' sums are added in order and sent to the CTA that adds up the cluster's.  With two turns one barrier a unit does: the results of the
+        // next one arrive in the other half of `arrived`, and those of the one behind it only after a barrier that this CTA reaches when it has
+        // read these.
 #pragma unroll
         for (int m = 0; m < MB; m++)
 #pragma unroll
@@ -227,223 +255,297 @@ down_kernel(const __grid_constant__ LowRankArgs a)
 #pragma unroll
                 for (int e = 0; e < 4; e++) sums[warp][j * 8 + quad * 2 + (e & 1)][m * 16 + row + (e >> 1) * 8] = acc[m][j][e];
         __syncthreads();
-        // the warps' sums, then the cluster's, each in order
-        float4 *const mine = reinterpret_cast<float4 *>(&sums[0][0][0]);
-        constexpr int QUADS = RANKS / 4, WARP_QUADS = TOKENS * PITCH / 4;
-        for (int i = tid; i < TOKENS * QUADS; i += 32 * kDownWarps) {
-            const int at = i / QUADS * (PITCH / 4) + i % QUADS;
+        const float4 *const mine = reinterpret_cast<const float4 *>(&sums[0][0][0]);
+        const uint32_t to = shared_addr(&arrived[turn][cta][0]);
+        for (int i = tid; i < QUADS; i += (32 * WARPS)) {
+            const int at = i / (RANKS / 4) * (PITCH / 4) + i % (RANKS / 4);
             float4 s = mine[at];
 #pragma unroll
-            for (int o = 1; o < kDownWarps; o++) {
+            for (int o = 1; o < WARPS; o++) {
                 const float4 y = mine[o * WARP_QUADS + at];
                 s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
             }
-            mine[at] = s;
+            st_dsmem_v4(mapa_shared(to + 16 * (i % SHARE), i / SHARE), s);
         }
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        for (int i = cta * 32 * kDownWarps + tid; i < TOKENS * QUADS; i += ctas * 32 * kDownWarps) {
-            const int token = i / QUADS, q = i % QUADS;
-            if (token >= tile.z || r0 + q * 4 >= rank) continue;
-            const uint32_t at = shared_addr(mine + token * (PITCH / 4) + q);
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int o = 0; o < ctas; o++) {
-                const uint32_t from = mapa_shared(at, o);
-                float4 y;
-                asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(from));
+        for (int i = tid; i < SHARE; i += (32 * WARPS)) {
+            const int token = (cta * SHARE + i) / (RANKS / 4), r = r0 + (cta * SHARE + i) % (RANKS / 4) * 4;
+            if (token >= tile.z || r >= rank) continue;
+            float4 s = arrived[turn][0][i];
+#pragma unroll
+            for (int o = 1; o < CTAS; o++) {
+                const float4 y = arrived[turn][o][i];
                 s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
             }
-            *reinterpret_cast<float4 *>(a.v + (int64_t)(tile.y + token) * d.rank + r0 + q * 4) = s;
+            *reinterpret_cast<float4 *>(a.v + (int64_t)(tile.y + token) * d.rank + r) = s;
         }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
+        if constexpr (TURNS == 2) {
+            turn ^= 1;
+        } else {
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+        }
     }
 }
 
 // ---- out = y + scale up v -------------------------------------------------------------------------------------------
-static_assert(kFewTokens == 32 * kDownWarps, "a thread per token");
-constexpr int kUpWarps = 4, kUpColumns = 32 * kUpWarps;
-
-// One unit of 32 columns by 64 ranks: rows of `up` as the 8-column operand, 4 tiles of 8 by 4 steps of 16 ranks.  Column c of tile j stands for
-// output column 8 (c / 2) + 2 j + c % 2, so that a lane's results over the four tiles are eight neighbours.
+// The products run over v in two 16-bit parts, so that it keeps what FP32 has of it.  In FP16 it is brought to the token's largest |v| in
+// [2^13, 2^14) by a power of two first (else it could leave FP16's range, or lose its small values): `down`, and `back` for the result.
+struct PowerOfTwo { float down, back; };
 template <class T>
-__device__ __forceinline__ void load_up(uint2 (&w)[4][4], const LowRankArgs &a, int e, int rank, int64_t n0, int r0, int lane)
+__device__ __forceinline__ PowerOfTwo bring_near(float top)
 {
-    const int row = lane >> 2, quad = lane & 3;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int64_t n = n0 + (row >> 1) * 8 + j * 2 + (row & 1);
-        const T *const p = (const T *)a.d.up + ((int64_t)e * a.d.N + n) * a.d.rank + r0 + quad * 4;
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            w[j][s] = make_uint2(0, 0);
-            if (n < a.d.N && r0 + s * 16 + quad * 4 < rank)
-                asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(w[j][s].x), "=r"(w[j][s].y) : "l"(p + s * 16));
-        }
-    }
+    const uint32_t exponent = __float_as_uint(top) >> 23;                      // top in [2^(exponent - 127), 2^(exponent - 126))
+    if (!std::is_same<T, __half>::value || exponent < 14 || exponent > 253) return {1.f, 1.f};      // (tiny, infinite or NaN as it is)
+    return {__uint_as_float((267 - exponent) << 23), __uint_as_float((exponent - 13) << 23)};
 }
+template <class T>
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    hi = Half<T>::pack(a, b);
+    const float2 f = Half<T>::unpack(hi);
+    lo = Half<T>::pack(a - f.x, b - f.y);
+}
+__device__ __forceinline__ float largest(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
-// MT tiles of 16 tokens
-template <class T, int MT, bool FEW>
-__global__ void __launch_bounds__(32 * kUpWarps)
+constexpr int kUpThreads = 128, kUpStages = 3;
+static_assert(kFewTokens == kUpThreads && kGroupThreads == 32 * 32, "a thread per token, a lane per warp");
+
+// Columns of a pair and the layout of a stage: rows of G ranks, 16 bytes of padding against bank conflicts
+template <int MT, int G>
+struct UpShape {
+    static constexpr int kTokens = MT * 16, kColumns = MT == 1 ? 128 : 64, kPieces = G / 8, kPitch = G * 2 + 16, kStage = kColumns * kPitch;
+    static int bytes(int padded) { return kUpStages * kStage + 64 + 2 * kTokens * (padded * 2 + 16); }
+};
+
+// The (tile, columns) pairs are numbered in a row and dealt evenly, a run of them to each CTA, so that v comes into shared memory about once per
+// CTA.  Rows of `up` arrive in a ring of three stages of up to 64 ranks, the first ones while down_kernel still runs; y is loaded a pair ahead.
+// Tiles of 16 tokens (MT = 1): a warp has 32 of 128 columns, bound by the weights.  Of 64 (MT = 4): a warp has 16 tokens and 64 columns, bound by
+// y and out.  Column c of 8 in product tile j stands for output column 8 (c / 2) + 2 j + c % 2 of 32, so that a lane's results over four
+// tiles are eight neighbours.
+template <class T, int MT, int G, bool FEW>
+__global__ void __launch_bounds__(kUpThreads, 4)
 up_kernel(const __grid_constant__ LowRankArgs a)
 {
-    constexpr int TOKENS = MT * 16;
-    constexpr bool NORMED = sizeof(T) == 2 && std::is_same<T, __half>::value;
+    using Shape = UpShape<MT, G>;
+    constexpr int TOKENS = Shape::kTokens, COLUMNS = Shape::kColumns, Q = MT == 1 ? 1 : COLUMNS / 32, S = kUpStages, PIECES = Shape::kPieces, PITCH = Shape::kPitch;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float factor[TOKENS];
     __shared__ __align__(16) unsigned char few_smem[FEW ? sizeof(FewTokens) : 16];
     const auto &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, row = lane >> 2;
-    const int padded = ((int)d.rank + 15) / 16 * 16, pitch = padded * 2 + 16;
-    unsigned char *const upper = smem, *const lower = smem + TOKENS * pitch;
-    // What is read in front of the wait was complete before down_kernel began (it lets this kernel start behind its own wait), or is
-    // a constant of the layer.
+    const int padded = a.padded, groups = G < 64 ? 1 : a.up_groups, v_pitch = padded * 2 + 16, N = (int)d.N;
+    unsigned char *const upper = smem + S * Shape::kStage + 64, *const lower = upper + TOKENS * v_pitch;
+    const int t0 = MT == 1 ? 0 : warp * 16, c0 = MT == 1 ? warp * 32 : 0;      // this warp's first token of the tile and column of the pair
+    // What is read in front of the wait was complete before down_kernel let this kernel start (it does so behind its own wait), or is a
+    // constant of the layer.
     griddep_launch();
     FewTokens &few = *reinterpret_cast<FewTokens *>(few_smem);
-    const int *order;
-    const int4 *tiles;
     int all;
     if constexpr (FEW) {
         const int2 n = group_few<TOKENS>(few, d);
         all = a.copies ? n.y : n.x;
-        order = few.order;
-        tiles = few.tiles;
     } else {
         all = __ldcg(a.heads + (a.copies ? 1 : 0));
-        order = a.order;
-        tiles = a.tiles;
     }
-    const int64_t blocks = (d.N + kUpColumns - 1) / kUpColumns;
-    // blocks of columns per unit: several where there are units enough, so that v is brought into place less often
-    int64_t span = all * blocks / ((int64_t)gridDim.x * 4);
-    span = span < 1 ? 1 : span < 8 ? span : 8;
-    const int64_t spans = (blocks + span - 1) / span, units = all * spans;
-    bool waited = false;
-    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        int4 tile;
-        if constexpr (FEW) tile = tiles[unit / spans];
-        else tile = __ldcg(tiles + unit / spans);
-        const int64_t first = unit % spans * span * kUpColumns, end = min(first + span * kUpColumns, d.N);
-        const int e = tile.x, rank = e < 0 ? 0 : rank_of(d, e);
-        uint2 w[4][4];
-        if (e >= 0) load_up<T>(w, a, e, rank, first + warp * 32, 0, lane);
-        if (!waited) griddep_wait();
-        waited = true;
-        __syncthreads();                         // the unit before is done with v
-        if (e >= 0) {
-            // v as two 16-bit parts, ranks in the order of the loads above; FP16: relative to the token's largest, by a power of two
-            for (int t = warp; t < TOKENS; t += kUpWarps) {
-                float4 x[2];
-                float top = 0.f;
+    auto tile_at = [&](int i) { if constexpr (FEW) return few.tiles[i]; else return __ldcg(a.tiles + i); };
+    const int64_t pairs = (int64_t)all * a.blocks, first = pairs * blockIdx.x / gridDim.x, end = pairs * (blockIdx.x + 1) / gridDim.x;
+    int left = (int)(end - first), to_issue = left;
+
+    // the copies of a step (pair, up to 64 ranks); each thread has PIECES (or half as many) of the 16-byte pieces
+    int next_group = 0, next_tile = left ? (int)(first / a.blocks) : 0, next_block = left ? (int)(first - (int64_t)next_tile * a.blocks) : 0;
+    int4 ahead = left ? tile_at(next_tile) : make_int4(-1, 0, 0, 0);
+    auto issue = [&](int stage) {
+        if (to_issue > 0) {
+            const int r0 = next_group * G;
+            if (ahead.x >= 0 && r0 < ahead.w) {
+                const uint32_t to = shared_addr(smem + stage * Shape::kStage);
+                const T *const from = (const T *)d.up + ((int64_t)ahead.x * N + next_block * COLUMNS) * d.rank + r0;
+                const int columns = N - next_block * COLUMNS, ranks = ahead.w - r0;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int r = (h * 32 + lane) * 4;
-                    x[h] = t < tile.z && r < rank ? __ldcg(reinterpret_cast<const float4 *>(a.v + (int64_t)(tile.y + t) * d.rank + r)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    top = fmaxf(top, fmaxf(fmaxf(fabsf(x[h].x), fabsf(x[h].y)), fmaxf(fabsf(x[h].z), fabsf(x[h].w))));
+                for (int u = 0; u < COLUMNS * PIECES / kUpThreads; u++) {
+                    const int i = u * kUpThreads + tid, n = i / PIECES, piece = i % PIECES;
+                    const bool on = n < columns && piece * 8 < ranks;
+                    const int at = (n & ~31) + (n >> 1 & 3) * 8 + (n >> 3 & 3) * 2 + (n & 1);      // product tile j = n / 2 % 4, its column c
+                    copy16_async(to + at * PITCH + piece * 16, on ? from + n * (int)d.rank + piece * 8 : from, on);
                 }
-                float back = 1.f;
-                if (NORMED) {
-#pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int exponent = (int)(__float_as_uint(top) >> 23);                   // top in [2^(exponent - 127), 2^(exponent - 126))
-                    if (exponent >= 14 && exponent <= 253) {                                  // (else: tiny, infinite or NaN as it is)
-                        const float down = __uint_as_float((uint32_t)(min(127 + 140 - exponent, 254)) << 23);
-                        back = __uint_as_float((uint32_t)(254 - min(127 + 140 - exponent, 254)) << 23);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) { x[h].x *= down; x[h].y *= down; x[h].z *= down; x[h].w *= down; }
-                    }
-                }
-                if (lane == 0) factor[t] = back * (d.scales ? __ldcg(d.scales + e) : 1.f);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int r = (h * 32 + lane) * 4;
-                    if (r >= padded) continue;
-                    const uint32_t u0 = Half<T>::pack(x[h].x, x[h].y), u1 = Half<T>::pack(x[h].z, x[h].w);
-                    const float2 f0 = Half<T>::unpack(u0), f1 = Half<T>::unpack(u1);
-                    const int at = t * pitch + (r >> 4) * 32 + (r & 15);                      // four ranks: two words, eight ranks apart
-                    *reinterpret_cast<uint32_t *>(upper + at) = u0;
-                    *reinterpret_cast<uint32_t *>(upper + at + 16) = u1;
-                    *reinterpret_cast<uint32_t *>(lower + at) = Half<T>::pack(x[h].x - f0.x, x[h].y - f0.y);
-                    *reinterpret_cast<uint32_t *>(lower + at + 16) = Half<T>::pack(x[h].z - f1.x, x[h].w - f1.y);
+            }
+            if (++next_group == groups) {
+                next_group = 0;
+                to_issue--;
+                if (++next_block == a.blocks && to_issue > 0) {
+                    next_block = 0;
+                    ahead = tile_at(++next_tile);
                 }
             }
         }
-        __syncthreads();
-        for (int64_t n0 = first + warp * 32; n0 < end; n0 += kUpColumns) {
-            const int64_t n = n0 + quad * 8;
-            float acc[MT][4][4];
+        copy_commit();
+    };
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+    for (int s = 0; s < S - 1; s++) issue(s);
+    griddep_wait();
+    if (left == 0) return;
+
+    int tile_number = (int)(first / a.blocks), block = (int)(first - (int64_t)tile_number * a.blocks), stage = 0;
+    bool new_tile = true;
+    int4 tile;
+    // this lane's place in its two tokens' rows of y and out: column c0 + 8 quad of the pair
+    const T *y_at[2];
+    T *out_at[2];
+    bool has[2];
+    uint4 y[Q][2];
+    auto load_y = [&]() {
+        if (a.vectors && (block + 1) * COLUMNS <= N) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-            const bool whole = a.vectors && n + 8 <= d.N;
-            for (int r0 = 0; r0 < rank; r0 += 64) {
-                uint2 next[4][4];
-                const bool more = r0 + 64 < rank || n0 + kUpColumns < end;
-                if (more) load_up<T>(next, a, e, rank, r0 + 64 < rank ? n0 : n0 + kUpColumns, r0 + 64 < rank ? r0 + 64 : 0, lane);
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    if (r0 + s * 16 >= rank) break;
+                for (int q = 0; q < Q; q++)
+                    if (has[h]) y[q][h] = load16(y_at[h] + q * 32);
+        }
+    };
+    for (;;) {
+        float acc[Q * 4][4];
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        if (m * 16 >= tile.z) break;
-                        uint32_t v[4];
-                        const int at = (m * 16 + (lane & 15)) * pitch + (r0 / 16 + s) * 32 + (lane >> 4) * 16;
-                        ldmatrix4(v, shared_addr(upper + at));
-#pragma unroll
-                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[m][j], v, w[j][s].x, w[j][s].y);
-                        ldmatrix4(v, shared_addr(lower + at));
-#pragma unroll
-                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[m][j], v, w[j][s].x, w[j][s].y);
-                    }
-                }
-                if (more) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int s = 0; s < 4; s++) w[j][s] = next[j][s];
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < MT; m++)
+        for (int j = 0; j < Q * 4; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        for (int group = 0; group < groups; group++) {
+            copy_wait<S - 2>();
+            __syncthreads();                     // the stage is there, and everybody is done with the one before it and with v
+            issue(stage == 0 ? S - 1 : stage - 1);
+            if (new_tile) {
+                new_tile = false;
+                tile = tile_at(tile_number);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int t = m * 16 + h * 8 + row;
-                    if (t >= tile.z || n >= d.N) continue;
-                    const int64_t token = FEW ? order[tile.y + t] : __ldcg(order + tile.y + t);
-                    const T *const y = (const T *)d.y + token * d.y_stride + n;
-                    T *const out = (T *)d.out + token * d.out_stride + n;
-                    const float f = e < 0 ? 0.f : factor[t];
-                    if (whole) {
-                        uint4 u = *reinterpret_cast<const uint4 *>(y);
-                        if (e >= 0) {
-                            uint32_t *const p = reinterpret_cast<uint32_t *>(&u);
+                    const int t = t0 + h * 8 + row;
+                    has[h] = t < tile.z;
+                    const int64_t token = !has[h] ? 0 : FEW ? few.order[tile.y + t] : __ldcg(a.order + tile.y + t);
+                    y_at[h] = (const T *)d.y + token * d.y_stride + block * COLUMNS + c0 + quad * 8;
+                    out_at[h] = (T *)d.out + token * d.out_stride + block * COLUMNS + c0 + quad * 8;
+                }
+                load_y();
+                if (tile.x >= 0) {
+                    const float scale = d.scales ? __ldcg(d.scales + tile.x) : 1.f;
+                    // lanes of a token: the power of two that holds a quarter of the rank, at most a warp (twice: above 128)
+                    const int width = padded <= 16 ? 4 : padded <= 32 ? 8 : padded <= 64 ? 16 : 32, rows = 32 / width, sub = lane & (width - 1);
+#pragma unroll 4
+                    for (int i = 0; i < TOKENS / 4; i += rows) {
+                        const int t = warp * (TOKENS / 4) + i + lane / width;
+                        if (TOKENS / 4 < rows && t >= (warp + 1) * (TOKENS / 4)) break;           // (a warp has four tokens, lanes for eight)
+                        float4 x[2];
+                        float top = 0.f;
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float2 was = Half<T>::unpack(p[j]);
-                                p[j] = Half<T>::pack(was.x + f * acc[m][j][2 * h], was.y + f * acc[m][j][2 * h + 1]);
-                            }
+                        for (int h = 0; h < 2; h++) {
+                            const int r = (h * 32 + sub) * 4;
+                            x[h] = t < tile.z && r < tile.w ? __ldcg(reinterpret_cast<const float4 *>(a.v + (int64_t)(tile.y + t) * d.rank + r))
+                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+                            top = fmaxf(top, largest(x[h]));
                         }
-                        *reinterpret_cast<uint4 *>(out) = u;
-                    } else {
+                        const uint32_t here = TOKENS / 4 < rows ? (1u << (TOKENS / 4 * width)) - 1 : 0xFFFFFFFFu;
+                        for (int o = width >> 1; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(here, top, o));
+                        const PowerOfTwo by = bring_near<T>(top);
+                        if (sub == 0) factor[t] = by.back * scale;
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (n + i < d.N) out[i] = e < 0 ? y[i] : Half<T>::from_float(Half<T>::to_float(y[i]) + f * acc[m][i >> 1][2 * h + (i & 1)]);
+                        for (int h = 0; h < 2; h++) {
+                            const int r = (h * 32 + sub) * 4;
+                            if (r >= padded) continue;
+                            uint32_t hi[2], lo[2];
+                            two_parts<T>(x[h].x * by.down, x[h].y * by.down, hi[0], lo[0]);
+                            two_parts<T>(x[h].z * by.down, x[h].w * by.down, hi[1], lo[1]);
+                            *reinterpret_cast<uint2 *>(upper + t * v_pitch + r * 2) = make_uint2(hi[0], hi[1]);
+                            *reinterpret_cast<uint2 *>(lower + t * v_pitch + r * 2) = make_uint2(lo[0], lo[1]);
+                        }
                     }
                 }
+                __syncthreads();
+            }
+            const int ranks = tile.x < 0 ? 0 : min(tile.w - group * G, G), steps = (ranks + 15) / 16;             // of 16 ranks
+            if (steps > 0 && t0 < tile.z) {
+                const uint32_t at = (uint32_t)((t0 + (lane & 15)) * v_pitch + group * (G * 2) + (lane >> 4) * 16);
+                const uint32_t from = shared_addr(smem + stage * Shape::kStage) + (uint32_t)((c0 + (lane & 7)) * PITCH + (lane >> 3) * 16);
+#pragma unroll
+                for (int k = 0; k < G / 16; k += 2) {
+                    if (k >= steps) break;
+                    const bool both = G > 16 && k + 1 < steps;
+                    uint32_t hi[2][4], lo[2][4];
+                    ldmatrix4(hi[0], shared_addr(upper) + at + k * 32);
+                    ldmatrix4(lo[0], shared_addr(lower) + at + k * 32);
+                    if (both) {
+                        ldmatrix4(hi[1], shared_addr(upper) + at + k * 32 + 32);
+                        ldmatrix4(lo[1], shared_addr(lower) + at + k * 32 + 32);
+                    }
+#pragma unroll
+                    for (int j = 0; j < Q * 4; j++) {
+                        uint32_t w[4];
+                        ldmatrix4(w, from + j * 8 * PITCH + k * 32);           // (with an odd number of steps the upper half is not used)
+                        Half<T>::mma(acc[j], hi[0], w[0], w[1]);
+                        Half<T>::mma(acc[j], lo[0], w[0], w[1]);
+                        if (both) {
+                            Half<T>::mma(acc[j], hi[1], w[2], w[3]);
+                            Half<T>::mma(acc[j], lo[1], w[2], w[3]);
+                        }
+                    }
+                }
+            }
+            if (++stage == S) stage = 0;
+        }
+        const bool adds = tile.x >= 0;
+        if (a.vectors && (block + 1) * COLUMNS <= N) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (!has[h]) continue;
+                const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
+#pragma unroll
+                for (int q = 0; q < Q; q++) {
+                    uint32_t p[4] = {y[q][h].x, y[q][h].y, y[q][h].z, y[q][h].w};
+                    if (adds) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float2 was = Half<T>::unpack(p[j]);
+                            p[j] = Half<T>::pack(was.x + f * acc[q * 4 + j][2 * h], was.y + f * acc[q * 4 + j][2 * h + 1]);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(out_at[h] + q * 32) = make_uint4(p[0], p[1], p[2], p[3]);
+                }
+            }
+        } else {                                 // rows that are not aligned, or the last columns: one by one
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (!has[h]) continue;
+                const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
+#pragma unroll
+                for (int q = 0; q < Q; q++) {
+                    const int rest = N - (block * COLUMNS + c0 + q * 32 + quad * 8);
+                    T was[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (i < rest) was[i] = y_at[h][q * 32 + i];
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (i < rest) out_at[h][q * 32 + i] = adds ? Half<T>::from_float(Half<T>::to_float(was[i]) + f * acc[q * 4 + (i >> 1)][2 * h + (i & 1)]) : was[i];
+                }
+            }
+        }
+        if (--left == 0) break;
+        if (++block == a.blocks) {
+            block = 0;
+            tile_number++;
+            new_tile = true;
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) { y_at[h] += COLUMNS; out_at[h] += COLUMNS; }
+            load_y();                            // under the next pair's products
         }
     }
-    if (!waited) griddep_wait();
 }
 
 static int check_low_rank(const ortho_b200_low_rank_desc *d)
 {
     if (!d) return ORTHO_B200_ERR_NULL;
     if (d->type != ORTHO_B200_TYPE_F16 && d->type != ORTHO_B200_TYPE_BF16) return ORTHO_B200_ERR_SHAPE;
-    if (d->tokens < 0 || d->tokens > 0x7FFFFFFF || d->K < 8 || d->K % 8 || d->K > 0x3FFFFFFF || d->N < 1 || d->N > 0x7FFFFFFF || d->adapters < 1 || d->adapters > kMostAdapters || d->rank < 8 || d->rank % 8 || d->rank > 256)
+    if (d->tokens < 0 || d->tokens > 0x7FFFFFFF || d->K < 8 || d->K % 8 || d->K > 0x3FFFFFFF || d->N < 1 || d->N > 0x3FFFFFFF || d->adapters < 1 || d->adapters > kMostAdapters || d->rank < 8 || d->rank % 8 || d->rank > 256)
         return ORTHO_B200_ERR_SHAPE;
     if (d->tokens == 0) return ORTHO_B200_OK;
     if (!d->x || !d->y || !d->out || !d->down || !d->up || !d->ids) return ORTHO_B200_ERR_NULL;
@@ -469,56 +571,64 @@ static LowRankSpace low_rank_space(const ortho_b200_low_rank_desc &d)
     return s;
 }
 
-template <class T, int MB, int NT, bool FEW>
-static int launch_down(LowRankArgs &a, int cluster, cudaStream_t stream)
+template <class T, int MB, int NT, int CTAS, int WARPS, bool FEW>
+static int launch_down(LowRankArgs &a, cudaStream_t stream)
 {
     const auto &d = a.d;
     const int tile = NT * 8;
     a.rank_groups = (int)ceil_div(d.rank, MB * 16);
     const int64_t most = d.tokens / tile + d.adapters, units = (most < d.tokens ? most : d.tokens) * a.rank_groups;
-    const int64_t room = 4 * (int64_t)device_sm_count(current_device_index()) / cluster;
+    const int64_t room = 4 * (int64_t)device_sm_count(current_device_index()) / CTAS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((units < room ? units : room) * cluster)); cfg.blockDim = dim3(32 * kDownWarps); cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)((units < room ? units : room) * CTAS)); cfg.blockDim = dim3(32 * WARPS); cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = CTAS; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    OB_CUDA(cudaLaunchKernelEx(&cfg, down_kernel<T, MB, NT, FEW>, a));
+    OB_CUDA(cudaLaunchKernelEx(&cfg, down_kernel<T, MB, NT, CTAS, WARPS, FEW>, a));
     count_launch();
     return ORTHO_B200_OK;
 }
 
-template <class T, int MT, bool FEW>
-static int launch_up(const LowRankArgs &a, cudaStream_t stream)
+template <class T, int MT, int G, bool FEW>
+static int launch_up_as(LowRankArgs &a, cudaStream_t stream)
 {
+    using Shape = UpShape<MT, G>;
     const auto &d = a.d;
-    const int64_t pitch = (d.rank + 15) / 16 * 32 + 16, smem = 2 * MT * 16 * pitch;
     const int dev = current_device_index();
     if (dev < 0) return ORTHO_B200_ERR_CUDA;
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
-        OB_CUDA(cudaFuncSetAttribute(up_kernel<T, MT, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * MT * 16 * (256 * 2 + 16)));
+        OB_CUDA(cudaFuncSetAttribute(up_kernel<T, MT, G, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes(256)));
         attr_set[dev] = true;
     }
-    const int64_t most = d.tokens / (MT * 16) + d.adapters + 1, units = (most < d.tokens ? most : d.tokens) * ceil_div(d.N, kUpColumns);
-    const int64_t room = (int64_t)device_sm_count(dev) * (FEW ? 4 : 3);
-    return launch_dependent(up_kernel<T, MT, FEW>, dim3((unsigned)(units < room ? units : room)), 32 * kUpWarps, (size_t)smem, stream, a);
+    a.blocks = (int)ceil_div(d.N, Shape::kColumns);
+    const int smem = Shape::bytes(a.padded), fit = 227 * 1024 / (smem + (FEW ? 7 : 2) * 1024);
+    const int64_t most = d.tokens / Shape::kTokens + d.adapters + 1, pairs = (most < d.tokens ? most : d.tokens) * a.blocks;
+    const int64_t room = (fit < 4 ? fit : 4) * (int64_t)device_sm_count(dev);
+    return launch_dependent(up_kernel<T, MT, G, FEW>, dim3((unsigned)(pairs < room ? pairs : room)), kUpThreads, (size_t)smem, stream, a);
+}
+template <class T, int MT, bool FEW>
+static int launch_up(LowRankArgs &a, cudaStream_t stream)
+{
+    return a.padded <= 16 ? launch_up_as<T, MT, 16, FEW>(a, stream) : a.padded <= 32 ? launch_up_as<T, MT, 32, FEW>(a, stream) : launch_up_as<T, MT, 64, FEW>(a, stream);
 }
 
 template <class T>
 static int launch_low_rank(LowRankArgs &a, cudaStream_t stream)
 {
     const auto &d = a.d;
-    int st;
-    if (d.tokens <= kFewTokens) {
-        st = d.rank <= 16 ? launch_down<T, 1, kFewTile / 8, true>(a, 8, stream)
-           : d.rank <= 32 ? launch_down<T, 2, kFewTile / 8, true>(a, 8, stream) : launch_down<T, 4, kFewTile / 8, true>(a, 8, stream);
-        return st ? st : launch_up<T, kFewTile / 16, true>(a, stream);
-    }
     const int dev = current_device_index();
     if (dev < 0) return ORTHO_B200_ERR_CUDA;
+    int st;
+    if (d.tokens <= kFewTokens) {
+        st = d.rank <= 16 ? launch_down<T, 1, kFewTile / 8, 8, 4, true>(a, stream)
+           : launch_down<T, 2, kFewTile / 8, 8, 4, true>(a, stream);
+        if (st) return st;
+        return launch_up<T, kFewTile / 16, true>(a, stream);
+    }
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
         OB_CUDA(cudaFuncSetAttribute(group_kernel<kManyTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 4 * (kMostAdapters + 1)));
@@ -526,8 +636,9 @@ static int launch_low_rank(LowRankArgs &a, cudaStream_t stream)
     }
     st = launch_dependent(group_kernel<kManyTile>, dim3(1), kGroupThreads, (size_t)(3 * 4 * (d.adapters + 1)), stream, a);
     if (st) return st;
-    st = d.rank <= 16 ? launch_down<T, 1, kManyTile / 8, false>(a, 4, stream) : launch_down<T, 2, kManyTile / 8, false>(a, 4, stream);
-    return st ? st : launch_up<T, kManyTile / 16, false>(a, stream);
+    st = d.rank <= 16 ? launch_down<T, 1, kManyTile / 8, 4, 4, false>(a, stream) : launch_down<T, 2, kManyTile / 8, 4, 4, false>(a, stream);
+    if (st) return st;
+    return launch_up<T, kManyTile / 16, false>(a, stream);
 }
 
 }  // namespace ob
@@ -555,6 +666,8 @@ extern "C" int ortho_b200_low_rank_add(const ortho_b200_low_rank_desc *d, void *
     a.order = reinterpret_cast<int *>(w + space.order);
     a.tiles = reinterpret_cast<int4 *>(w + space.tiles);
     a.v = reinterpret_cast<float *>(w + space.v);
+    a.padded = (int)((d->rank + 15) / 16 * 16);
+    a.up_groups = (int)ceil_div(d->rank, 64);
     a.vectors = (((uintptr_t)d->y | (uintptr_t)d->out) & 15u) == 0 && d->y_stride % 8 == 0 && d->out_stride % 8 == 0;
     a.copies = d->out != d->y || d->out_stride != d->y_stride;
     return d->type == ORTHO_B200_TYPE_F16 ? launch_low_rank<__half>(a, (cudaStream_t)stream) : launch_low_rank<__nv_bfloat16>(a, (cudaStream_t)stream);

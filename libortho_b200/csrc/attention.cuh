@@ -58,13 +58,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// 16 bytes, or zeros
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void *src, bool on)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
 // Shared memory of one CTA.  Rows of DP elements: 16-byte chunks exchanged within groups of eight by the row's number where a row is a multiple of

@@ -68,6 +68,21 @@ __device__ __forceinline__ void ldmatrix2(uint32_t &r0, uint32_t &r1, uint32_t a
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
 }
 
+// 16 bytes, or zeros
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void *src, bool on)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// 16 bytes, in the order of the program: the compiler keeps such loads in front of the products that use them, so that they are in flight together
+__device__ __forceinline__ uint4 load16(const void *p)
+{
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // n / d for 0 <= n < 2^31 and a divisor known at the launch: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d) < 2^32, the error of
 // n m / 2^(31 + s) is below n / 2^31 / d < 1 / d, so its integer part is the quotient.
 struct FastDiv {
