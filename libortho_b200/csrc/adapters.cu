@@ -578,7 +578,7 @@ static int launch_down(LowRankArgs &a, cudaStream_t stream)
     const int tile = NT * 8;
     a.rank_groups = (int)ceil_div(d.rank, MB * 16);
     const int64_t most = d.tokens / tile + d.adapters, units = (most < d.tokens ? most : d.tokens) * a.rank_groups;
-    const int64_t room = 4 * (int64_t)device_sm_count(current_device_index()) / CTAS;
+    const int64_t room = (FEW ? 4 : 2) * (int64_t)device_sm_count(current_device_index()) / CTAS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((units < room ? units : room) * CTAS)); cfg.blockDim = dim3(32 * WARPS); cfg.stream = stream;
     cudaLaunchAttribute attr[2];

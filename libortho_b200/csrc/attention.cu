@@ -20,7 +20,9 @@ static int check_attention(const ortho_b200_paged_attention_desc *d)
     return ORTHO_B200_OK;
 }
 
-template <int DP, int NT> static void take(AttnPlan &p) { p.dp = DP; p.ctas = AttnShape<DP, NT>::kPerSm; }
+template <int DP, int NT> static void take(AttnPlan &p) { p.dp = DP; p.ctas = AttnShape<DP, NT>::kPerSm; p.cluster = AttnShape<DP, NT>::kClusterPerSm; }
+
+constexpr int64_t kJoinUnits = 4;
 
 AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d)
 {
@@ -41,11 +43,23 @@ AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d)
     }
     OB_ATTENTION_DIMS(OB_CASE)
 #undef OB_CASE
-    p.ctas *= device_sm_count(current_device_index());
-    // never more CTAs than there can be units
+    const int64_t sms = device_sm_count(current_device_index());
     const int64_t keys = d.window > 0 && d.window < d.width * d.page_size ? d.window : d.width * d.page_size;
-    const int64_t units = ceil_div(keys, kUnitKeys) * p.groups * d.kv_heads;
-    if (units < p.ctas && units * d.batch < p.ctas) p.ctas = units * d.batch < 1 ? 1 : (int)(units * d.batch);
+    const int64_t units = ceil_div(keys, kUnitKeys), items = d.batch * d.kv_heads * p.groups;       // of one item at most; all items
+    // Items that find room on the GPU as clusters of two to eight CTAs are joined inside these (one launch, no partial sums in memory), unless an
+    // even cut over all CTAs is shorter by more than it takes to join: about as long as kJoinUnits units of one CTA.
+    int64_t cluster = p.cluster * sms / (items < 1 ? 1 : items);
+    cluster = cluster >= 8 ? 8 : cluster >= 4 ? 4 : cluster >= 2 ? 2 : 0;
+    while (cluster > 2 && cluster / 2 >= units) cluster /= 2;
+    p.ctas *= (int)sms;
+    if (cluster && ceil_div(units, cluster) > ceil_div(units * items, p.ctas) + kJoinUnits) cluster = 0;
+    p.cluster = (int)cluster;
+    if (cluster) {
+        p.ctas = (int)(items * cluster);
+        return p;
+    }
+    // never more CTAs than there can be costs
+    if (units < p.ctas && (units + 1) * items < p.ctas) p.ctas = (units + 1) * items < 1 ? 1 : (int)((units + 1) * items);
     const int64_t rows = 2 * (int64_t)p.ctas * p.nt * 8;
     p.bytes = (16 * (int64_t)p.ctas + 255) / 256 * 256 + (8 * rows + 255) / 256 * 256 + 4 * rows * d.head_dim;
     return p;
@@ -66,7 +80,7 @@ extern "C" int ortho_b200_paged_attention(const ortho_b200_paged_attention_desc 
     int st = check_attention(d);
     if (st || d->batch == 0) return st;
     const AttnPlan p = plan_attention(*d);
-    if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255u)) return ORTHO_B200_ERR_WORKSPACE;
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255u))) return ORTHO_B200_ERR_WORKSPACE;
     st = check_device();
     if (st) return st;
     AttentionArgs a;

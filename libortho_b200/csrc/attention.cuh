@@ -8,13 +8,16 @@
 // maximum and sum per query in FP32, then O^T += V^T P^T (16 elements x 8 queries).  Queries are the narrow operand because there are few of
 // them; P^T gets from accumulator to operand layout by an 8 x 8 transposition in registers.
 //
-// The work is cut evenly whatever the lengths are.  A unit is 64 keys of one request and key-value head (16 per warp).  The units of all requests
-// are numbered in a row, and CTA c of n takes the units [U c / n, U (c + 1) / n): every CTA finds its place by summing the lengths itself.
-// A request that lies within one CTA is finished there; of one that is cut each CTA leaves its sums in the workspace and
-// join_kernel, launched behind as a programmatic dependent, adds them in order.  No atomics: the same bits every time.
+// The work is cut evenly whatever the lengths are.  A unit is 64 keys of one request and key-value head (16 per warp); a request and head ("an
+// item") costs its units and one more for its start and end.  These costs are numbered in a row over all requests, and CTA c takes
+// [c per, (c + 1) per) of them: every CTA finds its place by summing the lengths itself.  An item that lies within one CTA is
+// finished there; of one that is cut each CTA leaves its sums in the workspace, and join_kernel, launched behind as a programmatic
+// dependent, adds them in order.  Few items (CLUSTER): a cluster of CTAs has an item and joins its sums through distributed shared memory.
+// Neither uses atomics: the same bits every time.
 #pragma once
 
 #include "launch.cuh"
+#include "tma.cuh"
 
 namespace ob {
 
@@ -24,8 +27,8 @@ struct AttentionArgs {
     float scale_log2;                            // scale log2 e: exponentials are powers of two
     int per_group, groups;                       // query heads of a key-value head in one unit, units' groups of them
     int ctas;
-    int4 *cut;                                   // [ctas] of a CTA's last request: {row, head group, last CTA, 1} if it goes on, {.., 0} if not
-    float2 *sums;                                // [2 ctas][rows] (max, sum) of cut requests: continued from the CTA before, going on behind
+    int4 *cut;                                   // [ctas] of a CTA's last item: {row, head group, last CTA, 1} if it goes on, {.., 0} if not
+    float2 *sums;                                // [2 ctas][rows] (max, sum) of cut items: continued from the CTA before, going on behind
     float *part;                                 // [2 ctas][rows][head_dim]
 };
 
@@ -69,11 +72,15 @@ struct AttnShape {
     static constexpr int kHalfTile = kWarpKeys * kPitch;                       // keys, then values
     static constexpr int kStage = 2 * kHalfTile;
     static constexpr int kQ = NT * 8 * kPitch;
-    static constexpr int kFold = kAttnWarps * 8 * 68 * 4;                      // 8 queries x 64 elements of every warp, rows apart by 4 banks
-    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kFold + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
+    static constexpr int kFoldPitch = DP + 4;                                  // 8 queries of a warp in FP32, rows apart by 4 banks: in a stage that is done with
+    static_assert(8 * kFoldPitch * 4 <= kStage, "room for 8 queries");
+    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
     static constexpr int kTwo = 115712, kOne = 232448;                         // room of a CTA with two or one on an SM
     static constexpr int kStages = bytes(4) <= kTwo ? 4 : bytes(3) <= kTwo ? 3 : bytes(2) <= kTwo ? 2 : bytes(4) <= kOne ? 4 : bytes(3) <= kOne ? 3 : 2;
     static constexpr int kBytes = bytes(kStages), kPerSm = kBytes <= kTwo ? 2 : 1;
+    static constexpr int kMostRanks = 8;                                       // of a cluster; what arrives from them: (max, sum) and a share of the sums
+    static constexpr int kArrived = kMostRanks * NT * 8 * 8 + NT * 8 * DP * 4 + kMostRanks * 16, kClusterBytes = (kBytes + 15) / 16 * 16 + kArrived;
+    static constexpr int kClusterPerSm = kClusterBytes <= kTwo ? 2 : kClusterBytes <= kOne ? 1 : 0;
     static constexpr bool kKeepQ = NT <= 2;                                    // query operands stay in registers
     static __device__ __forceinline__ uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((kSwap ? chunk ^ (row & 7) : chunk) << 4)); }
 };
@@ -93,14 +100,19 @@ __device__ __forceinline__ Span span_of(const ortho_b200_paged_attention_desc &d
     return s;
 }
 
-// Place in the row of all units: request, head group, 64 keys
+// Place in the row of all units: request, head group, 64 keys.  `left`: costs up to the end of this CTA's share, the unit's own among them
 struct Walk {
     int64_t b;
     int inner, unit;
     Span s;
+    long long left;
+    __device__ __forceinline__ bool last() const { return unit == s.units - 1; }
+    __device__ __forceinline__ bool more() const { return left > (last() ? 2 : 1); }
     __device__ __forceinline__ void step(const ortho_b200_paged_attention_desc &d, int inners)
     {
+        left--;
         if (++unit < s.units) return;
+        left--;
         unit = 0;
         if (++inner < inners) return;
         inner = 0;
@@ -108,7 +120,21 @@ struct Walk {
     }
 };
 
-template <class T, int DP, int NT>
+template <class T>
+__device__ __forceinline__ void store4(const ortho_b200_paged_attention_desc &d, int64_t b, int64_t head, int el, float4 x, float inverse)
+{
+    uint2 r;
+    r.x = Half<T>::pack(x.x * inverse, x.y * inverse);
+    r.y = Half<T>::pack(x.z * inverse, x.w * inverse);
+    *reinterpret_cast<uint2 *>((T *)d.out + b * d.out_token_stride + head * d.out_head_stride + el) = r;
+}
+template <class T>
+__device__ __forceinline__ float lse_of(float top, float sum)
+{
+    return sum == 0.f ? -INFINITY : (top - AttnType<T>::lift + __log2f(sum)) * 0.6931471805599453f;
+}
+
+template <class T, int DP, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP, NT>::kPerSm)
 paged_attention_kernel(const __grid_constant__ AttentionArgs a)
 {
@@ -120,62 +146,87 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = (int)d.head_dim;
     unsigned char *const ring = smem + warp * (S * Shape::kStage);
     unsigned char *const q_ring = smem + kAttnWarps * S * Shape::kStage;
-    float *const fold = reinterpret_cast<float *>(q_ring + S * Shape::kQ);
-    float2 *const sums = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(fold) + Shape::kFold);
+    float2 *const sums = reinterpret_cast<float2 *>(q_ring + S * Shape::kQ);
     uint32_t *const seen = reinterpret_cast<uint32_t *>(sums + kAttnWarps * NT * 8) + warp * S;
     const int inners = (int)d.kv_heads * a.groups, cta = blockIdx.x;
+    float2 *const arrived_sums = reinterpret_cast<float2 *>(smem + (Shape::kBytes + 15) / 16 * 16);           // [ranks][rows]
+    float4 *const arrived = reinterpret_cast<float4 *>(arrived_sums + Shape::kMostRanks * NT * 8);            // [ranks][this CTA's share]
 
+    if constexpr (CLUSTER) cluster_arrive();     // (waited for before anything is sent: the other CTAs have started then)
     griddep_wait();
     griddep_launch();
 
     // ---- this CTA's units -------------------------------------------------------------------------------------
-    __shared__ long long warp_units[kAttnWarps];
-    __shared__ long long first_b, first_rest;
-    const int64_t per = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * per, b1 = b0 + per < d.batch ? b0 + per : d.batch;
-    long long mine = 0;
-    for (int64_t b = b0; b < b1; b++) mine += span_of(d, b).units;
-    long long upto = mine;
+    Walk now;                                    // the unit that is computed
+    now.left = 0;
+    [[maybe_unused]] long long per = 0, item_at = 0;                           // costs of a CTA; cost number of the item's first cost
+    [[maybe_unused]] const int rank = CLUSTER ? (int)cluster_ctarank() : 0, ranks = CLUSTER ? (int)cluster_nctarank() : 1;
+    if constexpr (CLUSTER) {                     // an even share of the cluster's item
+        const int64_t item = cta / ranks;
+        now.b = item / inners;
+        now.inner = (int)(item - now.b * inners);
+        now.s = span_of(d, now.b);
+        now.unit = (int)((int64_t)now.s.units * rank / ranks);
+        now.left = (int64_t)now.s.units * (rank + 1) / ranks - now.unit;
+        __syncwarp();
+        cluster_wait();
+    } else {
+        __shared__ long long warp_cost[kAttnWarps];
+        __shared__ long long first_b, first_rest;
+        const int64_t chunk = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * chunk, b1 = b0 + chunk < d.batch ? b0 + chunk : d.batch;
+        long long mine = 0;
+        for (int64_t b = b0; b < b1; b++) {
+            const int units = span_of(d, b).units;
+            mine += units + (units > 0);
+        }
+        long long upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31) warp_units[warp] = upto;
-    __syncthreads();
-    long long total = 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) warp_cost[warp] = upto;
+        __syncthreads();
+        long long total = 0;
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; w++) {
-        if (w == warp) upto += total;
-        total += warp_units[w];
-    }
-    total *= inners;
-    const long long n = total < a.ctas ? total : a.ctas;                       // (every CTA that works has a unit)
-    const long long u0 = cta < n ? total * cta / n : 0, u1 = cta < n ? total * (cta + 1) / n : 0;
-    if (cta >= n && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
-    if (u0 < u1) {
-        const long long before = (upto - mine) * inners;
-        if (u0 >= before && u0 < upto * inners) {
-            long long rest = u0 - before;
-            int64_t b = b0;
-            for (;; b++) {
-                const long long here = (long long)span_of(d, b).units * inners;
-                if (rest < here) break;
-                rest -= here;
+        for (int w = 0; w < kAttnWarps; w++) {
+            if (w == warp) upto += total;
+            total += warp_cost[w];
+        }
+        total *= inners;
+        per = (total + a.ctas - 1) / a.ctas;
+        const long long from = per * cta, to = from + per < total ? from + per : total;
+        if (from < to) {
+            const long long before = (upto - mine) * inners;
+            if (from >= before && from < upto * inners) {
+                long long rest = from - before;
+                int64_t b = b0;
+                for (;; b++) {
+                    const int units = span_of(d, b).units;
+                    const long long here = (long long)(units + (units > 0)) * inners;
+                    if (rest < here) break;
+                    rest -= here;
+                }
+                first_b = b;
+                first_rest = rest;
             }
-            first_b = b;
-            first_rest = rest;
+        }
+        __syncthreads();
+        if (from < to) {
+            now.b = first_b;
+            now.s = span_of(d, now.b);
+            const int at = (int)(first_rest % (now.s.units + 1));                  // 0: the cost of the item's start and end, then its units
+            now.inner = (int)(first_rest / (now.s.units + 1));
+            now.unit = at > 0 ? at - 1 : 0;
+            now.left = to - from - (at == 0);
+            item_at = from - at;
         }
     }
-    __syncthreads();
-
-    if (u0 < u1) {
-        Walk now;                                // the unit that is computed
-        now.b = first_b;
-        now.s = span_of(d, now.b);
-        now.inner = (int)(first_rest / now.s.units);
-        now.unit = (int)(first_rest % now.s.units);
+    if (now.left <= 0) {                         // (a share of one cost may be that of an item's start alone)
+        if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
+    } else {
         Walk next = now;                         // the unit whose copies are issued next
-        long long left = u1 - u0;                // units not issued yet
+        bool issuing = true;
         int fresh_q = 0;                         // (request, head group) pairs issued so far: place in the ring of queries
         bool first_issue = true;
         // a lane's key of the unit `next`: its page is looked up one unit ahead of the copies
@@ -191,23 +242,25 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
             }
         };
         look_up();
+        const bool alike = d.k_page_stride == d.v_page_stride && d.k_slot_stride == d.v_slot_stride;
         auto issue = [&](int stage) {
-            if (left > 0) {
-                left--;
+            if (issuing) {
                 const int head = next.inner / a.groups, group = next.inner - head * a.groups;
                 if (page >= d.pages) page = -1;
                 const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
                 if (lane == 0) seen[stage] = ok;
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
                 const T *const k = (const T *)d.k_cache + head * d.k_head_stride, *const v = (const T *)d.v_cache + head * d.v_head_stride;
+                // a lane's own key's place in the caches; the lanes that copy a row get it from there
+                const int64_t k_mine = page >= 0 ? page * d.k_page_stride + place * d.k_slot_stride : -1;
+                const int64_t v_mine = alike || page < 0 ? k_mine : page * d.v_page_stride + place * d.v_slot_stride;
 #pragma unroll
                 for (int i = 0; i < Shape::kChunks / 2; i++) {
                     const int at = i * 32 + lane, row = at / Shape::kChunks, chunk = at % Shape::kChunks;
-                    const int pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
-                    const bool on = pg >= 0 && chunk * 8 < D;
-                    const int64_t p = on ? pg : 0, o = on ? pl : 0, e = on ? chunk * 8 : 0;
-                    copy16_async(dst + Shape::at(row, chunk), k + p * d.k_page_stride + o * d.k_slot_stride + e, on);
-                    copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), v + p * d.v_page_stride + o * d.v_slot_stride + e, on);
+                    const int64_t k_at = __shfl_sync(0xffffffffu, k_mine, row), v_at = alike ? k_at : __shfl_sync(0xffffffffu, v_mine, row);
+                    const bool on = k_at >= 0 && chunk * 8 < D;
+                    copy16_async(dst + Shape::at(row, chunk), on ? k + k_at + chunk * 8 : k, on);
+                    copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), on ? v + v_at + chunk * 8 : v, on);
                 }
                 if (next.unit == 0 || first_issue) {                           // its queries, a quarter per warp
                     const uint32_t qdst = shared_addr(q_ring + fresh_q * Shape::kQ);
@@ -222,7 +275,8 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     if (++fresh_q == S) fresh_q = 0;
                     first_issue = false;
                 }
-                if (left > 0) {
+                issuing = next.more();
+                if (issuing) {
                     next.step(d, inners);
                     look_up();
                 }
@@ -236,13 +290,13 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         float o[KS][NT][4], top[NT][2], sum[NT][2];
         int stage = 0, q_at = -1;
         bool started_here = true;                // the request's first unit is this CTA's
-        for (long long u = u0; u < u1; u++) {
+        for (bool first_unit = true, more = true; more; first_unit = false) {
             copy_wait<S - 2>();
             __syncwarp();
-            if (u == u0 || now.unit == 0) {
+            if (first_unit || now.unit == 0) {
                 started_here = now.unit == 0;
                 if (++q_at == S) q_at = 0;
-                __syncthreads();                 // every warp's part of the queries is there
+                __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
                 if constexpr (Shape::kKeepQ) {
                     const uint32_t src = shared_addr(q_ring + q_at * Shape::kQ);
 #pragma unroll
@@ -348,12 +402,13 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     }
                 }
             }
-            if (++stage == S) stage = 0;
-            const bool last = now.unit == now.s.units - 1;
-            if (last || u + 1 == u1) {
-                // ---- the four warps' sums over their keys of this request become one ---------------------------------------
+            const bool last = now.last();
+            more = now.more();
+            if (last || !more) {
+                // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
+                // issued behind the barrier above.
                 const int head = now.inner / a.groups, group = now.inner - head * a.groups;
-                const int h0 = head * (int)(d.q_heads / d.kv_heads) + group * a.per_group;
+                const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
                 const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
                 const bool whole = started_here && last;
                 const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
@@ -367,72 +422,98 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                         l += __shfl_xor_sync(0xffffffffu, l, 16);
                         if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(top[t][e], l);
                     }
-                __syncthreads();
-                float factor[NT][2];
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, sums[w * NT * 8 + t * 8 + 2 * (lane & 3) + e].x);
-                        factor[t][e] = top[t][e] == -INFINITY ? 0.f : exp2_approx(top[t][e] - m);
-                    }
-                const int fq = tid >> 4, fd = (tid & 15) * 4;                  // the query and the four elements that a thread adds up
+                float *const fold = reinterpret_cast<float *>(ring + stage * Shape::kStage) + 2 * (lane & 3) * Shape::kFoldPitch + (lane >> 2);
+                const float *const folds = reinterpret_cast<const float *>(smem + stage * Shape::kStage);
+                constexpr int WARP_FLOATS = S * Shape::kStage / 4;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    float m = -INFINITY, l = 0.f;
+                    __syncwarp();                // the warp has read its values
+                    if (t) __syncthreads();
 #pragma unroll
-                    for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, sums[w * NT * 8 + t * 8 + fq].x);
+                    for (int i = 0; i < KS; i++)
 #pragma unroll
-                    for (int w = 0; w < kAttnWarps; w++) {
-                        const float2 x = sums[w * NT * 8 + t * 8 + fq];
-                        l += x.x == -INFINITY ? x.y : x.y * exp2_approx(x.x - m);       // (nothing, or NaN)
-                    }
-                    const int row = t * 8 + fq;
-                    if (fd == 0 && row < heads) {
-                        if (!whole) a.sums[slot * NT * 8 + row] = make_float2(m, l);
-                        else if (d.lse) d.lse[now.b * d.q_heads + h0 + row] = l == 0.f ? -INFINITY : (m - Type::lift + __log2f(l)) * 0.6931471805599453f;
-                    }
-                    const float inverse = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                        for (int e = 0; e < 4; e++) fold[(e & 1) * Shape::kFoldPitch + i * 16 + (e >> 1) * 8] = o[i][t][e];
+                    __syncthreads();
+                    // a thread has one query and every 16th quad of its elements
+                    const int fq = tid >> 4, row = t * 8 + fq;
+                    if (row < heads) {
+                        float m = -INFINITY, l = 0.f, factor[kAttnWarps];
+                        float2 x[kAttnWarps];
 #pragma unroll
-                    for (int i0 = 0; i0 < KS; i0 += 4) {
-                        float *const to = fold + warp * 8 * 68 + 2 * (lane & 3) * 68 + (lane >> 2);
+                        for (int w = 0; w < kAttnWarps; w++) {
+                            x[w] = sums[w * NT * 8 + row];
+                            m = fmaxf(m, x[w].x);
+                        }
 #pragma unroll
-                        for (int i = i0; i < i0 + 4 && i < KS; i++)
+                        for (int w = 0; w < kAttnWarps; w++) {
+                            factor[w] = x[w].x == -INFINITY ? 0.f : exp2_approx(x[w].x - m);
+                            l += x[w].x == -INFINITY ? x[w].y : x[w].y * factor[w];               // (nothing, or NaN)
+                        }
+                        const float inverse = l == 0.f ? 0.f : 1.f / l;
+                        if constexpr (CLUSTER) {
+                            if ((tid & 15) < ranks) st_dsmem_v2(mapa_shared(shared_addr(arrived_sums + rank * NT * 8 + row), tid & 15), m, l);
+                        } else if ((tid & 15) == 0) {
+                            if (!whole) a.sums[slot * NT * 8 + row] = make_float2(m, l);
+                            else if (d.lse) d.lse[now.b * d.q_heads + h0 + row] = lse_of<T>(m, l);
+                        }
 #pragma unroll
-                            for (int e = 0; e < 4; e++) to[(e & 1) * 68 + (i - i0) * 16 + (e >> 1) * 8] = o[i][t][e] * factor[t][e & 1];
-                        __syncthreads();
-                        const int el = i0 * 16 + fd;
-                        if (row < heads && el < D) {
-                            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int i = 0; i < (DP + 63) / 64; i++) {
+                            const int el = i * 64 + (tid & 15) * 4;
+                            if (el >= D) break;
+                            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                             for (int w = 0; w < kAttnWarps; w++) {
-                                const float4 y = *reinterpret_cast<const float4 *>(fold + (w * 8 + fq) * 68 + fd);
-                                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                                const float4 z = *reinterpret_cast<const float4 *>(folds + w * WARP_FLOATS + fq * Shape::kFoldPitch + el);
+                                y.x += factor[w] * z.x; y.y += factor[w] * z.y; y.z += factor[w] * z.z; y.w += factor[w] * z.w;
                             }
-                            if (whole) {
-                                uint2 r;
-                                r.x = Half<T>::pack(x.x * inverse, x.y * inverse);
-                                r.y = Half<T>::pack(x.z * inverse, x.w * inverse);
-                                *reinterpret_cast<uint2 *>((T *)d.out + now.b * d.out_token_stride + (h0 + row) * d.out_head_stride + el) = r;
-                            } else {
-                                *reinterpret_cast<float4 *>(a.part + (slot * NT * 8 + row) * D + el) = x;
-                            }
+                            if constexpr (CLUSTER) {
+                                const int share = (heads * (D / 4) + ranks - 1) / ranks, at = row * (D / 4) + el / 4, to = at / share;
+                                st_dsmem_v4(mapa_shared(shared_addr(arrived + rank * share + (at - to * share)), to), y);
+                            } else if (whole) store4<T>(d, now.b, h0 + row, el, y, inverse);
+                            else *reinterpret_cast<float4 *>(a.part + (slot * NT * 8 + row) * D + el) = y;
                         }
-                        __syncthreads();
                     }
                 }
-                if (u + 1 == u1 && tid == 0) {
-                    const bool goes_on = started_here && !last;
-                    // the CTA of the request's last unit: the last one whose first unit is not behind it
-                    const long long end = u + (now.s.units - now.unit);
-                    a.cut[cta] = make_int4((int)now.b, now.inner, goes_on ? (int)((end * n - 1) / total) : 0, goes_on ? 1 : 0);
+                if constexpr (CLUSTER) {
+                    more = false;                // (a CTA has one item)
+                } else {
+                    if (!more && tid == 0) a.cut[cta] = make_int4((int)now.b, now.inner, (int)((item_at + now.s.units) / per), started_here && !last ? 1 : 0);
+                    item_at += now.s.units + 1;
                 }
             }
-            if (u + 1 < u1) now.step(d, inners);
+            if (++stage == S) stage = 0;
+            if (more) now.step(d, inners);
         }
         copy_wait<0>();
+    }
+    if constexpr (CLUSTER) {
+        // ---- the cluster's sums become one, a share of the elements in each CTA ----------------------------------------------
+        const int head = now.inner / a.groups, group = now.inner - head * a.groups;
+        const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
+        const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+        for (int i = tid; i < heads * ranks && now.left <= 0; i += kAttnThreads)                  // no unit: nothing is added
+            st_dsmem_v2(mapa_shared(shared_addr(arrived_sums + rank * NT * 8 + i / ranks), i % ranks), -INFINITY, 0.f);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        const int quads = D / 4, share = (heads * quads + ranks - 1) / ranks;
+        for (int i = tid; i < share && now.s.units > 0; i += kAttnThreads) {
+            const int at = rank * share + i, row = at / quads, el = (at - row * quads) * 4;
+            if (row >= heads) break;
+            float m = -INFINITY, l = 0.f;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < ranks; r++) m = fmaxf(m, arrived_sums[r * NT * 8 + row].x);
+            for (int r = 0; r < ranks; r++) {
+                const float2 x = arrived_sums[r * NT * 8 + row];
+                if (x.x == -INFINITY && x.y == 0.f) continue;                  // (nothing has arrived from a CTA without keys)
+                const float f = x.x == -INFINITY ? 0.f : exp2_approx(x.x - m);
+                const float4 z = arrived[r * share + i];
+                l += x.x == -INFINITY ? x.y : x.y * f;
+                y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+            }
+            store4<T>(d, now.b, h0 + row, el, y, l == 0.f ? 0.f : 1.f / l);
+            if (d.lse && el == 0) d.lse[now.b * d.q_heads + h0 + row] = lse_of<T>(m, l);
+        }
     }
     // ---- rows without keys ---------------------------------------------------------------------------------------
     for (int64_t b = cta; b < d.batch; b += gridDim.x) {
@@ -497,41 +578,55 @@ join_kernel(const __grid_constant__ AttentionArgs a, int rows)
         if (el >= D) continue;
 #pragma unroll
         for (int w = 0; w < 3; w++) { const float4 y = acc[w][h * 32 + lane]; x[h].x += y.x; x[h].y += y.y; x[h].z += y.z; x[h].w += y.w; }
-        uint2 r;
-        r.x = Half<T>::pack(x[h].x * inverse, x[h].y * inverse);
-        r.y = Half<T>::pack(x[h].z * inverse, x[h].w * inverse);
-        *reinterpret_cast<uint2 *>((T *)d.out + cut.x * d.out_token_stride + h0 * d.out_head_stride + el) = r;
+        store4<T>(d, cut.x, h0, el, x[h], inverse);
     }
-    if (d.lse && lane == 0) d.lse[cut.x * d.q_heads + h0] = l == 0.f ? -INFINITY : (m - AttnType<T>::lift + __log2f(l)) * 0.6931471805599453f;
+    if (d.lse && lane == 0) d.lse[cut.x * d.q_heads + h0] = lse_of<T>(m, l);
 }
 
 // ---- host: which variant, how much workspace -----------------------------------------------------------------
-struct AttnPlan { int dp, nt, per_group, groups, ctas; int64_t bytes; };
+struct AttnPlan { int dp, nt, per_group, groups, ctas, cluster; int64_t bytes; };
 AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d);             // attention.cu
 template <class T> int launch_attention(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream);
 
 template <class T, int DP, int NT>
-int launch_attention_as(const AttentionArgs &a, cudaStream_t stream)
+int launch_attention_as(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
 {
-    auto kern = paged_attention_kernel<T, DP, NT>;
-    static bool attr_set[kMaxDevices] = {};
+    using Shape = AttnShape<DP, NT>;
     const int dev = current_device_index();
     if (dev < 0) return ORTHO_B200_ERR_CUDA;
+    static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
-        OB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnShape<DP, NT>::kBytes));
+        OB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes));
+        if constexpr (Shape::kClusterPerSm > 0)
+            OB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kClusterBytes));
         attr_set[dev] = true;
     }
-    const int st = launch_dependent(kern, dim3((unsigned)a.ctas), kAttnThreads, AttnShape<DP, NT>::kBytes, stream, a);
+    if constexpr (Shape::kClusterPerSm > 0) {
+        if (p.cluster) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)a.ctas); cfg.blockDim = dim3(kAttnThreads); cfg.dynamicSmemBytes = Shape::kClusterBytes; cfg.stream = stream;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = (unsigned)p.cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+            cfg.attrs = attr; cfg.numAttrs = 2;
+            OB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_kernel<T, DP, NT, true>, a));
+            count_launch();
+            return ORTHO_B200_OK;
+        }
+    }
+    const int st = launch_dependent(paged_attention_kernel<T, DP, NT, false>, dim3((unsigned)a.ctas), kAttnThreads, Shape::kBytes, stream, a);
     if (st) return st;
     return launch_dependent(join_kernel<T>, dim3((unsigned)a.ctas, (unsigned)a.per_group), 128, 0, stream, a, NT * 8);
 }
 
 template <class T, int DP>
-int launch_attention_dim(const AttentionArgs &a, int nt, cudaStream_t stream)
+int launch_attention_dim(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
 {
-    if (nt == 1) return launch_attention_as<T, DP, 1>(a, stream);
-    if (nt == 2) return launch_attention_as<T, DP, 2>(a, stream);
-    if constexpr (DP <= 128) return launch_attention_as<T, DP, 4>(a, stream);
+    if (p.nt == 1) return launch_attention_as<T, DP, 1>(a, p, stream);
+    if (p.nt == 2) return launch_attention_as<T, DP, 2>(a, p, stream);
+    if constexpr (DP <= 128) return launch_attention_as<T, DP, 4>(a, p, stream);
     return ORTHO_B200_ERR_SHAPE;
 }
 
@@ -540,7 +635,7 @@ int launch_attention_dim(const AttentionArgs &a, int nt, cudaStream_t stream)
 template <class T>
 int launch_attention(const AttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
 {
-#define OB_CASE(DP) if (p.dp == DP) return launch_attention_dim<T, DP>(a, p.nt, stream);
+#define OB_CASE(DP) if (p.dp == DP) return launch_attention_dim<T, DP>(a, p, stream);
     OB_ATTENTION_DIMS(OB_CASE)
 #undef OB_CASE
     return ORTHO_B200_ERR_SHAPE;
