@@ -100,23 +100,28 @@ __device__ __forceinline__ Span span_of(const ortho_b200_paged_attention_desc &d
     return s;
 }
 
-// Place in the row of all units: request, head group, 64 keys.  `left`: costs up to the end of this CTA's share, the unit's own among them
+// Place in the row of all units: request, head group, 64 keys.  `left`: costs up to the end of this CTA's share, the unit's own among them.  In a
+// cluster a CTA has every `stride`-th unit of one item.
 struct Walk {
     int64_t b;
     int inner, unit;
     Span s;
     long long left;
     __device__ __forceinline__ bool last() const { return unit == s.units - 1; }
-    __device__ __forceinline__ bool more() const { return left > (last() ? 2 : 1); }
-    __device__ __forceinline__ void step(const ortho_b200_paged_attention_desc &d, int inners)
+    template <bool CLUSTER> __device__ __forceinline__ bool more(int stride) const { return CLUSTER ? unit + stride < s.units : left > (last() ? 2 : 1); }
+    template <bool CLUSTER> __device__ __forceinline__ void step(const ortho_b200_paged_attention_desc &d, int inners, int stride)
     {
-        left--;
-        if (++unit < s.units) return;
-        left--;
-        unit = 0;
-        if (++inner < inners) return;
-        inner = 0;
-        do b++, s = b < d.batch ? span_of(d, b) : Span{0, 0, 1, 0}; while (s.units == 0);
+        if constexpr (CLUSTER) {
+            unit += stride;
+        } else {
+            left--;
+            if (++unit < s.units) return;
+            left--;
+            unit = 0;
+            if (++inner < inners) return;
+            inner = 0;
+            do b++, s = b < d.batch ? span_of(d, b) : Span{0, 0, 1, 0}; while (s.units == 0);
+        }
     }
 };
 
@@ -161,18 +166,17 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     now.left = 0;
     [[maybe_unused]] long long per = 0, item_at = 0;                           // costs of a CTA; cost number of the item's first cost
     [[maybe_unused]] const int rank = CLUSTER ? (int)cluster_ctarank() : 0, ranks = CLUSTER ? (int)cluster_nctarank() : 1;
-    if constexpr (CLUSTER) {                     // an even share of the cluster's item
+    if constexpr (CLUSTER) {                     // every ranks-th unit of the cluster's item
         const int64_t item = cta / ranks;
         now.b = item / inners;
         now.inner = (int)(item - now.b * inners);
+        now.unit = rank;
         now.s = span_of(d, now.b);
-        now.unit = (int)((int64_t)now.s.units * rank / ranks);
-        now.left = (int64_t)now.s.units * (rank + 1) / ranks - now.unit;
-        __syncwarp();
-        cluster_wait();
+        now.left = rank < now.s.units;
     } else {
-        __shared__ long long warp_cost[kAttnWarps];
-        __shared__ long long first_b, first_rest;
+        __shared__ long long warp_cost[kAttnWarps], first_rest;
+        __shared__ int first_b;
+        // a thread's requests, one after the other; up to kAttnThreads requests each thread has one
         const int64_t chunk = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * chunk, b1 = b0 + chunk < d.batch ? b0 + chunk : d.batch;
         long long mine = 0;
         for (int64_t b = b0; b < b1; b++) {
@@ -194,29 +198,28 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
             total += warp_cost[w];
         }
         total *= inners;
-        per = (total + a.ctas - 1) / a.ctas;
+        // (32 bits where they do: a division in 64 takes some 200 cycles)
+        per = total < 0x7FFFFFFF ? ((uint32_t)total + a.ctas - 1) / (uint32_t)a.ctas : (total + a.ctas - 1) / a.ctas;
         const long long from = per * cta, to = from + per < total ? from + per : total;
-        if (from < to) {
-            const long long before = (upto - mine) * inners;
-            if (from >= before && from < upto * inners) {
-                long long rest = from - before;
-                int64_t b = b0;
-                for (;; b++) {
-                    const int units = span_of(d, b).units;
-                    const long long here = (long long)(units + (units > 0)) * inners;
-                    if (rest < here) break;
-                    rest -= here;
-                }
-                first_b = b;
-                first_rest = rest;
+        long long rest = from - (upto - mine) * inners;
+        if (from < to && rest >= 0 && rest < mine * inners) {
+            int64_t b = b0;
+            for (; b + 1 < b1; b++) {
+                const int units = span_of(d, b).units;
+                const long long here = (long long)(units + (units > 0)) * inners;
+                if (rest < here) break;
+                rest -= here;
             }
+            first_b = (int)b;
+            first_rest = rest;
         }
         __syncthreads();
         if (from < to) {
             now.b = first_b;
             now.s = span_of(d, now.b);
-            const int at = (int)(first_rest % (now.s.units + 1));                  // 0: the cost of the item's start and end, then its units
-            now.inner = (int)(first_rest / (now.s.units + 1));
+            const long long rest = first_rest;
+            now.inner = rest < 0x7FFFFFFF ? (int)((uint32_t)rest / (uint32_t)(now.s.units + 1)) : (int)(rest / (now.s.units + 1));
+            const int at = (int)(rest - (long long)now.inner * (now.s.units + 1));                // 0: the cost of the item's start and end, then its units
             now.unit = at > 0 ? at - 1 : 0;
             now.left = to - from - (at == 0);
             item_at = from - at;
@@ -225,28 +228,35 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     if (now.left <= 0) {                         // (a share of one cost may be that of an item's start alone)
         if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     } else {
-        Walk next = now;                         // the unit whose copies are issued next
-        bool issuing = true;
-        int fresh_q = 0;                         // (request, head group) pairs issued so far: place in the ring of queries
-        bool first_issue = true;
-        // a lane's key of the unit `next`: its page is looked up one unit ahead of the copies
-        int page, place;
-        auto look_up = [&]() {
-            const int key = next.s.from + next.unit * kUnitKeys + warp * kWarpKeys + (lane & 15);
-            page = -1;
-            place = 0;
-            if (key < next.s.n) {
+        // What the copies of a unit need.  The page of a lane's key is looked up well ahead of its use, those of the first units together.
+        struct Ticket { int64_t b; int inner, page, place; bool valid, queries; };
+        Walk ahead = now;                        // the unit of the next ticket
+        bool more_tickets = true;
+        auto ticket = [&]() {
+            Ticket t;
+            t.valid = more_tickets;
+            t.b = ahead.b;
+            t.inner = ahead.inner;
+            t.queries = CLUSTER ? ahead.unit == rank : ahead.unit == 0 || (ahead.b == now.b && ahead.inner == now.inner && ahead.unit == now.unit);
+            t.page = -1;
+            t.place = 0;
+            const int key = ahead.s.from + ahead.unit * kUnitKeys + warp * kWarpKeys + (lane & 15);
+            if (more_tickets && key < ahead.s.n) {
                 const int col = (int)a.by_page.quotient((uint32_t)key);
-                place = key - col * (int)d.page_size;
-                page = d.block_table[next.s.row * d.table_stride + col];
+                t.place = key - col * (int)d.page_size;
+                t.page = d.block_table[ahead.s.row * d.table_stride + col];
             }
+            if (more_tickets) {
+                more_tickets = ahead.more<CLUSTER>(ranks);
+                if (more_tickets) ahead.step<CLUSTER>(d, inners, ranks);
+            }
+            return t;
         };
-        look_up();
+        int fresh_q = 0;                         // items issued so far: place in the ring of queries
         const bool alike = d.k_page_stride == d.v_page_stride && d.k_slot_stride == d.v_slot_stride;
-        auto issue = [&](int stage) {
-            if (issuing) {
-                const int head = next.inner / a.groups, group = next.inner - head * a.groups;
-                if (page >= d.pages) page = -1;
+        auto issue = [&](const Ticket &t, int stage) {
+            if (t.valid) {
+                const int head = t.inner / a.groups, group = t.inner - head * a.groups, place = t.place, page = t.page < d.pages ? t.page : -1;
                 const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
                 if (lane == 0) seen[stage] = ok;
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
@@ -262,7 +272,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     copy16_async(dst + Shape::at(row, chunk), on ? k + k_at + chunk * 8 : k, on);
                     copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), on ? v + v_at + chunk * 8 : v, on);
                 }
-                if (next.unit == 0 || first_issue) {                           // its queries, a quarter per warp
+                if (t.queries) {                                               // its queries, a quarter per warp
                     const uint32_t qdst = shared_addr(q_ring + fresh_q * Shape::kQ);
                     const int h0 = head * (int)(d.q_heads / d.kv_heads) + group * a.per_group;
                     const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
@@ -270,21 +280,22 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                         const int row = at / Shape::kChunks, chunk = at % Shape::kChunks;
                         const bool on = row < heads && chunk * 8 < D;
                         copy16_async(qdst + Shape::at(row, chunk),
-                                     (const T *)d.q + next.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
+                                     (const T *)d.q + t.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
                     }
                     if (++fresh_q == S) fresh_q = 0;
-                    first_issue = false;
-                }
-                issuing = next.more();
-                if (issuing) {
-                    next.step(d, inners);
-                    look_up();
                 }
             }
             copy_commit();
         };
+        Ticket pending;
+        {
+            Ticket first[S - 1];
 #pragma unroll
-        for (int s = 0; s < S - 1; s++) issue(s);
+            for (int i = 0; i < S - 1; i++) first[i] = ticket();
+            pending = ticket();
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) issue(first[i], i);
+        }
 
         uint32_t q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? KS : 1][2];
         float o[KS][NT][4], top[NT][2], sum[NT][2];
@@ -293,7 +304,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         for (bool first_unit = true, more = true; more; first_unit = false) {
             copy_wait<S - 2>();
             __syncwarp();
-            if (first_unit || now.unit == 0) {
+            if (first_unit || (!CLUSTER && now.unit == 0)) {
                 started_here = now.unit == 0;
                 if (++q_at == S) q_at = 0;
                 __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
@@ -316,7 +327,8 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
             }
             const uint32_t ok = seen[stage];
             const uint32_t keys = shared_addr(ring + stage * Shape::kStage), values = keys + Shape::kHalfTile;
-            issue(stage == 0 ? S - 1 : stage - 1);
+            issue(pending, stage == 0 ? S - 1 : stage - 1);
+            pending = ticket();
             if (ok) {
                 float s[NT][4];
 #pragma unroll
@@ -403,8 +415,8 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                 }
             }
             const bool last = now.last();
-            more = now.more();
-            if (last || !more) {
+            more = now.more<CLUSTER>(ranks);
+            if (CLUSTER ? !more : last || !more) {
                 // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
                 // issued behind the barrier above.
                 const int head = now.inner / a.groups, group = now.inner - head * a.groups;
@@ -474,15 +486,13 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                         }
                     }
                 }
-                if constexpr (CLUSTER) {
-                    more = false;                // (a CTA has one item)
-                } else {
+                if constexpr (!CLUSTER) {
                     if (!more && tid == 0) a.cut[cta] = make_int4((int)now.b, now.inner, (int)((item_at + now.s.units) / per), started_here && !last ? 1 : 0);
                     item_at += now.s.units + 1;
                 }
             }
             if (++stage == S) stage = 0;
-            if (more) now.step(d, inners);
+            if (more) now.step<CLUSTER>(d, inners, ranks);
         }
         copy_wait<0>();
     }
@@ -501,15 +511,20 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
             const int at = rank * share + i, row = at / quads, el = (at - row * quads) * 4;
             if (row >= heads) break;
             float m = -INFINITY, l = 0.f;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int r = 0; r < ranks; r++) m = fmaxf(m, arrived_sums[r * NT * 8 + row].x);
-            for (int r = 0; r < ranks; r++) {
-                const float2 x = arrived_sums[r * NT * 8 + row];
-                if (x.x == -INFINITY && x.y == 0.f) continue;                  // (nothing has arrived from a CTA without keys)
-                const float f = x.x == -INFINITY ? 0.f : exp2_approx(x.x - m);
-                const float4 z = arrived[r * share + i];
-                l += x.x == -INFINITY ? x.y : x.y * f;
-                y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+            float2 x[Shape::kMostRanks];
+            float4 z[Shape::kMostRanks], y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int r = 0; r < Shape::kMostRanks; r++) {
+                x[r] = r < ranks ? arrived_sums[r * NT * 8 + row] : make_float2(-INFINITY, 0.f);
+                // (nothing has arrived from a CTA without keys)
+                z[r] = x[r].x == -INFINITY && x[r].y == 0.f ? y : arrived[r * share + i];
+                m = fmaxf(m, x[r].x);
+            }
+#pragma unroll
+            for (int r = 0; r < Shape::kMostRanks; r++) {
+                const float f = x[r].x == -INFINITY ? 0.f : exp2_approx(x[r].x - m);
+                l += x[r].x == -INFINITY ? x[r].y : x[r].y * f;
+                y.x += f * z[r].x; y.y += f * z[r].y; y.z += f * z[r].z; y.w += f * z[r].w;
             }
             store4<T>(d, now.b, h0 + row, el, y, l == 0.f ? 0.f : 1.f / l);
             if (d.lse && el == 0) d.lse[now.b * d.q_heads + h0 + row] = lse_of<T>(m, l);
@@ -527,7 +542,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     }
 }
 
-// Adds the parts of a request that was cut, in the order of its keys.  A CTA per CTA of the kernel above (the one where a cut request starts) and
+// Adds the parts of an item that was cut, in the order of its keys.  A CTA per CTA of the kernel above (the one where a cut item starts) and
 // query head; its warps take every fourth part, a lane four elements (eight: head dims above 128).
 template <class T>
 __global__ void __launch_bounds__(128)
