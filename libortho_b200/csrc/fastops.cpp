@@ -176,6 +176,7 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
     const Cache c = cache_of(a[3], a[4], type, k);
     const int64_t T = k.size(0);
     TORCH_CHECK_VALUE(c.heads == k.size(1) && c.D == k.size(2), "k and v must have the caches' heads and head_dim");
+    TORCH_CHECK_VALUE(c.D <= 8192, "head_dim must be at most 8192");
     const at::Tensor slots = list_of(a[5], "slots", at::kLong, T, k);
     const c10::cuda::CUDAGuard guard(k.device());
     ortho_b200_rotary_append_desc d;

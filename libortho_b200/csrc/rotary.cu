@@ -2,8 +2,8 @@
 //
 //     pair i < R / 2 of a head:  (a, b) -> (a c - b s, b c + a s),  c = table[p][i], s = table[p][R / 2 + i],  p = positions[axis(i)][t]
 //
-// Every value is read and written once.  An item is two vectors of VEC values of one head; a thread keeps an item's cosines and sines and
-// walks over the heads of its token, queries, keys and values alike.
+// Every value is read and written once: bound by HBM.  An item is two vectors of VEC values of one head; a thread has one item and walks over the
+// (token, head) pairs of its CTA, queries, keys and values alike.  Cosines and sines of the CTA's tokens pass through shared memory.
 #include "launch.cuh"
 
 namespace ob {
@@ -11,7 +11,8 @@ namespace ob {
 struct RotaryArgs {
     ortho_b200_rotary_append_desc d;
     int turned, items;                           // items of a head that turn, and all of them (two vectors each)
-    FastDiv by_items;
+    int together;                                // tokens of a CTA
+    FastDiv by_items, by_heads, by_half;
 };
 
 // VEC 16-bit values as they lie in memory
@@ -46,107 +47,140 @@ struct Raw {
     }
 };
 
-template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256)
-rotary_append_kernel(RotaryArgs a)
+// (a c - b s, b c + a s), the same bits in every variant: two products are rounded, the other two are not
+__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s)
 {
+    const float was = a;
+    a = __fmaf_rn(a, c, -__fmul_rn(b, s));
+    b = __fmaf_rn(b, c, __fmul_rn(was, s));
+}
+
+constexpr int kTurnsAhead = 2, kMostTogether = 4;  // turns of a thread whose values are in flight together; tokens of a CTA
+
+template <class T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4)
+rotary_append_kernel(const __grid_constant__ RotaryArgs a)
+{
+    constexpr int U = kTurnsAhead;
+    extern __shared__ __align__(16) float angles[];                            // [tokens][rotary]: cosines, then sines
+    __shared__ int64_t k_at[kMostTogether], v_at[kMostTogether];               // places in the caches, k_at -1 for none
     const auto &d = a.d;
-    const int64_t t = blockIdx.x;
-    const int half = (int)d.rotary / 2, all_heads = (int)(d.q_heads + 2 * d.kv_heads);
-    // a thread's item, and the first of its heads; the threads behind the last whole row of items rest
-    const int row = (int)a.by_items.quotient(threadIdx.x), item = threadIdx.x - row * a.items, rows = a.items <= 256 ? 256 / a.items : 1;
+    const int64_t t0 = (int64_t)blockIdx.x * a.together;
+    const int tokens = d.tokens - t0 < a.together ? (int)(d.tokens - t0) : a.together;
+    const int R = (int)d.rotary, half = R / 2, q_heads = (int)d.q_heads, kv_heads = (int)d.kv_heads, heads = q_heads + 2 * kv_heads, all = tokens * heads;
+    // a thread's item, and the first of its (token, head) pairs; the threads behind the last whole row of items rest
+    const int row = (int)a.by_items.quotient(threadIdx.x), rows = a.items <= 256 ? 256 / a.items : 1, step = (int)gridDim.y * rows;
+    const int first = row < rows ? (int)blockIdx.y * rows + row : all;
     griddep_wait();
     griddep_launch();
-    const int64_t slot = d.slots[t];
-    const bool kept = slot >= 0 && slot < d.pages * d.page_size;
-    int64_t page = 0, place = 0;
-    if (kept) { page = slot / d.page_size; place = slot - page * d.page_size; }
-    if (row >= rows) return;
-    for (int it = item; it < a.items; it += 256) {
-        const bool turns = it < a.turned;
+    bool ready = false;
+    for (int it0 = 0; it0 < a.items; it0 += 256) {
+        const int it = it0 + (int)threadIdx.x - row * a.items;
+        const bool some = it < a.items, turns = it < a.turned;
         // offsets of the two vectors
         int e0, e1;
-        if (!turns) { e0 = (int)d.rotary + 2 * (it - a.turned) * VEC; e1 = e0 + VEC; }
+        if (!turns) { e0 = R + 2 * (it - a.turned) * VEC; e1 = e0 + VEC; }
         else if (INTERLEAVED) { e0 = 2 * it * VEC; e1 = e0 + VEC; }
         else { e0 = it * VEC; e1 = e0 + half; }
-        float c[VEC], s[VEC];
-        if (turns) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-                const int i = it * VEC + j;
-                int axis = 0;
-#pragma unroll
-                for (int x = 0; x < ORTHO_B200_MAX_AXES - 1; x++) axis += x + 1 < d.axes && i >= d.section_ends[x];
-                const int32_t p = d.positions[axis * d.position_stride + t];
-                const bool in = p >= 0 && p < d.table_rows;
-                c[j] = in ? d.table[(int64_t)p * d.rotary + i] : 1.f;
-                s[j] = in ? d.table[(int64_t)p * d.rotary + half + i] : 0.f;
-            }
-        }
         const bool second = e1 < d.head_dim;
-        for (int h = (int)blockIdx.y * rows + row; h < all_heads; h += (int)gridDim.y * rows) {
-            const T *src;
-            T *dst;
-            bool turn = turns, write = true;
-            if (h < d.q_heads) {
-                src = (const T *)d.q + t * d.q_token_stride + h * d.q_head_stride;
-                dst = (T *)d.q_out + t * d.out_token_stride + h * d.out_head_stride;
-            } else if (h < d.q_heads + d.kv_heads) {
-                const int g = h - (int)d.q_heads;
-                src = (const T *)d.k + t * d.k_token_stride + g * d.k_head_stride;
-                dst = (T *)d.k_cache + page * d.k_page_stride + place * d.k_slot_stride + g * d.k_cache_head_stride;
-                write = kept;
-            } else {
-                const int g = h - (int)(d.q_heads + d.kv_heads);
-                src = (const T *)d.v + t * d.v_token_stride + g * d.v_head_stride;
-                dst = (T *)d.v_cache + page * d.v_page_stride + place * d.v_slot_stride + g * d.v_cache_head_stride;
-                turn = false;
-                write = kept;
+        for (int j0 = some ? first : all; j0 < all || !ready; j0 += U * step) {
+            Raw<VEC> r0[U], r1[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int j = j0 + u * step;
+                if (j >= all) break;
+                const int token = (int)a.by_heads.quotient(j), h = j - token * heads;
+                const int64_t t = t0 + token;
+                const T *const src = h < q_heads ? (const T *)d.q + t * d.q_token_stride + h * d.q_head_stride
+                                   : h < q_heads + kv_heads ? (const T *)d.k + t * d.k_token_stride + (h - q_heads) * d.k_head_stride
+                                                            : (const T *)d.v + t * d.v_token_stride + (h - q_heads - kv_heads) * d.v_head_stride;
+                r0[u].load(src + e0);
+                if (second) r1[u].load(src + e1);
             }
-            if (!write) continue;
-            Raw<VEC> r0, r1;
-            r0.load(src + e0);
-            if (second) r1.load(src + e1);
-            if (turn) {
-                float x0[VEC], x1[VEC];
-                r0.template to<T>(x0);
-                r1.template to<T>(x1);
-                if (INTERLEAVED && VEC > 1) {
-#pragma unroll
-                    for (int j = 0; j + 1 < VEC; j += 2) {
-                        const int i0 = j / 2, i1 = (VEC + j) / 2;
-                        const float a0 = x0[j], b0 = x0[j + 1], a1 = x1[j], b1 = x1[j + 1];
-                        x0[j] = a0 * c[i0] - b0 * s[i0]; x0[j + 1] = b0 * c[i0] + a0 * s[i0];
-                        x1[j] = a1 * c[i1] - b1 * s[i1]; x1[j + 1] = b1 * c[i1] + a1 * s[i1];
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; j++) {
-                        const float lo = x0[j], hi = x1[j];
-                        x0[j] = lo * c[j] - hi * s[j];
-                        x1[j] = hi * c[j] + lo * s[j];
-                    }
+            if (!ready) {                        // once, while the first values are under way: the tokens' places, cosines and sines
+                ready = true;
+                if ((int)threadIdx.x < tokens) {
+                    const int64_t slot = d.slots[t0 + threadIdx.x];
+                    const bool kept = slot >= 0 && slot < d.pages * d.page_size;
+                    const int64_t page = !kept ? 0 : slot <= 0x7FFFFFFF && d.page_size <= 0x7FFFFFFF ? (int64_t)((uint32_t)slot / (uint32_t)d.page_size) : slot / d.page_size;
+                    const int64_t place = slot - page * d.page_size;
+                    k_at[threadIdx.x] = kept ? page * d.k_page_stride + place * d.k_slot_stride : -1;
+                    v_at[threadIdx.x] = kept ? page * d.v_page_stride + place * d.v_slot_stride : -1;
                 }
-                r0.template from<T>(x0);
-                r1.template from<T>(x1);
+                for (int i = threadIdx.x; i < tokens * half; i += 256) {
+                    const int token = (int)a.by_half.quotient(i), pair = i - token * half;
+                    int axis = 0;
+#pragma unroll
+                    for (int x = 0; x < ORTHO_B200_MAX_AXES - 1; x++) axis += x + 1 < d.axes && pair >= d.section_ends[x];
+                    const int32_t p = d.positions[axis * d.position_stride + t0 + token];
+                    const bool in = p >= 0 && p < d.table_rows;
+                    angles[token * R + pair] = in ? d.table[(int64_t)p * R + pair] : 1.f;
+                    angles[token * R + half + pair] = in ? d.table[(int64_t)p * R + half + pair] : 0.f;
+                }
+                __syncthreads();
             }
-            r0.store(dst + e0);
-            if (second) r1.store(dst + e1);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int j = j0 + u * step;
+                if (j >= all) break;
+                const int token = (int)a.by_heads.quotient(j), h = j - token * heads;
+                const bool is_value = h >= q_heads + kv_heads;
+                if (turns && !is_value) {
+                    float x0[VEC], x1[VEC], c[VEC], s[VEC];
+                    const float *const at = angles + token * R + it * VEC;
+                    if constexpr (VEC > 1) {
+                        if (half % 4 == 0) {
+#pragma unroll
+                            for (int i = 0; i < VEC; i += 4) {
+                                const float4 x = *reinterpret_cast<const float4 *>(at + i), y = *reinterpret_cast<const float4 *>(at + half + i);
+                                c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+                                s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < VEC; i++) { c[i] = at[i]; s[i] = at[half + i]; }
+                        }
+                    } else { c[0] = at[0]; s[0] = at[half]; }
+                    r0[u].template to<T>(x0);
+                    r1[u].template to<T>(x1);
+                    if (INTERLEAVED && VEC > 1) {
+#pragma unroll
+                        for (int i = 0; i + 1 < VEC; i += 2) {
+                            turn_pair(x0[i], x0[i + 1], c[i / 2], s[i / 2]);
+                            turn_pair(x1[i], x1[i + 1], c[(VEC + i) / 2], s[(VEC + i) / 2]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) turn_pair(x0[i], x1[i], c[i], s[i]);
+                    }
+                    r0[u].template from<T>(x0);
+                    r1[u].template from<T>(x1);
+                }
+                const int64_t place = is_value ? v_at[token] : k_at[token];
+                if (h >= q_heads && k_at[token] < 0) continue;                 // (no place in the cache)
+                T *const dst = h < q_heads ? (T *)d.q_out + (t0 + token) * d.out_token_stride + h * d.out_head_stride
+                             : !is_value ? (T *)d.k_cache + place + (h - q_heads) * d.k_cache_head_stride
+                                         : (T *)d.v_cache + place + (h - q_heads - kv_heads) * d.v_cache_head_stride;
+                r0[u].store(dst + e0);
+                if (second) r1[u].store(dst + e1);
+            }
         }
     }
 }
 
 template <class T, int VEC>
-static int launch_rotary(const RotaryArgs &a, cudaStream_t stream)
+static int launch_rotary(RotaryArgs &a, cudaStream_t stream)
 {
-    const int64_t heads = a.d.q_heads + 2 * a.d.kv_heads, rows = a.items <= 256 ? 256 / a.items : 1;
-    // heads of a token over several CTAs only where the tokens alone do not fill the GPU
-    int64_t y = ceil_div(2 * device_sm_count(current_device_index()), a.d.tokens);
-    const int64_t most = ceil_div(heads, rows);
+    const int64_t heads = a.d.q_heads + 2 * a.d.kv_heads, rows = a.items <= 256 ? 256 / a.items : 1, sms = device_sm_count(current_device_index());
+    // Four tokens of a CTA share the time that their angles take to come; with few tokens one each, its heads over several CTAs until the GPU is full
+    a.together = a.d.tokens >= 2 * kMostTogether * sms && a.d.rotary <= 2048 ? kMostTogether : 1;
+    const int64_t ctas = ceil_div(a.d.tokens, a.together), most = ceil_div(heads * a.together, rows);
+    int64_t y = ceil_div(2 * sms, ctas);
     y = y < 1 ? 1 : y < most ? y : most;
-    const dim3 grid((unsigned)a.d.tokens, (unsigned)y);
-    return a.d.interleaved ? launch_dependent(rotary_append_kernel<T, VEC, true>, grid, 256, 0, stream, a)
-                           : launch_dependent(rotary_append_kernel<T, VEC, false>, grid, 256, 0, stream, a);
+    const dim3 grid((unsigned)ctas, (unsigned)y);
+    const size_t smem = (size_t)(a.together * a.d.rotary * 4);
+    return a.d.interleaved ? launch_dependent(rotary_append_kernel<T, VEC, true>, grid, 256, smem, stream, a)
+                           : launch_dependent(rotary_append_kernel<T, VEC, false>, grid, 256, smem, stream, a);
 }
 
 template <class T>
@@ -164,7 +198,7 @@ extern "C" int ortho_b200_rotary_append(const ortho_b200_rotary_append_desc *d, 
     if (!d) return ORTHO_B200_ERR_NULL;
     if (d->type != ORTHO_B200_TYPE_F16 && d->type != ORTHO_B200_TYPE_BF16) return ORTHO_B200_ERR_SHAPE;
     if (d->tokens < 0 || d->q_heads < 0 || d->kv_heads < 1 || d->head_dim < 1 || d->pages < 0 || d->page_size < 1
-        || d->tokens > 0x7FFFFFFF || d->q_heads > 65535 || d->kv_heads > 65535 || d->head_dim > 65536) return ORTHO_B200_ERR_SHAPE;
+        || d->tokens > 0x7FFFFFFF || d->q_heads > 65535 || d->kv_heads > 65535 || d->head_dim > 8192) return ORTHO_B200_ERR_SHAPE;
     if (d->rotary < 0 || d->rotary % 2 || d->rotary > d->head_dim) return ORTHO_B200_ERR_SHAPE;
     if (d->rotary) {
         if (d->axes < 1 || d->axes > ORTHO_B200_MAX_AXES || d->table_rows < 0 || d->section_ends[d->axes - 1] != d->rotary / 2) return ORTHO_B200_ERR_SHAPE;
@@ -193,6 +227,8 @@ extern "C" int ortho_b200_rotary_append(const ortho_b200_rotary_append_desc *d, 
     a.turned = (int)(d->rotary / 2 / vec);
     a.items = a.turned + (int)ceil_div(d->head_dim - d->rotary, 2 * vec);
     a.by_items = FastDiv((uint32_t)a.items);
+    a.by_heads = FastDiv((uint32_t)(d->q_heads + 2 * d->kv_heads));
+    a.by_half = FastDiv((uint32_t)(d->rotary ? d->rotary / 2 : 1));
     return d->type == ORTHO_B200_TYPE_F16 ? launch_rotary_of<__half>(a, vec, (cudaStream_t)stream)
                                           : launch_rotary_of<__nv_bfloat16>(a, vec, (cudaStream_t)stream);
 }
