@@ -311,18 +311,20 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t &hi, uint32
 }
 __device__ __forceinline__ float largest(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
-constexpr int kUpThreads = 128, kUpStages = 3;
+constexpr int kUpThreads = 128, kUpStages = 3;                                // (stages: 2 pairs are under way while one is worked on)
 static_assert(kFewTokens == kUpThreads && kGroupThreads == 32 * 32, "a thread per token, a lane per warp");
 
 // Columns of a pair and the layout of a stage: rows of G ranks, 16 bytes of padding against bank conflicts
 template <int MT, int G>
 struct UpShape {
-    static constexpr int kTokens = MT * 16, kColumns = MT == 1 ? 128 : 64, kPieces = G / 8, kPitch = G * 2 + 16, kStage = kColumns * kPitch;
-    static int bytes(int padded) { return kUpStages * kStage + 64 + 2 * kTokens * (padded * 2 + 16); }
+    static constexpr int kTokens = MT * 16, kColumns = MT == 1 ? 128 : 64, kPieces = G / 8, kPitch = G * 2 + 16, kWeights = kColumns * kPitch + 64;
+    static constexpr int kTaken = MT == 1 ? 2 : 4;                             // 16-byte pieces of y that a thread needs for its results of a pair
+    static constexpr int kStage = kWeights + kTaken * kUpThreads * 16;         // rows of `up`, then every thread's own pieces of y
+    static int bytes(int padded) { return kUpStages * kStage + 2 * kTokens * (padded * 2 + 16); }
 };
 
 // The (tile, columns) pairs are numbered in a row and dealt evenly, a run of them to each CTA, so that v comes into shared memory about once per
-// CTA.  Rows of `up` arrive in a ring of three stages of up to 64 ranks, the first ones while down_kernel still runs; y is loaded a pair ahead.
+// CTA.  Rows of `up` (up to 64 ranks) and y arrive in a ring of three stages, the first ones while down_kernel still runs.
 // Tiles of 16 tokens (MT = 1): a warp has 32 of 128 columns, bound by the weights.  Of 64 (MT = 4): a warp has 16 tokens and 64 columns, bound by
 // y and out.  Column c of 8 in product tile j stands for output column 8 (c / 2) + 2 j + c % 2 of 32, so that a lane's results over four
 // tiles are eight neighbours.
@@ -338,7 +340,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     const auto &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, row = lane >> 2;
     const int padded = a.padded, groups = G < 64 ? 1 : a.up_groups, v_pitch = padded * 2 + 16, N = (int)d.N;
-    unsigned char *const upper = smem + S * Shape::kStage + 64, *const lower = upper + TOKENS * v_pitch;
+    unsigned char *const upper = smem + S * Shape::kStage, *const lower = upper + TOKENS * v_pitch;
     const int t0 = MT == 1 ? 0 : warp * 16, c0 = MT == 1 ? warp * 32 : 0;      // this warp's first token of the tile and column of the pair
     // What is read in front of the wait was complete before down_kernel let this kernel start (it does so behind its own wait), or is a
     // constant of the layer.
@@ -357,10 +359,38 @@ up_kernel(const __grid_constant__ LowRankArgs a)
 
     // the copies of a step (pair, up to 64 ranks); each thread has PIECES (or half as many) of the 16-byte pieces
     int next_group = 0, next_tile = left ? (int)(first / a.blocks) : 0, next_block = left ? (int)(first - (int64_t)next_tile * a.blocks) : 0;
-    int4 ahead = left ? tile_at(next_tile) : make_int4(-1, 0, 0, 0);
+    int4 ahead = make_int4(-1, 0, 0, 0);
+    // this lane's place in its two tokens' rows of y, for the copies and (below) for the results: column c0 + 8 quad of a pair
+    struct Rows { const T *y[2]; T *out[2]; bool has[2]; };
+    auto rows_of = [&](const int4 &tile, int block) {
+        Rows r;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int t = t0 + h * 8 + row;
+            r.has[h] = t < tile.z;
+            const int64_t token = !r.has[h] ? 0 : FEW ? few.order[tile.y + t] : __ldcg(a.order + tile.y + t);
+            r.y[h] = (const T *)d.y + token * d.y_stride + block * COLUMNS + c0 + quad * 8;
+            r.out[h] = (T *)d.out + token * d.out_stride + block * COLUMNS + c0 + quad * 8;
+        }
+        return r;
+    };
+    Rows coming;
+    if (left) {
+        ahead = tile_at(next_tile);
+        coming = rows_of(ahead, next_block);
+    }
+    const uint32_t mine = Shape::kWeights + tid * 16;
     auto issue = [&](int stage) {
         if (to_issue > 0) {
             const int r0 = next_group * G;
+            if (next_group == groups - 1 && a.vectors && (next_block + 1) * COLUMNS <= N) {       // y comes with the last ranks
+                const uint32_t to = shared_addr(smem + stage * Shape::kStage) + mine;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int q = 0; q < Q; q++)
+                        if (coming.has[h]) copy16_async(to + (h * Q + q) * (kUpThreads * 16), coming.y[h] + q * 32, true);
+            }
             if (ahead.x >= 0 && r0 < ahead.w) {
                 const uint32_t to = shared_addr(smem + stage * Shape::kStage);
                 const T *const from = (const T *)d.up + ((int64_t)ahead.x * N + next_block * COLUMNS) * d.rank + r0;
@@ -376,9 +406,12 @@ up_kernel(const __grid_constant__ LowRankArgs a)
             if (++next_group == groups) {
                 next_group = 0;
                 to_issue--;
+#pragma unroll
+                for (int h = 0; h < 2; h++) coming.y[h] += COLUMNS;
                 if (++next_block == a.blocks && to_issue > 0) {
                     next_block = 0;
                     ahead = tile_at(++next_tile);
+                    coming = rows_of(ahead, 0);
                 }
             }
         }
@@ -392,21 +425,8 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     int tile_number = (int)(first / a.blocks), block = (int)(first - (int64_t)tile_number * a.blocks), stage = 0;
     bool new_tile = true;
     int4 tile;
-    // this lane's place in its two tokens' rows of y and out: column c0 + 8 quad of the pair
-    const T *y_at[2];
-    T *out_at[2];
-    bool has[2];
-    uint4 y[Q][2];
-    auto load_y = [&]() {
-        if (a.vectors && (block + 1) * COLUMNS <= N) {
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int q = 0; q < Q; q++)
-                    if (has[h]) y[q][h] = load16(y_at[h] + q * 32);
-        }
-    };
-    for (;;) {
+    Rows now;
+    for (int last = 0;;) {
         float acc[Q * 4][4];
 #pragma unroll
         for (int j = 0; j < Q * 4; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -417,15 +437,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
             if (new_tile) {
                 new_tile = false;
                 tile = tile_at(tile_number);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int t = t0 + h * 8 + row;
-                    has[h] = t < tile.z;
-                    const int64_t token = !has[h] ? 0 : FEW ? few.order[tile.y + t] : __ldcg(a.order + tile.y + t);
-                    y_at[h] = (const T *)d.y + token * d.y_stride + block * COLUMNS + c0 + quad * 8;
-                    out_at[h] = (T *)d.out + token * d.out_stride + block * COLUMNS + c0 + quad * 8;
-                }
-                load_y();
+                now = rows_of(tile, block);
                 if (tile.x >= 0) {
                     const float scale = d.scales ? __ldcg(d.scales + tile.x) : 1.f;
                     // lanes of a token: the power of two that holds a quarter of the rank, at most a warp (twice: above 128)
@@ -489,17 +501,19 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                     }
                 }
             }
+            last = stage;
             if (++stage == S) stage = 0;
         }
         const bool adds = tile.x >= 0;
         if (a.vectors && (block + 1) * COLUMNS <= N) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                if (!has[h]) continue;
+                if (!now.has[h]) continue;
                 const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
 #pragma unroll
                 for (int q = 0; q < Q; q++) {
-                    uint32_t p[4] = {y[q][h].x, y[q][h].y, y[q][h].z, y[q][h].w};
+                    const uint4 y = *reinterpret_cast<const uint4 *>(smem + last * Shape::kStage + mine + (h * Q + q) * (kUpThreads * 16));
+                    uint32_t p[4] = {y.x, y.y, y.z, y.w};
                     if (adds) {
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
@@ -507,13 +521,13 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                             p[j] = Half<T>::pack(was.x + f * acc[q * 4 + j][2 * h], was.y + f * acc[q * 4 + j][2 * h + 1]);
                         }
                     }
-                    *reinterpret_cast<uint4 *>(out_at[h] + q * 32) = make_uint4(p[0], p[1], p[2], p[3]);
+                    *reinterpret_cast<uint4 *>(now.out[h] + q * 32) = make_uint4(p[0], p[1], p[2], p[3]);
                 }
             }
         } else {                                 // rows that are not aligned, or the last columns: one by one
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                if (!has[h]) continue;
+                if (!now.has[h]) continue;
                 const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
 #pragma unroll
                 for (int q = 0; q < Q; q++) {
@@ -521,10 +535,10 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                     T was[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        if (i < rest) was[i] = y_at[h][q * 32 + i];
+                        if (i < rest) was[i] = now.y[h][q * 32 + i];
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        if (i < rest) out_at[h][q * 32 + i] = adds ? Half<T>::from_float(Half<T>::to_float(was[i]) + f * acc[q * 4 + (i >> 1)][2 * h + (i & 1)]) : was[i];
+                        if (i < rest) now.out[h][q * 32 + i] = adds ? Half<T>::from_float(Half<T>::to_float(was[i]) + f * acc[q * 4 + (i >> 1)][2 * h + (i & 1)]) : was[i];
                 }
             }
         }
@@ -535,8 +549,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
             new_tile = true;
         } else {
 #pragma unroll
-            for (int h = 0; h < 2; h++) { y_at[h] += COLUMNS; out_at[h] += COLUMNS; }
-            load_y();                            // under the next pair's products
+            for (int h = 0; h < 2; h++) { now.y[h] += COLUMNS; now.out[h] += COLUMNS; }
         }
     }
 }
