@@ -234,16 +234,15 @@ down_kernel(const __grid_constant__ LowRankArgs a)
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    if (j * 8 >= tile.z) continue;
+                for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int m = 0; m < MB; m++) {
-                        const uint32_t lo[4] = {wv[c][m][0].x, wv[c][m][1].x, wv[c][m][0].y, wv[c][m][1].y};
-                        const uint32_t hi[4] = {wv[c][m][0].z, wv[c][m][1].z, wv[c][m][0].w, wv[c][m][1].w};
-                        Half<T>::mma(acc[m][j], lo, xv[c][j].x, xv[c][j].y);
-                        Half<T>::mma(acc[m][j], hi, xv[c][j].z, xv[c][j].w);
+                        const uint4 w0 = wv[c][m][0], w1 = wv[c][m][1];
+                        const uint32_t part[4] = {h ? w0.z : w0.x, h ? w1.z : w1.x, h ? w0.w : w0.y, h ? w1.w : w1.y};
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+                            if (j * 8 < tile.z) Half<T>::mma(acc[m][j], part, h ? xv[c][j].z : xv[c][j].x, h ? xv[c][j].w : xv[c][j].y);
                     }
-                }
         }
         // The warps' sums are added in order and sent to the CTA that adds up the cluster's.  With two turns one barrier a unit does: the results of the
         // next one arrive in the other half of `arrived`, and those of the one behind it only after a barrier that this CTA reaches when it has
@@ -489,14 +488,19 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                         ldmatrix4(lo[1], shared_addr(lower) + at + k * 32 + 32);
                     }
 #pragma unroll
-                    for (int j = 0; j < Q * 4; j++) {
-                        uint32_t w[4];
-                        ldmatrix4(w, from + j * 8 * PITCH + k * 32);           // (with an odd number of steps the upper half is not used)
-                        Half<T>::mma(acc[j], hi[0], w[0], w[1]);
-                        Half<T>::mma(acc[j], lo[0], w[0], w[1]);
+                    for (int j0 = 0; j0 < Q * 4; j0 += 4) {
+                        uint32_t w[4][4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) ldmatrix4(w[j], from + (j0 + j) * 8 * PITCH + k * 32);        // (an odd number of steps: half of it)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[0], w[j][0], w[j][1]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[0], w[j][0], w[j][1]);
                         if (both) {
-                            Half<T>::mma(acc[j], hi[1], w[2], w[3]);
-                            Half<T>::mma(acc[j], lo[1], w[2], w[3]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[1], w[j][2], w[j][3]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[1], w[j][2], w[j][3]);
                         }
                     }
                 }

@@ -330,23 +330,26 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
             issue(pending, stage == 0 ? S - 1 : stage - 1);
             pending = ticket();
             if (ok) {
-                float s[NT][4];
+                float s[NT][4], odd[NT][4];
 #pragma unroll
-                for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+                for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = odd[t][0] = odd[t][1] = odd[t][2] = odd[t][3] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t k[4];
                     ldmatrix4(k, keys + Shape::at((lane & 7) + ((lane >> 3) & 1) * 8, ks * 2 + (lane >> 4)));
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        if constexpr (Shape::kKeepQ) {
-                            Half<T>::mma(s[t], k, q[t][ks][0], q[t][ks][1]);
-                        } else {
-                            uint32_t b0, b1;
-                            ldmatrix2(b0, b1, shared_addr(q_ring + q_at * Shape::kQ) + Shape::at(t * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
-                            Half<T>::mma(s[t], k, b0, b1);
-                        }
+                        uint32_t b0, b1;
+                        if constexpr (Shape::kKeepQ) { b0 = q[t][ks][0]; b1 = q[t][ks][1]; }
+                        else ldmatrix2(b0, b1, shared_addr(q_ring + q_at * Shape::kQ) + Shape::at(t * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+                        Half<T>::mma(NT <= 2 && (ks & 1) ? odd[t] : s[t], k, b0, b1);              // (two chains of products where there are few)
                     }
+                }
+                if constexpr (NT <= 2) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[t][e] += odd[t][e];
                 }
                 // rows (keys) lane / 4 and lane / 4 + 8, columns (queries) 2 (lane % 4) and the next
                 const bool on0 = (ok >> (lane >> 2)) & 1, on1 = (ok >> ((lane >> 2) + 8)) & 1;
@@ -404,14 +407,18 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < KS; i++) {
-                    uint32_t v[4];
-                    ldmatrix4_trans(v, values + Shape::at((lane & 7) + (lane >> 4) * 8, i * 2 + ((lane >> 3) & 1)));
+                for (int i0 = 0; i0 < KS; i0 += 2) {
+                    uint32_t v[2][4];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        Half<T>::mma(o[i][t], v, hi[t][0], hi[t][1]);
-                        Half<T>::mma(o[i][t], v, lo[t][0], lo[t][1]);
-                    }
+                    for (int i = 0; i < 2 && i0 + i < KS; i++)
+                        ldmatrix4_trans(v[i], values + Shape::at((lane & 7) + (lane >> 4) * 8, (i0 + i) * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int i = 0; i < 2 && i0 + i < KS; i++)
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+                                Half<T>::mma(o[i0 + i][t], v[i], part ? lo[t][0] : hi[t][0], part ? lo[t][1] : hi[t][1]);
                 }
             }
             const bool last = now.last();

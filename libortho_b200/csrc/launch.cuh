@@ -26,14 +26,19 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, 
 
 int check_device();                    // api.cu: ERR_DEVICE where the current device is no compute capability 10.x GPU
 
-// ---- 16-bit types ---------------------------------------------------------------------------------
+// ---- 16-bit types, and m16n8k16 products of them (a product waits some 23 cycles for the one before it on the same sums: keep four apart) ---------------------------------------------------------------------------------
 template <class T> struct Half;
 template <> struct Half<__half> {
     static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_half2(a, b); }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { mma_16816(d, a, b0, b1); }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+    {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
 };
 template <> struct Half<__nv_bfloat16> {
     static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -46,9 +51,7 @@ template <> struct Half<__nv_bfloat16> {
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
     {
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-            "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
