@@ -164,39 +164,30 @@ group_kernel(const __grid_constant__ LowRankArgs a)
 }
 
 // ---- v = down x ------------------------------------------------------------------------------------------------------
-// MB blocks of 16 ranks (the 16-row operand) by NT of 8 tokens, by a cluster of CTAS.  Few tokens: 64 warps a cluster, so that the K of usual layers
-// is in flight all at once.
-template <class T, int MB, int NT, int CTAS, int WARPS, bool FEW>
-__global__ void __launch_bounds__(32 * WARPS, 8 / WARPS)
-down_kernel(const __grid_constant__ LowRankArgs a)
+constexpr int kFewTile = 16, kFewCtas = 8, kManyTile = 64, kManyCtas = 8, kDownStages = 4;
+
+// Few tokens: MB blocks of 16 ranks (the 16-row operand) by 16 tokens, by a cluster of eight CTAs whose 32 warps have the K of usual layers in flight
+// almost at once.
+template <class T, int MB>
+__global__ void __launch_bounds__(128, 2)
+down_few_kernel(const __grid_constant__ LowRankArgs a)
 {
     // a step is 32 k; CHUNKS steps of a warp are loaded together, 64 to 128 registers
-    constexpr int TOKENS = NT * 8, RANKS = MB * 16, PITCH = RANKS + 4, CHUNKS = NT > 2 ? (MB == 1 ? 3 : 2) : 4;
+    constexpr int NT = kFewTile / 8, CTAS = kFewCtas, WARPS = 4, TOKENS = NT * 8, RANKS = MB * 16, PITCH = RANKS + 4, CHUNKS = 4;
     constexpr int QUADS = TOKENS * RANKS / 4, SHARE = QUADS / CTAS, WARP_QUADS = TOKENS * PITCH / 4;
     static_assert(QUADS % CTAS == 0, "every CTA adds up the same share");
     __shared__ __align__(16) float sums[WARPS][TOKENS][PITCH];
-    // this CTA's share of the results, from every CTA of the cluster; twice where there is room
-    constexpr int TURNS = NT > 2 ? 1 : 2;
-    __shared__ __align__(16) float4 arrived[TURNS][CTAS][SHARE];
-    __shared__ __align__(16) unsigned char few_smem[FEW ? sizeof(FewTokens) : 16];
+    // this CTA's share of the results, from every CTA of the cluster, of two units
+    __shared__ __align__(16) float4 arrived[2][CTAS][SHARE];
+    __shared__ FewTokens few;
     const auto &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = (int)cluster_ctarank();
     cluster_arrive();                            // (waited for before the first store into another CTA: it has started then)
     griddep_wait();
     griddep_launch();
-    FewTokens &few = *reinterpret_cast<FewTokens *>(few_smem);
-    const int *order;
-    const int4 *tiles;
-    int real;
-    if constexpr (FEW) {
-        real = group_few<TOKENS>(few, d).x;
-        order = few.order;
-        tiles = few.tiles;
-    } else {
-        real = a.heads[0];
-        order = a.order;
-        tiles = a.tiles;
-    }
+    const int real = group_few<TOKENS>(few, d).x;
+    const int *const order = few.order;
+    const int4 *const tiles = few.tiles;
     const int K = (int)d.K, steps = (K + 31) / 32, clusters = gridDim.x / CTAS;
     const int quad = lane & 3, row = lane >> 2;
     int turn = 0;
@@ -244,9 +235,8 @@ down_kernel(const __grid_constant__ LowRankArgs a)
                             if (j * 8 < tile.z) Half<T>::mma(acc[m][j], part, h ? xv[c][j].z : xv[c][j].x, h ? xv[c][j].w : xv[c][j].y);
                     }
         }
-        // The warps' sums are added in order and sent to the CTA that adds up the cluster's.  With two turns one barrier a unit does: the results of the
-        // next one arrive in the other half of `arrived`, and those of the one behind it only after a barrier that this CTA reaches when it has
-        // read these.
+        // The warps' sums are added in order and sent to the CTA that adds up the cluster's.  One barrier a unit: the results of the next one
+        // arrive in the other half of `arrived`, and those of the one behind it only after a barrier that this CTA reaches when it has read these.
 #pragma unroll
         for (int m = 0; m < MB; m++)
 #pragma unroll
@@ -280,9 +270,116 @@ down_kernel(const __grid_constant__ LowRankArgs a)
             }
             *reinterpret_cast<float4 *>(a.v + (int64_t)(tile.y + token) * d.rank + r) = s;
         }
-        if constexpr (TURNS == 2) {
-            turn ^= 1;
-        } else {
+        turn ^= 1;
+    }
+}
+
+// Many tokens: MB blocks of 16 ranks by 64 tokens, by a cluster of eight CTAs.  A CTA's share of K comes through a ring of four stages of 64 k; a warp
+// has 16 tokens and all ranks.  Bound by reading x.
+template <class T, int MB>
+__global__ void __launch_bounds__(128, 4)
+down_many_kernel(const __grid_constant__ LowRankArgs a)
+{
+    constexpr int S = kDownStages, RANKS = MB * 16, CTAS = kManyCtas, X_BYTES = kManyTile * 128, STAGE = X_BYTES + RANKS * 128, W_PIECES = RANKS * 8 / 128;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(16) float arrived[CTAS][kManyTile / CTAS][RANKS];     // sums of this CTA's share of the tokens, from every CTA of the cluster
+    const auto &d = a.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, row = lane >> 2, cta = (int)cluster_ctarank();
+    cluster_arrive();                            // (waited for before the first store into another CTA: it has started then)
+    griddep_wait();
+    griddep_launch();
+    const int real = a.heads[0], K = (int)d.K, blocks = (K + 63) / 64, first = blocks * cta / CTAS, count = blocks * (cta + 1) / CTAS - first;
+    // rows of 128 bytes in 16-byte chunks, exchanged by the row's number against bank conflicts; a thread copies the same chunk of every 16th row
+    auto at = [](int r, int chunk) { return (uint32_t)(r * 128 + ((chunk ^ (r & 7)) << 4)); };
+    const int chunk = tid & 7;
+    cluster_wait();
+    for (int64_t unit = blockIdx.x / CTAS; unit < (int64_t)real * a.rank_groups; unit += gridDim.x / CTAS) {
+        const int4 tile = a.tiles[unit / a.rank_groups];
+        const int r0 = (int)(unit % a.rank_groups) * RANKS, rank = tile.w;
+        if (r0 >= rank) continue;                // (the whole cluster)
+        const T *x[kManyTile / 16], *w[W_PIECES];
+#pragma unroll
+        for (int u = 0; u < kManyTile / 16; u++) {
+            const int t = u * 16 + (tid >> 3);
+            x[u] = t < tile.z ? (const T *)d.x + (int64_t)a.order[tile.y + t] * d.x_stride + first * 64 + chunk * 8 : nullptr;
+        }
+#pragma unroll
+        for (int u = 0; u < W_PIECES; u++) {
+            const int r = u * 16 + (tid >> 3);
+            w[u] = r0 + r < rank ? (const T *)d.down + ((int64_t)tile.x * d.rank + r0 + r) * d.K + first * 64 + chunk * 8 : nullptr;
+        }
+        int issued = 0;
+        auto issue = [&](int stage) {
+            if (issued < count) {
+                const uint32_t to = shared_addr(smem + stage * STAGE);
+                const bool in = (first + issued) * 64 + chunk * 8 < K;
+#pragma unroll
+                for (int u = 0; u < kManyTile / 16; u++) {
+                    const bool on = in && x[u];
+                    copy16_async(to + at(u * 16 + (tid >> 3), chunk), on ? x[u] + issued * 64 : d.x, on);
+                }
+#pragma unroll
+                for (int u = 0; u < W_PIECES; u++) {
+                    const bool on = in && w[u];
+                    copy16_async(to + X_BYTES + at(u * 16 + (tid >> 3), chunk), on ? w[u] + issued * 64 : d.down, on);
+                }
+                issued++;
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S - 1; s++) issue(s);
+        float acc[MB][2][4];
+#pragma unroll
+        for (int m = 0; m < MB; m++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+        for (int b = 0, stage = 0; b < count; b++) {
+            copy_wait<S - 2>();
+            __syncthreads();                     // the stage is there, and everybody is done with the one before it
+            issue(stage == 0 ? S - 1 : stage - 1);
+            const uint32_t xs = shared_addr(smem + stage * STAGE), ws = xs + X_BYTES;
+            if (warp * 16 < tile.z) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t v[4], r[MB][4];
+                    ldmatrix4(v, xs + at(warp * 16 + (lane & 7) + (lane >> 4) * 8, k * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                    for (int m = 0; m < MB; m++) ldmatrix4(r[m], ws + at(m * 16 + (lane & 15), k * 2 + (lane >> 4)));
+#pragma unroll
+                    for (int m = 0; m < MB; m++) {
+                        Half<T>::mma(acc[m][0], r[m], v[0], v[1]);
+                        Half<T>::mma(acc[m][1], r[m], v[2], v[3]);
+                    }
+                }
+            }
+            if (++stage == S) stage = 0;
+        }
+        copy_wait<0>();
+        // every CTA sends its sums of eight tokens to the CTA that adds them up
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t to = mapa_shared(shared_addr(&arrived[cta][0][0]), warp * 2 + j);
+#pragma unroll
+            for (int m = 0; m < MB; m++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) st_dsmem(to + ((quad * 2 + (e & 1)) * RANKS + m * 16 + row + (e >> 1) * 8) * 4, acc[m][j][e]);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        for (int i = tid; i < kManyTile / CTAS * RANKS / 4; i += 128) {
+            const int t = i / (RANKS / 4), r = i % (RANKS / 4) * 4, token = cta * (kManyTile / CTAS) + t;
+            if (token >= tile.z || r0 + r >= rank) continue;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int o = 0; o < CTAS; o++) {
+                const float4 y = *reinterpret_cast<const float4 *>(&arrived[o][t][r]);
+                s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
+            }
+            *reinterpret_cast<float4 *>(a.v + (int64_t)(tile.y + token) * d.rank + r0 + r) = s;
+        }
+        if (unit + gridDim.x / CTAS < (int64_t)real * a.rank_groups) {         // the next unit's sums may arrive, and its copies, when these are read
             __syncwarp();
             cluster_arrive();
             cluster_wait();
@@ -333,7 +430,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
 {
     using Shape = UpShape<MT, G>;
     constexpr int TOKENS = Shape::kTokens, COLUMNS = Shape::kColumns, Q = MT == 1 ? 1 : COLUMNS / 32, S = kUpStages, PIECES = Shape::kPieces, PITCH = Shape::kPitch;
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float factor[TOKENS];
     __shared__ __align__(16) unsigned char few_smem[FEW ? sizeof(FewTokens) : 16];
     const auto &d = a.d;
@@ -572,7 +669,6 @@ static int check_low_rank(const ortho_b200_low_rank_desc *d)
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 struct LowRankSpace { int64_t order, tiles, v, bytes; };
-constexpr int kFewTile = 16, kManyTile = 64;
 
 static LowRankSpace low_rank_space(const ortho_b200_low_rank_desc &d)
 {
@@ -588,23 +684,21 @@ static LowRankSpace low_rank_space(const ortho_b200_low_rank_desc &d)
     return s;
 }
 
-template <class T, int MB, int NT, int CTAS, int WARPS, bool FEW>
-static int launch_down(LowRankArgs &a, cudaStream_t stream)
+// `ranks` of a unit, tokens of its tile, CTAs of its cluster; `room`: clusters that find a place at once, about
+static int launch_down(LowRankArgs &a, void (*kernel)(LowRankArgs), int ranks, int tile, int ctas, int64_t room, size_t smem, cudaStream_t stream)
 {
     const auto &d = a.d;
-    const int tile = NT * 8;
-    a.rank_groups = (int)ceil_div(d.rank, MB * 16);
+    a.rank_groups = (int)ceil_div(d.rank, ranks);
     const int64_t most = d.tokens / tile + d.adapters, units = (most < d.tokens ? most : d.tokens) * a.rank_groups;
-    const int64_t room = (FEW ? 4 : 2) * (int64_t)device_sm_count(current_device_index()) / CTAS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((units < room ? units : room) * CTAS)); cfg.blockDim = dim3(32 * WARPS); cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)((units < room ? units : room) * ctas)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = CTAS; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = (unsigned)ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    OB_CUDA(cudaLaunchKernelEx(&cfg, down_kernel<T, MB, NT, CTAS, WARPS, FEW>, a));
+    OB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
     count_launch();
     return ORTHO_B200_OK;
 }
@@ -633,27 +727,35 @@ static int launch_up(LowRankArgs &a, cudaStream_t stream)
     return a.padded <= 16 ? launch_up_as<T, MT, 16, FEW>(a, stream) : a.padded <= 32 ? launch_up_as<T, MT, 32, FEW>(a, stream) : launch_up_as<T, MT, 64, FEW>(a, stream);
 }
 
+static constexpr size_t down_bytes(int mb) { return kDownStages * (kManyTile + mb * 16) * 128; }
+
 template <class T>
 static int launch_low_rank(LowRankArgs &a, cudaStream_t stream)
 {
     const auto &d = a.d;
     const int dev = current_device_index();
     if (dev < 0) return ORTHO_B200_ERR_CUDA;
+    const int64_t sms = device_sm_count(dev);
     int st;
     if (d.tokens <= kFewTokens) {
-        st = d.rank <= 16 ? launch_down<T, 1, kFewTile / 8, 8, 4, true>(a, stream)
-           : launch_down<T, 2, kFewTile / 8, 8, 4, true>(a, stream);
+        const int64_t room = 4 * sms / kFewCtas;
+        st = d.rank <= 16 ? launch_down(a, down_few_kernel<T, 1>, 16, kFewTile, kFewCtas, room, 0, stream)
+                          : launch_down(a, down_few_kernel<T, 2>, 32, kFewTile, kFewCtas, room, 0, stream);
         if (st) return st;
         return launch_up<T, kFewTile / 16, true>(a, stream);
     }
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
+        OB_CUDA(cudaFuncSetAttribute(down_many_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_bytes(1)));
+        OB_CUDA(cudaFuncSetAttribute(down_many_kernel<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_bytes(2)));
         OB_CUDA(cudaFuncSetAttribute(group_kernel<kManyTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 4 * (kMostAdapters + 1)));
         attr_set[dev] = true;
     }
     st = launch_dependent(group_kernel<kManyTile>, dim3(1), kGroupThreads, (size_t)(3 * 4 * (d.adapters + 1)), stream, a);
     if (st) return st;
-    st = d.rank <= 16 ? launch_down<T, 1, kManyTile / 8, 4, 4, false>(a, stream) : launch_down<T, 2, kManyTile / 8, 4, 4, false>(a, stream);
+    const int64_t room = 4 * sms / kManyCtas;
+    st = d.rank <= 16 ? launch_down(a, down_many_kernel<T, 1>, 16, kManyTile, kManyCtas, room, down_bytes(1), stream)
+                      : launch_down(a, down_many_kernel<T, 2>, 32, kManyTile, kManyCtas, room, down_bytes(2), stream);
     if (st) return st;
     return launch_up<T, kManyTile / 16, false>(a, stream);
 }

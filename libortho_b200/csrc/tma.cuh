@@ -175,6 +175,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
         if (mbar_try_wait_cluster(bar, parity)) return true;
     return false;
 }
+__device__ __forceinline__ void st_dsmem(uint32_t addr, float x) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory"); }
 __device__ __forceinline__ void st_dsmem_v2(uint32_t addr, float x, float y) {
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
 }
