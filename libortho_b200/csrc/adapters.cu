@@ -101,28 +101,26 @@ group_kernel(const __grid_constant__ LowRankArgs a)
     griddep_launch();
     for (int e = tid; e < E; e += kGroupThreads) counts[e] = 0;
     __syncthreads();
-    // the adapter of each token, its rank, and its number among its adapter's tokens
-    auto each = [&](auto &&use) {
-        for (int t0 = 0; t0 < T; t0 += AHEAD * kGroupThreads) {
-            int e[AHEAD], rank[AHEAD];
+    // AHEAD tokens of each thread: their adapters and ranks, and from the counters their numbers among their adapters' tokens
+    int e[AHEAD], rank[AHEAD], among[AHEAD];
+    auto number = [&](int t0) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const int t = t0 + i * kGroupThreads + tid;
-                rank[i] = 0;
-                e[i] = t < T ? adapter_of(d, t, rank[i]) : -1;
-            }
+        for (int i = 0; i < AHEAD; i++) {
+            const int t = t0 + i * kGroupThreads + tid;
+            rank[i] = 0;
+            e[i] = t < T ? adapter_of(d, t, rank[i]) : -1;
+        }
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                if (t0 + i * kGroupThreads >= T) break;
-                const uint32_t peers = __match_any_sync(0xffffffffu, e[i]);
-                const int leader = __ffs(peers) - 1;
-                int base = 0;
-                if (e[i] >= 0 && leader == lane) base = atomicAdd(counts + e[i], __popc(peers));
-                use(t0 + i * kGroupThreads + tid, e[i], rank[i], base, peers, leader);
-            }
+        for (int i = 0; i < AHEAD; i++) {
+            if (t0 + i * kGroupThreads >= T) break;
+            const uint32_t peers = __match_any_sync(0xffffffffu, e[i]);
+            const int leader = __ffs(peers) - 1;
+            int base = 0;
+            if (e[i] >= 0 && leader == lane) base = atomicAdd(counts + e[i], __popc(peers));
+            among[i] = __shfl_sync(0xffffffffu, base, leader) + __popc(peers & ((1u << lane) - 1));
         }
     };
-    each([](int, int, int, int, uint32_t, int) {});
+    for (int t0 = 0; t0 < T; t0 += AHEAD * kGroupThreads) number(t0);
     __syncthreads();
     int2 before = make_int2(0, 0);               // tokens and tiles of the adapters before
     for (int e0 = 0; e0 < E; e0 += kGroupThreads) {
@@ -151,16 +149,19 @@ group_kernel(const __grid_constant__ LowRankArgs a)
         before.y += __shfl_sync(0xffffffffu, w.y, 31);
         __syncthreads();
     }
-    each([&](int t, int e, int rank, int base, uint32_t peers, int leader) {
-        base = __shfl_sync(0xffffffffu, base, leader);
-        if (e < 0) return;
-        const int among = base + __popc(peers & ((1u << lane) - 1)), at = start[e] + among;
-        a.order[at] = t;
-        if (among % TILE == 0) {
-            const int end = e + 1 < E ? start[e + 1] : T;
-            a.tiles[first_tile[e] + among / TILE] = make_int4(e + 1 < E ? e : -1, at, min(TILE, end - at), rank);
+    for (int t0 = 0; t0 < T; t0 += AHEAD * kGroupThreads) {
+        if (T > AHEAD * kGroupThreads) number(t0);                             // (else they are at hand)
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (e[i] < 0) continue;
+            const int at = start[e[i]] + among[i];
+            a.order[at] = t0 + i * kGroupThreads + tid;
+            if (among[i] % TILE == 0) {
+                const int end = e[i] + 1 < E ? start[e[i] + 1] : T;
+                a.tiles[first_tile[e[i]] + among[i] / TILE] = make_int4(e[i] + 1 < E ? e[i] : -1, at, min(TILE, end - at), rank[i]);
+            }
         }
-    });
+    }
 }
 
 // ---- v = down x ------------------------------------------------------------------------------------------------------
