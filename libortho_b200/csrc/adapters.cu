@@ -6,12 +6,11 @@
 // token).  The operations are a few per byte either way, so both products run on m16n8k16 tensor-core instructions.
 //
 // Tokens are grouped first, so that an adapter's weights are read once for all its tokens: `order` lists them by adapter, a tile is up to
-// kTile of them with one adapter.  Up to kFewTokens tokens every CTA groups them for itself; more are grouped by a kernel in front.
+// 16 or 64 of them with one adapter.
 //
-// down_kernel: a cluster of CTAs per tile and 16 or 32 ranks, K split over its warps, their sums joined through distributed shared memory in a fixed
-// order.  Operands come straight from global memory, 16 bytes a lane: the order of k inside an instruction is free as long as both use
-// the same one.  up_kernel is launched as a programmatic dependent and fetches its first weights (constants of the layer) while down_kernel
-// still runs.
+// Up to kFewTokens tokens every CTA groups them for itself, and where there is little to do few_kernel does it all.  Else a kernel computes v
+// (down_few_kernel or down_many_kernel; more tokens are grouped by a kernel in front) and up_kernel the outputs: it starts beside the kernel for v
+// and fetches its first weights (constants of the layer) and rows of y meanwhile.
 #include "launch.cuh"
 #include "tma.cuh"
 
@@ -411,20 +410,128 @@ __device__ __forceinline__ float largest(float4 v) { return fmaxf(fmaxf(fabsf(v.
 constexpr int kUpThreads = 128, kUpStages = 3;                                // (stages: 2 pairs are under way while one is worked on)
 static_assert(kFewTokens == kUpThreads && kGroupThreads == 32 * 32, "a thread per token, a lane per warp");
 
-// Columns of a pair and the layout of a stage: rows of G ranks, 16 bytes of padding against bank conflicts
+// Columns of a unit of work and the layout of a stage: rows of G ranks, 16 bytes of padding against bank conflicts, then every thread's own pieces of y.
+// Column c of 8 in product tile j stands for output column 8 (c / 2) + 2 j + c % 2 of 32, so that a lane's results over four tiles are
+// eight neighbours.
 template <int MT, int G>
 struct UpShape {
     static constexpr int kTokens = MT * 16, kColumns = MT == 1 ? 128 : 64, kPieces = G / 8, kPitch = G * 2 + 16, kWeights = kColumns * kPitch + 64;
-    static constexpr int kTaken = MT == 1 ? 2 : 4;                             // 16-byte pieces of y that a thread needs for its results of a pair
-    static constexpr int kStage = kWeights + kTaken * kUpThreads * 16;         // rows of `up`, then every thread's own pieces of y
-    static int bytes(int padded) { return kUpStages * kStage + 2 * kTokens * (padded * 2 + 16); }
+    static constexpr int kTaken = MT == 1 ? 2 : 4;                             // 16-byte pieces of y that a thread needs for its results
+    static constexpr int kStage = kWeights + kTaken * kUpThreads * 16;
+    static __device__ __forceinline__ int at(int n) { return (n & ~31) + (n >> 1 & 3) * 8 + (n >> 3 & 3) * 2 + (n & 1); }      // row of a column in a stage
 };
 
-// The (tile, columns) pairs are numbered in a row and dealt evenly, a run of them to each CTA, so that v comes into shared memory about once per
-// CTA.  Rows of `up` (up to 64 ranks) and y arrive in a ring of three stages, the first ones while down_kernel still runs.
-// Tiles of 16 tokens (MT = 1): a warp has 32 of 128 columns, bound by the weights.  Of 64 (MT = 4): a warp has 16 tokens and 64 columns, bound by
-// y and out.  Column c of 8 in product tile j stands for output column 8 (c / 2) + 2 j + c % 2 of 32, so that a lane's results over four
-// tiles are eight neighbours.
+// A lane's place in its two tokens' rows of y and out
+template <class T> struct Rows { const T *y[2]; T *out[2]; bool has[2]; };
+
+// v as two 16-bit parts into shared memory, rows `pitch` bytes apart, and the factor of each token's result.  `from(t, r)`: four ranks of token t.
+template <class T, int TOKENS, class F>
+__device__ __forceinline__ void place_v(unsigned char *upper, unsigned char *lower, float *factor, int pitch, int padded, float scale, F &&from)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // lanes of a token: the power of two that holds a quarter of the rank, at most a warp (twice: above 128)
+    const int width = padded <= 16 ? 4 : padded <= 32 ? 8 : padded <= 64 ? 16 : 32, rows = 32 / width, sub = lane & (width - 1);
+#pragma unroll 4
+    for (int i = 0; i < TOKENS / 4; i += rows) {
+        const int t = warp * (TOKENS / 4) + i + lane / width;
+        if (TOKENS / 4 < rows && t >= (warp + 1) * (TOKENS / 4)) break;        // (a warp has four tokens, lanes for eight)
+        float4 x[2];
+        float top = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            x[h] = from(t, (h * 32 + sub) * 4);
+            top = fmaxf(top, largest(x[h]));
+        }
+        const uint32_t here = TOKENS / 4 < rows ? (1u << (TOKENS / 4 * width)) - 1 : 0xFFFFFFFFu;
+        for (int o = width >> 1; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(here, top, o));
+        const PowerOfTwo by = bring_near<T>(top);
+        if (sub == 0) factor[t] = by.back * scale;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = (h * 32 + sub) * 4;
+            if (r >= padded) continue;
+            uint32_t hi[2], lo[2];
+            two_parts<T>(x[h].x * by.down, x[h].y * by.down, hi[0], lo[0]);
+            two_parts<T>(x[h].z * by.down, x[h].w * by.down, hi[1], lo[1]);
+            *reinterpret_cast<uint2 *>(upper + t * pitch + r * 2) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2 *>(lower + t * pitch + r * 2) = make_uint2(lo[0], lo[1]);
+        }
+    }
+}
+
+// acc += v up over `steps` times 16 ranks of a stage, for 16 tokens and 4 J columns' tiles of 8.  v_at: this lane's row of v in the upper part, `apart` to the lower.
+template <class T, int G, int J>
+__device__ __forceinline__ void multiply_up(float (&acc)[J][4], uint32_t v_at, uint32_t apart, uint32_t weights, int steps)
+{
+    constexpr int PITCH = G * 2 + 16;
+#pragma unroll
+    for (int k = 0; k < G / 16; k += 2) {
+        if (k >= steps) break;
+        const bool both = G > 16 && k + 1 < steps;
+        uint32_t hi[2][4], lo[2][4];
+        ldmatrix4(hi[0], v_at + k * 32);
+        ldmatrix4(lo[0], v_at + apart + k * 32);
+        if (both) {
+            ldmatrix4(hi[1], v_at + k * 32 + 32);
+            ldmatrix4(lo[1], v_at + apart + k * 32 + 32);
+        }
+#pragma unroll
+        for (int j0 = 0; j0 < J; j0 += 4) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) ldmatrix4(w[j], weights + (j0 + j) * 8 * PITCH + k * 32);          // (an odd number of steps: half of it)
+#pragma unroll
+            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[0], w[j][0], w[j][1]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[0], w[j][0], w[j][1]);
+            if (both) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[1], w[j][2], w[j][3]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[1], w[j][2], w[j][3]);
+            }
+        }
+    }
+}
+
+// out = y + factor acc of a lane's two tokens.  whole: y has come to `staged` (pieces of a thread 16 kUpThreads bytes apart); else rows that are not aligned, or
+// the last columns (`rest` of them from this lane's first one on), one by one.
+template <class T, int Q>
+__device__ __forceinline__ void write_out(const Rows<T> &now, const float (&acc)[Q * 4][4], const float *factor, int t, bool adds, bool whole, const unsigned char *staged, int rest)
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (!now.has[h]) continue;
+        const float f = adds ? factor[t + h * 8] : 0.f;
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            if (whole) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(staged + (h * Q + q) * (kUpThreads * 16));
+                uint32_t p[4] = {y.x, y.y, y.z, y.w};
+                if (adds) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float2 was = Half<T>::unpack(p[j]);
+                        p[j] = Half<T>::pack(was.x + f * acc[q * 4 + j][2 * h], was.y + f * acc[q * 4 + j][2 * h + 1]);
+                    }
+                }
+                *reinterpret_cast<uint4 *>(now.out[h] + q * 32) = make_uint4(p[0], p[1], p[2], p[3]);
+            } else {
+                T was[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < rest - q * 32) was[i] = now.y[h][q * 32 + i];
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < rest - q * 32) now.out[h][q * 32 + i] = adds ? Half<T>::from_float(Half<T>::to_float(was[i]) + f * acc[q * 4 + (i >> 1)][2 * h + (i & 1)]) : was[i];
+            }
+        }
+    }
+}
+
+// The (tile, columns) pairs are numbered in a row and dealt evenly, a run of them to each CTA, so that v comes into shared memory about once per CTA.
+// Rows of `up` (up to 64 ranks) and y arrive in a ring of three stages, the first ones while the kernel for v still runs.  Tiles of 16 tokens (MT = 1):
+// a warp has 32 of 128 columns, bound by the weights.  Of 64 (MT = 4): a warp has 16 tokens and 64 columns, bound by y and out.
 template <class T, int MT, int G, bool FEW>
 __global__ void __launch_bounds__(kUpThreads, 4)
 up_kernel(const __grid_constant__ LowRankArgs a)
@@ -437,9 +544,9 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     const auto &d = a.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, row = lane >> 2;
     const int padded = a.padded, groups = G < 64 ? 1 : a.up_groups, v_pitch = padded * 2 + 16, N = (int)d.N;
-    unsigned char *const upper = smem + S * Shape::kStage, *const lower = upper + TOKENS * v_pitch;
     const int t0 = MT == 1 ? 0 : warp * 16, c0 = MT == 1 ? warp * 32 : 0;      // this warp's first token of the tile and column of the pair
-    // What is read in front of the wait was complete before down_kernel let this kernel start (it does so behind its own wait), or is a
+    unsigned char *const upper = smem + S * Shape::kStage, *const lower = upper + TOKENS * v_pitch;
+    // What is read in front of the wait was complete before the kernel for v let this kernel start (it does so behind its own wait), or is a
     // constant of the layer.
     griddep_launch();
     FewTokens &few = *reinterpret_cast<FewTokens *>(few_smem);
@@ -453,14 +560,8 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     auto tile_at = [&](int i) { if constexpr (FEW) return few.tiles[i]; else return __ldcg(a.tiles + i); };
     const int64_t pairs = (int64_t)all * a.blocks, first = pairs * blockIdx.x / gridDim.x, end = pairs * (blockIdx.x + 1) / gridDim.x;
     int left = (int)(end - first), to_issue = left;
-
-    // the copies of a step (pair, up to 64 ranks); each thread has PIECES (or half as many) of the 16-byte pieces
-    int next_group = 0, next_tile = left ? (int)(first / a.blocks) : 0, next_block = left ? (int)(first - (int64_t)next_tile * a.blocks) : 0;
-    int4 ahead = make_int4(-1, 0, 0, 0);
-    // this lane's place in its two tokens' rows of y, for the copies and (below) for the results: column c0 + 8 quad of a pair
-    struct Rows { const T *y[2]; T *out[2]; bool has[2]; };
     auto rows_of = [&](const int4 &tile, int block) {
-        Rows r;
+        Rows<T> r;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int t = t0 + h * 8 + row;
@@ -471,7 +572,10 @@ up_kernel(const __grid_constant__ LowRankArgs a)
         }
         return r;
     };
-    Rows coming;
+    // the copies of a step (pair, up to 64 ranks); each thread has some of the 16-byte pieces of `up` and its own of y, which come with the last ranks
+    int next_group = 0, next_tile = left ? (int)(first / a.blocks) : 0, next_block = left ? (int)(first - (int64_t)next_tile * a.blocks) : 0;
+    int4 ahead = make_int4(-1, 0, 0, 0);
+    Rows<T> coming;
     if (left) {
         ahead = tile_at(next_tile);
         coming = rows_of(ahead, next_block);
@@ -480,7 +584,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     auto issue = [&](int stage) {
         if (to_issue > 0) {
             const int r0 = next_group * G;
-            if (next_group == groups - 1 && a.vectors && (next_block + 1) * COLUMNS <= N) {       // y comes with the last ranks
+            if (next_group == groups - 1 && a.vectors && (next_block + 1) * COLUMNS <= N) {
                 const uint32_t to = shared_addr(smem + stage * Shape::kStage) + mine;
 #pragma unroll
                 for (int h = 0; h < 2; h++)
@@ -496,8 +600,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                 for (int u = 0; u < COLUMNS * PIECES / kUpThreads; u++) {
                     const int i = u * kUpThreads + tid, n = i / PIECES, piece = i % PIECES;
                     const bool on = n < columns && piece * 8 < ranks;
-                    const int at = (n & ~31) + (n >> 1 & 3) * 8 + (n >> 3 & 3) * 2 + (n & 1);      // product tile j = n / 2 % 4, its column c
-                    copy16_async(to + at * PITCH + piece * 16, on ? from + n * (int)d.rank + piece * 8 : from, on);
+                    copy16_async(to + Shape::at(n) * PITCH + piece * 16, on ? from + n * (int)d.rank + piece * 8 : from, on);
                 }
             }
             if (++next_group == groups) {
@@ -522,7 +625,7 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     int tile_number = (int)(first / a.blocks), block = (int)(first - (int64_t)tile_number * a.blocks), stage = 0;
     bool new_tile = true;
     int4 tile;
-    Rows now;
+    Rows<T> now;
     for (int last = 0;;) {
         float acc[Q * 4][4];
 #pragma unroll
@@ -535,115 +638,20 @@ up_kernel(const __grid_constant__ LowRankArgs a)
                 new_tile = false;
                 tile = tile_at(tile_number);
                 now = rows_of(tile, block);
-                if (tile.x >= 0) {
-                    const float scale = d.scales ? __ldcg(d.scales + tile.x) : 1.f;
-                    // lanes of a token: the power of two that holds a quarter of the rank, at most a warp (twice: above 128)
-                    const int width = padded <= 16 ? 4 : padded <= 32 ? 8 : padded <= 64 ? 16 : 32, rows = 32 / width, sub = lane & (width - 1);
-#pragma unroll 4
-                    for (int i = 0; i < TOKENS / 4; i += rows) {
-                        const int t = warp * (TOKENS / 4) + i + lane / width;
-                        if (TOKENS / 4 < rows && t >= (warp + 1) * (TOKENS / 4)) break;           // (a warp has four tokens, lanes for eight)
-                        float4 x[2];
-                        float top = 0.f;
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int r = (h * 32 + sub) * 4;
-                            x[h] = t < tile.z && r < tile.w ? __ldcg(reinterpret_cast<const float4 *>(a.v + (int64_t)(tile.y + t) * d.rank + r))
-                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
-                            top = fmaxf(top, largest(x[h]));
-                        }
-                        const uint32_t here = TOKENS / 4 < rows ? (1u << (TOKENS / 4 * width)) - 1 : 0xFFFFFFFFu;
-                        for (int o = width >> 1; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(here, top, o));
-                        const PowerOfTwo by = bring_near<T>(top);
-                        if (sub == 0) factor[t] = by.back * scale;
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int r = (h * 32 + sub) * 4;
-                            if (r >= padded) continue;
-                            uint32_t hi[2], lo[2];
-                            two_parts<T>(x[h].x * by.down, x[h].y * by.down, hi[0], lo[0]);
-                            two_parts<T>(x[h].z * by.down, x[h].w * by.down, hi[1], lo[1]);
-                            *reinterpret_cast<uint2 *>(upper + t * v_pitch + r * 2) = make_uint2(hi[0], hi[1]);
-                            *reinterpret_cast<uint2 *>(lower + t * v_pitch + r * 2) = make_uint2(lo[0], lo[1]);
-                        }
-                    }
-                }
+                if (tile.x >= 0)
+                    place_v<T, TOKENS>(upper, lower, factor, v_pitch, padded, d.scales ? __ldcg(d.scales + tile.x) : 1.f, [&](int t, int r) {
+                        return t < tile.z && r < tile.w ? __ldcg(reinterpret_cast<const float4 *>(a.v + (int64_t)(tile.y + t) * d.rank + r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    });
                 __syncthreads();
             }
             const int ranks = tile.x < 0 ? 0 : min(tile.w - group * G, G), steps = (ranks + 15) / 16;             // of 16 ranks
-            if (steps > 0 && t0 < tile.z) {
-                const uint32_t at = (uint32_t)((t0 + (lane & 15)) * v_pitch + group * (G * 2) + (lane >> 4) * 16);
-                const uint32_t from = shared_addr(smem + stage * Shape::kStage) + (uint32_t)((c0 + (lane & 7)) * PITCH + (lane >> 3) * 16);
-#pragma unroll
-                for (int k = 0; k < G / 16; k += 2) {
-                    if (k >= steps) break;
-                    const bool both = G > 16 && k + 1 < steps;
-                    uint32_t hi[2][4], lo[2][4];
-                    ldmatrix4(hi[0], shared_addr(upper) + at + k * 32);
-                    ldmatrix4(lo[0], shared_addr(lower) + at + k * 32);
-                    if (both) {
-                        ldmatrix4(hi[1], shared_addr(upper) + at + k * 32 + 32);
-                        ldmatrix4(lo[1], shared_addr(lower) + at + k * 32 + 32);
-                    }
-#pragma unroll
-                    for (int j0 = 0; j0 < Q * 4; j0 += 4) {
-                        uint32_t w[4][4];
-#pragma unroll
-                        for (int j = 0; j < 4; j++) ldmatrix4(w[j], from + (j0 + j) * 8 * PITCH + k * 32);        // (an odd number of steps: half of it)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[0], w[j][0], w[j][1]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[0], w[j][0], w[j][1]);
-                        if (both) {
-#pragma unroll
-                            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], hi[1], w[j][2], w[j][3]);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) Half<T>::mma(acc[j0 + j], lo[1], w[j][2], w[j][3]);
-                        }
-                    }
-                }
-            }
+            if (steps > 0 && t0 < tile.z)
+                multiply_up<T, G, Q * 4>(acc, shared_addr(upper) + (uint32_t)((t0 + (lane & 15)) * v_pitch + group * (G * 2) + (lane >> 4) * 16), (uint32_t)(TOKENS * v_pitch),
+                                         shared_addr(smem + stage * Shape::kStage) + (uint32_t)((c0 + (lane & 7)) * PITCH + (lane >> 3) * 16), steps);
             last = stage;
             if (++stage == S) stage = 0;
         }
-        const bool adds = tile.x >= 0;
-        if (a.vectors && (block + 1) * COLUMNS <= N) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (!now.has[h]) continue;
-                const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
-#pragma unroll
-                for (int q = 0; q < Q; q++) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(smem + last * Shape::kStage + mine + (h * Q + q) * (kUpThreads * 16));
-                    uint32_t p[4] = {y.x, y.y, y.z, y.w};
-                    if (adds) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float2 was = Half<T>::unpack(p[j]);
-                            p[j] = Half<T>::pack(was.x + f * acc[q * 4 + j][2 * h], was.y + f * acc[q * 4 + j][2 * h + 1]);
-                        }
-                    }
-                    *reinterpret_cast<uint4 *>(now.out[h] + q * 32) = make_uint4(p[0], p[1], p[2], p[3]);
-                }
-            }
-        } else {                                 // rows that are not aligned, or the last columns: one by one
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (!now.has[h]) continue;
-                const float f = adds ? factor[t0 + h * 8 + row] : 0.f;
-#pragma unroll
-                for (int q = 0; q < Q; q++) {
-                    const int rest = N - (block * COLUMNS + c0 + q * 32 + quad * 8);
-                    T was[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i < rest) was[i] = now.y[h][q * 32 + i];
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i < rest) now.out[h][q * 32 + i] = adds ? Half<T>::from_float(Half<T>::to_float(was[i]) + f * acc[q * 4 + (i >> 1)][2 * h + (i & 1)]) : was[i];
-                }
-            }
-        }
+        write_out<T, Q>(now, acc, factor, t0 + row, tile.x >= 0, a.vectors && (block + 1) * COLUMNS <= N, smem + last * Shape::kStage + mine, N - (block * COLUMNS + c0 + quad * 8));
         if (--left == 0) break;
         if (++block == a.blocks) {
             block = 0;
@@ -653,6 +661,201 @@ up_kernel(const __grid_constant__ LowRankArgs a)
 #pragma unroll
             for (int h = 0; h < 2; h++) { now.y[h] += COLUMNS; now.out[h] += COLUMNS; }
         }
+    }
+}
+
+// ---- few tokens and columns: both products in one kernel ------------------------------------------------------------------------------
+// A cluster of eight CTAs has a tile of up to 16 tokens and a share of the columns.  It computes v of the tile (again in every cluster that has some of its
+// columns: the weights come from L2 then), K split over its 32 warps; every CTA sends its sums to all the others and adds up what
+// arrives, in order.  Then every CTA has some blocks of 128 columns, a warp 32 of them.  The first rows of `up` and of y are under way from the
+// start.  Bound by the weights, and at a token or two by the chain of loads: ids, weights and x, exchange, results.
+template <int MB>
+struct FewShape {
+    static constexpr int kRanks = MB * 16, kCtas = 8, kPitch = kRanks + 4;
+    using Up = UpShape<1, kRanks>;
+    static constexpr int kSums = 4 * 16 * kPitch * 4, kArrived = 2 * kCtas * 16 * kRanks * 4;
+    static int bytes(int padded) { return kUpStages * Up::kStage + kSums + kArrived + 2 * 16 * (padded * 2 + 16) + 16 * padded * 4; }
+};
+
+template <class T, int MB>
+__global__ void __launch_bounds__(kUpThreads, 2)
+few_kernel(const __grid_constant__ LowRankArgs a)
+{
+    using Shape = FewShape<MB>;
+    using Up = typename Shape::Up;
+    constexpr int S = kUpStages, CTAS = Shape::kCtas, RANKS = Shape::kRanks, PITCH = Shape::kPitch, CHUNKS = 4, STRIDE = CTAS * 4, COLUMNS = Up::kColumns, PIECES = Up::kPieces;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ FewTokens few;
+    __shared__ float factor[16];
+    const auto &d = a.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, row = lane >> 2, cta = (int)cluster_ctarank();
+    const int padded = a.padded, v_pitch = padded * 2 + 16, K = (int)d.K, N = (int)d.N, steps_k = (K + 31) / 32;
+    float *const sums = reinterpret_cast<float *>(smem + S * Up::kStage);      // [4 warps][16 tokens][PITCH]
+    float4 *const arrived = reinterpret_cast<float4 *>(reinterpret_cast<unsigned char *>(sums) + Shape::kSums);           // [2][CTAS][16 tokens][RANKS]
+    float *const v = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(arrived) + Shape::kArrived);             // [16][padded]
+    unsigned char *const upper = reinterpret_cast<unsigned char *>(v + 16 * padded), *const lower = upper + 16 * v_pitch;
+    cluster_arrive();                            // (waited for before the first store into another CTA: it has started then)
+    griddep_wait();
+    griddep_launch();
+    const int2 count = group_few<16>(few, d);
+    const int all = a.copies ? count.y : count.x, clusters = gridDim.x / CTAS;
+    // clusters of a tile
+    const int shares = all > 0 ? max(1, min(clusters / all, (a.blocks + CTAS - 1) / CTAS)) : 1;
+    int turn = 0;
+    cluster_wait();
+    for (int unit = blockIdx.x / CTAS; unit < all * shares; unit += clusters) {
+        const int4 tile = few.tiles[unit / shares];
+        const int part = unit % shares * CTAS + cta, parts = shares * CTAS;
+        int block = (int)((int64_t)a.blocks * part / parts);
+        const int end = (int)((int64_t)a.blocks * (part + 1) / parts), rank = tile.x < 0 ? 0 : tile.w, groups = rank ? (rank + RANKS - 1) / RANKS : 1;
+        const float scale = rank && d.scales ? __ldcg(d.scales + tile.x) : 1.f;
+        Rows<T> now;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int t = h * 8 + row;
+            now.has[h] = t < tile.z;
+            const int64_t token = now.has[h] ? few.order[tile.y + t] : 0;
+            now.y[h] = (const T *)d.y + token * d.y_stride + block * COLUMNS + warp * 32 + quad * 8;
+            now.out[h] = (T *)d.out + token * d.out_stride + block * COLUMNS + warp * 32 + quad * 8;
+        }
+        // the copies of a step: up to RANKS ranks of a block of columns, y with the last of them
+        int next_block = block, next_group = 0;
+        const uint32_t mine = Up::kWeights + tid * 16;
+        auto issue = [&](int stage) {
+            if (next_block < end) {
+                const uint32_t to = shared_addr(smem + stage * Up::kStage);
+                if (next_group == groups - 1 && a.vectors && (next_block + 1) * COLUMNS <= N) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (now.has[h]) copy16_async(to + mine + h * (kUpThreads * 16), now.y[h] + (next_block - block) * COLUMNS, true);
+                }
+                if (rank) {
+                    const int r0 = next_group * RANKS, columns = N - next_block * COLUMNS, ranks = rank - r0;
+                    const T *const from = (const T *)d.up + ((int64_t)tile.x * N + next_block * COLUMNS) * d.rank + r0;
+#pragma unroll
+                    for (int u = 0; u < COLUMNS * PIECES / kUpThreads; u++) {
+                        const int i = u * kUpThreads + tid, n = i / PIECES, piece = i % PIECES;
+                        const bool on = n < columns && piece * 8 < ranks;
+                        copy16_async(to + Up::at(n) * Up::kPitch + piece * 16, on ? from + n * (int)d.rank + piece * 8 : from, on);
+                    }
+                }
+                if (++next_group == groups) {
+                    next_group = 0;
+                    next_block++;
+                }
+            }
+            copy_commit();
+        };
+        __syncthreads();                         // the unit before is done with the stages and with v
+#pragma unroll
+        for (int s = 0; s < S - 1; s++) issue(s);
+
+        // ---- v = down x: 32 k a step, 8 of them (16 bytes of every row) a lane, steps dealt to the cluster's warps in turn
+        const T *x[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) x[j] = (const T *)d.x + (int64_t)few.order[tile.y + min(j * 8 + row, tile.z - 1)] * d.x_stride;
+        for (int r0 = 0; r0 < rank; r0 += RANKS) {
+            const T *const w = (const T *)d.down + ((int64_t)tile.x * d.rank + r0 + row) * d.K;
+            float acc[MB][2][4];
+#pragma unroll
+            for (int m = 0; m < MB; m++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+            for (int s0 = cta * 4 + warp; s0 < steps_k; s0 += CHUNKS * STRIDE) {
+                uint4 wv[CHUNKS][MB][2], xv[CHUNKS][2];
+#pragma unroll
+                for (int c = 0; c < CHUNKS; c++) {
+                    const int k = (s0 + c * STRIDE) * 32 + quad * 8;
+                    const bool on = k < K;
+#pragma unroll
+                    for (int m = 0; m < MB; m++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            wv[c][m][h] = on && r0 + m * 16 + h * 8 + row < rank ? load16(w + (int64_t)(m * 16 + h * 8) * d.K + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) xv[c][j] = on && j * 8 < tile.z ? load16(x[j] + k) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int m = 0; m < MB; m++) {
+                            const uint4 w0 = wv[c][m][0], w1 = wv[c][m][1];
+                            const uint32_t half[4] = {h ? w0.z : w0.x, h ? w1.z : w1.x, h ? w0.w : w0.y, h ? w1.w : w1.y};
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                if (j * 8 < tile.z) Half<T>::mma(acc[m][j], half, h ? xv[c][j].z : xv[c][j].x, h ? xv[c][j].w : xv[c][j].y);
+                        }
+            }
+#pragma unroll
+            for (int m = 0; m < MB; m++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sums[(warp * 16 + j * 8 + quad * 2 + (e & 1)) * PITCH + m * 16 + row + (e >> 1) * 8] = acc[m][j][e];
+            __syncthreads();
+            // The CTA's sums go to every CTA of the cluster.  One barrier: the next ones arrive in the other half of `arrived`, and those behind them only
+            // after a barrier that this CTA reaches when it has read these.
+            constexpr int QUADS = 16 * RANKS / 4;
+            const uint32_t to = shared_addr(arrived + (turn * CTAS + cta) * QUADS);
+            for (int i = tid; i < QUADS; i += kUpThreads) {
+                const int t = i / (RANKS / 4), q = i % (RANKS / 4) * 4;
+                if (t >= tile.z) break;
+                float4 s = *reinterpret_cast<const float4 *>(sums + t * PITCH + q);
+#pragma unroll
+                for (int o = 1; o < 4; o++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(sums + (o * 16 + t) * PITCH + q);
+                    s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
+                }
+#pragma unroll
+                for (int o = 0; o < CTAS; o++) st_dsmem_v4(mapa_shared(to + 16 * i, o), s);
+            }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            for (int i = tid; i < QUADS; i += kUpThreads) {
+                const int t = i / (RANKS / 4), r = r0 + i % (RANKS / 4) * 4;
+                if (t >= tile.z) break;
+                if (r >= padded) continue;
+                float4 s = arrived[turn * CTAS * QUADS + i];
+#pragma unroll
+                for (int o = 1; o < CTAS; o++) {
+                    const float4 y = arrived[(turn * CTAS + o) * QUADS + i];
+                    s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w;
+                }
+                *reinterpret_cast<float4 *>(v + t * padded + r) = r < rank ? s : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            turn ^= 1;
+        }
+        if (rank) {
+            __syncthreads();
+            place_v<T, 16>(upper, lower, factor, v_pitch, padded, scale, [&](int t, int r) {
+                return t < tile.z && r < rank ? *reinterpret_cast<const float4 *>(v + t * padded + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            });
+        }
+
+        // ---- out = y + scale up v (the barrier in the loop is also that of v)
+        for (int stage = 0, last = 0; block < end; block++) {
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            for (int group = 0; group < groups; group++) {
+                copy_wait<S - 2>();
+                __syncthreads();                 // the stage is there, and everybody is done with the one before it
+                issue(stage == 0 ? S - 1 : stage - 1);
+                const int ranks = min(rank - group * RANKS, RANKS);
+                if (ranks > 0)
+                    multiply_up<T, RANKS, 4>(acc, shared_addr(upper) + (uint32_t)((lane & 15) * v_pitch + group * (RANKS * 2) + (lane >> 4) * 16), (uint32_t)(16 * v_pitch),
+                                             shared_addr(smem + stage * Up::kStage) + (uint32_t)((warp * 32 + (lane & 7)) * Up::kPitch + (lane >> 3) * 16), (ranks + 15) / 16);
+                last = stage;
+                if (++stage == S) stage = 0;
+            }
+            write_out<T, 1>(now, acc, factor, row, rank > 0, a.vectors && (block + 1) * COLUMNS <= N, smem + last * Up::kStage + mine, N - (block * COLUMNS + warp * 32 + quad * 8));
+#pragma unroll
+            for (int h = 0; h < 2; h++) { now.y[h] += COLUMNS; now.out[h] += COLUMNS; }
+        }
+        copy_wait<0>();
     }
 }
 
@@ -671,28 +874,42 @@ static int check_low_rank(const ortho_b200_low_rank_desc *d)
 // ---- host -------------------------------------------------------------------------------------------------------------
 struct LowRankSpace { int64_t order, tiles, v, bytes; };
 
+// the most tiles that these tokens can have: an adapter's last tile may hold fewer tokens
+static int64_t most_tiles(const ortho_b200_low_rank_desc &d, int tile)
+{
+    const int64_t most = d.tokens / tile + d.adapters + 1;
+    return most < d.tokens ? most : d.tokens;
+}
+
+// Up to kFewTokens tokens both products run in one kernel where every tile finds room at once as a cluster for each eight blocks of columns (or two, one
+// after the other): one launch and no exchange through memory.  Where there is more to do, the two kernels use the GPU more evenly and the second
+// one's weights come while the first runs.  Measured, both ways: 1 token, 4096 -> 12288, rank 16: 4.7 us in one kernel, 5.0 in two; 77 tokens,
+// 2912 -> 1003, rank 8: 6.7, 7.4; 64 tokens over twenty adapters of rank 8 to 64, 8192 -> 10240: 24.5, 18.4 (and two launches of host time).
+static bool in_one_kernel(const ortho_b200_low_rank_desc &d)
+{
+    const int64_t units = most_tiles(d, kFewTile) * ceil_div(ceil_div(d.N, UpShape<1, 16>::kColumns), FewShape<1>::kCtas);
+    return d.tokens <= kFewTokens && units <= 4 * (int64_t)device_sm_count(current_device_index()) / FewShape<1>::kCtas;
+}
+
 static LowRankSpace low_rank_space(const ortho_b200_low_rank_desc &d)
 {
     auto room = [](int64_t b) { return (b + 255) / 256 * 256; };
     LowRankSpace s = {};
+    if (in_one_kernel(d)) return s;
     if (d.tokens > kFewTokens) {
         s.order = 256;
         s.tiles = s.order + room(4 * d.tokens);
-        const int64_t most = d.tokens / kManyTile + d.adapters + 1;             // an adapter's last tile may hold fewer tokens
-        s.v = s.tiles + room(16 * (most < d.tokens ? most : d.tokens));
+        s.v = s.tiles + room(16 * most_tiles(d, kManyTile));
     }
     s.bytes = s.v + room(4 * d.tokens * d.rank);
     return s;
 }
 
-// `ranks` of a unit, tokens of its tile, CTAs of its cluster; `room`: clusters that find a place at once, about
-static int launch_down(LowRankArgs &a, void (*kernel)(LowRankArgs), int ranks, int tile, int ctas, int64_t room, size_t smem, cudaStream_t stream)
+// clusters of `ctas` CTAs, `count` of them, as a programmatic dependent
+static int launch_clusters(void (*kernel)(LowRankArgs), int64_t count, int ctas, size_t smem, const LowRankArgs &a, cudaStream_t stream)
 {
-    const auto &d = a.d;
-    a.rank_groups = (int)ceil_div(d.rank, ranks);
-    const int64_t most = d.tokens / tile + d.adapters, units = (most < d.tokens ? most : d.tokens) * a.rank_groups;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((units < room ? units : room) * ctas)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(count * ctas)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -703,32 +920,62 @@ static int launch_down(LowRankArgs &a, void (*kernel)(LowRankArgs), int ranks, i
     count_launch();
     return ORTHO_B200_OK;
 }
-
-template <class T, int MT, int G, bool FEW>
-static int launch_up_as(LowRankArgs &a, cudaStream_t stream)
+template <class T, int MB>
+static int launch_few(LowRankArgs &a, int dev, cudaStream_t stream)
 {
-    using Shape = UpShape<MT, G>;
-    const auto &d = a.d;
-    const int dev = current_device_index();
-    if (dev < 0) return ORTHO_B200_ERR_CUDA;
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
-        OB_CUDA(cudaFuncSetAttribute(up_kernel<T, MT, G, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::bytes(256)));
+        OB_CUDA(cudaFuncSetAttribute(few_kernel<T, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<MB>::bytes(256)));
         attr_set[dev] = true;
     }
-    a.blocks = (int)ceil_div(d.N, Shape::kColumns);
-    const int smem = Shape::bytes(a.padded), fit = 227 * 1024 / (smem + (FEW ? 7 : 2) * 1024);
-    const int64_t most = d.tokens / Shape::kTokens + d.adapters + 1, pairs = (most < d.tokens ? most : d.tokens) * a.blocks;
-    const int64_t room = (fit < 4 ? fit : 4) * (int64_t)device_sm_count(dev);
-    return launch_dependent(up_kernel<T, MT, G, FEW>, dim3((unsigned)(pairs < room ? pairs : room)), kUpThreads, (size_t)smem, stream, a);
-}
-template <class T, int MT, bool FEW>
-static int launch_up(LowRankArgs &a, cudaStream_t stream)
-{
-    return a.padded <= 16 ? launch_up_as<T, MT, 16, FEW>(a, stream) : a.padded <= 32 ? launch_up_as<T, MT, 32, FEW>(a, stream) : launch_up_as<T, MT, 64, FEW>(a, stream);
+    a.blocks = (int)ceil_div(a.d.N, UpShape<1, 16>::kColumns);
+    const int64_t units = most_tiles(a.d, kFewTile) * ceil_div(a.blocks, FewShape<MB>::kCtas), room = 2 * (int64_t)device_sm_count(dev) / FewShape<MB>::kCtas;
+    return launch_clusters(few_kernel<T, MB>, units < room ? units : room, FewShape<MB>::kCtas, (size_t)FewShape<MB>::bytes(a.padded), a, stream);
 }
 
-static constexpr size_t down_bytes(int mb) { return kDownStages * (kManyTile + mb * 16) * 128; }
+template <class T, int MB, bool FEW>
+static int launch_down(LowRankArgs &a, int dev, cudaStream_t stream)
+{
+    a.rank_groups = (int)ceil_div(a.d.rank, MB * 16);
+    const int64_t units = most_tiles(a.d, FEW ? kFewTile : kManyTile) * a.rank_groups, room = 4 * (int64_t)device_sm_count(dev) / kManyCtas;
+    static_assert(kFewCtas == kManyCtas, "clusters of one size");
+    if constexpr (FEW) {
+        return launch_clusters(down_few_kernel<T, MB>, units < room ? units : room, kFewCtas, 0, a, stream);
+    } else {
+        constexpr int smem = kDownStages * (kManyTile + MB * 16) * 128;
+        static bool attr_set[kMaxDevices] = {};
+        if (!attr_set[dev]) {
+            OB_CUDA(cudaFuncSetAttribute(down_many_kernel<T, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            attr_set[dev] = true;
+        }
+        return launch_clusters(down_many_kernel<T, MB>, units < room ? units : room, kManyCtas, smem, a, stream);
+    }
+}
+
+template <class T, int G, bool FEW>
+static int launch_up(LowRankArgs &a, int dev, cudaStream_t stream)
+{
+    constexpr int MT = FEW ? kFewTile / 16 : kManyTile / 16;
+    using Shape = UpShape<MT, G>;
+    auto bytes = [](int padded) { return kUpStages * Shape::kStage + 2 * Shape::kTokens * (padded * 2 + 16); };
+    static bool attr_set[kMaxDevices] = {};
+    if (!attr_set[dev]) {
+        OB_CUDA(cudaFuncSetAttribute(up_kernel<T, MT, G, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(256)));
+        attr_set[dev] = true;
+    }
+    a.blocks = (int)ceil_div(a.d.N, Shape::kColumns);
+    const int smem = bytes(a.padded), fit = 227 * 1024 / (smem + (FEW ? 7 : 2) * 1024);
+    const int64_t pairs = most_tiles(a.d, Shape::kTokens) * a.blocks, room = (fit < 4 ? fit : 4) * (int64_t)device_sm_count(dev);
+    return launch_dependent(up_kernel<T, MT, G, FEW>, dim3((unsigned)(pairs < room ? pairs : room)), kUpThreads, (size_t)smem, stream, a);
+}
+
+template <class T, bool FEW>
+static int launch_two(LowRankArgs &a, int dev, cudaStream_t stream)
+{
+    const int st = a.d.rank <= 16 ? launch_down<T, 1, FEW>(a, dev, stream) : launch_down<T, 2, FEW>(a, dev, stream);
+    if (st) return st;
+    return a.padded <= 16 ? launch_up<T, 16, FEW>(a, dev, stream) : a.padded <= 32 ? launch_up<T, 32, FEW>(a, dev, stream) : launch_up<T, 64, FEW>(a, dev, stream);
+}
 
 template <class T>
 static int launch_low_rank(LowRankArgs &a, cudaStream_t stream)
@@ -736,29 +983,15 @@ static int launch_low_rank(LowRankArgs &a, cudaStream_t stream)
     const auto &d = a.d;
     const int dev = current_device_index();
     if (dev < 0) return ORTHO_B200_ERR_CUDA;
-    const int64_t sms = device_sm_count(dev);
-    int st;
-    if (d.tokens <= kFewTokens) {
-        const int64_t room = 4 * sms / kFewCtas;
-        st = d.rank <= 16 ? launch_down(a, down_few_kernel<T, 1>, 16, kFewTile, kFewCtas, room, 0, stream)
-                          : launch_down(a, down_few_kernel<T, 2>, 32, kFewTile, kFewCtas, room, 0, stream);
-        if (st) return st;
-        return launch_up<T, kFewTile / 16, true>(a, stream);
-    }
+    if (in_one_kernel(d)) return d.rank <= 16 ? launch_few<T, 1>(a, dev, stream) : launch_few<T, 2>(a, dev, stream);
+    if (d.tokens <= kFewTokens) return launch_two<T, true>(a, dev, stream);
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
-        OB_CUDA(cudaFuncSetAttribute(down_many_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_bytes(1)));
-        OB_CUDA(cudaFuncSetAttribute(down_many_kernel<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_bytes(2)));
         OB_CUDA(cudaFuncSetAttribute(group_kernel<kManyTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 4 * (kMostAdapters + 1)));
         attr_set[dev] = true;
     }
-    st = launch_dependent(group_kernel<kManyTile>, dim3(1), kGroupThreads, (size_t)(3 * 4 * (d.adapters + 1)), stream, a);
-    if (st) return st;
-    const int64_t room = 4 * sms / kManyCtas;
-    st = d.rank <= 16 ? launch_down(a, down_many_kernel<T, 1>, 16, kManyTile, kManyCtas, room, down_bytes(1), stream)
-                      : launch_down(a, down_many_kernel<T, 2>, 32, kManyTile, kManyCtas, room, down_bytes(2), stream);
-    if (st) return st;
-    return launch_up<T, kManyTile / 16, false>(a, stream);
+    const int st = launch_dependent(group_kernel<kManyTile>, dim3(1), kGroupThreads, (size_t)(3 * 4 * (d.adapters + 1)), stream, a);
+    return st ? st : launch_two<T, false>(a, dev, stream);
 }
 
 }  // namespace ob
@@ -776,7 +1009,7 @@ extern "C" int ortho_b200_low_rank_add(const ortho_b200_low_rank_desc *d, void *
     int st = check_low_rank(d);
     if (st || d->tokens == 0) return st;
     const LowRankSpace space = low_rank_space(*d);
-    if (!workspace || workspace_bytes < space.bytes || ((uintptr_t)workspace & 255u)) return ORTHO_B200_ERR_WORKSPACE;
+    if (space.bytes && (!workspace || workspace_bytes < space.bytes || ((uintptr_t)workspace & 255u))) return ORTHO_B200_ERR_WORKSPACE;
     st = check_device();
     if (st) return st;
     LowRankArgs a = {};

@@ -94,7 +94,7 @@ def test_paged_attention_refuses(change, want):
 @pytest.mark.parametrize("change,want", [
     ({"type": 2}, SHAPE), ({"tokens": -1}, SHAPE), ({"K": 60}, SHAPE), ({"N": 0}, SHAPE), ({"adapters": 0}, SHAPE), ({"rank": 12}, SHAPE),
     ({"rank": 264}, SHAPE), ({"x": None}, NULL), ({"ids": None}, NULL), ({"x": 258}, ALIGN), ({"up": 264}, ALIGN), ({"x_stride": 60}, ALIGN),
-    ({}, WORKSPACE), ({"tokens": 0, "x": None}, OK)])
+    ({"tokens": 200}, WORKSPACE), ({"tokens": 0, "x": None}, OK)])
 def test_low_rank_add_refuses(change, want):
     assert status("low_rank_add", low_rank(), **change) == want
     assert _lib.lib().ortho_b200_low_rank_add(None, None, 0, None) == NULL

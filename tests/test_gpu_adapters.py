@@ -66,6 +66,17 @@ def test_widths_of_prompts():
         check(*make(200, K, N, 3, 24, BF16, seed=K))
 
 
+@pytest.mark.parametrize("T,E,K,N,R", [(40, 40, 264, 2100, 24), (128, 3, 64, 12000, 8), (90, 60, 520, 3001, 72), (100, 100, 96, 1500, 256), (3, 3, 1024, 26000, 16),
+                                       (17, 17, 4096, 5000, 64)])
+def test_few_tokens_with_much_to_do(T, E, K, N, R):
+    """More tiles and columns than clusters find room for: two kernels instead of one."""
+    for dtype in (F16, BF16):
+        x, y, down, up, ids, scales = make(T, K, N, E, R, dtype, seed=T)
+        check(x, y, down, up, ids, scales, torch.arange(E, device=DEV, dtype=torch.int32) % (R + 3))
+        ids[:] = torch.arange(T, device=DEV) % E
+        check(x, y, down, up, ids)
+
+
 def test_more_adapters_than_tokens_and_the_reverse():
     check(*make(20, 256, 128, 300, 8, F16))
     check(*make(600, 256, 128, 1, 8, F16))
