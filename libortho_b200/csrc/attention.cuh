@@ -34,10 +34,13 @@ struct AttentionArgs {
 
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps, kWarpKeys = 16, kUnitKeys = kWarpKeys * kAttnWarps;
 
-// Probabilities are powers of two of s - max + kLift: in FP16 the largest is then 2^12 and what is 2^-36 of it still has a value
+// Probabilities are powers of two of s - reference + lift.  The reference is the running maximum, but it stays where it is until a score is kSlack above it:
+// the search for the maximum over the lanes and the scaling of what has been summed are then left out in almost every tile, and the result does
+// not depend on the reference.  In FP16 the largest probability is 2^15 and what is 2^-32 of the reference still has a value.
+constexpr float kSlack = 7.f;
 template <class T> struct AttnType;
 template <> struct AttnType<__half> {
-    static constexpr float lift = 12.f, below = 1.f - 1.f / 1024.f;
+    static constexpr float lift = 8.f, below = 1.f - 1.f / 1024.f;
     static __device__ __forceinline__ uint32_t pack_rz(float lo, float hi)
     {
         uint32_t r;
@@ -262,15 +265,16 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
                 const T *const k = (const T *)d.k_cache + head * d.k_head_stride, *const v = (const T *)d.v_cache + head * d.v_head_stride;
                 // a lane's own key's place in the caches; the lanes that copy a row get it from there
-                const int64_t k_mine = page >= 0 ? page * d.k_page_stride + place * d.k_slot_stride : -1;
+                const int64_t k_mine = page >= 0 ? page * d.k_page_stride + place * d.k_slot_stride : 0;
                 const int64_t v_mine = alike || page < 0 ? k_mine : page * d.v_page_stride + place * d.v_slot_stride;
 #pragma unroll
                 for (int i = 0; i < Shape::kChunks / 2; i++) {
                     const int at = i * 32 + lane, row = at / Shape::kChunks, chunk = at % Shape::kChunks;
                     const int64_t k_at = __shfl_sync(0xffffffffu, k_mine, row), v_at = alike ? k_at : __shfl_sync(0xffffffffu, v_mine, row);
-                    const bool on = k_at >= 0 && chunk * 8 < D;
-                    copy16_async(dst + Shape::at(row, chunk), on ? k + k_at + chunk * 8 : k, on);
-                    copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), on ? v + v_at + chunk * 8 : v, on);
+                    const bool on = (ok >> row & 1) && chunk * 8 < D;          // (else zeros; the address is that of the first page)
+                    const int e = chunk * 8 < D ? chunk * 8 : 0;
+                    copy16_async(dst + Shape::at(row, chunk), k + k_at + e, on);
+                    copy16_async(dst + Shape::kHalfTile + Shape::at(row, chunk), v + v_at + e, on);
                 }
                 if (t.queries) {                                               // its queries, a quarter per warp
                     const uint32_t qdst = shared_addr(q_ring + fresh_q * Shape::kQ);
@@ -353,7 +357,6 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                 }
                 // rows (keys) lane / 4 and lane / 4 + 8, columns (queries) 2 (lane % 4) and the next
                 const bool on0 = (ok >> (lane >> 2)) & 1, on1 = (ok >> ((lane >> 2) + 8)) & 1;
-                float now_top[NT][2];
                 bool grows = false;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
@@ -361,12 +364,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                     for (int e = 0; e < 2; e++) {
                         s[t][e] = on0 ? s[t][e] * a.scale_log2 : -INFINITY;
                         s[t][e + 2] = on1 ? s[t][e + 2] * a.scale_log2 : -INFINITY;
-                        float m = fmaxf(s[t][e], s[t][e + 2]);
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        grows = grows || m > top[t][e];
-                        now_top[t][e] = fmaxf(top[t][e], m);
+                        grows = grows || fmaxf(s[t][e], s[t][e + 2]) > top[t][e] + kSlack;
                     }
                 if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -374,8 +372,13 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
                         float keep[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            keep[e] = now_top[t][e] == -INFINITY ? 1.f : exp2_approx(top[t][e] - now_top[t][e]);
-                            top[t][e] = now_top[t][e];
+                            float m = fmaxf(s[t][e], s[t][e + 2]);
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                            m = fmaxf(m, top[t][e]);
+                            keep[e] = m == -INFINITY ? 1.f : exp2_approx(top[t][e] - m);
+                            top[t][e] = m;
                             sum[t][e] *= keep[e];
                         }
 #pragma unroll
