@@ -428,8 +428,7 @@ ORTHO_B200_API int ortho_b200_paged_attention(const ortho_b200_paged_attention_d
 /* Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + scales[e] * up[e] (down[e] x[t]) with
  * e = ids[t]; out[t] = y[t] where ids[t] is not in [0, adapters).  ranks[e] (NULL: all `rank`) is the number of rows of down[e] and
  * columns of up[e] that are used, rounded up to a multiple of 8; scales NULL: 1.  The inner sums are FP32 and stay so (two 16-bit
- * parts in the second product), out is rounded once.  out may be y.  down and up are constants of the layer in the sense stated
- * at ortho_b200_forward.  K a multiple of 8, rank a multiple of 8 up to 256, up to 8192 adapters; x, down and up 16-byte aligned, x_stride a multiple of 8.
+ * parts in the second product), out is rounded once.  out may be y.  K a multiple of 8, rank a multiple of 8 up to 256, up to 8192 adapters; x, down and up 16-byte aligned, x_stride a multiple of 8.
  * workspace: ortho_b200_low_rank_add_workspace_bytes(d) bytes, 256-byte aligned; what it holds before does not matter. */
 typedef struct ortho_b200_low_rank_desc {
     const void *x, *y;                  /* [tokens, K], [tokens, N] */

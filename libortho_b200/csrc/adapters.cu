@@ -10,7 +10,7 @@
 //
 // Up to kFewTokens tokens every CTA groups them for itself, and where there is little to do few_kernel does it all.  Else a kernel computes v
 // (down_few_kernel or down_many_kernel; more tokens are grouped by a kernel in front) and up_kernel the outputs: it starts beside the kernel for v
-// and fetches its first weights (constants of the layer) and rows of y meanwhile.
+// and fetches its first weights and rows of y meanwhile.
 #include "launch.cuh"
 #include "tma.cuh"
 
@@ -26,7 +26,7 @@ struct LowRankArgs {
     int *order;                                  // [tokens] grouped by adapter, those without one last
     int4 *tiles;                                 // {adapter or -1, first place in order, tokens, rank}
     float *v;                                    // [tokens][rank], by place in order
-    int rank_groups;                             // of down_kernel's ranks
+    int rank_groups;                             // groups of ranks that the kernel for v computes apart
     int blocks, padded, up_groups;               // of up_kernel's columns; rank in whole 16; groups of 64 ranks
     bool vectors, copies;                        // rows of y and out in 16-byte pieces; out is not y
 };
@@ -48,20 +48,18 @@ __device__ __forceinline__ int adapter_of(const ortho_b200_low_rank_desc &d, int
 // ---- grouping ----------------------------------------------------------------------------------------------------
 struct FewTokens { int adapter[kFewTokens], order[kFewTokens]; int4 at[kFewTokens], tiles[kFewTokens]; int count[kFewTokens / 32]; };
 
-// by a CTA of kFewTokens threads or more; returns (tiles with an adapter, all tiles)
+// by a CTA of kFewTokens threads; returns (tiles with an adapter, all tiles)
 template <int TILE>
 __device__ __forceinline__ int2 group_few(FewTokens &g, const ortho_b200_low_rank_desc &d)
 {
     const int t = threadIdx.x, T = (int)d.tokens, lane = t & 31, warp = t >> 5;
     int rank = 0;
     const int e = t < T ? adapter_of(d, t, rank) : 0x7FFFFFFF;
-    if (t < kFewTokens) {
-        g.adapter[t] = e;
-        g.at[t] = make_int4(-2, 0, 0, 0);
-    }
+    g.adapter[t] = e;
+    g.at[t] = make_int4(-2, 0, 0, 0);
     __syncthreads();
     int less = 0, before = 0, same = 0;
-    for (int i = 0; i < T && t < T; i += 4) {
+    for (int i = 0; i < T; i += 4) {
         const int4 o = *reinterpret_cast<const int4 *>(g.adapter + i);
         less += (o.x < e) + (o.y < e) + (o.z < e) + (o.w < e);
         same += (o.x == e) + (o.y == e) + (o.z == e) + (o.w == e);
@@ -73,12 +71,12 @@ __device__ __forceinline__ int2 group_few(FewTokens &g, const ortho_b200_low_ran
         if (before % TILE == 0) g.at[place] = make_int4(e < d.adapters ? e : -1, place, min(TILE, same - before), rank);
     }
     __syncthreads();
-    const int4 mine = t < kFewTokens ? g.at[t] : make_int4(-2, 0, 0, 0);
+    const int4 mine = g.at[t];
     const uint32_t leads = __ballot_sync(0xffffffffu, mine.x != -2);
-    if (lane == 0 && t < kFewTokens) g.count[warp] = __popc(leads);
+    if (lane == 0) g.count[warp] = __popc(leads);
     const int real = __syncthreads_count(mine.x >= 0), all = __syncthreads_count(mine.x != -2);
     int at = __popc(leads & ((1u << lane) - 1));
-    for (int w = 0; w < warp && t < kFewTokens; w++) at += g.count[w];
+    for (int w = 0; w < warp; w++) at += g.count[w];
     if (mine.x != -2) g.tiles[at] = mine;
     __syncthreads();
     return make_int2(real, all);
@@ -546,8 +544,8 @@ up_kernel(const __grid_constant__ LowRankArgs a)
     const int padded = a.padded, groups = G < 64 ? 1 : a.up_groups, v_pitch = padded * 2 + 16, N = (int)d.N;
     const int t0 = MT == 1 ? 0 : warp * 16, c0 = MT == 1 ? warp * 32 : 0;      // this warp's first token of the tile and column of the pair
     unsigned char *const upper = smem + S * Shape::kStage, *const lower = upper + TOKENS * v_pitch;
-    // What is read in front of the wait was complete before the kernel for v let this kernel start (it does so behind its own wait), or is a
-    // constant of the layer.
+    // What is read in front of the wait was complete before the kernel for v let this kernel start: it does so behind its own wait.  (From L2: this SM's L1 may
+    // hold older values.)
     griddep_launch();
     FewTokens &few = *reinterpret_cast<FewTokens *>(few_smem);
     int all;
@@ -887,6 +885,9 @@ static int64_t most_tiles(const ortho_b200_low_rank_desc &d, int tile)
 // 2912 -> 1003, rank 8: 6.7, 7.4; 64 tokens over twenty adapters of rank 8 to 64, 8192 -> 10240: 24.5, 18.4 (and two launches of host time).
 static bool in_one_kernel(const ortho_b200_low_rank_desc &d)
 {
+    // (a cluster reads x while another writes: not where out lies in x)
+    const char *const x = static_cast<const char *>(d.x), *const out = static_cast<const char *>(d.out);
+    if (out < x + 2 * ((d.tokens - 1) * d.x_stride + d.K) && x < out + 2 * ((d.tokens - 1) * d.out_stride + d.N)) return false;
     const int64_t units = most_tiles(d, kFewTile) * ceil_div(ceil_div(d.N, UpShape<1, 16>::kColumns), FewShape<1>::kCtas);
     return d.tokens <= kFewTokens && units <= 4 * (int64_t)device_sm_count(current_device_index()) / FewShape<1>::kCtas;
 }

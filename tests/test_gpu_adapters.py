@@ -143,6 +143,22 @@ def test_strides_shapes_streams_and_capture():
     assert torch.equal(got, _C_ops.low_rank_add(x, y, down, up, ids.flip(0), scales=scales))
 
 
+@pytest.mark.parametrize("T", [1, 5, 64, 128, 200])
+def test_one_tensor_as_input_base_and_output(T):
+    """x + up (down x), written over x."""
+    x, _, down, up, ids, scales = make(T, 512, 512, 4, 16, F16, seed=T)
+    for _ in range(5):
+        mine = x.clone()
+        want = _C_ops.low_rank_add(x, x, down, up, ids, scales=scales)
+        assert _C_ops.low_rank_add(mine, mine, down, up, ids, scales=scales, out=mine) is mine and torch.equal(mine, want)
+    # and where the output begins inside x
+    wide = torch.zeros(T, 1200, dtype=F16, device=DEV)
+    wide[:, :512] = x
+    y = torch.randn(T, 512, device=DEV).to(F16)
+    want = _C_ops.low_rank_add(x, y, down, up, ids, scales=scales)
+    assert torch.equal(_C_ops.low_rank_add(wide[:, :512], y, down, up, ids, scales=scales, out=wide[:, 264:776]), want)
+
+
 def test_the_module():
     g = torch.Generator(device=DEV).manual_seed(2)
     r = lambda *s: torch.randn(*s, generator=g, device=DEV) * 0.1             # noqa: E731
