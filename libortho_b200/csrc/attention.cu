@@ -22,7 +22,7 @@ static int check_attention(const ortho_b200_paged_attention_desc *d)
 
 template <int DP, int NT> static void take(AttnPlan &p) { p.dp = DP; p.ctas = AttnShape<DP, NT>::kPerSm; p.cluster = AttnShape<DP, NT>::kClusterPerSm; }
 
-constexpr int64_t kJoinUnits = 4;
+constexpr int64_t kJoinUnits = 10;
 
 AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d)
 {
@@ -46,13 +46,17 @@ AttnPlan plan_attention(const ortho_b200_paged_attention_desc &d)
     const int64_t sms = device_sm_count(current_device_index());
     const int64_t keys = d.window > 0 && d.window < d.width * d.page_size ? d.window : d.width * d.page_size;
     const int64_t units = ceil_div(keys, kUnitKeys), items = d.batch * d.kv_heads * p.groups;       // of one item at most; all items
-    // Items that find room on the GPU as clusters of two to eight CTAs are joined inside these (one launch, no partial sums in memory), unless an
-    // even cut over all CTAs is shorter by more than it takes to join: about as long as kJoinUnits units of one CTA.
-    int64_t cluster = p.cluster * sms / (items < 1 ? 1 : items);
-    cluster = cluster >= 8 ? 8 : cluster >= 4 ? 4 : cluster >= 2 ? 2 : 0;
-    while (cluster > 2 && cluster / 2 >= units) cluster /= 2;
+    // An item to a cluster of one to eight CTAs: one launch, nothing passes through memory, but all wait for the longest item.  Or an even cut of all
+    // units over all CTAs and join_kernel behind, which takes as long as kJoinUnits units of one CTA more.  The host knows the table's width, not
+    // the lengths, so the cut is reckoned with requests of half that on the average.  Measured, clusters / cut, us: 64 + 2 x 8 heads of 128,
+    // 1 request of 1000 / 4000 / 8000 keys 5.4 / 10.5 / 19.3, 9.7 / 13.4 / 16.1; 4 of 1000 / 8000 6.6 / 32.0, 12.0 / 30.8; 32 of 100 / 1000
+    // 6.7 / 25.5, 10.4 / 32.4, of up to 1000 / 4000 log-spread 18.5 / 64, 14.0 / 22.4; 128 of 100 27.6, 23.8.
+    const int64_t room = p.cluster * sms;
+    int64_t cluster = items < 1 ? 0 : room / items;
+    cluster = cluster >= 8 ? 8 : cluster >= 4 ? 4 : cluster >= 2 ? 2 : p.cluster ? 1 : 0;
+    while (cluster > 1 && cluster / 2 >= units) cluster /= 2;
     p.ctas *= (int)sms;
-    if (cluster && ceil_div(units, cluster) > ceil_div(units * items, p.ctas) + kJoinUnits) cluster = 0;
+    if (cluster && ceil_div(items * cluster, room) * (ceil_div(units, cluster) + 2) > units * items / (2 * p.ctas) + kJoinUnits) cluster = 0;
     p.cluster = (int)cluster;
     if (cluster) {
         p.ctas = (int)(items * cluster);

@@ -78,12 +78,16 @@ struct AttnShape {
     static constexpr int kFoldPitch = DP + 4;                                  // 8 queries of a warp in FP32, rows apart by 4 banks: in a stage that is done with
     static_assert(8 * kFoldPitch * 4 <= kStage, "room for 8 queries");
     static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
-    static constexpr int kTwo = 115712, kOne = 232448;                         // room of a CTA with two or one on an SM
-    static constexpr int kStages = bytes(4) <= kTwo ? 4 : bytes(3) <= kTwo ? 3 : bytes(2) <= kTwo ? 2 : bytes(4) <= kOne ? 4 : bytes(3) <= kOne ? 3 : 2;
-    static constexpr int kBytes = bytes(kStages), kPerSm = kBytes <= kTwo ? 2 : 1;
+    // Room of a CTA with three, two or one on an SM.  Three where registers and a ring of two stages allow it, up to 8 queries and head dims up to 112:
+    // a CTA waits for its own chain of steps in every unit, which more warps fill (3 against 2, us: heads of 64, 200 requests of 1000 keys with 4 key-value
+    // heads 46.7, 59.5; of 96 75, 79; of 112, 2 x 32768 keys with 8 heads 50, 62; of 128 53.7, 51.5: two).
+    static constexpr int kThree = 73728, kTwo = 115712, kOne = 232448;
+    static constexpr bool kTriple = NT == 1 && DP <= 112 && bytes(2) <= kThree;
+    static constexpr int kRoom = kTriple ? kThree : bytes(2) <= kTwo ? kTwo : kOne;
+    static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2, kBytes = bytes(kStages), kPerSm = kTriple ? 3 : kBytes <= kTwo ? 2 : 1;
     static constexpr int kMostRanks = 8;                                       // of a cluster; what arrives from them: (max, sum) and a share of the sums
     static constexpr int kArrived = kMostRanks * NT * 8 * 8 + NT * 8 * DP * 4 + kMostRanks * 16, kClusterBytes = (kBytes + 15) / 16 * 16 + kArrived;
-    static constexpr int kClusterPerSm = kClusterBytes <= kTwo ? 2 : kClusterBytes <= kOne ? 1 : 0;
+    static constexpr int kClusterPerSm = kTriple && kClusterBytes <= kThree + 2048 ? 3 : kClusterBytes <= kTwo ? 2 : kClusterBytes <= kOne ? 1 : 0;
     static constexpr bool kKeepQ = NT <= 2;                                    // query operands stay in registers
     static __device__ __forceinline__ uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((kSwap ? chunk ^ (row & 7) : chunk) << 4)); }
 };
