@@ -14,6 +14,10 @@
 // finished there; of one that is cut each CTA leaves its sums in the workspace, and join_kernel, launched behind as a programmatic
 // dependent, adds them in order.  Few items (CLUSTER): a cluster of CTAs has an item and joins its sums through distributed shared memory.
 // Neither uses atomics: the same bits every time.
+// Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 1.07 GB: 163 to 166 = 6.5 TB/s, 170 in long runs at the clock that the power cap leaves;
+// 32 requests of up to 4096 keys, log-spread, 74 MB: 22.8, of which 2.6 pass before the first copy (lengths, place, pages, each from memory) and 4.2
+// with join_kernel; 1 x 1000 keys of 32 heads, 16 MB: 6.2.  Joining cut items in this kernel, by the last CTA to count itself in, took 7 us more than
+// join_kernel (fence, counter, two rounds of reads, one after the other in one CTA).
 #pragma once
 
 #include "launch.cuh"

@@ -3,7 +3,9 @@
 //     pair i < R / 2 of a head:  (a, b) -> (a c - b s, b c + a s),  c = table[p][i], s = table[p][R / 2 + i],  p = positions[axis(i)][t]
 //
 // Every value is read and written once: bound by HBM.  An item is two vectors of VEC values of one head; a thread has one item and walks over the
-// (token, head) pairs of its CTA, queries, keys and values alike.  Cosines and sines of the CTA's tokens pass through shared memory.
+// (token, head) pairs of its CTA, queries, keys and values alike.  Cosines and sines of the CTA's tokens pass through shared memory: in registers
+// they leave too little room for values under way (4096 tokens of 96 heads of 128, 204 MB: 36.9 us = 5.5 TB/s; 40 us with a token a CTA and its angles in
+// registers, 49 to 64 with values loaded ahead there).  64 tokens of 80 heads: 2.7 us, launch and the chain slot, position, angle.
 #include "launch.cuh"
 
 namespace ob {

@@ -98,7 +98,8 @@ class PagedAttentionBlock(nn.Module):
                 positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` [tokens, in_features]: the step's new tokens, request after request, as ``step`` lists them.
         ``positions``: rotary positions where they are not those in the request, [tokens] or [axes, tokens].  Every token sees its
-        request up to itself.  Places behind the step's last token give what an empty attention gives."""
+        request up to itself and reads its keys for itself: meant for decoding and short prompts.  Places behind the step's
+        last token give what an empty attention gives."""
         T, D = x.shape[0], self.head_dim
         qkv = self.qkv(x)
         if self.qkv_adapters is not None and ids is not None:
