@@ -184,6 +184,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         now.unit = rank;
         now.s = span_of(d, now.b);
         now.left = rank < now.s.units;
+        cluster_wait();
     } else {
         __shared__ long long warp_cost[kAttnWarps], first_rest;
         __shared__ int first_b;

@@ -1,5 +1,6 @@
 """The operators around the projections without a GPU: what the C entries and the Python surface refuse before any launch."""
 import ctypes
+from pathlib import Path
 
 import pytest
 import torch
@@ -157,3 +158,13 @@ def test_the_plain_forms_by_hand():
     assert torch.allclose(out[0, 0], (v[1, 0, 0] + v[1, 1, 0] + v[0, 0, 0]).double() / 3) and abs(float(lse[0, 0]) - 1.0986122886681098) < 1e-12
     out, _ = plain_ops.low_rank(torch.ones(1, 8), torch.ones(1, 2), torch.ones(1, 8, 8), torch.ones(1, 2, 8), torch.tensor([0]))
     assert out.tolist() == [[65.0, 65.0]]
+
+
+def test_every_arrival_at_a_cluster_barrier_is_waited_for():
+    """A second arrival before the wait for the first one is undefined, and what is sent between them may meet a CTA that has not started."""
+    sources = Path(_lib.__file__).parent / "csrc"
+    for path in sorted(sources.glob("*.cu*")):
+        if path.name == "tma.cuh":                           # (their definitions)
+            continue
+        text = path.read_text()
+        assert text.count("cluster_arrive()") == text.count("cluster_wait()"), path.name

@@ -96,6 +96,20 @@ def test_a_long_cache():
         check(*make([100000, 33], Hq, Hkv, 64, 256, dtype))
 
 
+def test_ctas_of_a_cluster_that_start_and_end_at_different_times():
+    """Few items of very different lengths, behind a kernel that leaves the CTAs' room bit by bit: the same bits every time."""
+    args = make([1, 3000, 64, 0, 513, 65], 4, 2, 64, 16, F16)
+    want = check(*args)
+    x, y, down, up, ids = (torch.randn(64, 2048, device=DEV, dtype=F16), torch.randn(64, 2048, device=DEV, dtype=F16),
+                           torch.randn(9, 16, 2048, device=DEV, dtype=F16), torch.randn(9, 2048, 16, device=DEV, dtype=F16),
+                           torch.arange(64, device=DEV, dtype=torch.int32) % 9)
+    got = []
+    for _ in range(100):
+        _C_ops.low_rank_add(x, y, down, up, ids)
+        got.append(_C_ops.paged_attention(*args))
+    assert all(torch.equal(g, want) for g in got)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 100, 1000])
 def test_windows(window):
     check(*make([0, 1, 50, 64, 101, 700], 6, 2, 64, 8, F16, seed=window), window=window)
