@@ -366,7 +366,8 @@ ORTHO_B200_API int ortho_b200_sieve(const float *w, const float *h_inv_diag, int
  *   request_of[tokens]        request; -1 behind the last token
  *   counts    [3]             tokens and pages asked for, pages left (0 if too few)
  * `tokens` is the size of the token arrays: more tokens than that get their pages, but no place in the arrays.  The free list
- * is not changed: the next step passes counts + 2 as `available`. */
+ * is not changed: the next step passes counts + 2 as `available`.  lengths may be cached and counts + 2 available (a step in
+ * place, in one CTA); no other output overlaps an input. */
 typedef struct ortho_b200_page_step_desc {
     const int32_t *cached, *fresh;      /* [requests] */
     int32_t *block_table;               /* [requests, width], rows table_stride apart */

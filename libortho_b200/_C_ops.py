@@ -455,7 +455,8 @@ def page_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
     more.  New pages are taken, request after request, from the end of the first ``available[0]`` entries of ``free_pages``
     (the last one first) and written to ``block_table`` [requests, pages] in place; where the pool or the table has no
     room the tokens get slot -1.  ``tokens`` is the size of the token arrays, which list the requests' new tokens one
-    request after the other.  The next step's ``available`` is ``counts[2:]``.  ``out``: a result (or its six tensors) to write into.
+    request after the other.  The next step's ``available`` is ``counts[2:]``.  ``out``: a result (or its six tensors) to write into; its
+    ``lengths`` may be ``cached`` and its ``counts[2:]`` ``available``, a step in place.
     All inputs are int32 tensors on the GPU; nothing is read back by the host."""
     got = _lib.fast().page_step(cached, fresh, block_table, free_pages, available, page_size, tokens, out)
     return got if isinstance(got, PageStep) else PageStep(*got)

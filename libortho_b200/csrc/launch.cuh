@@ -1,6 +1,6 @@
 // Launches of the operators around the projections: every kernel is a programmatic dependent of what precedes it on the stream
-// (it starts beside that kernel's tail and calls griddep_wait() before it touches anything that is not a layer's constant) and lets its
-// own successor start early.
+// (it starts beside that kernel's tail and calls griddep_wait() before it touches memory; one that reads ahead says why it may) and lets its own
+// successor start early, behind its wait or where what it reads is complete before.
 #pragma once
 
 #include "common.cuh"

@@ -81,7 +81,8 @@ page_step_kernel(ortho_b200_page_step_desc d)
             d.starts[b] = as_count(first.tokens);
         }
         __syncthreads();
-        for (unsigned long long p = before.pages + (unsigned long long)blockIdx.x * kPageThreads + tid; p < total.pages;
+        const unsigned long long granted = total.pages < n ? total.pages : n;                     // (none is left for those behind)
+        for (unsigned long long p = before.pages + (unsigned long long)blockIdx.x * kPageThreads + tid; p < granted;
              p += (unsigned long long)gridDim.x * kPageThreads) {
             const int i = last_not_above(pages_at, in_chunk, p);
             const unsigned long long col = have_of[i] + (p - pages_at[i]);
@@ -129,6 +130,10 @@ extern "C" int ortho_b200_page_step(const ortho_b200_page_step_desc *d, void *st
     if (d->tokens && (!d->slots || !d->positions || !d->request_of)) return ORTHO_B200_ERR_NULL;
     const int st = check_device();
     if (st) return st;
-    const int64_t sms = device_sm_count(current_device_index()), want = ceil_div(d->tokens, kPageThreads);
+    // Where this step's lengths take the place of the last one's, or its counts those that `available` lies in, no CTA may write them while another
+    // still reads: one CTA does it all then, whose threads read theirs first.
+    auto meet = [](const int32_t *a, int64_t n, const int32_t *b, int64_t m) { return a < b + m && b < a + n; };
+    const bool in_place = meet(d->lengths, d->requests, d->cached, d->requests) || meet(d->counts, 3, d->available, 1);
+    const int64_t sms = in_place ? 1 : device_sm_count(current_device_index()), want = ceil_div(d->tokens, kPageThreads);
     return launch_dependent(page_step_kernel, dim3((unsigned)(want < 1 ? 1 : want < sms ? want : sms)), kPageThreads, 0, (cudaStream_t)stream, *d);
 }

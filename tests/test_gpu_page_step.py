@@ -91,6 +91,25 @@ def test_strided_tables_reused_outputs_streams_and_capture():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_steps_in_place():
+    """Lengths and counts that are the next step's inputs, more tokens than one CTA has threads and more requests than one chunk."""
+    P, B, T, pages = 8, 700, 3000, 9000
+    rng = random.Random(11)
+    free = list(range(pages))
+    rng.shuffle(free)
+    table, lengths, available = [[-1] * 12 for _ in range(B)], [0] * B, pages
+    dev_table, dev_free = i32(table), i32(free)
+    step = _C_ops.page_step(i32(lengths), i32([0] * B), dev_table, dev_free, i32([available]), P, T)
+    for _ in range(8):
+        fresh = [rng.randint(0, 8) for _ in range(B)]
+        want = plain_ops.page_step(lengths, fresh, table, free, available, P, T)
+        got = _C_ops.page_step(step.lengths, i32(fresh), dev_table, dev_free, step.counts[2:], P, T, out=step)
+        for g, w in zip((*got, dev_table), want):
+            assert g.flatten().tolist() == (sum(w, []) if isinstance(w[0], list) else w)
+        lengths, table, available = want[0], want[6], want[5][2]
+        assert got is step
+
+
 def test_a_pool_over_steps():
     """Prompts, decoding and requests that leave: no page is held twice, and all come back."""
     rng = random.Random(3)
