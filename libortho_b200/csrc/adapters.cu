@@ -396,8 +396,8 @@ struct PowerOfTwo { float down, back; };
 template <class T>
 __device__ __forceinline__ PowerOfTwo bring_near(float top)
 {
-    const uint32_t exponent = __float_as_uint(top) >> 23;                      // top in [2^(exponent - 127), 2^(exponent - 126))
-    if (!std::is_same<T, __half>::value || exponent < 14 || exponent > 253) return {1.f, 1.f};      // (tiny, infinite or NaN as it is)
+    const uint32_t exponent = min(__float_as_uint(top) >> 23, 254u);           // top in [2^(exponent - 127), 2^(exponent - 126)), or infinite
+    if (!std::is_same<T, __half>::value || exponent < 14) return {1.f, 1.f};   // (tiny as it is)
     return {__uint_as_float((267 - exponent) << 23), __uint_as_float((exponent - 13) << 23)};
 }
 template <class T>
@@ -405,7 +405,7 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t &hi, uint32
 {
     hi = Half<T>::pack(a, b);
     const float2 f = Half<T>::unpack(hi);
-    lo = Half<T>::pack(a - f.x, b - f.y);
+    lo = Half<T>::pack(isinf(f.x) ? 0.f : a - f.x, isinf(f.y) ? 0.f : b - f.y);                    // (what is infinite stays so: no infinity minus another)
 }
 __device__ __forceinline__ float largest(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
@@ -865,7 +865,7 @@ static int check_low_rank(const ortho_b200_low_rank_desc *d)
 {
     if (!d) return ORTHO_B200_ERR_NULL;
     if (d->type != ORTHO_B200_TYPE_F16 && d->type != ORTHO_B200_TYPE_BF16) return ORTHO_B200_ERR_SHAPE;
-    if (d->tokens < 0 || d->tokens > 0x7FFFFFFF || d->K < 8 || d->K % 8 || d->K > 0x3FFFFFFF || d->N < 1 || d->N > 0x3FFFFFFF || d->adapters < 1 || d->adapters > kMostAdapters || d->rank < 8 || d->rank % 8 || d->rank > 256)
+    if (d->tokens < 0 || d->tokens > 0x7FFF0000 || d->K < 8 || d->K % 8 || d->K > 0x3FFFFFFF || d->N < 1 || d->N > 0x3FFFFFFF || d->adapters < 1 || d->adapters > kMostAdapters || d->rank < 8 || d->rank % 8 || d->rank > 256)
         return ORTHO_B200_ERR_SHAPE;
     if (d->tokens == 0) return ORTHO_B200_OK;
     if (!d->x || !d->y || !d->out || !d->down || !d->up || !d->ids) return ORTHO_B200_ERR_NULL;

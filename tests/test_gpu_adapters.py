@@ -112,6 +112,22 @@ def test_infinite_and_nan_activations_stay_with_their_token():
         assert torch.equal(got[even], clean[even]) and not torch.isfinite(got[1]).any()
 
 
+def test_inner_values_that_overflow_are_infinite():
+    """1e30 * 1e30 is infinite in FP32 and so is what it is added to, with the sign of `up`."""
+    for T in (12, 150):
+        x, y, down, up, ids, scales = make(T, 128, 100, 2, 16, BF16)
+        ids[:] = torch.arange(T, device=DEV) % 2
+        clean = _C_ops.low_rank_add(x, y, down, up, ids)
+        x[3] = 1e30
+        down[1] = 0
+        down[1, 2] = 1e30
+        up[1, :, 2] = torch.where(torch.arange(100, device=DEV) % 3 == 0, -0.5, 2.0)
+        got = _C_ops.low_rank_add(x, y, down, up, ids)
+        assert torch.equal(got[3].float(), torch.where(torch.arange(100, device=DEV) % 3 == 0, -math.inf, math.inf))
+        even = [t for t in range(T) if t % 2 == 0]
+        assert torch.equal(got[even], clean[even])
+
+
 def test_strides_shapes_streams_and_capture():
     x, y, down, up, ids, scales = make(24, 256, 120, 3, 16, F16)
     want = check(x, y, down, up, ids, scales)
