@@ -168,7 +168,8 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     float2 *const arrived_sums = reinterpret_cast<float2 *>(smem + (Shape::kBytes + 15) / 16 * 16);           // [ranks][rows]
     float4 *const arrived = reinterpret_cast<float4 *>(arrived_sums + Shape::kMostRanks * NT * 8);            // [ranks][this CTA's share]
 
-    if constexpr (CLUSTER) cluster_arrive();     // (waited for before anything is sent: the other CTAs have started then)
+    if constexpr (CLUSTER) cluster_arrive();
+    auto others_started = [&]() { if constexpr (CLUSTER) { __syncwarp(); cluster_wait(); } };         // before anything is sent to them, once the first copies are under way
     griddep_wait();
     griddep_launch();
 
@@ -184,7 +185,6 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         now.unit = rank;
         now.s = span_of(d, now.b);
         now.left = rank < now.s.units;
-        cluster_wait();
     } else {
         __shared__ long long warp_cost[kAttnWarps], first_rest;
         __shared__ int first_b;
@@ -238,6 +238,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         }
     }
     if (now.left <= 0) {                         // (a share of one cost may be that of an item's start alone)
+        others_started();
         if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     } else {
         // What the copies of a unit need.  The page of a lane's key is looked up well ahead of its use, those of the first units together.
@@ -309,6 +310,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
 #pragma unroll
             for (int i = 0; i < S - 1; i++) issue(first[i], i);
         }
+        others_started();
 
         uint32_t q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? KS : 1][2];
         float o[KS][NT][4], top[NT][2], sum[NT][2];
