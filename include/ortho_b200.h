@@ -356,15 +356,16 @@ ORTHO_B200_API int ortho_b200_sieve(const float *w, const float *h_inv_diag, int
  * ------------------------------------------------------------------------------------------- */
 
 /* One step's pages, slots and positions from the requests' lengths.  With c = max(cached, 0) and f = max(fresh, 0) tokens of
- * request b: the pages ceil(c / P) .. ceil((c + f) / P) - 1 of every request are new and are taken, request after request, from
- * the end of the first n = clamp(*available, 0, free_count) entries of free_pages: free_pages[n - 1] first.  They are written to
- * block_table; a page that the pool or the table has no place for is not, and its tokens get slot -1.
+ * request b: the pages ceil(c / P) .. ceil((c + f) / P) - 1 of every request are new.  Those that block_table has a column for (numbers
+ * below width) are taken, request after request, from the end of the first n = clamp(*available, 0, free_count) entries of
+ * free_pages, free_pages[n - 1] first, and written to block_table.  No page is taken for tokens behind the last column; these, and those whose
+ * page the pool does not have, get slot -1.
  *   lengths   [requests]      c + f
  *   starts    [requests + 1]  first token of each request in this step, and their number
  *   slots     [tokens]        slot, or -1 where the token has no page; -1 behind the last token
  *   positions [tokens]        position in the request (from c on, 2^31 - 1 at most); -1 behind the last token
  *   request_of[tokens]        request; -1 behind the last token
- *   counts    [3]             tokens and pages asked for, pages left (0 if too few)
+ *   counts    [3]             tokens, pages asked for (those with a column), pages left (0 if too few)
  * `tokens` is the size of the token arrays: more tokens than that get their pages, but no place in the arrays.  The free list
  * is not changed: the next step passes counts + 2 as `available`.  lengths may be cached and counts + 2 available (a step in
  * place, in one CTA); no other output overlaps an input. */

@@ -1,7 +1,7 @@
 // Pages, slots and positions of a step's new tokens from the requests' lengths: running sums of two small quantities per request
 // (tokens and new pages), then one independent lookup per page and per token.
 //
-//     c, f = cached, fresh;  have = ceil(c / P), want = ceil((c + f) / P)
+//     c, f = cached, fresh;  have = min(ceil(c / P), W), want = min(ceil((c + f) / P), W)   (W: columns of the table)
 //     starts = exclusive sums of f, first = exclusive sums of want - have
 //     block_table[b][have + j] = free[n - 1 - (first[b] + j)];  slot of token t of b = page(c + t - starts[b]) * P + (c + t - starts[b]) % P
 //
@@ -38,7 +38,7 @@ page_step_kernel(ortho_b200_page_step_desc d)
     __shared__ uint32_t cached_of[kPageThreads], have_of[kPageThreads];
     __shared__ PageSums warp_sum[kPageThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t P = (uint32_t)d.page_size;
+    const uint32_t P = (uint32_t)d.page_size, W = d.width < 0xFFFFFFFFll ? (uint32_t)d.width : 0xFFFFFFFFu;
     const unsigned long long share = ((unsigned long long)d.tokens + gridDim.x - 1) / gridDim.x;
     const unsigned long long t0 = share * blockIdx.x, t1 = t0 + share < (unsigned long long)d.tokens ? t0 + share : (unsigned long long)d.tokens;
     griddep_wait();
@@ -55,7 +55,8 @@ page_step_kernel(ortho_b200_page_step_desc d)
             c = (uint32_t)max(d.cached[b], 0);
             f = (uint32_t)max(d.fresh[b], 0);
         }
-        const uint32_t have = c / P + (c % P != 0), all = c + f, want = all / P + (all % P != 0);
+        // (only pages that the table has a column for: one without could not be given back)
+        const uint32_t all = c + f, have = min(c / P + (c % P != 0), W), want = min(all / P + (all % P != 0), W);
         PageSums mine = {f, want - have}, sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -87,14 +88,14 @@ page_step_kernel(ortho_b200_page_step_desc d)
             const int i = last_not_above(pages_at, in_chunk, p);
             const unsigned long long col = have_of[i] + (p - pages_at[i]);
             const int32_t page = new_page(p);
-            if (page >= 0 && col < (unsigned long long)d.width) d.block_table[(b0 + i) * d.table_stride + (int64_t)col] = page;
+            if (page >= 0) d.block_table[(b0 + i) * d.table_stride + (int64_t)col] = page;
         }
         const unsigned long long from = before.tokens > t0 ? before.tokens : t0, to = total.tokens < t1 ? total.tokens : t1;
         for (unsigned long long t = from + tid; t < to; t += kPageThreads) {
             const int i = last_not_above(tokens_at, in_chunk, t);
             const uint32_t pos = cached_of[i] + (uint32_t)(t - tokens_at[i]), col = pos / P;
             int32_t page = -1;
-            if (col < (unsigned long long)d.width)
+            if (col < W)
                 page = col < have_of[i] ? d.block_table[(b0 + i) * d.table_stride + col] : new_page(pages_at[i] + (col - have_of[i]));
             d.slots[t] = page >= 0 ? (int64_t)page * P + pos % P : -1;
             d.positions[t] = (int32_t)min(pos, 0x7FFFFFFFu);

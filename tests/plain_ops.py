@@ -25,11 +25,11 @@ def page_step(cached, fresh, table, free, available, P, T):
     pages = 0
     for b, (c, f) in enumerate(zip(cached, fresh)):
         c, f = max(c, 0), max(f, 0)
-        have, want = -(-c // P), -(-(c + f) // P)
+        have, want = min(-(-c // P), W), min(-(-(c + f) // P), W)
         new = {}
         for col in range(have, want):
             new[col] = free[n - 1 - pages] if pages < n else -1
-            if new[col] >= 0 and col < W:
+            if new[col] >= 0:
                 table[b][col] = new[col]
             pages += 1
         for pos in range(c, min(c + f, c + T - len(slots))):        # (what has a place)

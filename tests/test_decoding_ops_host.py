@@ -168,3 +168,12 @@ def test_every_arrival_at_a_cluster_barrier_is_waited_for():
             continue
         text = path.read_text()
         assert text.count("cluster_arrive()") == text.count("cluster_wait()"), path.name
+
+
+def test_the_plain_page_step_takes_only_pages_that_the_table_holds():
+    """The oracle by hand: a table of two columns of four tokens, then one of three."""
+    got = plain_ops.page_step([8, 0], [8, 1], [[0, 1], [-1, -1]], [2, 3, 4, 5], 4, 4, 9)
+    assert got == ([16, 1], [0, 8, 9], [-1] * 8 + [20], [8, 9, 10, 11, 12, 13, 14, 15, 0], [0] * 8 + [1], [9, 1, 3], [[0, 1], [5, -1]])
+    got = plain_ops.page_step([8], [8], [[0, 1, -1]], [2, 3], 2, 4, 8)
+    assert got[2] == [12, 13, 14, 15, -1, -1, -1, -1] and got[5] == [8, 1, 1] and got[6] == [[0, 1, 3]]
+    assert plain_ops.page_step([2 ** 31 - 1], [5], [[0, 1]], [2, 3], 2, 4, 1)[5] == [5, 0, 2]

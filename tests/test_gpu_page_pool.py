@@ -1,0 +1,47 @@
+"""Pages of a pool over steps that go wrong: no page is lost, none is held twice."""
+import pytest
+import torch
+
+from libortho_b200 import PagePool, _C_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def held(pool):
+    """Pages in the table, and the free ones."""
+    return [p for row in pool.block_table.tolist() for p in row if p >= 0], pool.free_pages.tolist()[:int(pool.available)]
+
+
+@pytest.mark.parametrize("tokens_a_step", [1, 3, 40])
+def test_a_request_past_the_table_loses_no_page(tokens_a_step):
+    """Two columns of four tokens: the request's tokens from the ninth on have no place, and what is free stays so."""
+    pool = PagePool(2, 12, 4, max_pages=2, device=DEV)
+    pool.step(i32([8, 1]), 9)
+    n = 8
+    while n < 48:
+        f = min(tokens_a_step, 48 - n)
+        step = pool.step(i32([f, 0]), f)
+        n += f
+        assert step.slots.tolist() == [-1] * f and step.positions.tolist() == list(range(n - f, n))
+        assert step.counts.tolist() == [f, 0, 9] and pool.lengths.tolist() == [n, 1]
+    used, free = held(pool)
+    assert len(used) == 3 and sorted(used + free) == list(range(12))
+    # the other request still gets a page
+    step = pool.step(i32([0, 7]), 7)
+    assert (step.slots >= 0).all()
+    pool.release(torch.tensor([True, True], device=DEV))
+    used, free = held(pool)
+    assert not used and sorted(free) == list(range(12)) and pool.lengths.tolist() == [0, 0]
+
+
+def test_a_step_that_ends_behind_the_table_takes_what_the_table_holds():
+    """Eight tokens cached, eight more, a table of three columns of four: one page, not two."""
+    table = i32([[3, 5, -1], [-1, -1, -1]])
+    step = _C_ops.page_step(i32([8, 0]), i32([8, 1]), table, i32([0, 1, 2, 4]), i32([4]), 4, 9)
+    assert step.counts.tolist() == [9, 2, 2] and table.tolist() == [[3, 5, 4], [2, -1, -1]]
+    assert step.slots.tolist() == [16, 17, 18, 19, -1, -1, -1, -1, 8]
