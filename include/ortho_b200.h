@@ -358,8 +358,8 @@ ORTHO_B200_API int ortho_b200_sieve(const float *w, const float *h_inv_diag, int
 /* One step's pages, slots and positions from the requests' lengths.  With c = max(cached, 0) and f = max(fresh, 0) tokens of
  * request b: the pages ceil(c / P) .. ceil((c + f) / P) - 1 of every request are new.  Those that block_table has a column for (numbers
  * below width) are taken, request after request, from the end of the first n = clamp(*available, 0, free_count) entries of
- * free_pages, free_pages[n - 1] first, and written to block_table.  No page is taken for tokens behind the last column; these, and those whose
- * page the pool does not have, get slot -1.
+ * free_pages, free_pages[n - 1] first, and written to block_table; a column that gets none is set to -1, whatever it held.  No page is
+ * taken for tokens behind the last column; these, and those whose page the pool does not have, get slot -1.
  *   lengths   [requests]      c + f
  *   starts    [requests + 1]  first token of each request in this step, and their number
  *   slots     [tokens]        slot, or -1 where the token has no page; -1 behind the last token

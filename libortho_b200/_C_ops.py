@@ -454,7 +454,7 @@ def page_step(cached: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tens
     """Pages, slots and positions of a step in which request ``b`` has ``cached[b]`` tokens in the cache and gets ``fresh[b]``
     more.  New pages are taken, request after request, from the end of the first ``available[0]`` entries of ``free_pages``
     (the last one first) and written to ``block_table`` [requests, pages] in place; where the pool or the table has no
-    room the tokens get slot -1, and no page is taken that the table has no column for.  ``tokens`` is the size of the token arrays, which list the requests' new tokens one
+    room the tokens get slot -1, a column that gets no page is set to -1, and no page is taken that the table has no column for.  ``tokens`` is the size of the token arrays, which list the requests' new tokens one
     request after the other.  The next step's ``available`` is ``counts[2:]``.  ``out``: a result (or its six tensors) to write into; its
     ``lengths`` may be ``cached`` and its ``counts[2:]`` ``available``, a step in place.
     All inputs are int32 tensors on the GPU; nothing is read back by the host."""

@@ -3,7 +3,7 @@
 //
 //     c, f = cached, fresh;  have = min(ceil(c / P), W), want = min(ceil((c + f) / P), W)   (W: columns of the table)
 //     starts = exclusive sums of f, first = exclusive sums of want - have
-//     block_table[b][have + j] = free[n - 1 - (first[b] + j)];  slot of token t of b = page(c + t - starts[b]) * P + (c + t - starts[b]) % P
+//     block_table[b][have + j] = free[n - 1 - (first[b] + j)], -1 where none is left;  slot of token t of b = page(c + t - starts[b]) * P + (c + t - starts[b]) % P
 //
 // 16 bytes per request and per token, 8 per page: bound by latency (a load of the lengths, the sums, a load of the page).  Every CTA forms
 // the sums of all requests for itself, a chunk of them at a time in shared memory, and serves its share of the tokens and pages, so
@@ -82,13 +82,12 @@ page_step_kernel(ortho_b200_page_step_desc d)
             d.starts[b] = as_count(first.tokens);
         }
         __syncthreads();
-        const unsigned long long granted = total.pages < n ? total.pages : n;                     // (none is left for those behind)
-        for (unsigned long long p = before.pages + (unsigned long long)blockIdx.x * kPageThreads + tid; p < granted;
+        // a column that gets no page says so: what it held may be another request's by now
+        for (unsigned long long p = before.pages + (unsigned long long)blockIdx.x * kPageThreads + tid; p < total.pages;
              p += (unsigned long long)gridDim.x * kPageThreads) {
             const int i = last_not_above(pages_at, in_chunk, p);
             const unsigned long long col = have_of[i] + (p - pages_at[i]);
-            const int32_t page = new_page(p);
-            if (page >= 0) d.block_table[(b0 + i) * d.table_stride + (int64_t)col] = page;
+            d.block_table[(b0 + i) * d.table_stride + (int64_t)col] = max(new_page(p), -1);
         }
         const unsigned long long from = before.tokens > t0 ? before.tokens : t0, to = total.tokens < t1 ? total.tokens : t1;
         for (unsigned long long t = from + tid; t < to; t += kPageThreads) {

@@ -29,8 +29,7 @@ def page_step(cached, fresh, table, free, available, P, T):
         new = {}
         for col in range(have, want):
             new[col] = free[n - 1 - pages] if pages < n else -1
-            if new[col] >= 0:
-                table[b][col] = new[col]
+            table[b][col] = max(new[col], -1)
             pages += 1
         for pos in range(c, min(c + f, c + T - len(slots))):        # (what has a place)
             col = pos // P

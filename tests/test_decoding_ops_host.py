@@ -177,3 +177,8 @@ def test_the_plain_page_step_takes_only_pages_that_the_table_holds():
     got = plain_ops.page_step([8], [8], [[0, 1, -1]], [2, 3], 2, 4, 8)
     assert got[2] == [12, 13, 14, 15, -1, -1, -1, -1] and got[5] == [8, 1, 1] and got[6] == [[0, 1, 3]]
     assert plain_ops.page_step([2 ** 31 - 1], [5], [[0, 1]], [2, 3], 2, 4, 1)[5] == [5, 0, 2]
+
+
+def test_the_plain_page_step_names_no_page_where_none_is_left():
+    got = plain_ops.page_step([4, 3], [5, 2], [[0, 7, 6], [1, 7, 6]], [5, 4], 1, 4, 7)
+    assert got[6] == [[0, 5, -1], [1, -1, 6]] and got[2] == [20, 21, 22, 23, -1, 7, -1] and got[5] == [7, 3, 0]

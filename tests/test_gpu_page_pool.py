@@ -1,7 +1,8 @@
-"""Pages of a pool over steps that go wrong: no page is lost, none is held twice."""
+"""Pages of a pool over steps that go wrong: no page is lost, none is held twice, no request sees another's."""
 import pytest
 import torch
 
+import plain_ops
 from libortho_b200 import PagePool, _C_ops
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +46,24 @@ def test_a_step_that_ends_behind_the_table_takes_what_the_table_holds():
     step = _C_ops.page_step(i32([8, 0]), i32([8, 1]), table, i32([0, 1, 2, 4]), i32([4]), 4, 9)
     assert step.counts.tolist() == [9, 2, 2] and table.tolist() == [[3, 5, 4], [2, -1, -1]]
     assert step.slots.tolist() == [16, 17, 18, 19, -1, -1, -1, -1, 8]
+
+
+@pytest.mark.parametrize("available", [0, 1])
+def test_a_column_without_a_page_names_no_page(available):
+    """The table's rows held other requests' pages; those of columns that get none may not be taken for this request's."""
+    P, D = 4, 64
+    table = i32([[0, 7, 6], [1, 7, 6]])
+    free = i32([5, 4])
+    step = _C_ops.page_step(i32([4, 3]), i32([5, 2]), table, free, i32([available]), P, 7)
+    granted = 5 if available else -1
+    assert table.tolist() == [[0, granted, -1], [1, -1, 6]]
+    want = plain_ops.page_step([4, 3], [5, 2], [[0, 7, 6], [1, 7, 6]], [5, 4], available, P, 7)
+    assert step.slots.tolist() == want[2] and step.counts.tolist() == want[5] and table.tolist() == want[6]
+    # the step after: nothing is written to page 7 or 6, and nothing is read from there
+    step = _C_ops.page_step(step.lengths, i32([1, 1]), table, free, step.counts[2:], P, 2)
+    assert step.slots.tolist() == [-1, -1]
+    k, v = (torch.randn(8, P, 1, D, device=DEV).half() for _ in range(2))
+    q = torch.randn(2, 1, D, device=DEV).half()
+    before = _C_ops.paged_attention(q, k, v, table, step.lengths)
+    k[6:], v[6:] = 9.0, 9.0
+    assert torch.equal(_C_ops.paged_attention(q, k, v, table, step.lengths), before)
