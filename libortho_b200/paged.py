@@ -33,7 +33,8 @@ class PagePool:
 
     ``step(fresh, tokens)`` takes in ``fresh[b]`` new tokens of every request and returns the ``PageStep`` for all
     layers; ``release(which)`` gives the pages of finished requests back.  Pages that ran out show in ``PageStep.counts``
-    (pages asked for against those left before) and as slots of -1."""
+    (pages asked for against those left before) and as slots of -1.  The pool's tensors stay where they are and change in
+    place, so both may be captured and replayed; a ``PageStep`` is its own and keeps what it says."""
 
     def __init__(self, requests: int, pages: int, page_size: int, max_pages: Optional[int] = None, device=None):
         if requests < 1 or pages < 1 or page_size < 1:
@@ -47,7 +48,7 @@ class PagePool:
 
     def step(self, fresh: torch.Tensor, tokens: int) -> PageStep:
         s = _C.page_step(self.lengths, fresh, self.block_table, self.free_pages, self.available, self.page_size, tokens)
-        self.lengths, self.available = s.lengths, s.counts[2:]
+        torch._foreach_copy_([self.lengths, self.available], [s.lengths, s.counts[2:]])    # (one launch)
         return s
 
     def release(self, which: torch.Tensor) -> None:
@@ -59,10 +60,10 @@ class PagePool:
         # entries that give nothing back aim behind the list
         room = torch.cat((self.free_pages, self.free_pages.new_empty(1)))
         room.scatter_(0, torch.where(mine.flatten(), place, self.free_pages.numel()).long(), pages)
-        self.free_pages = room[:-1]
-        self.available = self.available + count[-1:]
+        self.free_pages.copy_(room[:-1])
+        self.available += count[-1:]
         self.block_table.masked_fill_(which.unsqueeze(1), -1)
-        self.lengths = torch.where(which, 0, self.lengths)
+        self.lengths.masked_fill_(which, 0)
 
 
 class PagedCache:

@@ -1,4 +1,4 @@
-"""Pages of a pool over steps that go wrong: no page is lost, none is held twice, no request sees another's."""
+"""Pages of a pool over steps that go wrong or are replayed: no page is lost, none is held twice, no request sees another's."""
 import pytest
 import torch
 
@@ -67,3 +67,34 @@ def test_a_column_without_a_page_names_no_page(available):
     before = _C_ops.paged_attention(q, k, v, table, step.lengths)
     k[6:], v[6:] = 9.0, 9.0
     assert torch.equal(_C_ops.paged_attention(q, k, v, table, step.lengths), before)
+
+
+def test_a_captured_step_goes_on_at_every_replay():
+    B, pages, P, T = 3, 20, 4, 6
+    eager, pool = (PagePool(B, pages, P, max_pages=6, device=DEV) for _ in range(2))
+    fresh = i32([0, 0, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step = pool.step(fresh, T)
+    for f, gone in (([3, 1, 2], None), ([1, 4, 1], [False, True, False]), ([1, 2, 3], None), ([0, 1, 1], [True, False, True]), ([2, 2, 2], None)):
+        want = eager.step(i32(f), T)
+        fresh.copy_(i32(f))
+        graph.replay()
+        for name, g, w in zip(want._fields, step, want):
+            assert torch.equal(g, w), name
+        for p in (eager, pool):
+            if gone:
+                p.release(torch.tensor(gone, device=DEV))
+        for a, b in ((pool.lengths, eager.lengths), (pool.block_table, eager.block_table), (pool.available, eager.available), (pool.free_pages, eager.free_pages)):
+            assert torch.equal(a, b)
+        used, free = held(pool)
+        assert sorted(used + free) == list(range(pages))
+
+
+def test_an_earlier_step_keeps_what_it_said():
+    pool = PagePool(2, 20, 4, device=DEV)
+    first = pool.step(i32([5, 1]), 6)
+    was = [t.tolist() for t in first]
+    pool.step(i32([1, 1]), 2)
+    pool.release(torch.tensor([True, False], device=DEV))
+    assert [t.tolist() for t in first] == was
