@@ -33,7 +33,9 @@ class PagePool:
 
     ``step(fresh, tokens)`` takes in ``fresh[b]`` new tokens of every request and returns the ``PageStep`` for all
     layers; ``release(which)`` gives the pages of finished requests back.  Pages that ran out show in ``PageStep.counts``
-    (pages asked for against those left before) and as slots of -1.  The pool's tensors stay where they are and change in
+    (pages asked for against those left before) and as slots of -1: such tokens count in the request's length, but their keys are
+    nowhere, then and later, and attention goes on without them.  ``incomplete()`` names the requests that this happened to, or that
+    went past ``max_pages``; release them and bring their tokens again.  The pool's tensors stay where they are and change in
     place, so both may be captured and replayed; a ``PageStep`` is its own and keeps what it says."""
 
     def __init__(self, requests: int, pages: int, page_size: int, max_pages: Optional[int] = None, device=None):
@@ -50,6 +52,13 @@ class PagePool:
         s = _C.page_step(self.lengths, fresh, self.block_table, self.free_pages, self.available, self.page_size, tokens)
         torch._foreach_copy_([self.lengths, self.available], [s.lengths, s.counts[2:]])    # (one launch)
         return s
+
+    def incomplete(self) -> torch.Tensor:
+        """bool [requests]: those of whose tokens some found no page."""
+        columns = self.block_table.shape[1]
+        need = (self.lengths.long().unsqueeze(1) + self.page_size - 1) // self.page_size
+        lacks = (self.block_table < 0) & (torch.arange(columns, device=need.device) < need)
+        return lacks.any(dim=1) | (need[:, 0] > columns)
 
     def release(self, which: torch.Tensor) -> None:
         """``which``: bool [requests].  Their pages go back to the pool, their lengths to zero."""

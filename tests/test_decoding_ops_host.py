@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import plain_ops
-from libortho_b200 import LowRankAdapters, _C_ops, _lib, rotary_table
+from libortho_b200 import LowRankAdapters, PagePool, _C_ops, _lib, rotary_table
 
 OK, NULL, SHAPE, ALIGN, WORKSPACE = 0, 1, 2, 3, 5
 
@@ -182,3 +182,10 @@ def test_the_plain_page_step_takes_only_pages_that_the_table_holds():
 def test_the_plain_page_step_names_no_page_where_none_is_left():
     got = plain_ops.page_step([4, 3], [5, 2], [[0, 7, 6], [1, 7, 6]], [5, 4], 1, 4, 7)
     assert got[6] == [[0, 5, -1], [1, -1, 6]] and got[2] == [20, 21, 22, 23, -1, 7, -1] and got[5] == [7, 3, 0]
+
+
+def test_a_pool_names_requests_that_lack_pages():
+    pool = PagePool(5, 9, 4, max_pages=2, device="cpu")
+    pool.block_table.copy_(torch.tensor([[3, 1], [-1, 2], [4, -1], [5, -1], [6, 7]]))
+    pool.lengths.copy_(torch.tensor([8, 5, 4, 5, 2 ** 31 - 1]))
+    assert pool.incomplete().tolist() == [False, True, False, True, True]

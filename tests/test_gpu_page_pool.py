@@ -98,3 +98,23 @@ def test_an_earlier_step_keeps_what_it_said():
     pool.step(i32([1, 1]), 2)
     pool.release(torch.tensor([True, False], device=DEV))
     assert [t.tolist() for t in first] == was
+
+
+def test_requests_that_lack_pages_are_named():
+    """Five pages of four tokens: the third request's second page is not there, the first one's table ends."""
+    pool = PagePool(4, 5, 4, max_pages=3, device=DEV)
+    assert pool.incomplete().tolist() == [False] * 4
+    pool.step(i32([9, 4, 3, 0]), 16)                         # 3 + 1 + 1 pages: just enough
+    assert pool.incomplete().tolist() == [False] * 4
+    step = pool.step(i32([0, 0, 2, 0]), 2)
+    assert (step.slots >= 0).tolist() == [True, False] and pool.incomplete().tolist() == [False, False, True, False]
+    pool.release(torch.tensor([False, True, False, False], device=DEV))
+    step = pool.step(i32([0, 0, 1, 0]), 1)                   # a page is free again, but it is not the one that the fifth token lacks
+    assert step.slots.tolist() == [-1] and pool.incomplete().tolist() == [False, False, True, False]
+    pool.release(torch.tensor([False, False, True, False], device=DEV))
+    pool.step(i32([3, 0, 6, 0]), 9)
+    assert pool.incomplete().tolist() == [False] * 4
+    pool.step(i32([1, 0, 0, 0]), 1)
+    assert pool.incomplete().tolist() == [True, False, False, False]
+    pool.release(torch.tensor([True, False, False, False], device=DEV))
+    assert pool.incomplete().tolist() == [False] * 4
