@@ -387,7 +387,8 @@ ORTHO_B200_API int ortho_b200_page_step(const ortho_b200_page_step_desc *d, void
  * section_ends[0] turn with axis 0, those below section_ends[1] with axis 1, and so on (section_ends[axes - 1] = rotary / 2).  A
  * position outside the table turns nothing.  Computed in FP32, rounded once; the other elements and the values are copied.
  * q and q_out may be NULL together (keys and values alone); rotary = 0 turns nothing and then neither table nor positions are
- * read.  q_out may be q.  A token whose slot lies outside the cache is not written to it.  Two tokens with one slot: either.
+ * read.  q_out may be q.  A token whose slot lies outside the cache is not written to it (pages = 0: none
+ * is, and the caches may be NULL).  Two tokens with one slot: either.
  * head_dim up to 8192; any alignment. */
 #define ORTHO_B200_MAX_AXES 4
 typedef struct ortho_b200_rotary_append_desc {

@@ -208,7 +208,7 @@ extern "C" int ortho_b200_rotary_append(const ortho_b200_rotary_append_desc *d, 
             if (d->section_ends[i] < (i ? d->section_ends[i - 1] : 0)) return ORTHO_B200_ERR_SHAPE;
     }
     if (d->tokens == 0) return ORTHO_B200_OK;
-    if (!d->k || !d->v || !d->k_cache || !d->v_cache || !d->slots || (d->q_heads && (!d->q || !d->q_out))) return ORTHO_B200_ERR_NULL;
+    if (!d->k || !d->v || !d->slots || (d->pages && (!d->k_cache || !d->v_cache)) || (d->q_heads && (!d->q || !d->q_out))) return ORTHO_B200_ERR_NULL;
     if (d->rotary && (!d->positions || (d->table_rows && !d->table))) return ORTHO_B200_ERR_NULL;
     const int st = check_device();
     if (st) return st;

@@ -189,3 +189,9 @@ def test_a_pool_names_requests_that_lack_pages():
     pool.block_table.copy_(torch.tensor([[3, 1], [-1, 2], [4, -1], [5, -1], [6, 7]]))
     pool.lengths.copy_(torch.tensor([8, 5, 4, 5, 2 ** 31 - 1]))
     assert pool.incomplete().tolist() == [False, True, False, True, True]
+
+
+def test_rotary_append_needs_caches_only_where_there_are_pages():
+    for k_cache, v_cache in ((None, 256), (256, None), (None, None)):
+        assert status("rotary_append", rotary(), k_cache=k_cache, v_cache=v_cache) == NULL
+        assert status("rotary_append", rotary(), k_cache=k_cache, v_cache=v_cache, pages=0, tokens=0) == OK

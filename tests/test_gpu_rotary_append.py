@@ -188,3 +188,14 @@ def test_refusals():
     refused(ValueError, "out", out=q[:3])
     refused(ValueError, "out is for q", q=None, out=q)
     refused(TypeError, "v must be a tensor", v=None)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_cache_without_pages_keeps_nothing_and_queries_are_turned(interleaved):
+    for T, D in ((1, 64), (12, 64), (5, 20)):
+        q, k, v, caches, slots = make(T, 4, 2, D, 4, 8, F16)
+        table, positions = rotary_table(64, D, device=DEV), torch.arange(T, dtype=torch.int32, device=DEV) * 3
+        want = _C_ops.rotary_append(q, k, v, *(c.clone() for c in caches), slots, positions, table, interleaved=interleaved)
+        got = _C_ops.rotary_append(q, k, v, caches[0][:0], caches[1][:0], slots, positions, table, interleaved=interleaved)
+        assert torch.equal(got, want)
+        assert _C_ops.rotary_append(None, k, v, caches[0][:0], caches[1][:0], slots, positions, table) is None
