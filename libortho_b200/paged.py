@@ -104,6 +104,13 @@ class PagedAttentionBlock(nn.Module):
         self.sections, self.interleaved, self.window = sections, interleaved, window
         self.register_buffer("table", table, persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        table = self.table
+        out = super()._apply(fn, recurse)
+        if self.table.dtype != table.dtype:        # .half() and the like are for weights: angles of late positions do not fit 16 bits
+            self.table = table.to(self.table.device)
+        return out
+
     def forward(self, x: torch.Tensor, cache: PagedCache, pool: PagePool, step: PageStep, ids: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` [tokens, in_features]: the step's new tokens, request after request, as ``step`` lists them.

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import plain_ops
-from libortho_b200 import LowRankAdapters, PagePool, _C_ops, _lib, rotary_table
+from libortho_b200 import LowRankAdapters, OrthoLinear, PagedAttentionBlock, PagePool, _C_ops, _lib, rotary_table
 
 OK, NULL, SHAPE, ALIGN, WORKSPACE = 0, 1, 2, 3, 5
 
@@ -195,3 +195,10 @@ def test_rotary_append_needs_caches_only_where_there_are_pages():
     for k_cache, v_cache in ((None, 256), (256, None), (None, None)):
         assert status("rotary_append", rotary(), k_cache=k_cache, v_cache=v_cache) == NULL
         assert status("rotary_append", rotary(), k_cache=k_cache, v_cache=v_cache, pages=0, tokens=0) == OK
+
+
+def test_a_block_keeps_its_angles_in_32_bits():
+    table = rotary_table(5000, 16)
+    for convert in (lambda m: m.half(), lambda m: m.bfloat16().float(), lambda m: m.to(torch.float64), lambda m: m.half().float()):
+        block = convert(PagedAttentionBlock(OrthoLinear(64, 64), OrthoLinear(32, 64), 2, 1, table))
+        assert block.table.dtype == torch.float32 and torch.equal(block.table, table)

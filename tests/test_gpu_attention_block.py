@@ -68,3 +68,20 @@ def test_steps_against_dense_attention(dtype):
         # six roundings to 16 bits on the way (activations of the projections to FP16 as well), each relative to values of the outputs' size
         off = (got[:sum(fresh)].double() - want).norm() / want.norm()
         assert off <= 6 * plain_ops.U[dtype], float(off)
+
+
+def test_a_block_that_is_converted_turns_by_the_same_angles():
+    """``half()`` and the like are for weights; angles of late positions do not fit 16 bits."""
+    width, Hq, Hkv, D, P = 256, 4, 2, 64, 8
+    qkv = wl.make_layer(width, (Hq + 2 * Hkv) * D, 0.01, seed=1, device=DEV).to_module()
+    proj = wl.make_layer(Hq * D, width, 0.01, seed=2, device=DEV).to_module()
+    table = rotary_table(4096, D, device=DEV)
+    x = torch.randn(9, width, device=DEV).half()
+
+    def step(block):
+        pool, cache = PagePool(2, 40, P, device=DEV), PagedCache(40, P, Hkv, D, device=DEV)
+        s = pool.step(torch.tensor([7, 2], dtype=torch.int32, device=DEV), 9)
+        return block(x, cache, pool, s, positions=s.positions + 4000)
+    want = step(PagedAttentionBlock(qkv, proj, Hq, Hkv, table))
+    got = step(PagedAttentionBlock(qkv, proj, Hq, Hkv, table).half())
+    assert torch.equal(got, want)
