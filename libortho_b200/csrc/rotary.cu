@@ -130,17 +130,12 @@ rotary_append_kernel(const __grid_constant__ RotaryArgs a)
                 if (turns && !is_value) {
                     float x0[VEC], x1[VEC], c[VEC], s[VEC];
                     const float *const at = angles + token * R + it * VEC;
-                    if constexpr (VEC > 1) {
-                        if (half % 4 == 0) {
+                    if constexpr (VEC > 1) {               // (half is a multiple of VEC)
 #pragma unroll
-                            for (int i = 0; i < VEC; i += 4) {
-                                const float4 x = *reinterpret_cast<const float4 *>(at + i), y = *reinterpret_cast<const float4 *>(at + half + i);
-                                c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
-                                s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < VEC; i++) { c[i] = at[i]; s[i] = at[half + i]; }
+                        for (int i = 0; i < VEC; i += 4) {
+                            const float4 x = *reinterpret_cast<const float4 *>(at + i), y = *reinterpret_cast<const float4 *>(at + half + i);
+                            c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+                            s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
                         }
                     } else { c[0] = at[0]; s[0] = at[half]; }
                     r0[u].template to<T>(x0);
