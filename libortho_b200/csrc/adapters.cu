@@ -22,7 +22,7 @@
 
 namespace ob {
 
-constexpr int kFewTokens = 128, kMostAdapters = 8192, kGroupThreads = 1024;
+constexpr int kFewTokens = 128, kFewRank = 64, kMostAdapters = 8192, kGroupThreads = 1024;       // kFewRank: few_kernel's highest
 
 struct LowRankArgs {
     ortho_b200_low_rank_desc d;
@@ -883,17 +883,24 @@ static int64_t most_tiles(const ortho_b200_low_rank_desc &d, int tile)
     return most < d.tokens ? most : d.tokens;
 }
 
-// Up to kFewTokens tokens both products run in one kernel where every tile finds room at once as a cluster for each eight blocks of columns (or two, one
-// after the other): one launch and no exchange through memory.  Where there is more to do, the two kernels use the GPU more evenly and the second
-// one's weights come while the first runs.  Measured, both ways: 1 token, 4096 -> 12288, rank 16: 4.7 us in one kernel, 5.0 in two; 77 tokens,
-// 2912 -> 1003, rank 8: 6.7, 7.4; 64 tokens over twenty adapters of rank 8 to 64, 8192 -> 10240: 24.5, 18.4 (and two launches of host time).
+// Up to kFewTokens tokens both products run in one kernel (one launch, no exchange through memory) where it is not the slower way.  A unit is a tile and eight blocks
+// of columns, the work of a cluster, of which the GPU holds some 32 at once.  Every cluster computes v of its tile for itself, 32 ranks a round that ends with an
+// exchange: several clusters of a tile (wide) do that over again, and two kernels split ranks and columns over the whole GPU.  Tiles are reckoned as one per
+// adapter that can be in use.  Measured, one kernel / two, GPU us, first K = 4096 then 14336:
+//   wide,   1 token, 12288 columns (12 units): rank 16 4.7 / 5.0, 7.2 / 7.4;  32 5.5 / 5.6, 9.0 / 8.7;  48 8.0 / 6.1;  256 23.4 / 9.8
+//   wide,   24 units: rank 16 5.2 / 5.1, 8.0 / 7.6;  32 6.2 / 5.6, 10.7 / 9.0;  48 9.2 / 6.2.   32 units: rank 16 6.4 / 5.2;  32 8.7 / 5.8.   48: rank 16 9.9 / 5.6
+//   narrow, 1 unit: rank 16 4.7 / 5.1;  32 5.5 / 5.7, 8.9 / 8.8;  48 7.9 / 6.3;  256 22.9 / 9.1.   16 units: rank 32 6.5 / 7.0;  48 9.4 / 7.9
+//   narrow, 28 units: rank 16 5.8 / 7.0;  32 7.0 / 7.7;  48 10.0 / 12.2;  64 10.3 / 12.4;  128 17.8 / 17.8;  256 49.8 / 29.3.   36 units: rank 16 10.2 / 7.3
 static bool in_one_kernel(const ortho_b200_low_rank_desc &d)
 {
     // (a cluster reads x while another writes: not where out lies in x)
     const char *const x = static_cast<const char *>(d.x), *const out = static_cast<const char *>(d.out);
     if (out < x + 2 * ((d.tokens - 1) * d.x_stride + d.K) && x < out + 2 * ((d.tokens - 1) * d.out_stride + d.N)) return false;
-    const int64_t units = most_tiles(d, kFewTile) * ceil_div(ceil_div(d.N, UpShape<1, 16>::kColumns), FewShape<1>::kCtas);
-    return d.tokens <= kFewTokens && units <= 4 * (int64_t)device_sm_count(current_device_index()) / FewShape<1>::kCtas;
+    if (d.tokens > kFewTokens || d.rank > kFewRank) return false;
+    const int64_t sms = device_sm_count(current_device_index()), clusters = ceil_div(ceil_div(d.N, UpShape<1, 16>::kColumns), FewShape<1>::kCtas);
+    const int64_t in_use = d.tokens < d.adapters ? d.tokens : d.adapters, full = ceil_div(d.tokens, kFewTile), units = (in_use > full ? in_use : full) * clusters;
+    if (clusters > 1) return units <= sms / (d.rank <= 16 ? 6 : 12) && d.rank <= 32;
+    return units <= 2 * sms / 9 && (d.rank <= 32 || units >= sms / 6);
 }
 
 static LowRankSpace low_rank_space(const ortho_b200_low_rank_desc &d)
@@ -930,7 +937,7 @@ static int launch_few(LowRankArgs &a, int dev, cudaStream_t stream)
 {
     static bool attr_set[kMaxDevices] = {};
     if (!attr_set[dev]) {
-        OB_CUDA(cudaFuncSetAttribute(few_kernel<T, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<MB>::bytes(256)));
+        OB_CUDA(cudaFuncSetAttribute(few_kernel<T, MB>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<MB>::bytes(kFewRank)));
         attr_set[dev] = true;
     }
     a.blocks = (int)ceil_div(a.d.N, UpShape<1, 16>::kColumns);

@@ -226,3 +226,18 @@ def test_refusals():
     refused(ValueError, "out", out=y[:4])
     refused(ValueError, "out", out=torch.zeros(40, 5, dtype=F16, device=DEV).T)
     refused(TypeError, "up must be a tensor", up=None)
+
+
+@pytest.mark.parametrize("T,K,N,E,R,kernels", [
+    (1, 4096, 12288, 8, 16, 1), (1, 4096, 12288, 8, 32, 1), (1, 4096, 12288, 8, 40, 2), (1, 4096, 1000, 8, 48, 2), (1, 512, 1000, 8, 256, 2),
+    (4, 4096, 4096, 32, 16, 1), (4, 4096, 4096, 32, 24, 2), (4, 4096, 12288, 32, 16, 2), (16, 1024, 2048, 16, 8, 2), (16, 1024, 1000, 16, 32, 1),
+    (77, 2912, 1003, 12, 8, 1), (28, 264, 1000, 28, 48, 1), (32, 264, 900, 40, 64, 1), (28, 264, 1000, 28, 72, 2), (36, 264, 1000, 36, 16, 2), (128, 264, 1000, 30, 24, 1)])
+def test_one_kernel_where_two_are_not_faster(T, K, N, E, R, kernels):
+    """Several rounds of 32 ranks, columns over several clusters, more tiles than clusters find room for: measured beside the rule."""
+    x, y, down, up, ids, scales = make(T, K, N, E, R, BF16 if R % 16 else F16, seed=T + R)
+    check(x, y, down, up, ids, scales, torch.arange(E, device=DEV, dtype=torch.int32) % (R + 3))
+    ids[:] = torch.arange(T, device=DEV) % E
+    check(x, y, down, up, ids)
+    before = _lib.lib().ortho_b200_launch_count()
+    _C_ops.low_rank_add(x, y, down, up, ids)
+    assert _lib.lib().ortho_b200_launch_count() - before == kernels
