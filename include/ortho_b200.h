@@ -411,7 +411,7 @@ ORTHO_B200_API int ortho_b200_rotary_append(const ortho_b200_rotary_append_desc 
  * the tokens of a prompt with their own lengths.  Query head h reads KV head h / (q_heads / kv_heads).  A row without
  * keys (length 0, a table row out of range) gives 0 and -inf; a key on a page outside the cache is left out.  What lies behind a
  * length, NaN too, has no effect.  Scores, softmax and sums are FP32; the probabilities enter the matrix products as two 16-bit
- * parts.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned, strides of q and caches multiples of 8.
+ * parts, which hold them to 2^-14 (BF16) or 2^-20 (FP16).  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned, strides of q and caches multiples of 8.
  * workspace: ortho_b200_paged_attention_workspace_bytes(d) bytes, 256-byte aligned (partial sums of requests that are split over CTAs;
  * what it holds before does not matter). */
 typedef struct ortho_b200_paged_attention_desc {
@@ -430,8 +430,8 @@ ORTHO_B200_API int ortho_b200_paged_attention(const ortho_b200_paged_attention_d
 
 /* Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + scales[e] * up[e] (down[e] x[t]) with
  * e = ids[t]; out[t] = y[t] where ids[t] is not in [0, adapters).  ranks[e] (NULL: all `rank`) is the number of rows of down[e] and
- * columns of up[e] that are used, rounded up to a multiple of 8; scales NULL: 1.  The inner sums are FP32 and stay so (two 16-bit
- * parts in the second product), out is rounded once.  out may be y.  K a multiple of 8, rank a multiple of 8 up to 256, up to 8192 adapters; x, down and up 16-byte aligned, x_stride a multiple of 8.
+ * columns of up[e] that are used, rounded up to a multiple of 8; scales NULL: 1.  Both sums are FP32; the second product takes the inner
+ * one's results as two 16-bit parts, which hold them to 2^-16 (BF16) or 2^-22 (FP16); out is rounded once.  out may be y.  K a multiple of 8, rank a multiple of 8 up to 256, up to 8192 adapters; x, down and up 16-byte aligned, x_stride a multiple of 8.
  * workspace: ortho_b200_low_rank_add_workspace_bytes(d) bytes, 256-byte aligned; what it holds before does not matter. */
 typedef struct ortho_b200_low_rank_desc {
     const void *x, *y;                  /* [tokens, K], [tokens, N] */

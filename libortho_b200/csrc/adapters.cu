@@ -12,7 +12,8 @@
 // (down_few_kernel or down_many_kernel; more tokens are grouped by a kernel in front) and up_kernel the outputs: it starts beside the kernel for v
 // and fetches its first weights and rows of y meanwhile.
 //
-// Measured (GPU time, us): 1 token, 4096 -> 12288, rank 16: 4.6; 64 tokens over twenty adapters of rank 8 to 64, 8192 -> 10240, 26 MB: 18.5; 4096 tokens,
+// Measured (GPU time, us): 1 token, 4096 -> 12288, rank 16: 4.7; 64 tokens over twenty adapters of rank 8 to 64, 8192 -> 10240, 26 MB: 18.9 (38 MB are read: a
+// column's row of `up` has the highest rank's 128 bytes, of which an adapter of rank 8 uses 16 and memory delivers more); 4096 tokens,
 // six adapters of rank 32, 4096 -> 12288, 241 MB: 65, of which grouping 5, v 9, outputs 49 (4.1 TB/s: no pipe is full, the chain of barrier, operands,
 // products and results of 16 warps an SM).
 #include "launch.cuh"
@@ -390,8 +391,9 @@ down_many_kernel(const __grid_constant__ LowRankArgs a)
 }
 
 // ---- out = y + scale up v -------------------------------------------------------------------------------------------
-// The products run over v in two 16-bit parts, so that it keeps what FP32 has of it.  In FP16 it is brought to the token's largest |v| in
-// [2^13, 2^14) by a power of two first (else it could leave FP16's range, or lose its small values): `down`, and `back` for the result.
+// The products run over v in two 16-bit parts, which hold a value to 2^-16 of it in BF16 and 2^-22 in FP16 (one part alone would add an error as large as
+// the output's own rounding, up to 2^-8 and 2^-11).  In FP16 it is brought to the token's largest |v| in [2^13, 2^14) by a power of two first (else it
+// could leave FP16's range, or lose its small values; what is left of these is off by 2^-38 of the largest): `down`, and `back` for the result.
 struct PowerOfTwo { float down, back; };
 template <class T>
 __device__ __forceinline__ PowerOfTwo bring_near(float top)

@@ -29,7 +29,8 @@ def rotary_table(positions: int, rotary_dim: int, base: float = 10000.0, device=
 
 
 class PagePool:
-    """Block table and free pages of up to ``requests`` requests, on the GPU; no call waits for it.
+    """Block table and free pages of up to ``requests`` requests, on the GPU; no call waits for it.  A request has at most ``max_pages`` pages
+    (all, if not given); attention goes by that number when it divides its work, so it should be what the longest request needs.
 
     ``step(fresh, tokens)`` takes in ``fresh[b]`` new tokens of every request and returns the ``PageStep`` for all
     layers; ``release(which)`` gives the pages of finished requests back.  Pages that ran out show in ``PageStep.counts``
