@@ -85,3 +85,26 @@ def test_a_block_that_is_converted_turns_by_the_same_angles():
     want = step(PagedAttentionBlock(qkv, proj, Hq, Hkv, table))
     got = step(PagedAttentionBlock(qkv, proj, Hq, Hkv, table).half())
     assert torch.equal(got, want)
+
+
+def test_a_captured_step_through_the_block():
+    """Step and block in one graph, replayed for token after token: what the same steps give one by one."""
+    width, Hq, Hkv, D, P, B = 256, 4, 2, 64, 8, 3
+    qkv = wl.make_layer(width, (Hq + 2 * Hkv) * D, 0.01, seed=1, device=DEV).to_module()
+    proj = wl.make_layer(Hq * D, width, 0.01, seed=2, device=DEV).to_module()
+    block = PagedAttentionBlock(qkv, proj, Hq, Hkv, rotary_table(128, D, device=DEV))
+    g = torch.Generator(device=DEV).manual_seed(5)
+    tokens = torch.randn(12, B, width, generator=g, device=DEV).half()
+    fresh = torch.ones(B, dtype=torch.int32, device=DEV)
+    pools, caches = zip(*((PagePool(B, 20, P, max_pages=4, device=DEV), PagedCache(20, P, Hkv, D, device=DEV)) for _ in range(2)))
+    want = [block(x, caches[0], pools[0], pools[0].step(fresh, B)) for x in tokens]
+    first = [block(x, caches[1], pools[1], pools[1].step(fresh, B)) for x in tokens[:2]]
+    x, graph = tokens[2].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = block(x, caches[1], pools[1], pools[1].step(fresh, B))
+    for i, one in enumerate(want):
+        if i >= 2:
+            x.copy_(tokens[i])
+            graph.replay()
+        assert torch.equal(first[i] if i < 2 else got, one)
+    assert torch.equal(caches[1].k, caches[0].k) and torch.equal(caches[1].v, caches[0].v) and pools[1].lengths.tolist() == [12] * B
