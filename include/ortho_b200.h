@@ -428,6 +428,44 @@ typedef struct ortho_b200_paged_attention_desc {
 ORTHO_B200_API int64_t ortho_b200_paged_attention_workspace_bytes(const ortho_b200_paged_attention_desc *d);
 ORTHO_B200_API int ortho_b200_paged_attention(const ortho_b200_paged_attention_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* A paged cache held in 4 bits.  The elements of a head are `groups` groups, each a whole head (groups = 1) or 64 elements (groups = head_dim / 64);
+ * a token's group is held as 4-bit codes and a pair (scale, zero) of the model's type, and stands for zero + scale * code.  Codes: two a byte,
+ * the even element in the low half; head h of the token at place o of page p starts p * page_stride + o * slot_stride + h * head_stride bytes
+ * behind the base.  Scales: [groups][2], at strides that count pairs.  Base and strides of the codes are multiples of 4 bytes
+ * (multiples of 16, with head_dim a multiple of 32, are faster), the scales' base is too.  head_dim: a multiple of 8 up to 256. */
+typedef struct ortho_b200_quantised_cache {
+    void *k, *v;                        /* codes */
+    void *k_scales, *v_scales;
+    int64_t pages, page_size, kv_heads, head_dim, groups;
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int64_t ks_page_stride, ks_slot_stride, ks_head_stride, vs_page_stride, vs_slot_stride, vs_head_stride;
+} ortho_b200_quantised_cache;
+
+/* ortho_b200_rotary_append into a cache held in 4 bits; the record's fields of a cache are not read.  A key is turned, a key or value x of a group
+ * quantised: zero = min x and scale = (max x - min x) / 15, each rounded to the type, code = clamp(rint((x - zero) / scale), 0, 15), ties to even, and
+ * 0 where the scale is 0; all of it as in exact arithmetic on the turned key (the codes do not depend on how FP32 rounds).  Where zero + 15 scale would
+ * round to infinity the scale is the next smaller number of the type.  A group with a value that is not finite, or whose zero is not in
+ * the type, gets the scale NaN: it stands for NaN.  Values below FP32's normal numbers count as zero.  rotary: a multiple of 8; q, k and v
+ * 8-byte aligned with strides that are multiples of 4. */
+ORTHO_B200_API int ortho_b200_rotary_append_quantised(const ortho_b200_rotary_append_desc *d, const ortho_b200_quantised_cache *cache, void *stream);
+
+/* What a cache held in 4 bits stands for, in the model's type, rounded once: token i of the outputs is the cache's token at slots[i], zeros where that
+ * lies outside the cache.  k_out and v_out [count, kv_heads, head_dim] 16-byte aligned, strides multiples of 8. */
+typedef struct ortho_b200_read_quantised_desc {
+    const int64_t *slots;               /* [count] */
+    void *k_out, *v_out;
+    int64_t count, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int32_t type, reserved;
+} ortho_b200_read_quantised_desc;
+ORTHO_B200_API int ortho_b200_read_quantised(const ortho_b200_read_quantised_desc *d, const ortho_b200_quantised_cache *cache, void *stream);
+
+/* ortho_b200_paged_attention over a cache held in 4 bits; the record's fields of a cache (k_cache to head_dim's, pages, strides) are not read but kv_heads
+ * and head_dim, which are the cache's.  Codes enter the matrix products as the whole numbers they are, scales and zeros in FP32; a probability times a
+ * scale enters as two FP16 parts, which hold it to 2^-21, a query in FP16 that was brought into range by a power of two.  Scales are not negative. */
+ORTHO_B200_API int64_t ortho_b200_paged_attention_quantised_workspace_bytes(const ortho_b200_paged_attention_desc *d, const ortho_b200_quantised_cache *cache);
+ORTHO_B200_API int ortho_b200_paged_attention_quantised(const ortho_b200_paged_attention_desc *d, const ortho_b200_quantised_cache *cache,
+                                                        void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + scales[e] * up[e] (down[e] x[t]) with
  * e = ids[t]; out[t] = y[t] where ids[t] is not in [0, adapters).  ranks[e] (NULL: all `rank`) is the number of rows of down[e] and
  * columns of up[e] that are used, rounded up to a multiple of 8; scales NULL: 1.  Both sums are FP32; the second product takes the inner

@@ -10,7 +10,7 @@ stream, and any failure raises instead of being dropped.
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple, Optional, Sequence
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -489,6 +489,38 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``head_dim ** -0.5``.  A row without keys gives zeros.  ``lse`` (float32 [batch, q_heads], written): logarithm of the sum of the exponentials, by which
     results over parts of a cache are joined.  head_dim: a multiple of 8 up to 256."""
     return _lib.fast().paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window, rows, out, lse)
+
+
+# A paged cache held in 4 bits: ``k_cache`` / ``v_cache`` uint8 [pages, page_size, kv_heads, head_dim / 2] (two codes a byte, the even element in
+# the low half), ``k_scales`` / ``v_scales`` [pages, page_size, kv_heads, groups, 2] of the model's type (a scale and a zero for each group of a token: a whole head, or
+# 64 elements of one).  An element is ``zero + scale * code``.  Any strides but those of the codes' last dimension and the scales' last two; a page that lies head
+# by head (``QuantisedCache``) is read fastest.  head_dim: a multiple of 8 up to 256.
+
+def rotary_append_quantised(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            k_scales: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                            table: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                            out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``rotary_append`` into a cache held in 4 bits: keys, turned, and values are quantised as they are written.
+
+    Of a group's elements ``zero`` is the least and ``scale`` a 15th of the range, both rounded to the type; codes are ``(x - zero) / scale`` rounded, ties to
+    even, within 0 to 15, as in exact arithmetic.  A group with an element that is not finite in the type reads back as NaN.  No two tokens of a call may have
+    one slot.  rotary_dim: a multiple of 8.  The other arguments and the turned queries are those of ``rotary_append``."""
+    return _lib.fast().rotary_append_quantised(q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, table, sections, interleaved, out)
+
+
+def read_quantised(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor,
+                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [tokens, kv_heads, head_dim] of the tokens at ``slots`` (int64), in the model's type, rounded once; zeros where a slot lies outside the
+    cache.  ``out``: two tensors to write into."""
+    return _lib.fast().read_quantised(k_cache, v_cache, k_scales, v_scales, slots, out)
+
+
+def paged_attention_quantised(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                              block_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                              rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                              lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attention`` over a cache held in 4 bits: scores, softmax and sums are of what the codes, scales and zeros stand for, in FP32."""
+    return _lib.fast().paged_attention_quantised(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, scale, window, rows, out, lse)
 
 
 def low_rank_add(x: torch.Tensor, y: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,

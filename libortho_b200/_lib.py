@@ -60,6 +60,19 @@ class LowRankDesc(ctypes.Structure):
                        (ctypes.c_int64, "tokens K N adapters rank x_stride y_stride out_stride"), (ctypes.c_int32, "type"))
 
 
+class QuantisedCacheDesc(ctypes.Structure):
+    """``ortho_b200_quantised_cache``."""
+    _fields_ = _fields((ctypes.c_void_p, "k v k_scales v_scales"),
+                       (ctypes.c_int64, "pages page_size kv_heads head_dim groups k_page_stride k_slot_stride k_head_stride v_page_stride v_slot_stride "
+                        "v_head_stride ks_page_stride ks_slot_stride ks_head_stride vs_page_stride vs_slot_stride vs_head_stride"))
+
+
+class ReadQuantisedDesc(ctypes.Structure):
+    """``ortho_b200_read_quantised_desc``."""
+    _fields_ = _fields((ctypes.c_void_p, "slots k_out v_out"),
+                       (ctypes.c_int64, "count k_token_stride k_head_stride v_token_stride v_head_stride"), (ctypes.c_int32, "type reserved"))
+
+
 class OrthoB200Error(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -163,6 +176,15 @@ def _declare(l):
             fn = getattr(l, f"ortho_b200_{name}_workspace_bytes")
             fn.restype = i64
             fn.argtypes = [c.POINTER(desc)]
+    cache = c.POINTER(QuantisedCacheDesc)
+    l.ortho_b200_rotary_append_quantised.restype = c.c_int
+    l.ortho_b200_rotary_append_quantised.argtypes = [c.POINTER(RotaryAppendDesc), cache, vp]
+    l.ortho_b200_read_quantised.restype = c.c_int
+    l.ortho_b200_read_quantised.argtypes = [c.POINTER(ReadQuantisedDesc), cache, vp]
+    l.ortho_b200_paged_attention_quantised.restype = c.c_int
+    l.ortho_b200_paged_attention_quantised.argtypes = [c.POINTER(PagedAttentionDesc), cache, vp, i64, vp]
+    l.ortho_b200_paged_attention_quantised_workspace_bytes.restype = i64
+    l.ortho_b200_paged_attention_quantised_workspace_bytes.argtypes = [c.POINTER(PagedAttentionDesc), cache]
 
 
 # every symbol include/ortho_b200.h declares
@@ -181,6 +203,8 @@ EXPORTS = [
     "ortho_b200_forward_multi", "ortho_b200_multi_workspace_bytes", "ortho_b200_forward_typed", "ortho_b200_typed_scratch_bytes",
     "ortho_b200_page_step", "ortho_b200_rotary_append", "ortho_b200_paged_attention", "ortho_b200_paged_attention_workspace_bytes",
     "ortho_b200_low_rank_add", "ortho_b200_low_rank_add_workspace_bytes",
+    "ortho_b200_rotary_append_quantised", "ortho_b200_read_quantised", "ortho_b200_paged_attention_quantised",
+    "ortho_b200_paged_attention_quantised_workspace_bytes",
 ]
 
 
@@ -219,7 +243,8 @@ def fast():
         f.set_operators(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in
                           (l.ortho_b200_page_step, l.ortho_b200_rotary_append, l.ortho_b200_paged_attention,
                            l.ortho_b200_paged_attention_workspace_bytes, l.ortho_b200_low_rank_add, l.ortho_b200_low_rank_add_workspace_bytes,
-                           l.ortho_b200_strerror, l.ortho_b200_last_cuda_error)))
+                           l.ortho_b200_strerror, l.ortho_b200_last_cuda_error, l.ortho_b200_rotary_append_quantised, l.ortho_b200_read_quantised,
+                           l.ortho_b200_paged_attention_quantised, l.ortho_b200_paged_attention_quantised_workspace_bytes)))
         _fast = f
     return _fast
 

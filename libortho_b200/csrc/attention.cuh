@@ -96,8 +96,9 @@ struct AttnShape {
     static __device__ __forceinline__ uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((kSwap ? chunk ^ (row & 7) : chunk) << 4)); }
 };
 
-// One request as the units see it
+// One request as the units of UNIT keys see it
 struct Span { int from, n, units; int64_t row; };
+template <int UNIT>
 __device__ __forceinline__ Span span_of(const ortho_b200_paged_attention_desc &d, int64_t b)
 {
     Span s;
@@ -107,12 +108,13 @@ __device__ __forceinline__ Span span_of(const ortho_b200_paged_attention_desc &d
     n = n < 0 ? 0 : n < most ? n : most;
     s.n = n;
     s.from = d.window > 0 && n > d.window ? n - (int)d.window : 0;
-    s.units = (n - s.from + kUnitKeys - 1) / kUnitKeys;
+    s.units = (n - s.from + UNIT - 1) / UNIT;
     return s;
 }
 
-// Place in the row of all units: request, head group, 64 keys.  `left`: costs up to the end of this CTA's share, the unit's own among them.  In a
+// Place in the row of all units: request, head group, UNIT keys.  `left`: costs up to the end of this CTA's share, the unit's own among them.  In a
 // cluster a CTA has every `stride`-th unit of one item.
+template <int UNIT>
 struct Walk {
     int64_t b;
     int inner, unit;
@@ -131,10 +133,79 @@ struct Walk {
             unit = 0;
             if (++inner < inners) return;
             inner = 0;
-            do b++, s = b < d.batch ? span_of(d, b) : Span{0, 0, 1, 0}; while (s.units == 0);
+            do b++, s = b < d.batch ? span_of<UNIT>(d, b) : Span{0, 0, 1, 0}; while (s.units == 0);
         }
     }
 };
+
+// A CTA's first unit, and how many costs it has.  per: costs of a CTA; item_at: number of the item's first cost.
+template <int UNIT, bool CLUSTER>
+__device__ __forceinline__ Walk<UNIT> first_unit(const ortho_b200_paged_attention_desc &d, int inners, int ctas, int rank, int ranks, long long &per, long long &item_at)
+{
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+    Walk<UNIT> now;
+    now.left = 0;
+    if constexpr (CLUSTER) {                     // every ranks-th unit of the cluster's item
+        const int64_t item = cta / ranks;
+        now.b = item / inners;
+        now.inner = (int)(item - now.b * inners);
+        now.unit = rank;
+        now.s = span_of<UNIT>(d, now.b);
+        now.left = rank < now.s.units;
+    } else {
+        __shared__ long long warp_cost[kAttnWarps], first_rest;
+        __shared__ int first_b;
+        // a thread's requests, one after the other; up to kAttnThreads requests each thread has one
+        const int64_t chunk = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * chunk, b1 = b0 + chunk < d.batch ? b0 + chunk : d.batch;
+        long long mine = 0;
+        for (int64_t b = b0; b < b1; b++) {
+            const int units = span_of<UNIT>(d, b).units;
+            mine += units + (units > 0);
+        }
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 31) warp_cost[warp] = upto;
+        __syncthreads();
+        long long total = 0;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; w++) {
+            if (w == warp) upto += total;
+            total += warp_cost[w];
+        }
+        total *= inners;
+        // (32 bits where they do: a division in 64 takes some 200 cycles)
+        per = total < 0x7FFFFFFF ? ((uint32_t)total + ctas - 1) / (uint32_t)ctas : (total + ctas - 1) / ctas;
+        const long long from = per * cta, to = from + per < total ? from + per : total;
+        long long rest = from - (upto - mine) * inners;
+        if (from < to && rest >= 0 && rest < mine * inners) {
+            int64_t b = b0;
+            for (; b + 1 < b1; b++) {
+                const int units = span_of<UNIT>(d, b).units;
+                const long long here = (long long)(units + (units > 0)) * inners;
+                if (rest < here) break;
+                rest -= here;
+            }
+            first_b = (int)b;
+            first_rest = rest;
+        }
+        __syncthreads();
+        if (from < to) {
+            now.b = first_b;
+            now.s = span_of<UNIT>(d, now.b);
+            const long long rest = first_rest;
+            now.inner = rest < 0x7FFFFFFF ? (int)((uint32_t)rest / (uint32_t)(now.s.units + 1)) : (int)(rest / (now.s.units + 1));
+            const int at = (int)(rest - (long long)now.inner * (now.s.units + 1));                // 0: the cost of the item's start and end, then its units
+            now.unit = at > 0 ? at - 1 : 0;
+            now.left = to - from - (at == 0);
+            item_at = from - at;
+        }
+    }
+    return now;
+}
 
 template <class T>
 __device__ __forceinline__ void store4(const ortho_b200_paged_attention_desc &d, int64_t b, int64_t head, int el, float4 x, float inverse)
@@ -148,6 +219,102 @@ template <class T>
 __device__ __forceinline__ float lse_of(float top, float sum)
 {
     return sum == 0.f ? -INFINITY : (top - AttnType<T>::lift + __log2f(sum)) * 0.6931471805599453f;
+}
+
+// The four warps' sums over their keys of query t * 8 + (0 .. 7) of an item become one: to the output, to the workspace, or to the cluster's CTAs.
+// folds: [warps][8 queries][elements], the warps WARP_FLOATS and the queries FOLD apart; sums: (maximum, sum) of [warps][NT * 8 queries].
+template <class T, int DP, int NT, bool CLUSTER, int WARP_FLOATS, int FOLD>
+__device__ __forceinline__ void add_warps(const AttentionArgs &a, const float *folds, const float2 *sums, int t, int64_t b, int64_t h0, int heads, bool whole, int64_t slot,
+                      int rank, int ranks, float2 *arrived_sums, float4 *arrived)
+{
+    const auto &d = a.d;
+    const int tid = threadIdx.x, D = (int)d.head_dim;
+    // a thread has one query and every 16th quad of its elements
+    const int fq = tid >> 4, row = t * 8 + fq;
+    if (row < heads) {
+        float m = -INFINITY, l = 0.f, factor[kAttnWarps];
+        float2 x[kAttnWarps];
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; w++) {
+            x[w] = sums[w * NT * 8 + row];
+            m = fmaxf(m, x[w].x);
+        }
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; w++) {
+            factor[w] = x[w].x == -INFINITY ? 0.f : exp2_approx(x[w].x - m);
+            l += x[w].x == -INFINITY ? x[w].y : x[w].y * factor[w];               // (nothing, or NaN)
+        }
+        const float inverse = l == 0.f ? 0.f : 1.f / l;
+        if constexpr (CLUSTER) {
+            if ((tid & 15) < ranks) st_dsmem_v2(mapa_shared(shared_addr(arrived_sums + rank * NT * 8 + row), tid & 15), m, l);
+        } else if ((tid & 15) == 0) {
+            if (!whole) a.sums[slot * NT * 8 + row] = make_float2(m, l);
+            else if (d.lse) d.lse[b * d.q_heads + h0 + row] = lse_of<T>(m, l);
+        }
+#pragma unroll
+        for (int i = 0; i < (DP + 63) / 64; i++) {
+            const int el = i * 64 + (tid & 15) * 4;
+            if (el >= D) break;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; w++) {
+                const float4 z = *reinterpret_cast<const float4 *>(folds + w * WARP_FLOATS + fq * FOLD + el);
+                y.x += factor[w] * z.x; y.y += factor[w] * z.y; y.z += factor[w] * z.z; y.w += factor[w] * z.w;
+            }
+            if constexpr (CLUSTER) {
+                const int share = (heads * (D / 4) + ranks - 1) / ranks, at = row * (D / 4) + el / 4, to = at / share;
+                st_dsmem_v4(mapa_shared(shared_addr(arrived + rank * share + (at - to * share)), to), y);
+            } else if (whole) store4<T>(d, b, h0 + row, el, y, inverse);
+            else *reinterpret_cast<float4 *>(a.part + (slot * NT * 8 + row) * D + el) = y;
+        }
+    }
+}
+
+// This CTA's share of an item's elements from what its cluster's CTAs have sent
+template <class T, int NT, int MOST>
+__device__ __forceinline__ void add_cluster(const AttentionArgs &a, int64_t b, int64_t h0, int heads, int rank, int ranks, const float2 *arrived_sums, const float4 *arrived)
+{
+    const auto &d = a.d;
+    const int tid = threadIdx.x, D = (int)d.head_dim;
+    const int quads = D / 4, share = (heads * quads + ranks - 1) / ranks;
+    for (int i = tid; i < share; i += kAttnThreads) {
+        const int at = rank * share + i, row = at / quads, el = (at - row * quads) * 4;
+        if (row >= heads) break;
+        float m = -INFINITY, l = 0.f;
+        float2 x[MOST];
+        float4 z[MOST], y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < MOST; r++) {
+            x[r] = r < ranks ? arrived_sums[r * NT * 8 + row] : make_float2(-INFINITY, 0.f);
+            // (nothing has arrived from a CTA without keys)
+            z[r] = x[r].x == -INFINITY && x[r].y == 0.f ? y : arrived[r * share + i];
+            m = fmaxf(m, x[r].x);
+        }
+#pragma unroll
+        for (int r = 0; r < MOST; r++) {
+            const float f = x[r].x == -INFINITY ? 0.f : exp2_approx(x[r].x - m);
+            l += x[r].x == -INFINITY ? x[r].y : x[r].y * f;
+            y.x += f * z[r].x; y.y += f * z[r].y; y.z += f * z[r].z; y.w += f * z[r].w;
+        }
+        store4<T>(d, b, h0 + row, el, y, l == 0.f ? 0.f : 1.f / l);
+        if (d.lse && el == 0) d.lse[b * d.q_heads + h0 + row] = lse_of<T>(m, l);
+    }
+}
+
+// Rows without keys
+template <class T, int UNIT>
+__device__ __forceinline__ void empty_rows(const ortho_b200_paged_attention_desc &d)
+{
+    const int tid = threadIdx.x, D = (int)d.head_dim;
+    for (int64_t b = blockIdx.x; b < d.batch; b += gridDim.x) {
+        if (span_of<UNIT>(d, b).units) continue;
+        const int chunks = D / 8;
+        for (int i = tid; i < (int)d.q_heads * chunks; i += kAttnThreads) {
+            const int h = i / chunks, c = i - h * chunks;
+            *reinterpret_cast<uint4 *>((T *)d.out + b * d.out_token_stride + h * d.out_head_stride + c * 8) = make_uint4(0, 0, 0, 0);
+            if (d.lse && c == 0) d.lse[b * d.q_heads + h] = -INFINITY;
+        }
+    }
 }
 
 template <class T, int DP, int NT, bool CLUSTER>
@@ -174,76 +341,16 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
     griddep_launch();
 
     // ---- this CTA's units -------------------------------------------------------------------------------------
-    Walk now;                                    // the unit that is computed
-    now.left = 0;
     [[maybe_unused]] long long per = 0, item_at = 0;                           // costs of a CTA; cost number of the item's first cost
     [[maybe_unused]] const int rank = CLUSTER ? (int)cluster_ctarank() : 0, ranks = CLUSTER ? (int)cluster_nctarank() : 1;
-    if constexpr (CLUSTER) {                     // every ranks-th unit of the cluster's item
-        const int64_t item = cta / ranks;
-        now.b = item / inners;
-        now.inner = (int)(item - now.b * inners);
-        now.unit = rank;
-        now.s = span_of(d, now.b);
-        now.left = rank < now.s.units;
-    } else {
-        __shared__ long long warp_cost[kAttnWarps], first_rest;
-        __shared__ int first_b;
-        // a thread's requests, one after the other; up to kAttnThreads requests each thread has one
-        const int64_t chunk = (d.batch + kAttnThreads - 1) / kAttnThreads, b0 = tid * chunk, b1 = b0 + chunk < d.batch ? b0 + chunk : d.batch;
-        long long mine = 0;
-        for (int64_t b = b0; b < b1; b++) {
-            const int units = span_of(d, b).units;
-            mine += units + (units > 0);
-        }
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        if (lane == 31) warp_cost[warp] = upto;
-        __syncthreads();
-        long long total = 0;
-#pragma unroll
-        for (int w = 0; w < kAttnWarps; w++) {
-            if (w == warp) upto += total;
-            total += warp_cost[w];
-        }
-        total *= inners;
-        // (32 bits where they do: a division in 64 takes some 200 cycles)
-        per = total < 0x7FFFFFFF ? ((uint32_t)total + a.ctas - 1) / (uint32_t)a.ctas : (total + a.ctas - 1) / a.ctas;
-        const long long from = per * cta, to = from + per < total ? from + per : total;
-        long long rest = from - (upto - mine) * inners;
-        if (from < to && rest >= 0 && rest < mine * inners) {
-            int64_t b = b0;
-            for (; b + 1 < b1; b++) {
-                const int units = span_of(d, b).units;
-                const long long here = (long long)(units + (units > 0)) * inners;
-                if (rest < here) break;
-                rest -= here;
-            }
-            first_b = (int)b;
-            first_rest = rest;
-        }
-        __syncthreads();
-        if (from < to) {
-            now.b = first_b;
-            now.s = span_of(d, now.b);
-            const long long rest = first_rest;
-            now.inner = rest < 0x7FFFFFFF ? (int)((uint32_t)rest / (uint32_t)(now.s.units + 1)) : (int)(rest / (now.s.units + 1));
-            const int at = (int)(rest - (long long)now.inner * (now.s.units + 1));                // 0: the cost of the item's start and end, then its units
-            now.unit = at > 0 ? at - 1 : 0;
-            now.left = to - from - (at == 0);
-            item_at = from - at;
-        }
-    }
+    Walk<kUnitKeys> now = first_unit<kUnitKeys, CLUSTER>(d, inners, a.ctas, rank, ranks, per, item_at);       // the unit that is computed
     if (now.left <= 0) {                         // (a share of one cost may be that of an item's start alone)
         others_started();
         if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     } else {
         // What the copies of a unit need.  The page of a lane's key is looked up well ahead of its use, those of the first units together.
         struct Ticket { int64_t b; int inner, page, place; bool valid, queries; };
-        Walk ahead = now;                        // the unit of the next ticket
+        Walk<kUnitKeys> ahead = now;                        // the unit of the next ticket
         bool more_tickets = true;
         auto ticket = [&]() {
             Ticket t;
@@ -469,45 +576,7 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
 #pragma unroll
                         for (int e = 0; e < 4; e++) fold[(e & 1) * Shape::kFoldPitch + i * 16 + (e >> 1) * 8] = o[i][t][e];
                     __syncthreads();
-                    // a thread has one query and every 16th quad of its elements
-                    const int fq = tid >> 4, row = t * 8 + fq;
-                    if (row < heads) {
-                        float m = -INFINITY, l = 0.f, factor[kAttnWarps];
-                        float2 x[kAttnWarps];
-#pragma unroll
-                        for (int w = 0; w < kAttnWarps; w++) {
-                            x[w] = sums[w * NT * 8 + row];
-                            m = fmaxf(m, x[w].x);
-                        }
-#pragma unroll
-                        for (int w = 0; w < kAttnWarps; w++) {
-                            factor[w] = x[w].x == -INFINITY ? 0.f : exp2_approx(x[w].x - m);
-                            l += x[w].x == -INFINITY ? x[w].y : x[w].y * factor[w];               // (nothing, or NaN)
-                        }
-                        const float inverse = l == 0.f ? 0.f : 1.f / l;
-                        if constexpr (CLUSTER) {
-                            if ((tid & 15) < ranks) st_dsmem_v2(mapa_shared(shared_addr(arrived_sums + rank * NT * 8 + row), tid & 15), m, l);
-                        } else if ((tid & 15) == 0) {
-                            if (!whole) a.sums[slot * NT * 8 + row] = make_float2(m, l);
-                            else if (d.lse) d.lse[now.b * d.q_heads + h0 + row] = lse_of<T>(m, l);
-                        }
-#pragma unroll
-                        for (int i = 0; i < (DP + 63) / 64; i++) {
-                            const int el = i * 64 + (tid & 15) * 4;
-                            if (el >= D) break;
-                            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                            for (int w = 0; w < kAttnWarps; w++) {
-                                const float4 z = *reinterpret_cast<const float4 *>(folds + w * WARP_FLOATS + fq * Shape::kFoldPitch + el);
-                                y.x += factor[w] * z.x; y.y += factor[w] * z.y; y.z += factor[w] * z.z; y.w += factor[w] * z.w;
-                            }
-                            if constexpr (CLUSTER) {
-                                const int share = (heads * (D / 4) + ranks - 1) / ranks, at = row * (D / 4) + el / 4, to = at / share;
-                                st_dsmem_v4(mapa_shared(shared_addr(arrived + rank * share + (at - to * share)), to), y);
-                            } else if (whole) store4<T>(d, now.b, h0 + row, el, y, inverse);
-                            else *reinterpret_cast<float4 *>(a.part + (slot * NT * 8 + row) * D + el) = y;
-                        }
-                    }
+                    add_warps<T, DP, NT, CLUSTER, WARP_FLOATS, Shape::kFoldPitch>(a, folds, sums, t, now.b, h0, heads, whole, slot, rank, ranks, arrived_sums, arrived);
                 }
                 if constexpr (!CLUSTER) {
                     if (!more && tid == 0) a.cut[cta] = make_int4((int)now.b, now.inner, (int)((item_at + now.s.units) / per), started_here && !last ? 1 : 0);
@@ -529,40 +598,9 @@ paged_attention_kernel(const __grid_constant__ AttentionArgs a)
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        const int quads = D / 4, share = (heads * quads + ranks - 1) / ranks;
-        for (int i = tid; i < share && now.s.units > 0; i += kAttnThreads) {
-            const int at = rank * share + i, row = at / quads, el = (at - row * quads) * 4;
-            if (row >= heads) break;
-            float m = -INFINITY, l = 0.f;
-            float2 x[Shape::kMostRanks];
-            float4 z[Shape::kMostRanks], y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int r = 0; r < Shape::kMostRanks; r++) {
-                x[r] = r < ranks ? arrived_sums[r * NT * 8 + row] : make_float2(-INFINITY, 0.f);
-                // (nothing has arrived from a CTA without keys)
-                z[r] = x[r].x == -INFINITY && x[r].y == 0.f ? y : arrived[r * share + i];
-                m = fmaxf(m, x[r].x);
-            }
-#pragma unroll
-            for (int r = 0; r < Shape::kMostRanks; r++) {
-                const float f = x[r].x == -INFINITY ? 0.f : exp2_approx(x[r].x - m);
-                l += x[r].x == -INFINITY ? x[r].y : x[r].y * f;
-                y.x += f * z[r].x; y.y += f * z[r].y; y.z += f * z[r].z; y.w += f * z[r].w;
-            }
-            store4<T>(d, now.b, h0 + row, el, y, l == 0.f ? 0.f : 1.f / l);
-            if (d.lse && el == 0) d.lse[now.b * d.q_heads + h0 + row] = lse_of<T>(m, l);
-        }
+        if (now.s.units > 0) add_cluster<T, NT, Shape::kMostRanks>(a, now.b, h0, heads, rank, ranks, arrived_sums, arrived);
     }
-    // ---- rows without keys ---------------------------------------------------------------------------------------
-    for (int64_t b = cta; b < d.batch; b += gridDim.x) {
-        if (span_of(d, b).units) continue;
-        const int chunks = D / 8;
-        for (int i = tid; i < (int)d.q_heads * chunks; i += kAttnThreads) {
-            const int h = i / chunks, c = i - h * chunks;
-            *reinterpret_cast<uint4 *>((T *)d.out + b * d.out_token_stride + h * d.out_head_stride + c * 8) = make_uint4(0, 0, 0, 0);
-            if (d.lse && c == 0) d.lse[b * d.q_heads + h] = -INFINITY;
-        }
-    }
+    empty_rows<T, kUnitKeys>(d);
 }
 
 // Adds the parts of an item that was cut, in the order of its keys.  A CTA per CTA of the kernel above (the one where a cut item starts) and

@@ -1,0 +1,581 @@
+// Attention of one new token per row over a paged cache held in 4 bits (quantised.cuh; one source for both 16-bit types):
+//
+//     s_j = scale sum_g (ks_jg sum_i q_i c_ji + kz_jg sum_i q_i),     out_i = sum_j p_j (vs_jg (d_ji - 8) + vz_jg + 8 vs_jg) / sum_j p_j,     p_j = exp(s_j - max)
+//
+// with codes c and d of keys and values, scales and zeros of their groups g.  The division of the work, the ring of asynchronous copies per warp and the joining are those of
+// attention.cuh; here the bytes are a quarter, so what bounds it is the warps' instructions: unpacking, about one a code and 32 lanes.
+// Codes enter the products as whole numbers, and scales and zeros are applied to what 64 elements or 16 keys have in common:
+//   * S^T = K Q^T: a lane reads 8 codes of a key as one word; the halves of the word, masked and joined with an exponent, are four operands of 64 + c
+//     in FP16 (c in the upper bits of the mantissa).  Elements are taken in the order in which a word has them, the queries likewise; the 64 comes off with
+//     the zero's term, ks q.c + (kz - 64 ks) sum q.  A sum of 64 q loses at most 2^-23 of itself, some 2^-19 of a typical q.c.
+//   * O^T += V^T P^T: a pair of keys' words are joined by halves, then unpacked to d - 8 exactly: codes around zero keep the sums as small as the outputs
+//     of a long average are, where 0 to 15 against a zero at the other end would lose two digits.  p vs enters as two FP16 parts, brought into
+//     range by a power of two of the warp's largest scale; p (vz + 8 vs) is summed in FP32 per query.
+// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element near 2^8.
+#pragma once
+
+#include <type_traits>
+
+#include "attention.cuh"
+#include "quantised.cuh"
+
+namespace ob {
+
+struct QuantisedAttentionArgs {
+    AttentionArgs a;                             // (d.kv_heads, head_dim, pages, page_size are the cache's; the other fields of a cache are not read)
+    ortho_b200_quantised_cache c;
+    int wide;                                    // rows of the cache are whole 16-byte pieces
+};
+
+constexpr int kQWarpKeys = 32, kQUnitKeys = kQWarpKeys * kAttnWarps;
+
+template <int DP, int NT, bool GROUPED>
+struct QuantisedShape {
+    static constexpr int kGroups = GROUPED ? DP / kQuantGroup : 1;
+    // Rows are an odd number of 16-byte pieces, so that the words that a warp reads together (8 keys x 4 words; 4 pairs of keys x 8 words) lie in 32 banks
+    static constexpr int kPitch = DP / 2 + (DP / 32 % 2 ? 0 : 16), kPieces = DP / 32;
+    static constexpr int kCodes = kQWarpKeys * kPitch, kScales = kQWarpKeys * kGroups * 4;
+    static constexpr int kStage = 2 * (kCodes + kScales);
+    static constexpr int kQPitch = DP * 2 + 16, kQ = NT * 8 * kQPitch;
+    static constexpr int kFoldPitch = DP + 4;
+    static_assert(8 * kFoldPitch * 4 <= kStage, "room for 8 queries");
+    static constexpr bool kKeepQ = NT * DP <= 256;                             // query operands stay in registers
+    static constexpr int kOperands = kKeepQ ? 0 : NT * DP / 32 * 512;
+    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
+    static constexpr int kFour = 57088, kThree = 76458, kTwo = 115712, kOne = 232448;
+    static constexpr int kRegs = NT * DP;                                      // a measure of the sums that a thread holds
+    static constexpr int kWanted = kRegs <= 128 ? 4 : kRegs <= 192 ? 3 : kRegs <= 256 ? 2 : 1;
+    static constexpr int kRoom = kWanted == 4 && bytes(2) <= kFour ? kFour : kWanted >= 3 && bytes(2) <= kThree ? kThree : kWanted >= 2 && bytes(2) <= kTwo ? kTwo : kOne;
+    static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2, kBytes = bytes(kStages);
+    static constexpr int kPerSm = kRoom == kFour ? 4 : kRoom == kThree ? 3 : kRoom == kTwo ? 2 : 1;
+    static constexpr int kMostRanks = 8;
+    static constexpr int kArrived = kMostRanks * NT * 8 * 8 + NT * 8 * DP * 4 + kMostRanks * 16, kClusterBytes = (kBytes + 15) / 16 * 16 + kArrived;
+    static constexpr int kClusterPerSm = kClusterBytes <= kFour && kPerSm >= 4 ? 4 : kClusterBytes <= kThree && kPerSm >= 3 ? 3 : kClusterBytes <= kTwo && kPerSm >= 2 ? 2 : kClusterBytes <= kOne ? 1 : 0;
+};
+
+__device__ __forceinline__ uint32_t load_shared(uint32_t addr) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory"); return v; }
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void *src, bool on)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+// Codes at bits 4 to 7 and 20 to 23 as 64 + code
+__device__ __forceinline__ uint32_t codes_64(uint32_t w) { return (w & 0x00F000F0u) | 0x54005400u; }
+// Codes at bits 0 to 3 and 16 to 19 (LOW), or 4 to 7 and 20 to 23, less 8
+template <bool LOW> __device__ __forceinline__ uint32_t codes_centred(uint32_t w)
+{
+    const uint32_t b = LOW ? (w & 0x000F000Fu) | 0x64006400u : (w & 0x00F000F0u) | 0x54005400u, off = LOW ? 0x64086408u : 0x54805480u;      // 1024 + 8, 64 + 8
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&off));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <class T> __device__ __forceinline__ float2 scale_and_zero(uint32_t w) { return Half<T>::unpack(w); }
+
+// Eight elements of a query, in memory's order, as the products take them: (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ uint4 as_codes_lie(uint4 w)
+{
+    return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632));
+}
+
+// One query's operands: `row` is its place in shared memory, thread t of four has the words 4 j + t.  f: what the products are to be multiplied by;
+// sums: of its elements, per group.
+template <class T, int DP, int GROUPS>
+__device__ __forceinline__ void query_operands(uint32_t row, int t, uint4 (&w)[DP / 32], float &f, float (&sums)[GROUPS])
+{
+    constexpr int J = DP / 32, PER = J / GROUPS;
+    f = 1.f;
+#pragma unroll
+    for (int j = 0; j < J; j++) w[j] = load_shared16(row + (4 * j + t) * 16);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            most = __vmaxu2(__vmaxu2(__vmaxu2(w[j].x & 0x7FFF7FFFu, w[j].y & 0x7FFF7FFFu), __vmaxu2(w[j].z & 0x7FFF7FFFu, w[j].w & 0x7FFF7FFFu)), most);
+        }
+        most = max(most & 0xFFFFu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // exponent e of the largest: elements times 2^(8 - e).  (Infinity and NaN stay what they are; of rows below 2^-100 nothing is lost that FP32 shows.)
+        const int e = min(max((int)(most >> 7), 27), 254);
+        const float by = __uint_as_float((uint32_t)(262 - e) << 23);
+        f = __uint_as_float((uint32_t)(e - 8) << 23);
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            uint32_t *const x = reinterpret_cast<uint32_t *>(&w[j]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 v = Half<T>::unpack(x[i]);
+                x[i] = Half<__half>::pack(v.x * by, v.y * by);
+            }
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = g * PER; j < (g + 1) * PER; j++) {
+            const uint32_t *const x = reinterpret_cast<const uint32_t *>(&w[j]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) { const float2 v = Half<__half>::unpack(x[i]); s += v.x + v.y; }
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        sums[g] = s;
+    }
+#pragma unroll
+    for (int j = 0; j < J; j++) w[j] = as_codes_lie(w[j]);
+}
+
+template <class T, int DP, int NT, bool GROUPED, bool CLUSTER>
+__global__ void __launch_bounds__(kAttnThreads, QuantisedShape<DP, NT, GROUPED>::kPerSm)
+paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs args)
+{
+    using Shape = QuantisedShape<DP, NT, GROUPED>;
+    using Type = AttnType<__half>;
+    constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
+    constexpr uint32_t kAll = 0xffffffffu;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const AttentionArgs &a = args.a;
+    const auto &d = a.d;
+    const auto &c = args.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t4 = lane & 3, D = (int)d.head_dim;
+    unsigned char *const ring = smem + warp * (S * Shape::kStage);
+    unsigned char *const q_ring = smem + kAttnWarps * S * Shape::kStage;
+    unsigned char *const operands = q_ring + S * Shape::kQ;                    // (of queries that do not stay in registers) [NT][J][32] x 16 bytes
+    float2 *const sums = reinterpret_cast<float2 *>(operands + Shape::kOperands);
+    uint32_t *const seen = reinterpret_cast<uint32_t *>(sums + kAttnWarps * NT * 8) + warp * S;
+    const int inners = (int)d.kv_heads * a.groups, cta = blockIdx.x;
+    float2 *const arrived_sums = reinterpret_cast<float2 *>(smem + (Shape::kBytes + 15) / 16 * 16);           // [ranks][rows]
+    float4 *const arrived = reinterpret_cast<float4 *>(arrived_sums + Shape::kMostRanks * NT * 8);            // [ranks][this CTA's share]
+
+    if constexpr (CLUSTER) cluster_arrive();
+    auto others_started = [&]() { if constexpr (CLUSTER) { __syncwarp(); cluster_wait(); } };         // before anything is sent to them, once the first copies are under way
+    griddep_wait();
+    griddep_launch();
+
+    [[maybe_unused]] long long per = 0, item_at = 0;                           // costs of a CTA; cost number of the item's first cost
+    [[maybe_unused]] const int rank = CLUSTER ? (int)cluster_ctarank() : 0, ranks = CLUSTER ? (int)cluster_nctarank() : 1;
+    Walk<kQUnitKeys> now = first_unit<kQUnitKeys, CLUSTER>(d, inners, a.ctas, rank, ranks, per, item_at);     // the unit that is computed
+    if (now.left <= 0) {                         // (a share of one cost may be that of an item's start alone)
+        others_started();
+        if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
+    } else {
+        // What the copies of a unit need; a lane has a key of the warp's 32, and looks its page up well ahead of its use
+        struct Ticket { int64_t b; int inner, page, place; bool valid, queries; };
+        Walk<kQUnitKeys> ahead = now;            // the unit of the next ticket
+        bool more_tickets = true;
+        auto ticket = [&]() {
+            Ticket t;
+            t.valid = more_tickets;
+            t.b = ahead.b;
+            t.inner = ahead.inner;
+            t.queries = CLUSTER ? ahead.unit == rank : ahead.unit == 0 || (ahead.b == now.b && ahead.inner == now.inner && ahead.unit == now.unit);
+            t.page = -1;
+            t.place = 0;
+            const int key = ahead.s.from + ahead.unit * kQUnitKeys + warp * kQWarpKeys + lane;
+            if (more_tickets && key < ahead.s.n) {
+                const int col = (int)a.by_page.quotient((uint32_t)key);
+                t.place = key - col * (int)d.page_size;
+                t.page = d.block_table[ahead.s.row * d.table_stride + col];
+            }
+            if (more_tickets) {
+                more_tickets = ahead.template more<CLUSTER>(ranks);
+                if (more_tickets) ahead.template step<CLUSTER>(d, inners, ranks);
+            }
+            return t;
+        };
+        int fresh_q = 0;                         // items issued so far: place in the ring of queries
+        const bool alike = c.k_page_stride == c.v_page_stride && c.k_slot_stride == c.v_slot_stride;
+        auto issue = [&](const Ticket &t, int stage) {
+            if (t.valid) {
+                const int head = t.inner / a.groups, group = t.inner - head * a.groups, place = t.place, page = t.page < d.pages ? t.page : -1;
+                const uint32_t ok = __ballot_sync(kAll, page >= 0);
+                if (lane == 0) seen[stage] = ok;
+                const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
+                const unsigned char *const k = (const unsigned char *)c.k + head * c.k_head_stride, *const v = (const unsigned char *)c.v + head * c.v_head_stride;
+                // a lane's own key's place in the caches; the lanes that copy a row get it from there
+                const int64_t k_mine = page >= 0 ? page * c.k_page_stride + place * c.k_slot_stride : 0;
+                const int64_t v_mine = alike || page < 0 ? k_mine : page * c.v_page_stride + place * c.v_slot_stride;
+                {
+                    const int64_t ks = page >= 0 ? page * c.ks_page_stride + place * c.ks_slot_stride : 0, vs = page >= 0 ? page * c.vs_page_stride + place * c.vs_slot_stride : 0;
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        copy4_async(dst + 2 * Shape::kCodes + (lane * G + g) * 4, (const uint32_t *)c.k_scales + ks + head * c.ks_head_stride + g, page >= 0);
+                        copy4_async(dst + 2 * Shape::kCodes + Shape::kScales + (lane * G + g) * 4, (const uint32_t *)c.v_scales + vs + head * c.vs_head_stride + g, page >= 0);
+                    }
+                }
+                if (args.wide) {
+#pragma unroll
+                    for (int i = 0; i < Shape::kPieces; i++) {
+                        const int at = i * 32 + lane, row = at / Shape::kPieces, piece = at % Shape::kPieces;
+                        const int64_t k_at = __shfl_sync(kAll, k_mine, row), v_at = alike ? k_at : __shfl_sync(kAll, v_mine, row);
+                        const bool on = (ok >> row & 1) && piece * 32 < D;     // (else zeros; the address is that of the first page)
+                        const int e = piece * 32 < D ? piece * 16 : 0;
+                        copy16_async(dst + row * Shape::kPitch + piece * 16, k + k_at + e, on);
+                        copy16_async(dst + Shape::kCodes + row * Shape::kPitch + piece * 16, v + v_at + e, on);
+                    }
+                } else {
+                    for (int at = lane; at < kQWarpKeys * (DP / 8); at += 32) {
+                        const int row = at / (DP / 8), word = at % (DP / 8);
+                        const int64_t k_at = __shfl_sync(kAll, k_mine, row), v_at = alike ? k_at : __shfl_sync(kAll, v_mine, row);
+                        const bool on = (ok >> row & 1) && word * 8 < D;
+                        const int e = word * 8 < D ? word * 4 : 0;
+                        copy4_async(dst + row * Shape::kPitch + word * 4, k + k_at + e, on);
+                        copy4_async(dst + Shape::kCodes + row * Shape::kPitch + word * 4, v + v_at + e, on);
+                    }
+                }
+                if (t.queries) {                                               // its queries, a quarter per warp
+                    const uint32_t qdst = shared_addr(q_ring + fresh_q * Shape::kQ);
+                    const int h0 = head * (int)(d.q_heads / d.kv_heads) + group * a.per_group;
+                    const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+                    for (int at = tid; at < NT * DP; at += kAttnThreads) {
+                        const int row = at / (DP / 8), chunk = at % (DP / 8);
+                        const bool on = row < heads && chunk * 8 < D;
+                        copy16_async(qdst + row * Shape::kQPitch + chunk * 16, (const T *)d.q + t.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
+                    }
+                    if (++fresh_q == S) fresh_q = 0;
+                }
+            }
+            copy_commit();
+        };
+        Ticket pending;
+        {
+            Ticket first[S - 1];
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) first[i] = ticket();
+            pending = ticket();
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) issue(first[i], i);
+        }
+        others_started();
+
+        uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
+        float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
+        float o[2 * J][NT][4], top[NT][2], sum[NT][2], zeros[NT][G][2];
+        float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
+        int stage = 0, q_at = -1;
+        bool started_here = true;                // the request's first unit is this CTA's
+        for (bool first_one = true, more = true; more; first_one = false) {
+            copy_wait<S - 2>();
+            __syncwarp();
+            if (first_one || (!CLUSTER && now.unit == 0)) {
+                started_here = now.unit == 0;
+                if (++q_at == S) q_at = 0;
+                __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
+                const uint32_t src = shared_addr(q_ring + q_at * Shape::kQ) + r * Shape::kQPitch;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    uint4 w[J];
+                    float f, s[G];
+                    query_operands<T, DP, G>(src + t * 8 * Shape::kQPitch, t4, w, f, s);
+                    if constexpr (Shape::kKeepQ) {
+#pragma unroll
+                        for (int j = 0; j < J; j++) q[t][j] = w[j];
+                    } else if (t % kAttnWarps == warp) {
+#pragma unroll
+                        for (int j = 0; j < J; j++) reinterpret_cast<uint4 *>(operands)[(t * J + j) * 32 + lane] = w[j];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * a.scale_log2;
+#pragma unroll
+                        for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
+                    }
+                    top[t][0] = top[t][1] = -INFINITY;
+                    sum[t][0] = sum[t][1] = 0.f;
+#pragma unroll
+                    for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 2 * J; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
+                }
+                if constexpr (!Shape::kKeepQ) __syncthreads();
+            }
+            const uint32_t ok = seen[stage];
+            const uint32_t keys = shared_addr(ring + stage * Shape::kStage), values = keys + Shape::kCodes, scales = values + Shape::kCodes;
+            issue(pending, stage == 0 ? S - 1 : stage - 1);
+            pending = ticket();
+#pragma unroll
+            for (int h = 0; h < 2; h++) {        // 16 keys
+                if (!(ok >> (16 * h) & 0xFFFFu)) continue;
+                float s[NT][4];
+                // rows (keys) r and r + 8 of the tile, columns (queries) 2 t4 and the next
+                const uint32_t k_row = keys + (16 * h + r) * Shape::kPitch + t4 * 4;
+#pragma unroll
+                for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    float x[NT][4], odd[NT][4];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) x[t][0] = x[t][1] = x[t][2] = x[t][3] = odd[t][0] = odd[t][1] = odd[t][2] = odd[t][3] = 0.f;
+#pragma unroll
+                    for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
+                        const uint32_t w0 = load_shared(k_row + j * 16), w1 = load_shared(k_row + 8 * Shape::kPitch + j * 16);
+                        const uint32_t lower[4] = {codes_64(w0 << 4), codes_64(w1 << 4), codes_64(w0), codes_64(w1)};
+                        const uint32_t upper[4] = {codes_64(w0 >> 4), codes_64(w1 >> 4), codes_64(w0 >> 8), codes_64(w1 >> 8)};
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            uint4 b;
+                            if constexpr (Shape::kKeepQ) b = q[t][j];
+                            else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
+                            Half<__half>::mma(x[t], lower, b.x, b.y);
+                            Half<__half>::mma(NT <= 2 ? odd[t] : x[t], upper, b.z, b.w);           // (two chains of products where there are few)
+                        }
+                    }
+                    const float2 h0 = scale_and_zero<T>(load_shared(scales + ((16 * h + r) * G + g) * 4)), h1 = scale_and_zero<T>(load_shared(scales + ((16 * h + r + 8) * G + g) * 4));
+                    const float z0 = h0.y - 64.f * h0.x, z1 = h1.y - 64.f * h1.x;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            s[t][e] += h0.x * (NT <= 2 ? x[t][e] + odd[t][e] : x[t][e]) + z0 * q_sum[t][g][e];
+                            s[t][e + 2] += h1.x * (NT <= 2 ? x[t][e + 2] + odd[t][e + 2] : x[t][e + 2]) + z1 * q_sum[t][g][e];
+                        }
+                }
+                float2 v0[G], v1[G];             // scales and zeros of the two keys' values
+                const bool on0 = (ok >> (16 * h + r)) & 1, on1 = (ok >> (16 * h + r + 8)) & 1;
+                bool grows = false;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    v0[g] = scale_and_zero<T>(load_shared(scales + Shape::kScales + ((16 * h + r) * G + g) * 4));
+                    v1[g] = scale_and_zero<T>(load_shared(scales + Shape::kScales + ((16 * h + r + 8) * G + g) * 4));
+                    grows = grows || fmaxf(v0[g].x, v1[g].x) > largest;
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        s[t][e] = on0 ? s[t][e] * factor[t][e] : -INFINITY;
+                        s[t][e + 2] = on1 ? s[t][e + 2] * factor[t][e] : -INFINITY;
+                        grows = grows || fmaxf(s[t][e], s[t][e + 2]) > top[t][e] + kSlack;
+                    }
+                if (__any_sync(kAll, grows)) {
+                    float most = largest;
+#pragma unroll
+                    for (int g = 0; g < G; g++) most = fmaxf(most, fmaxf(v0[g].x, v1[g].x));
+                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 4));
+                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 8));
+                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 16));
+                    // the power of two at or above it, between 2^-100 and 2^126
+                    const uint32_t up = min(max((__float_as_uint(most) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
+                    const float was = largest;
+                    largest = __uint_as_float(up);
+                    to_one = __uint_as_float((254u << 23) - up);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        float keep[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float m = fmaxf(s[t][e], s[t][e + 2]);
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
+                            m = fmaxf(m, top[t][e]);
+                            keep[e] = m == -INFINITY ? 1.f : exp2_approx(top[t][e] - m);
+                            top[t][e] = m;
+                            sum[t][e] *= keep[e];
+#pragma unroll
+                            for (int g = 0; g < G; g++) zeros[t][g][e] *= keep[e];
+                            keep[e] *= was * to_one;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2 * J; i++) {
+                            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1]; o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
+                        }
+                    }
+                }
+                float p[NT][4];
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float base = (top[t][e] == -INFINITY ? 0.f : top[t][e]) - Type::lift;
+                        p[t][e] = exp2_approx(s[t][e] - base);
+                        p[t][e + 2] = exp2_approx(s[t][e + 2] - base);
+                        sum[t][e] += p[t][e] + p[t][e + 2];
+                    }
+                // a lane's pairs of keys are 2 t4 and 2 t4 + 8 with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
+                const uint32_t v_row = values + (16 * h + 2 * t4) * Shape::kPitch + r * 4;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    uint32_t hi[NT][2], lo[NT][2];
+                    const float f0 = v0[g].x * to_one, f1 = v1[g].x * to_one, z0 = v0[g].y + 8.f * v0[g].x, z1 = v1[g].y + 8.f * v1[g].x;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        zeros[t][g][0] += p[t][0] * z0 + p[t][2] * z1;
+                        zeros[t][g][1] += p[t][1] * z0 + p[t][3] * z1;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float y0 = p[t][2 * i] * (i ? f1 : f0), y1 = p[t][2 * i + 1] * (i ? f1 : f0);
+                            const uint32_t up = pack_half2(y0, y1);
+                            const float2 f = Half<__half>::unpack(up);
+                            hi[t][i] = transpose8x8(up);
+                            lo[t][i] = transpose8x8(pack_half2(y0 - f.x, y1 - f.y));
+                        }
+                    }
+                    auto products = [&](int at, const uint32_t (&v)[2][4]) {   // two tiles of 16 elements
+#pragma unroll
+                        for (int part = 0; part < 2; part++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+#pragma unroll
+                                for (int t = 0; t < NT; t++) Half<__half>::mma(o[at + i][t], v[i], part ? lo[t][0] : hi[t][0], part ? lo[t][1] : hi[t][1]);
+                    };
+                    auto unpacked = [&](int at, uint32_t x, uint32_t y) {      // four codes each of a pair of keys, and of the pair 8 behind
+                        const uint32_t x8 = x >> 8, y8 = y >> 8;
+                        const uint32_t v[2][4] = {{codes_centred<true>(x), codes_centred<false>(x), codes_centred<true>(y), codes_centred<false>(y)},
+                                                  {codes_centred<true>(x8), codes_centred<false>(x8), codes_centred<true>(y8), codes_centred<false>(y8)}};
+                        products(at, v);
+                    };
+#pragma unroll
+                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++) {
+                        const uint32_t at = v_row + ch * 32;
+                        const uint32_t w0 = load_shared(at), w1 = load_shared(at + Shape::kPitch), w2 = load_shared(at + 8 * Shape::kPitch), w3 = load_shared(at + 9 * Shape::kPitch);
+                        unpacked(4 * ch, __byte_perm(w0, w1, 0x5410), __byte_perm(w2, w3, 0x5410));
+                        unpacked(4 * ch + 2, __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x7632));
+                    }
+                    if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
+                        const uint32_t at = values + (16 * h + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4, half = r & 1 ? 0x7632 : 0x5410;
+                        const uint32_t w0 = load_shared(at), w1 = load_shared(at + Shape::kPitch), w2 = load_shared(at + 8 * Shape::kPitch), w3 = load_shared(at + 9 * Shape::kPitch);
+                        unpacked(4 * CH, __byte_perm(w0, w1, half), __byte_perm(w2, w3, half));
+                    }
+                }
+            }
+            const bool last = now.last();
+            more = now.template more<CLUSTER>(ranks);
+            if (CLUSTER ? !more : last || !more) {
+                // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
+                // issued behind the barrier above.  What was 2^lift and `largest` times too large is brought back here.
+                const int head = now.inner / a.groups, group = now.inner - head * a.groups;
+                const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
+                const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+                const bool whole = started_here && last;
+                const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
+                constexpr float kDown = 1.f / 256.f;
+                static_assert(Type::lift == 8.f, "the power of two above");
+                auto over_keys = [](float x) {
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    return x + __shfl_xor_sync(0xffffffffu, x, 16);
+                };
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float l = over_keys(sum[t][e]);
+                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(top[t][e] + AttnType<T>::lift, l * kDown);
+#pragma unroll
+                        for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
+                    }
+                float *const fold = reinterpret_cast<float *>(ring + stage * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
+                const float *const folds = reinterpret_cast<const float *>(smem + stage * Shape::kStage);
+                constexpr int WARP_FLOATS = S * Shape::kStage / 4;
+                const float times = largest * kDown;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    __syncwarp();                // the warp has read its values
+                    if (t) __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < 2 * J; i++) {
+                        const int el = i < 4 * CH ? (i / 4) * 64 + 8 * r + 2 * (i % 4) : CH * 64 + 4 * r + 2 * (i % 4);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float z = zeros[t][GROUPED ? i / 4 : 0][e];
+                            *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times + z);
+                        }
+                    }
+                    __syncthreads();
+                    add_warps<T, DP, NT, CLUSTER, WARP_FLOATS, Shape::kFoldPitch>(a, folds, sums, t, now.b, h0, heads, whole, slot, rank, ranks, arrived_sums, arrived);
+                }
+                if constexpr (!CLUSTER) {
+                    if (!more && tid == 0) a.cut[cta] = make_int4((int)now.b, now.inner, (int)((item_at + now.s.units) / per), started_here && !last ? 1 : 0);
+                    item_at += now.s.units + 1;
+                }
+            }
+            if (++stage == S) stage = 0;
+            if (more) now.template step<CLUSTER>(d, inners, ranks);
+        }
+        copy_wait<0>();
+    }
+    if constexpr (CLUSTER) {
+        // ---- the cluster's sums become one, a share of the elements in each CTA
+        const int head = now.inner / a.groups, group = now.inner - head * a.groups;
+        const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
+        const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+        for (int i = tid; i < heads * ranks && now.left <= 0; i += kAttnThreads)                  // no unit: nothing is added
+            st_dsmem_v2(mapa_shared(shared_addr(arrived_sums + rank * NT * 8 + i / ranks), i % ranks), -INFINITY, 0.f);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (now.s.units > 0) add_cluster<T, NT, Shape::kMostRanks>(a, now.b, h0, heads, rank, ranks, arrived_sums, arrived);
+    }
+    empty_rows<T, kQUnitKeys>(d);
+}
+
+// ---- host: which variant, how much workspace -----------------------------------------------------------------
+template <class T> int launch_attention_quantised(const QuantisedAttentionArgs &a, const AttnPlan &p, bool grouped, cudaStream_t stream);
+
+template <class T, int DP, int NT, bool GROUPED>
+int launch_attention_quantised_as(const QuantisedAttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
+{
+    using Shape = QuantisedShape<DP, NT, GROUPED>;
+    const int dev = current_device_index();
+    if (dev < 0) return ORTHO_B200_ERR_CUDA;
+    static bool attr_set[kMaxDevices] = {};
+    if (!attr_set[dev]) {
+        OB_CUDA(cudaFuncSetAttribute(paged_attention_quantised_kernel<T, DP, NT, GROUPED, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes));
+        if constexpr (Shape::kClusterPerSm > 0)
+            OB_CUDA(cudaFuncSetAttribute(paged_attention_quantised_kernel<T, DP, NT, GROUPED, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kClusterBytes));
+        attr_set[dev] = true;
+    }
+    if constexpr (Shape::kClusterPerSm > 0) {
+        if (p.cluster) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)a.a.ctas); cfg.blockDim = dim3(kAttnThreads); cfg.dynamicSmemBytes = Shape::kClusterBytes; cfg.stream = stream;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = (unsigned)p.cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+            cfg.attrs = attr; cfg.numAttrs = 2;
+            OB_CUDA(cudaLaunchKernelEx(&cfg, paged_attention_quantised_kernel<T, DP, NT, GROUPED, true>, a));
+            count_launch();
+            return ORTHO_B200_OK;
+        }
+    }
+    const int st = launch_dependent(paged_attention_quantised_kernel<T, DP, NT, GROUPED, false>, dim3((unsigned)a.a.ctas), kAttnThreads, Shape::kBytes, stream, a);
+    if (st) return st;
+    return launch_dependent(join_kernel<T>, dim3((unsigned)a.a.ctas, (unsigned)a.a.per_group), 128, 0, stream, a.a, NT * 8);
+}
+
+template <class T, int DP, bool GROUPED>
+int launch_attention_quantised_dim(const QuantisedAttentionArgs &a, const AttnPlan &p, cudaStream_t stream)
+{
+    if (p.nt == 1) return launch_attention_quantised_as<T, DP, 1, GROUPED>(a, p, stream);
+    if (p.nt == 2) return launch_attention_quantised_as<T, DP, 2, GROUPED>(a, p, stream);
+    if constexpr (DP <= 128) return launch_attention_quantised_as<T, DP, 4, GROUPED>(a, p, stream);
+    return ORTHO_B200_ERR_SHAPE;
+}
+
+#define OB_QUANTISED_DIMS(X) X(64) X(96) X(128) X(192) X(256)
+
+template <class T>
+int launch_attention_quantised(const QuantisedAttentionArgs &a, const AttnPlan &p, bool grouped, cudaStream_t stream)
+{
+#define OB_CASE(DP)                                                                                              \
+    if (p.dp == DP) {                                                                                            \
+        if constexpr (DP % kQuantGroup == 0 && DP > kQuantGroup)                                                 \
+            if (grouped) return launch_attention_quantised_dim<T, DP, true>(a, p, stream);                       \
+        return launch_attention_quantised_dim<T, DP, false>(a, p, stream);                                       \
+    }
+    OB_QUANTISED_DIMS(OB_CASE)
+#undef OB_CASE
+    return ORTHO_B200_ERR_SHAPE;
+}
+
+}  // namespace ob

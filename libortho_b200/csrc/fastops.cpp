@@ -1,4 +1,4 @@
-// Host path of the operators around the projections (_C_ops.page_step, rotary_append, paged_attention, low_rank_add): argument checks,
+// Host path of the operators around the projections (_C_ops.page_step, rotary_append, paged_attention, low_rank_add, and those of a cache held in 4 bits): argument checks,
 // outputs and scratch, the C record, the launch.  Part of the extension module of fastcall.cpp; wrong arguments raise here, with the
 // device guard, the current stream and torch's allocator taken as any torch operator takes them.
 #include <Python.h>
@@ -21,6 +21,10 @@ int (*attention_c)(const ortho_b200_paged_attention_desc *, void *, int64_t, voi
 int64_t (*attention_ws_c)(const ortho_b200_paged_attention_desc *) = nullptr;
 int (*low_rank_c)(const ortho_b200_low_rank_desc *, void *, int64_t, void *) = nullptr;
 int64_t (*low_rank_ws_c)(const ortho_b200_low_rank_desc *) = nullptr;
+int (*append_quantised_c)(const ortho_b200_rotary_append_desc *, const ortho_b200_quantised_cache *, void *) = nullptr;
+int (*read_quantised_c)(const ortho_b200_read_quantised_desc *, const ortho_b200_quantised_cache *, void *) = nullptr;
+int (*attention_quantised_c)(const ortho_b200_paged_attention_desc *, const ortho_b200_quantised_cache *, void *, int64_t, void *) = nullptr;
+int64_t (*attention_quantised_ws_c)(const ortho_b200_paged_attention_desc *, const ortho_b200_quantised_cache *) = nullptr;
 const char *(*strerror_c)(int) = nullptr;
 int (*last_cuda_error_c)() = nullptr;
 
@@ -105,6 +109,43 @@ Cache cache_of(PyObject *k, PyObject *v, at::ScalarType type, const at::Tensor &
     return c;
 }
 
+// One held in 4 bits, from its four tensors
+struct QuantisedCache : Cache { at::Tensor ks, vs; ortho_b200_quantised_cache record; };
+QuantisedCache quantised_cache_of(PyObject *const *a, at::ScalarType type, const at::Tensor &like)
+{
+    QuantisedCache c;
+    c.k = output(a[0], "k_cache", at::kByte, like);
+    c.v = output(a[1], "v_cache", at::kByte, like);
+    c.ks = output(a[2], "k_scales", type, like);
+    c.vs = output(a[3], "v_scales", type, like);
+    TORCH_CHECK_VALUE(c.k.dim() == 4 && c.v.sizes() == c.k.sizes(), "k_cache and v_cache must be [pages, page_size, kv_heads, head_dim / 2] alike");
+    TORCH_CHECK_VALUE(c.k.stride(3) == 1 && c.v.stride(3) == 1, "the caches' last dimension must be contiguous");
+    c.pages = c.k.size(0); c.page_size = c.k.size(1); c.heads = c.k.size(2); c.D = 2 * c.k.size(3);
+    TORCH_CHECK_VALUE(c.page_size >= 1 && c.heads >= 1, "k_cache and v_cache must have pages of at least one token");
+    TORCH_CHECK_VALUE(c.D >= 8 && c.D % 8 == 0 && c.D <= 256, "head_dim must be a multiple of 8 up to 256");
+    TORCH_CHECK_VALUE(c.ks.dim() == 5 && c.vs.sizes() == c.ks.sizes() && c.ks.size(0) == c.pages && c.ks.size(1) == c.page_size && c.ks.size(2) == c.heads && c.ks.size(4) == 2,
+                      "k_scales and v_scales must be [pages, page_size, kv_heads, groups, 2] alike");
+    const int64_t groups = c.ks.size(3);
+    TORCH_CHECK_VALUE(groups == 1 || groups * 64 == c.D, "a group must be a whole head or 64 elements of one");
+    auto stride = [](const at::Tensor &t, int i, int of) {
+        if (t.size(i) <= 1) return (int64_t)0;
+        TORCH_CHECK_VALUE(t.stride(i) % of == 0, "codes must lie at multiples of 4 bytes and scales at multiples of 2 elements");
+        return t.stride(i) / (of == 4 ? 1 : of);
+    };
+    for (const at::Tensor *t : {&c.k, &c.v, &c.ks, &c.vs})
+        TORCH_CHECK_VALUE(((uintptr_t)t->const_data_ptr() & 3u) == 0, "codes and scales must be 4-byte aligned");
+    for (const at::Tensor *t : {&c.ks, &c.vs})
+        TORCH_CHECK_VALUE(t->stride(4) == 1 && (groups == 1 || t->stride(3) == 2), "the scales' last two dimensions must be contiguous");
+    ortho_b200_quantised_cache &r = c.record;
+    r.k = ptr<void>(c.k); r.v = ptr<void>(c.v); r.k_scales = ptr<void>(c.ks); r.v_scales = ptr<void>(c.vs);
+    r.pages = c.pages; r.page_size = c.page_size; r.kv_heads = c.heads; r.head_dim = c.D; r.groups = groups;
+    r.k_page_stride = stride(c.k, 0, 4); r.k_slot_stride = stride(c.k, 1, 4); r.k_head_stride = stride(c.k, 2, 4);
+    r.v_page_stride = stride(c.v, 0, 4); r.v_slot_stride = stride(c.v, 1, 4); r.v_head_stride = stride(c.v, 2, 4);
+    r.ks_page_stride = stride(c.ks, 0, 2); r.ks_slot_stride = stride(c.ks, 1, 2); r.ks_head_stride = stride(c.ks, 2, 2);
+    r.vs_page_stride = stride(c.vs, 0, 2); r.vs_slot_stride = stride(c.vs, 1, 2); r.vs_head_stride = stride(c.vs, 2, 2);
+    return c;
+}
+
 // page_step(cached, fresh, block_table, free_pages, available, page_size, tokens, out or None) -> six tensors
 PyObject *page_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
@@ -160,20 +201,30 @@ PyObject *page_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
-// rotary_append(q or None, k, v, k_cache, v_cache, slots, positions, table, sections, interleaved, out) -> q_out or None
+// rotary_append(q or None, k, v, k_cache, v_cache, slots, positions, table, sections, interleaved, out) -> q_out or None; a cache held in 4 bits has
+// k_scales and v_scales behind v_cache
+template <bool QUANTISED>
 PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    TORCH_CHECK_TYPE(n == 11, "rotary_append takes 11 arguments");
-    const auto type = half_type(tensor(a[1], "k"), "k");
+    TORCH_CHECK_TYPE(n == (QUANTISED ? 13 : 11), QUANTISED ? "rotary_append_quantised takes 13 arguments" : "rotary_append takes 11 arguments");
+    PyObject *const *const caches = a + 3;
+    if (QUANTISED) a += 2;                       // what follows the caches keeps its number
+    PyObject *const q_arg = caches[-3], *const k_arg = caches[-2], *const v_arg = caches[-1];
+    const auto type = half_type(tensor(k_arg, "k"), "k");
+    // (codes are made of vectors of four values at least)
+    auto fits = [](const at::Tensor &t) { return ((uintptr_t)t.const_data_ptr() & 7u) == 0 && t.stride(0) % 4 == 0 && t.stride(1) % 4 == 0; };
     auto heads = [&](PyObject *o, const char *name, const at::Tensor *like) {
         at::Tensor t = input(o, name, type, like);
         three_dims(t, name, like ? like->size(0) : -1, like ? like->size(2) : -1);
+        if (QUANTISED && (t.stride(2) != 1 || !fits(t))) return t.clone(at::MemoryFormat::Contiguous);
         return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous();
     };
-    const at::Tensor k = heads(a[1], "k", nullptr), v = heads(a[2], "v", &k);
+    const at::Tensor k = heads(k_arg, "k", nullptr), v = heads(v_arg, "v", &k);
     TORCH_CHECK_VALUE(v.size(1) == k.size(1), "k and v must have the same heads");
-    const Cache c = cache_of(a[3], a[4], type, k);
+    std::conditional_t<QUANTISED, QuantisedCache, Cache> c;
+    if constexpr (QUANTISED) c = quantised_cache_of(caches, type, k);
+    else c = cache_of(caches[0], caches[1], type, k);
     const int64_t T = k.size(0);
     TORCH_CHECK_VALUE(c.heads == k.size(1) && c.D == k.size(2), "k and v must have the caches' heads and head_dim");
     TORCH_CHECK_VALUE(c.D <= 8192, "head_dim must be at most 8192");
@@ -189,6 +240,7 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (positions.stride(-1) != 1 && T > 1) positions = positions.contiguous();
         table = input(a[7], "table", at::kFloat, &k);
         TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) >= 2 && table.size(1) % 2 == 0 && table.size(1) <= c.D, "table must be [positions, rotary_dim], rotary_dim even and at most head_dim");
+        TORCH_CHECK_VALUE(!QUANTISED || table.size(1) % 8 == 0, "rotary_dim must be a multiple of 8");
         if (!table.is_contiguous()) table = table.contiguous();
         d.axes = positions.dim() == 1 ? 1 : (int32_t)positions.size(0);
         TORCH_CHECK_VALUE(d.axes >= 1 && d.axes <= ORTHO_B200_MAX_AXES, "positions must have one to ", ORTHO_B200_MAX_AXES, " axes");
@@ -212,12 +264,13 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
         }
         d.positions = ptr<int32_t>(positions); d.table = ptr<float>(table); d.table_rows = table.size(0);
     }
-    if (given(a[0])) {
+    if (given(q_arg)) {
         TORCH_CHECK_VALUE(given(a[7]), "without positions there is nothing to do for q");
-        q = heads(a[0], "q", &k);
+        q = heads(q_arg, "q", &k);
         if (given(a[10])) {
             out = output(a[10], "out", type, k);
             TORCH_CHECK_VALUE(out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) <= 1), "out must have q's shape and a contiguous last dimension");
+            TORCH_CHECK_VALUE(!QUANTISED || fits(out), "out must be 8-byte aligned, with strides that are multiples of 4");
         } else {
             out = at::empty(q.sizes(), q.options());
         }
@@ -228,39 +281,93 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     const int truth = PyObject_IsTrue(a[9]);
     if (truth < 0) throw python_error();
-    d.k = ptr<void>(k); d.v = ptr<void>(v); d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v); d.slots = ptr<int64_t>(slots);
+    d.k = ptr<void>(k); d.v = ptr<void>(v); d.slots = ptr<int64_t>(slots);
     d.tokens = T; d.kv_heads = c.heads; d.head_dim = c.D; d.pages = c.pages; d.page_size = c.page_size;
     d.k_token_stride = k.stride(0); d.k_head_stride = k.stride(1); d.v_token_stride = v.stride(0); d.v_head_stride = v.stride(1);
-    d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_cache_head_stride = c.k.stride(2);
-    d.v_page_stride = c.v.stride(0); d.v_slot_stride = c.v.stride(1); d.v_cache_head_stride = c.v.stride(2);
+    if (!QUANTISED) {
+        d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v);
+        d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_cache_head_stride = c.k.stride(2);
+        d.v_page_stride = c.v.stride(0); d.v_slot_stride = c.v.stride(1); d.v_cache_head_stride = c.v.stride(2);
+    }
     d.interleaved = truth; d.type = type_number(type);
     void *stream = current_stream(k);
     int st = 0;
     if (c.pages > 0 || d.q_heads > 0) {          // (a cache without pages keeps nothing)
         Py_BEGIN_ALLOW_THREADS
-        st = rotary_append_c(&d, stream);
+        if constexpr (QUANTISED) st = append_quantised_c(&d, &c.record, stream);
+        else st = rotary_append_c(&d, stream);
         Py_END_ALLOW_THREADS
     }
-    check_status(st, "ortho_b200_rotary_append");
+    check_status(st, QUANTISED ? "ortho_b200_rotary_append_quantised" : "ortho_b200_rotary_append");
     if (!out.defined()) Py_RETURN_NONE;
     return given(a[10]) ? Py_NewRef(a[10]) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
 
-// paged_attention(q, k_cache, v_cache, block_table, lengths, scale or None, window, rows or None, out or None, lse or None) -> out
+// read_quantised(k_cache, v_cache, k_scales, v_scales, slots, out or None) -> (k, v)
+PyObject *read_quantised(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 6, "read_quantised takes 6 arguments");
+    const at::Tensor &scales = tensor(a[2], "k_scales");
+    const auto type = half_type(scales, "k_scales");
+    const QuantisedCache c = quantised_cache_of(a, type, scales);
+    at::Tensor slots = input(a[4], "slots", at::kLong, &scales);
+    TORCH_CHECK_VALUE(slots.dim() == 1, "slots must be one-dimensional");
+    const int64_t T = slots.size(0);
+    TORCH_CHECK_VALUE(T <= std::numeric_limits<int32_t>::max(), "slots must be fewer than 2^31");
+    if (!slots.is_contiguous()) slots = slots.contiguous();
+    const c10::cuda::CUDAGuard guard(scales.device());
+    at::Tensor out[2];
+    static const char *names[2] = {"out[0]", "out[1]"};
+    if (given(a[5])) {
+        TORCH_CHECK_TYPE(PyTuple_Check(a[5]) && PyTuple_GET_SIZE(a[5]) == 2, "out must be a pair of tensors");
+        for (int i = 0; i < 2; i++) {
+            out[i] = output(PyTuple_GET_ITEM(a[5], i), names[i], type, scales);
+            TORCH_CHECK_VALUE(out[i].dim() == 3 && out[i].size(0) == T && out[i].size(1) == c.heads && out[i].size(2) == c.D && out[i].stride(2) == 1 && aligned(out[i])
+                              && out[i].stride(0) % 8 == 0 && out[i].stride(1) % 8 == 0,
+                              names[i], " must be [tokens, kv_heads, head_dim] with a contiguous last dimension, 16-byte alignment and strides that are multiples of 8");
+        }
+    } else {
+        for (int i = 0; i < 2; i++) out[i] = at::empty({T, c.heads, c.D}, scales.options().memory_format(at::MemoryFormat::Contiguous));
+    }
+    ortho_b200_read_quantised_desc d;
+    memset(&d, 0, sizeof(d));
+    d.slots = ptr<int64_t>(slots); d.k_out = ptr<void>(out[0]); d.v_out = ptr<void>(out[1]); d.count = T; d.type = type_number(type);
+    d.k_token_stride = out[0].stride(0); d.k_head_stride = out[0].stride(1); d.v_token_stride = out[1].stride(0); d.v_head_stride = out[1].stride(1);
+    void *stream = current_stream(scales);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = read_quantised_c(&d, &c.record, stream);
+    Py_END_ALLOW_THREADS
+    check_status(st, "ortho_b200_read_quantised");
+    if (given(a[5])) return Py_NewRef(a[5]);
+    PyObject *r = PyTuple_New(2);
+    if (!r) return nullptr;
+    for (int i = 0; i < 2; i++) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_cache, v_cache, block_table, lengths, scale or None, window, rows or None, out or None, lse or None) -> out; a cache held in
+// 4 bits has k_scales and v_scales behind v_cache
+template <bool QUANTISED>
 PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    TORCH_CHECK_TYPE(n == 10, "paged_attention takes 10 arguments");
+    TORCH_CHECK_TYPE(n == (QUANTISED ? 12 : 10), QUANTISED ? "paged_attention_quantised takes 12 arguments" : "paged_attention takes 10 arguments");
     const auto type = half_type(tensor(a[0], "q"), "q");
     at::Tensor q = input(a[0], "q", type);
     three_dims(q, "q", -1, -1);
-    const Cache c = cache_of(a[1], a[2], type, q);
+    std::conditional_t<QUANTISED, QuantisedCache, Cache> c;
+    if constexpr (QUANTISED) c = quantised_cache_of(a + 1, type, q);
+    else c = cache_of(a[1], a[2], type, q);
+    if (QUANTISED) a += 2;                       // what follows the caches keeps its number
     const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
     TORCH_CHECK_VALUE(D == c.D && H >= 1 && H % c.heads == 0, "q must have the caches' head_dim and a multiple of their heads");
     TORCH_CHECK_VALUE(D % 8 == 0 && D <= 256, "head_dim must be a multiple of 8 up to 256");
     for (const at::Tensor *t : {&c.k, &c.v})
-        TORCH_CHECK_VALUE(aligned(*t) && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0,
+        TORCH_CHECK_VALUE(QUANTISED || (aligned(*t) && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0),
                           "the caches must be 16-byte aligned, with strides that are multiples of 8");
     const at::Tensor table = input(a[3], "block_table", at::kInt, &q);
     TORCH_CHECK_VALUE(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), "block_table must be [requests, pages] with contiguous rows");
@@ -291,26 +398,32 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
         TORCH_CHECK_VALUE(lse.dim() == 2 && lse.size(0) == B && lse.size(1) == H && lse.is_contiguous(), "lse must be a contiguous [requests, heads] tensor");
         d.lse = ptr<float>(lse);
     }
-    d.q = ptr<void>(q); d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v); d.out = ptr<void>(out);
+    d.q = ptr<void>(q); d.out = ptr<void>(out);
     d.block_table = ptr<int32_t>(table); d.lengths = ptr<int32_t>(lengths); d.row_of = rows.defined() ? ptr<int32_t>(rows) : nullptr;
     d.batch = B; d.q_heads = H; d.kv_heads = c.heads; d.head_dim = D; d.rows = table.size(0); d.width = table.size(1); d.table_stride = table.stride(0);
     d.pages = c.pages; d.page_size = c.page_size; d.window = window;
     d.q_token_stride = q.stride(0); d.q_head_stride = q.stride(1); d.out_token_stride = out.stride(0); d.out_head_stride = out.stride(1);
-    d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_head_stride = c.k.stride(2);
-    d.v_page_stride = c.v.stride(0); d.v_slot_stride = c.v.stride(1); d.v_head_stride = c.v.stride(2);
+    if (!QUANTISED) {
+        d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v);
+        d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_head_stride = c.k.stride(2);
+        d.v_page_stride = c.v.stride(0); d.v_slot_stride = c.v.stride(1); d.v_head_stride = c.v.stride(2);
+    }
     d.scale = (float)scale; d.type = type_number(type);
     if (c.pages == 0) { d.width = 0; d.k_cache = d.v_cache = d.q; }        // nothing is cached: no row has a key
     int st = 0;
     if (B) {
-        const int64_t need = attention_ws_c(&d);
+        int64_t need;
+        if constexpr (QUANTISED) need = attention_quantised_ws_c(&d, &c.record);
+        else need = attention_ws_c(&d);
         at::Tensor ws;
         if (need > 0) ws = scratch(need, q);
         void *wsp = need > 0 ? ws.mutable_data_ptr() : nullptr, *stream = current_stream(q);
         Py_BEGIN_ALLOW_THREADS
-        st = attention_c(&d, wsp, need, stream);
+        if constexpr (QUANTISED) st = attention_quantised_c(&d, &c.record, wsp, need, stream);
+        else st = attention_c(&d, wsp, need, stream);
         Py_END_ALLOW_THREADS
     }
-    check_status(st, "ortho_b200_paged_attention");
+    check_status(st, QUANTISED ? "ortho_b200_paged_attention_quantised" : "ortho_b200_paged_attention");
     return given(a[8]) ? Py_NewRef(a[8]) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -375,9 +488,9 @@ PyObject *low_rank_add(PyObject *, PyObject *const *a, Py_ssize_t n)
 // addresses in the loaded library, in the order below
 PyObject *set_operators(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (n != 8) { PyErr_SetString(PyExc_TypeError, "set_operators takes 8 arguments"); return nullptr; }
-    void *p[8];
-    for (int i = 0; i < 8; i++) p[i] = PyLong_AsVoidPtr(a[i]);
+    if (n != 12) { PyErr_SetString(PyExc_TypeError, "set_operators takes 12 arguments"); return nullptr; }
+    void *p[12];
+    for (int i = 0; i < 12; i++) p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
     page_step_c = reinterpret_cast<decltype(page_step_c)>(p[0]);
     rotary_append_c = reinterpret_cast<decltype(rotary_append_c)>(p[1]);
@@ -387,6 +500,10 @@ PyObject *set_operators(PyObject *, PyObject *const *a, Py_ssize_t n)
     low_rank_ws_c = reinterpret_cast<decltype(low_rank_ws_c)>(p[5]);
     strerror_c = reinterpret_cast<decltype(strerror_c)>(p[6]);
     last_cuda_error_c = reinterpret_cast<decltype(last_cuda_error_c)>(p[7]);
+    append_quantised_c = reinterpret_cast<decltype(append_quantised_c)>(p[8]);
+    read_quantised_c = reinterpret_cast<decltype(read_quantised_c)>(p[9]);
+    attention_quantised_c = reinterpret_cast<decltype(attention_quantised_c)>(p[10]);
+    attention_quantised_ws_c = reinterpret_cast<decltype(attention_quantised_ws_c)>(p[11]);
     Py_RETURN_NONE;
 }
 
@@ -394,8 +511,11 @@ PyObject *set_operators(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 PyMethodDef ortho_operator_methods[] = {
     {"page_step", (PyCFunction)(void (*)(void))page_step, METH_FASTCALL, nullptr},
-    {"rotary_append", (PyCFunction)(void (*)(void))rotary_append, METH_FASTCALL, nullptr},
-    {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
+    {"rotary_append", (PyCFunction)(void (*)(void))rotary_append<false>, METH_FASTCALL, nullptr},
+    {"rotary_append_quantised", (PyCFunction)(void (*)(void))rotary_append<true>, METH_FASTCALL, nullptr},
+    {"read_quantised", (PyCFunction)(void (*)(void))read_quantised, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))paged_attention<false>, METH_FASTCALL, nullptr},
+    {"paged_attention_quantised", (PyCFunction)(void (*)(void))paged_attention<true>, METH_FASTCALL, nullptr},
     {"low_rank_add", (PyCFunction)(void (*)(void))low_rank_add, METH_FASTCALL, nullptr},
     {"set_operators", (PyCFunction)(void (*)(void))set_operators, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

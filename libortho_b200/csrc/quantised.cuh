@@ -1,0 +1,22 @@
+// The paged cache held in 4 bits (include/ortho_b200.h has the format): checks of its record, and the unpacking of codes.
+#pragma once
+
+#include "launch.cuh"
+
+namespace ob {
+
+constexpr int kQuantGroup = 64;                  // elements of a group that is not a whole head
+
+inline int check_quantised(const ortho_b200_quantised_cache *c)
+{
+    if (!c) return ORTHO_B200_ERR_NULL;
+    if (c->pages < 0 || c->pages > 0x7FFFFFFF || c->page_size < 1 || c->page_size > 0x7FFFFF00 || c->kv_heads < 1 || c->kv_heads > 65535 || c->head_dim < 8 || c->head_dim > 256
+        || c->head_dim % 8 || c->groups < 1 || (c->groups > 1 && c->groups * kQuantGroup != c->head_dim)) return ORTHO_B200_ERR_SHAPE;
+    if (c->pages && (!c->k || !c->v || !c->k_scales || !c->v_scales)) return ORTHO_B200_ERR_NULL;
+    if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 3u) return ORTHO_B200_ERR_ALIGN;
+    for (int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride})
+        if (s % 4) return ORTHO_B200_ERR_ALIGN;
+    return ORTHO_B200_OK;
+}
+
+}  // namespace ob

@@ -6,7 +6,7 @@
 // (token, head) pairs of its CTA, queries, keys and values alike.  Cosines and sines of the CTA's tokens pass through shared memory: in registers
 // they leave too little room for values under way (4096 tokens of 96 heads of 128, 204 MB: 36.9 us = 5.5 TB/s; 40 us with a token a CTA and its angles in
 // registers, 49 to 64 with values loaded ahead there).  64 tokens of 80 heads: 2.7 us, launch and the chain slot, position, angle.
-#include "launch.cuh"
+#include "rotary.cuh"
 
 namespace ob {
 
@@ -16,46 +16,6 @@ struct RotaryArgs {
     int together;                                // tokens of a CTA
     FastDiv by_items, by_heads, by_half;
 };
-
-// VEC 16-bit values as they lie in memory
-template <int VEC>
-struct Raw {
-    uint32_t w[VEC > 1 ? VEC / 2 : 1];
-    __device__ __forceinline__ void load(const void *p)
-    {
-        if constexpr (VEC == 8) { const uint4 u = *reinterpret_cast<const uint4 *>(p); w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; }
-        else if constexpr (VEC == 4) { const uint2 u = *reinterpret_cast<const uint2 *>(p); w[0] = u.x; w[1] = u.y; }
-        else w[0] = *reinterpret_cast<const uint16_t *>(p);
-    }
-    __device__ __forceinline__ void store(void *p) const
-    {
-        if constexpr (VEC == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        else if constexpr (VEC == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
-    }
-    template <class T> __device__ __forceinline__ void to(float (&o)[VEC]) const
-    {
-#pragma unroll
-        for (int j = 0; j < (VEC + 1) / 2; j++) {
-            const float2 f = Half<T>::unpack(w[j]);
-            o[2 * j] = f.x;
-            if (VEC > 1) o[VEC > 1 ? 2 * j + 1 : 0] = f.y;
-        }
-    }
-    template <class T> __device__ __forceinline__ void from(const float (&o)[VEC])
-    {
-#pragma unroll
-        for (int j = 0; j < (VEC + 1) / 2; j++) w[j] = Half<T>::pack(o[2 * j], VEC > 1 ? o[VEC > 1 ? 2 * j + 1 : 0] : 0.f);
-    }
-};
-
-// (a c - b s, b c + a s), the same bits in every variant: two products are rounded, the other two are not
-__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s)
-{
-    const float was = a;
-    a = __fmaf_rn(a, c, -__fmul_rn(b, s));
-    b = __fmaf_rn(b, c, __fmul_rn(was, s));
-}
 
 constexpr int kTurnsAhead = 2, kMostTogether = 4;  // turns of a thread whose values are in flight together; tokens of a CTA
 
@@ -109,16 +69,7 @@ rotary_append_kernel(const __grid_constant__ RotaryArgs a)
                     k_at[threadIdx.x] = kept ? page * d.k_page_stride + place * d.k_slot_stride : -1;
                     v_at[threadIdx.x] = kept ? page * d.v_page_stride + place * d.v_slot_stride : -1;
                 }
-                for (int i = threadIdx.x; i < tokens * half; i += 256) {
-                    const int token = (int)a.by_half.quotient(i), pair = i - token * half;
-                    int axis = 0;
-#pragma unroll
-                    for (int x = 0; x < ORTHO_B200_MAX_AXES - 1; x++) axis += x + 1 < d.axes && pair >= d.section_ends[x];
-                    const int32_t p = d.positions[axis * d.position_stride + t0 + token];
-                    const bool in = p >= 0 && p < d.table_rows;
-                    angles[token * R + pair] = in ? d.table[(int64_t)p * R + pair] : 1.f;
-                    angles[token * R + half + pair] = in ? d.table[(int64_t)p * R + half + pair] : 0.f;
-                }
+                angles_of(d, a.by_half, t0, tokens, angles);
                 __syncthreads();
             }
 #pragma unroll
