@@ -78,7 +78,7 @@ __device__ __forceinline__ Held held_of(double lo, double hi)
 }
 
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, 2)
 quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
 {
     constexpr int U = 2;                         // rows of a segment whose values are in flight together

@@ -1,13 +1,13 @@
 """A paged key-value cache and the attention part of a decoder block on it.
 
-``PagePool`` keeps the requests' block table and the free pages on the GPU, ``PagedCache`` one layer's keys and values,
+``PagePool`` keeps the requests' block table and the free pages on the GPU, ``PagedCache`` one layer's keys and values (``QuantisedCache``: in 4 bits),
 ``PagedAttentionBlock`` runs a step: fused QKV projection (``OrthoLinear``), adapters, rotary positions with the write into
 the cache, attention, output projection, adapters.  One step serves requests that decode (one new token) and
 requests that bring a prompt (several) alike.  The reference has no counterpart; its operator ends with the projection.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -84,6 +84,49 @@ class PagedCache:
         self.k = torch.zeros(pages, page_size, kv_heads, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
 
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: Optional[torch.Tensor] = None,
+               table: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+        """Turns queries and keys, writes keys and values to ``slots``; the turned queries (``_C_ops.rotary_append``)."""
+        return _C.rotary_append(q, k, v, self.k, self.v, slots, positions, table, sections=sections, interleaved=interleaved)
+
+    def attention(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                  rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of one token per row (``_C_ops.paged_attention``)."""
+        return _C.paged_attention(q, self.k, self.v, block_table, lengths, scale=scale, window=window, rows=rows)
+
+
+class QuantisedCache:
+    """Keys and values of one layer in 4 bits: ``PagedCache`` in three tenths of its room.
+
+    Each token's head, or every ``group`` = 64 elements of one, has a scale and a zero of its own.  ``read(slots)`` gives tokens back in ``dtype``.  A page lies head by
+    head, so that attention reads whole lines of memory."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, group: Optional[int] = None, device=None, dtype=torch.float16):
+        if head_dim < 8 or head_dim % 8 or head_dim > 256:
+            raise ValueError("head_dim must be a multiple of 8 up to 256")
+        if group not in (None, head_dim) and (group != 64 or head_dim % 64):
+            raise ValueError("group must be 64, of a head_dim that is a multiple of it, or the whole head")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("scales are float16 or bfloat16")
+        device = torch.device("cuda" if device is None else device)
+        groups = head_dim // (group or head_dim)
+        self.k, self.v = (torch.zeros(pages, kv_heads, page_size, head_dim // 2, dtype=torch.uint8, device=device).transpose(1, 2) for _ in range(2))
+        self.k_scales, self.v_scales = (torch.zeros(pages, kv_heads, page_size, groups, 2, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
+
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: Optional[torch.Tensor] = None,
+               table: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+        """Turns queries and keys, quantises keys and values as it writes them to ``slots``; the turned queries (``_C_ops.rotary_append_quantised``)."""
+        return _C.rotary_append_quantised(q, k, v, self.k, self.v, self.k_scales, self.v_scales, slots, positions, table, sections=sections, interleaved=interleaved)
+
+    def attention(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                  rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of one token per row (``_C_ops.paged_attention_quantised``)."""
+        return _C.paged_attention_quantised(q, self.k, self.v, self.k_scales, self.v_scales, block_table, lengths, scale=scale, window=window, rows=rows)
+
+    def read(self, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [tokens, kv_heads, head_dim] of the tokens at ``slots`` (``_C_ops.read_quantised``)."""
+        return _C.read_quantised(self.k, self.v, self.k_scales, self.v_scales, slots)
+
 
 class PagedAttentionBlock(nn.Module):
     """The attention part of a decoder block for serving.
@@ -112,7 +155,7 @@ class PagedAttentionBlock(nn.Module):
             self.table = table.to(self.table.device)
         return out
 
-    def forward(self, x: torch.Tensor, cache: PagedCache, pool: PagePool, step: PageStep, ids: Optional[torch.Tensor] = None,
+    def forward(self, x: torch.Tensor, cache: Union[PagedCache, QuantisedCache], pool: PagePool, step: PageStep, ids: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` [tokens, in_features]: the step's new tokens, request after request, as ``step`` lists them.
         ``positions``: rotary positions where they are not those in the request, [tokens] or [axes, tokens].  Every token sees its
@@ -124,9 +167,9 @@ class PagedAttentionBlock(nn.Module):
             qkv = self.qkv_adapters(x, qkv, ids, out=qkv)
         heads = qkv.view(T, self.q_heads + 2 * self.kv_heads, D)
         q, k, v = heads.split((self.q_heads, self.kv_heads, self.kv_heads), dim=1)
-        q = _C.rotary_append(q, k, v, cache.k, cache.v, step.slots, step.positions if positions is None else positions, self.table,
-                             sections=self.sections, interleaved=self.interleaved)
-        o = _C.paged_attention(q, cache.k, cache.v, pool.block_table, step.positions + 1, window=self.window, rows=step.requests)
+        q = cache.append(q, k, v, step.slots, step.positions if positions is None else positions, self.table,
+                         sections=self.sections, interleaved=self.interleaved)
+        o = cache.attention(q, pool.block_table, step.positions + 1, window=self.window, rows=step.requests)
         o = o.view(T, self.q_heads * D)
         y = self.proj(o)
         if self.proj_adapters is not None and ids is not None:

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import quantised_ops
-from libortho_b200 import _C_ops, _lib
+from libortho_b200 import QuantisedCache, _C_ops, _lib
 from test_decoding_ops_host import ALIGN, NULL, OK, SHAPE, WORKSPACE, attention, rotary
 
 F16, BF16 = torch.float16, torch.bfloat16
@@ -94,6 +94,18 @@ def test_cpu_tensors_raise():
                  lambda: _C_ops.paged_attention_quantised(h, *c, i.view(2, 1), i)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_a_cache_is_made_and_checked_on_the_host():
+    c = QuantisedCache(3, 16, 2, 128, 64, device="cpu", dtype=BF16)
+    assert c.k.shape == c.v.shape == (3, 16, 2, 64) and c.k_scales.shape == (3, 16, 2, 2, 2) and c.v_scales.dtype == BF16 and not c.k.any()
+    assert c.k.stride() == (2048, 64, 1024, 1) and c.k_scales.stride() == (128, 4, 64, 2, 1)
+    assert QuantisedCache(3, 16, 2, 72, device="cpu").k_scales.shape == QuantisedCache(3, 16, 2, 72, 72, device="cpu").k_scales.shape == (3, 16, 2, 1, 2)
+    for bad in ((3, 16, 2, 60), (3, 16, 2, 264), (3, 16, 2, 96, 64), (3, 16, 2, 128, 32), (3, 16, 2, 0)):
+        with pytest.raises(ValueError):
+            QuantisedCache(*bad, device="cpu")
+    with pytest.raises(TypeError):
+        QuantisedCache(3, 16, 2, 64, device="cpu", dtype=torch.float32)
 
 
 def test_the_plain_forms_by_hand():
