@@ -5,10 +5,14 @@
 // Rounding to 4 bits turns a difference in the last place of FP32 into a whole step wherever x lies next to a border, so the codes are those of exact
 // arithmetic: FP32 does the work and knows its own error, and what lies within that of a border is taken again in FP64 from the raw values (a key in
 // some 1500 groups, and ties).  A turned key is a c - b s of an 11-bit and a 24-bit factor each, exact in FP64 up to its last sum.
+#include <cfloat>
+
 #include "quantised.cuh"
 #include "rotary.cuh"
 
 namespace ob {
+
+constexpr int kMostTogether = 4;                 // tokens of a CTA
 
 struct QuantiseArgs {
     ortho_b200_rotary_append_desc d;
@@ -30,9 +34,15 @@ template <> struct QuantType<__nv_bfloat16> {
 };
 template <class T> __device__ __forceinline__ uint32_t bits16(T v) { return *reinterpret_cast<const uint16_t *>(&v); }
 
+// Least and largest, NaN where one is
+__device__ __forceinline__ float least_of(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float most_of(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float least_of(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float most_of(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
 // Element e of a head in FP64, turned or not
 template <class T, bool INTERLEAVED>
-__device__ __noinline__ double exact_element(const T *src, int e, const float *angles, int rotary)
+__device__ __forceinline__ double exact_element(const T *src, int e, const float *angles, int rotary)
 {
     if (e >= rotary) return (double)Half<T>::to_float(src[e]);
     const int half = rotary / 2, pair = INTERLEAVED ? e >> 1 : e < half ? e : e - half;
@@ -51,13 +61,12 @@ template <class T>
 __device__ __forceinline__ bool held_of(float lo, float hi, float tol, Held &h)
 {
     const float q = (hi - lo) * (1.f / 15.f), tq = tol * (2.f / 15.f) + q * 0x1p-21f;
-    const T z = Half<T>::from_float(lo), s = Half<T>::from_float(q);
-    h.z = Half<T>::to_float(z);
-    h.s = Half<T>::to_float(s);
-    h.bits = bits16(s) | bits16(z) << 16;
-    return bits16(Half<T>::from_float(lo - tol)) == bits16(Half<T>::from_float(lo + tol))
-        && bits16(Half<T>::from_float(q - tq)) == bits16(Half<T>::from_float(q + tq))
-        && fmaxf(fabsf(lo), fabsf(hi)) < QuantType<T>::safe && (q > 1e-30f || (lo == hi && tol == 0.f));
+    h.bits = Half<T>::pack(q, lo);
+    const float2 f = Half<T>::unpack(h.bits);
+    h.s = f.x;
+    h.z = f.y;
+    return Half<T>::pack(q - tq, lo - tol) == Half<T>::pack(q + tq, lo + tol) && fmaxf(fabsf(lo), fabsf(hi)) < QuantType<T>::safe
+        && (q > 1e-30f || (lo == hi && tol == 0.f));
 }
 template <class T>
 __device__ __forceinline__ Held held_of(double lo, double hi)
@@ -77,14 +86,50 @@ __device__ __forceinline__ Held held_of(double lo, double hi)
     return h;
 }
 
+// Scales and zeros of a warp's heads in FP64: of the groups g0 and g1 that a thread's vectors at e0 and e1 (-1: none) belong to.  src NULL: no head.
+struct HeldTwo { Held of[2]; };
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 2)
+__device__ __noinline__ HeldTwo exact_held(const T *src, int e0, int e1, const float *angles, int rotary, int groups, int g0, int g1, int lanes)
+{
+    double least[2] = {INFINITY, INFINITY}, most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        const int e = v ? e1 : e0;
+        if (!src || e < 0) break;
+#pragma unroll 1
+        for (int i = 0; i < VEC; i++) {
+            const double x = exact_element<T, INTERLEAVED>(src, e + i, angles, rotary);
+            least[v] = x < least[v] ? x : least[v];
+            most[v] = x > most[v] ? x : most[v];
+            if (!(fabs(x) < INFINITY)) most[v] = INFINITY;
+        }
+    }
+    HeldTwo r = {};
+    for (int g = 0; g < groups; g++) {
+        double l = INFINITY, m = -INFINITY;
+        if (g0 == g) { l = least[0]; m = most[0]; }
+        if (g1 == g) { l = least[1] < l ? least[1] : l; m = most[1] > m ? most[1] : m; }
+        for (int o = lanes >> 1; o >= 1; o >>= 1) {
+            const double l2 = __shfl_xor_sync(0xffffffffu, l, o), m2 = __shfl_xor_sync(0xffffffffu, m, o);
+            l = l2 < l ? l2 : l;
+            m = m2 > m ? m2 : m;
+        }
+        const Held h = held_of<T>(l, m);
+        if (g0 == g) r.of[0] = h;
+        if (g1 == g) r.of[1] = h;
+    }
+    return r;
+}
+
+template <class T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 3)
 quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
 {
-    constexpr int U = 2;                         // rows of a segment whose values are in flight together
+    constexpr int U = 1;                    // rows of a segment whose values are in flight together
     constexpr uint32_t kAll = 0xffffffffu;
     extern __shared__ __align__(16) float angles[];                            // [tokens][rotary]: cosines, then sines
-    __shared__ int64_t places[4][4];             // of a token in codes and scales of keys and values; the first -1 for none
+    struct Places { const T *from[3]; void *to[3]; uint32_t *scales[2]; };     // of a token's queries, keys and values; no place in the cache: NULL
+    __shared__ Places places[kMostTogether];
     const auto &d = a.d;
     const auto &c = a.c;
     const int64_t t0 = (int64_t)blockIdx.x * a.together;
@@ -101,50 +146,56 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
     const int g0 = groups == 1 ? 0 : e0 / kQuantGroup, g1 = groups == 1 ? 0 : e1 / kQuantGroup;
     griddep_wait();
     griddep_launch();
-    bool ready = false;
+    if ((int)threadIdx.x < tokens) {
+        const int64_t t = t0 + threadIdx.x, slot = d.slots[t];
+        const bool kept = slot >= 0 && slot < c.pages * c.page_size;
+        const int64_t page = kept ? slot / c.page_size : 0, place = slot - page * c.page_size;
+        Places &p = places[threadIdx.x];
+        p.from[0] = (const T *)d.q + t * d.q_token_stride;
+        p.from[1] = (const T *)d.k + t * d.k_token_stride;
+        p.from[2] = (const T *)d.v + t * d.v_token_stride;
+        p.to[0] = (T *)d.q_out + t * d.out_token_stride;
+        p.to[1] = kept ? (unsigned char *)c.k + page * c.k_page_stride + place * c.k_slot_stride : nullptr;
+        p.to[2] = kept ? (unsigned char *)c.v + page * c.v_page_stride + place * c.v_slot_stride : nullptr;
+        p.scales[0] = kept ? (uint32_t *)c.k_scales + page * c.ks_page_stride + place * c.ks_slot_stride : nullptr;
+        p.scales[1] = kept ? (uint32_t *)c.v_scales + page * c.vs_page_stride + place * c.vs_slot_stride : nullptr;
+    }
+    angles_of(d, a.by_half, t0, tokens, angles);
+    __syncthreads();
     // (a warp's segments go round the loop together: they meet in shuffles)
-    for (int j0 = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2); j0 < all || !ready; j0 += U * step) {
+    for (int j0 = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2); j0 < all; j0 += U * step) {
         Raw<VEC> r0[U], r1[U];
-        const T *from[U];
+        // 0: queries, 1: keys, 2: values; and the head among them
+        auto kind_of = [&](int h, int &own) {
+            const int kind = (h >= q_heads) + (h >= q_heads + kv_heads);
+            own = h - (kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + kv_heads);
+            return kind;
+        };
+        auto source = [&](int token, int kind, int own) { return places[token].from[kind] + own * (kind == 0 ? d.q_head_stride : kind == 1 ? d.k_head_stride : d.v_head_stride); };
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int j = j0 + u * step + seg;
-            from[u] = nullptr;
             if (j >= all || !some) continue;
-            const int token = (int)a.by_heads.quotient(j), h = j - token * heads;
-            const int64_t t = t0 + token;
-            const T *const src = h < q_heads ? (const T *)d.q + t * d.q_token_stride + h * d.q_head_stride
-                               : h < q_heads + kv_heads ? (const T *)d.k + t * d.k_token_stride + (h - q_heads) * d.k_head_stride
-                                                        : (const T *)d.v + t * d.v_token_stride + (h - q_heads - kv_heads) * d.v_head_stride;
-            from[u] = src;
+            const int token = (int)a.by_heads.quotient(j);
+            int own;
+            const int kind = kind_of(j - token * heads, own);
+            const T *const src = source(token, kind, own);
             r0[u].load(src + e0);
             if (second) r1[u].load(src + e1);
-        }
-        if (!ready) {                            // once, while the first values are under way
-            ready = true;
-            if ((int)threadIdx.x < tokens) {
-                const int64_t slot = d.slots[t0 + threadIdx.x];
-                const bool kept = slot >= 0 && slot < c.pages * c.page_size;
-                const int64_t page = kept ? slot / c.page_size : 0, place = slot - page * c.page_size;
-                places[threadIdx.x][0] = kept ? page * c.k_page_stride + place * c.k_slot_stride : -1;
-                places[threadIdx.x][1] = page * c.v_page_stride + place * c.v_slot_stride;
-                places[threadIdx.x][2] = page * c.ks_page_stride + place * c.ks_slot_stride;
-                places[threadIdx.x][3] = page * c.vs_page_stride + place * c.vs_slot_stride;
-            }
-            angles_of(d, a.by_half, t0, tokens, angles);
-            __syncthreads();
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (j0 + u * step >= all) break;     // (the whole warp)
-            const int j = j0 + u * step + seg, token = j < all ? (int)a.by_heads.quotient(j) : 0, h = j - token * heads;
-            const bool is_query = h < q_heads, is_value = h >= q_heads + kv_heads;
+            const int j = j0 + u * step + seg, token = j < all ? (int)a.by_heads.quotient(j) : 0;
+            int own;
+            const int kind = kind_of(j - token * heads, own);
             const float *const angle = angles + token * R;
+            const bool mine = j < all && some;
             float x0[VEC], x1[VEC];
-            if (from[u]) {
+            if (mine) {
                 r0[u].template to<T>(x0);
                 if (second) r1[u].template to<T>(x1);
-                if (turns && !is_value) {
+                if (turns && kind != 2) {
                     float cs[VEC], sn[VEC];
                     const float *const at = angle + it * VEC;
 #pragma unroll
@@ -164,112 +215,118 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
                         for (int i = 0; i < VEC; i++) turn_pair(x0[i], x1[i], cs[i], sn[i]);
                     }
                 }
-                if (is_query) {
-                    r0[u].template from<T>(x0);
-                    T *const dst = (T *)d.q_out + (t0 + token) * d.out_token_stride + h * d.out_head_stride;
-                    r0[u].store(dst + e0);
-                    if (second) {
-                        r1[u].template from<T>(x1);
-                        r1[u].store(dst + e1);
-                    }
+            }
+            void *const to = places[token].to[kind];
+            if (mine && kind == 0) {
+                r0[u].template from<T>(x0);
+                T *const dst = (T *)to + own * d.out_head_stride;
+                r0[u].store(dst + e0);
+                if (second) {
+                    r1[u].template from<T>(x1);
+                    r1[u].store(dst + e1);
                 }
             }
-            const bool kept = from[u] && !is_query && places[token][0] >= 0;
+            const bool kept = mine && kind != 0 && to;
             if (!__any_sync(kAll, kept)) continue;
             // ---- least and largest value of the groups of this thread's vectors, and largest size in the head
             float least[2] = {INFINITY, INFINITY}, most[2] = {-INFINITY, -INFINITY};
             if (kept) {
+                least[0] = most[0] = x0[0];
 #pragma unroll
-                for (int i = 0; i < VEC; i++) { least[0] = fminf(least[0], x0[i]); most[0] = fmaxf(most[0], x0[i]); }
+                for (int i = 1; i + 1 < VEC; i += 2) { least[0] = least_of(least[0], x0[i], x0[i + 1]); most[0] = most_of(most[0], x0[i], x0[i + 1]); }
+                least[0] = least_of(least[0], x0[VEC - 1]);
+                most[0] = most_of(most[0], x0[VEC - 1]);
                 if (second) {
+                    least[1] = most[1] = x1[0];
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) { least[1] = fminf(least[1], x1[i]); most[1] = fmaxf(most[1], x1[i]); }
+                    for (int i = 1; i + 1 < VEC; i += 2) { least[1] = least_of(least[1], x1[i], x1[i + 1]); most[1] = most_of(most[1], x1[i], x1[i + 1]); }
+                    least[1] = least_of(least[1], x1[VEC - 1]);
+                    most[1] = most_of(most[1], x1[VEC - 1]);
                 }
             }
-            float lo[2], hi[2], size = 0.f;
-            for (int g = 0; g < groups; g++) {
-                float l = fminf(g0 == g ? least[0] : INFINITY, g1 == g ? least[1] : INFINITY), m = fmaxf(g0 == g ? most[0] : -INFINITY, g1 == g ? most[1] : -INFINITY);
-                for (int o = L >> 1; o >= 1; o >>= 1) {
-                    l = fminf(l, __shfl_xor_sync(kAll, l, o));
-                    m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+            float lo[2], hi[2], size;
+            auto over_lanes = [&](float &l, float &m) {
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1)
+                    if (o < L) {
+                        l = least_of(l, __shfl_xor_sync(kAll, l, o));
+                        m = most_of(m, __shfl_xor_sync(kAll, m, o));
+                    }
+            };
+            if (groups == 1) {
+                lo[0] = least_of(least[0], least[1]);
+                hi[0] = most_of(most[0], most[1]);
+                over_lanes(lo[0], hi[0]);
+                lo[1] = lo[0];
+                hi[1] = hi[0];
+                size = most_of(-lo[0], hi[0]);
+            } else {
+                size = 0.f;
+                for (int g = 0; g < groups; g++) {
+                    float l = least_of(g0 == g ? least[0] : INFINITY, g1 == g ? least[1] : INFINITY), m = most_of(g0 == g ? most[0] : -INFINITY, g1 == g ? most[1] : -INFINITY);
+                    over_lanes(l, m);
+                    if (g0 == g) { lo[0] = l; hi[0] = m; }
+                    if (g1 == g) { lo[1] = l; hi[1] = m; }
+                    size = most_of(size, -l, m);
                 }
-                if (g0 == g) { lo[0] = l; hi[0] = m; }
-                if (g1 == g) { lo[1] = l; hi[1] = m; }
-                size = fmaxf(size, fmaxf(fabsf(l), fabsf(m)));
+                if (!second) { lo[1] = lo[0]; hi[1] = hi[0]; }
             }
-            if (!second) { lo[1] = lo[0]; hi[1] = hi[0]; }
             // A turned value a c - b s is off by at most 2^-24 (|b s| + |x|), and both are at most sqrt(c c + s s) |(a, b)| = |(x, y)| <= 2 size
-            const float tol = is_value || R == 0 ? 0.f : 0x1p-22f * size;
+            const float tol = kind == 2 || R == 0 ? 0.f : 0x1p-22f * size;
             Held held[2] = {};
             bool sure = true;
             if (kept) {
                 sure = held_of<T>(lo[0], hi[0], tol, held[0]);
-                if (g1 == g0) held[1] = held[0];
-                else sure = held_of<T>(lo[1], hi[1], tol, held[1]) && sure;
+                held[1] = held[0];
+                if (g1 != g0) sure = held_of<T>(lo[1], hi[1], tol, held[1]) && sure;
             }
             if (!__all_sync(kAll, sure)) {       // the same in FP64, for the whole warp
-                double l0[2] = {INFINITY, INFINITY}, m0[2] = {-INFINITY, -INFINITY};
-                if (kept) {
-                    for (int v = 0; v < (second ? 2 : 1); v++)
-#pragma unroll 1
-                        for (int i = 0; i < VEC; i++) {
-                            const double x = exact_element<T, INTERLEAVED>(from[u], (v ? e1 : e0) + i, angle, is_value ? 0 : R);
-                            l0[v] = x < l0[v] ? x : l0[v];
-                            m0[v] = x > m0[v] ? x : m0[v];
-                            if (!(fabs(x) < INFINITY)) m0[v] = INFINITY;
-                        }
-                }
-                for (int g = 0; g < groups; g++) {
-                    double l = INFINITY, m = -INFINITY;
-                    for (int v = 0; v < 2; v++)
-                        if ((v ? g1 : g0) == g) { l = l0[v] < l ? l0[v] : l; m = m0[v] > m ? m0[v] : m; }
-                    for (int o = L >> 1; o >= 1; o >>= 1) {
-                        const double l2 = __shfl_xor_sync(kAll, l, o), m2 = __shfl_xor_sync(kAll, m, o);
-                        l = l2 < l ? l2 : l;
-                        m = m2 > m ? m2 : m;
-                    }
-                    if (!kept) continue;
-                    if (g0 == g) held[0] = held_of<T>(l, m);
-                    if (g1 == g) held[1] = held_of<T>(l, m);
-                }
-            }
-            // ---- codes.  What is left of a value behind its code, x - zero - code scale, shows in FP32 whether the code is the next one; it is off by
-            // tol and the rounding of x - zero (2^-24 of at most 15.5 scales; in a value it is 0 where there is a tie)
-            uint32_t word[2] = {0, 0};
-            bool odd[2] = {false, false};        // a value that is no number
-            if (kept) {
-#pragma unroll
-                for (int v = 0; v < 2; v++) {
-                    if (v && !second) break;
-                    const float s = held[v].s, z = held[v].z, inverse = s > 0.f ? __frcp_rn(s) : 0.f;
-                    const float limit = s > 0.f ? 0.5f * s - (is_value ? 0.f : tol + s * 0x1p-20f) : INFINITY;
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        const float x = (v ? x1[i] : x0[i]) - z;
-                        const float m = fminf(fmaxf(x * inverse, 0.f), 15.f) + 12582912.f;        // (1.5 2^23: the sum's last bits are the code)
-                        uint32_t code = __float_as_uint(m) & 15u;
-                        if (!(fabsf(__fmaf_rn(-(m - 12582912.f), s, x)) < limit)) {
-                            const double exact = exact_element<T, INTERLEAVED>(from[u], (v ? e1 : e0) + i, angle, is_value ? 0 : R);
-                            odd[v] = odd[v] || !(fabs(exact) < INFINITY);
-                            const double y = rint((exact - (double)z) / (double)s);
-                            code = s > 0.f && y > 0.0 ? (y < 15.0 ? (uint32_t)y : 15u) : 0u;
-                        }
-                        word[v] |= code << (4 * i);
-                    }
-                }
-            }
-            if (__any_sync(kAll, odd[0] || odd[1])) {
-                for (int g = 0; g < groups; g++) {
-                    const uint32_t who = __ballot_sync(kAll, (odd[0] && g0 == g) || (odd[1] && g1 == g));
-                    if (!(who >> (seg << a.lanes_log2) & (L == 32 ? kAll : (1u << L) - 1))) continue;
-                    if (g0 == g) { word[0] = 0; held[0].bits = kNoNumber; }
-                    if (g1 == g) { word[1] = 0; held[1].bits = kNoNumber; }
-                }
+                const HeldTwo exact = exact_held<T, VEC, INTERLEAVED>(kept ? source(token, kind, own) : nullptr, e0, second ? e1 : -1, angle, kind == 2 ? 0 : R, groups, g0, g1, L);
+                if (kept) { held[0] = exact.of[0]; held[1] = exact.of[1]; }
             }
             if (!kept) continue;
-            const int hk = h - q_heads - (is_value ? kv_heads : 0);
-            unsigned char *const codes = is_value ? (unsigned char *)c.v + places[token][1] + hk * c.v_head_stride : (unsigned char *)c.k + places[token][0] + hk * c.k_head_stride;
-            uint32_t *const scales = is_value ? (uint32_t *)c.v_scales + places[token][3] + hk * c.vs_head_stride : (uint32_t *)c.k_scales + places[token][2] + hk * c.ks_head_stride;
+            // ---- codes: 15 times a saturated (x - zero) / (15 scale), and how far that is from a whole number.  Off by 15 2^-21.5 for the inverse and the sums' roundings, by
+            // 2^-24 of the zero's own quotient, and for a key by tol: what is that near a half is taken again.
+            uint32_t word[2], unsure = 0;
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                if (v && !second) break;
+                const float s = held[v].s, z = held[v].z, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f, by = inverse * (1.f / 15.f), less = -z * by;
+                // (quotients that are no normal numbers of FP32: all of them again)
+                const float limit = s > 0.f && !(s > 0x1p-100f && s < 0x1p100f) ? -1.f : 0.5f - (0x1p-17f + 0x1p-23f * fabsf(z * inverse) + tol * inverse);
+                uint32_t sum = 0;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    const float t = __saturatef(__fmaf_rn(v ? x1[i] : x0[i], by, less)), m = __fmaf_rn(t, 15.f, 12582912.f);      // (1.5 2^23: the sum's last bits are the code)
+                    if (!(fabsf(__fmaf_rn(t, 15.f, -(m - 12582912.f))) < limit)) unsure |= 1u << (v * VEC + i);
+                    sum += __float_as_uint(m) << (4 * i);
+                }
+                word[v] = sum - 0x4B400000u * (VEC == 8 ? 0x11111111u : 0x1111u);
+            }
+            while (unsure) {
+                const int n = __ffs(unsure) - 1, v = n >= VEC, i = n - v * VEC, e = (v ? e1 : e0) + i;
+                unsure &= unsure - 1;
+                const float s = v ? held[1].s : held[0].s, z = v ? held[1].z : held[0].z;
+                const T *const src = source(token, kind, own);
+                uint32_t code;
+                const float raw = Half<T>::to_float(src[e]), x = raw - z;
+                if (kind == 2 && s > 0.f && fabsf(x) <= FLT_MAX) {
+                    // A value: what is left behind a code is exact, and half a scale is a tie unless x - zero was rounded
+                    const float m = fminf(fmaxf(x * __fdividef(1.f, s), 0.f), 15.f) + 12582912.f, left = __fmaf_rn(-(m - 12582912.f), s, x);
+                    const float lost = (raw - (x + z)) + ((x + z) - x - z);                       // raw = z + x + lost
+                    const float over = fabsf(left) == 0.5f * s ? (left > 0.f ? lost : -lost) : fabsf(left) - 0.5f * s;
+                    code = __float_as_uint(m) & 15u;
+                    if (over > 0.f || (over == 0.f && (code & 1u))) code = (uint32_t)min(max((int)code + (left > 0.f ? 1 : -1), 0), 15);
+                } else {
+                    const double exact = exact_element<T, INTERLEAVED>(src, e, angle, kind == 2 ? 0 : R), y = rint((exact - (double)z) / (double)s);
+                    code = s > 0.f && y > 0.0 ? (y < 15.0 ? (uint32_t)y : 15u) : 0u;
+                }
+                const uint32_t keep = ~(15u << (4 * i)), put = code << (4 * i);
+                if (v) word[1] = (word[1] & keep) | put;
+                else word[0] = (word[0] & keep) | put;
+            }
+            unsigned char *const codes = (unsigned char *)to + own * (kind == 2 ? c.v_head_stride : c.k_head_stride);
+            uint32_t *const scales = places[token].scales[kind - 1] + own * (kind == 2 ? c.vs_head_stride : c.ks_head_stride);
 #pragma unroll
             for (int v = 0; v < 2; v++) {
                 if (v && !second) break;
@@ -287,7 +344,7 @@ static int launch_quantise(QuantiseArgs &a, cudaStream_t stream)
 {
     const int64_t heads = a.d.q_heads + 2 * a.c.kv_heads, rows = 256 >> a.lanes_log2, sms = device_sm_count(current_device_index());
     // as rotary_append_kernel does it: four tokens of a CTA where there are many, the heads of one over several CTAs where there are few
-    a.together = a.d.tokens >= 8 * sms ? 4 : 1;
+    a.together = a.d.tokens >= 2 * kMostTogether * sms ? kMostTogether : 1;
     const int64_t ctas = ceil_div(a.d.tokens, a.together), most = ceil_div(heads * a.together, rows);
     int64_t y = ceil_div(2 * sms, ctas);
     y = y < 1 ? 1 : y < most ? y : most;
@@ -298,8 +355,8 @@ static int launch_quantise(QuantiseArgs &a, cudaStream_t stream)
 }
 
 // ---- reading back: value = round16(zero + scale code), one multiply-add in the type itself ------------------------------------------------------
-// An item is 8 codes of a head, 4 bytes in and 16 out; a CTA has a few tokens, whose places pass through shared memory.  Bound by HBM, four fifths of it
-// what is written.
+// An item is 8 codes of a head, 4 bytes in and 16 out.  A thread has an item of every token (or every few) of its CTA, whose places pass through shared memory.
+// Bound by HBM, four fifths of it what is written.
 struct ReadArgs {
     ortho_b200_read_quantised_desc d;
     ortho_b200_quantised_cache c;
@@ -334,53 +391,57 @@ __global__ void __launch_bounds__(256)
 read_quantised_kernel(const __grid_constant__ ReadArgs a)
 {
     constexpr int U = 4;                         // items of a thread in flight together
-    __shared__ int64_t places[kMostRead][4];
+    struct Places { const unsigned char *codes[2]; const uint32_t *scales[2]; };                  // of a token's keys and values; outside the cache: NULL
+    __shared__ Places places[kMostRead];
     const auto &d = a.d;
     const auto &c = a.c;
     const int64_t t0 = (int64_t)blockIdx.x * a.together;
-    const int tokens = d.count - t0 < a.together ? (int)(d.count - t0) : a.together, chunks = (int)c.head_dim / 8, per_cache = (int)c.kv_heads * chunks, all = tokens * 2 * per_cache;
+    const int tokens = d.count - t0 < a.together ? (int)(d.count - t0) : a.together, chunks = (int)c.head_dim / 8, per_cache = (int)c.kv_heads * chunks, per_token = 2 * per_cache;
     griddep_wait();
     griddep_launch();
     if ((int)threadIdx.x < tokens) {
         const int64_t slot = d.slots[t0 + threadIdx.x];
         const bool in = slot >= 0 && slot < c.pages * c.page_size;
         const int64_t page = in ? slot / c.page_size : 0, place = slot - page * c.page_size;
-        places[threadIdx.x][0] = in ? page * c.k_page_stride + place * c.k_slot_stride : -1;
-        places[threadIdx.x][1] = page * c.v_page_stride + place * c.v_slot_stride;
-        places[threadIdx.x][2] = page * c.ks_page_stride + place * c.ks_slot_stride;
-        places[threadIdx.x][3] = page * c.vs_page_stride + place * c.vs_slot_stride;
+        Places &p = places[threadIdx.x];
+        p.codes[0] = in ? (const unsigned char *)c.k + page * c.k_page_stride + place * c.k_slot_stride : nullptr;
+        p.codes[1] = in ? (const unsigned char *)c.v + page * c.v_page_stride + place * c.v_slot_stride : nullptr;
+        p.scales[0] = (const uint32_t *)c.k_scales + page * c.ks_page_stride + place * c.ks_slot_stride;
+        p.scales[1] = (const uint32_t *)c.v_scales + page * c.vs_page_stride + place * c.vs_slot_stride;
     }
     __syncthreads();
-    for (int i0 = (int)(blockIdx.y * blockDim.x + threadIdx.x); i0 < all; i0 += U * (int)(gridDim.y * blockDim.x)) {
-        uint32_t code[U], held[U];
-        uint4 *to[U];
+    // several tokens side by side where one has few items; the threads behind the last whole token rest
+    const int row = (int)a.by_token.quotient(threadIdx.x), rows = per_token <= 256 ? 256 / per_token : 1;
+    for (int at = (int)(blockIdx.y * 256 + threadIdx.x) - row * per_token; at < per_token && row < rows; at += (int)gridDim.y * 256) {
+        const int is_value = at >= per_cache, rest = at - (is_value ? per_cache : 0), h = (int)a.by_chunk.quotient(rest), chunk = rest - h * chunks;
+        const int64_t code_at = h * (is_value ? c.v_head_stride : c.k_head_stride) + chunk * 4;
+        const int64_t scale_at = h * (is_value ? c.vs_head_stride : c.ks_head_stride) + (int)a.by_group.quotient(chunk);
+        const int64_t stride = is_value ? d.v_token_stride : d.k_token_stride;
+        T *const out = (T *)(is_value ? d.v_out : d.k_out) + t0 * stride + h * (is_value ? d.v_head_stride : d.k_head_stride) + chunk * 8;
+        for (int token0 = row; token0 < tokens; token0 += U * rows) {
+            uint32_t code[U], held[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = i0 + u * (int)(gridDim.y * blockDim.x);
-            to[u] = nullptr;
-            if (i >= all) break;
-            const int token = (int)a.by_token.quotient(i), at = i - token * 2 * per_cache;
-            const bool is_value = at >= per_cache;
-            const int rest = at - (is_value ? per_cache : 0), h = (int)a.by_chunk.quotient(rest), chunk = rest - h * chunks, group = (int)a.by_group.quotient(chunk);
-            to[u] = reinterpret_cast<uint4 *>((T *)(is_value ? d.v_out : d.k_out) + (t0 + token) * (is_value ? d.v_token_stride : d.k_token_stride)
-                                              + h * (is_value ? d.v_head_stride : d.k_head_stride) + chunk * 8);
-            code[u] = held[u] = 0;
-            if (places[token][0] < 0) continue;
-            code[u] = *reinterpret_cast<const uint32_t *>(is_value ? (const unsigned char *)c.v + places[token][1] + h * c.v_head_stride + chunk * 4
-                                                                   : (const unsigned char *)c.k + places[token][0] + h * c.k_head_stride + chunk * 4);
-            held[u] = *(is_value ? (const uint32_t *)c.v_scales + places[token][3] + h * c.vs_head_stride + group
-                                 : (const uint32_t *)c.k_scales + places[token][2] + h * c.ks_head_stride + group);
-        }
+            for (int u = 0; u < U; u++) {
+                const int token = token0 + u * rows;
+                code[u] = held[u] = 0;
+                if (token >= tokens) break;
+                const unsigned char *const codes = places[token].codes[is_value];
+                if (!codes) continue;
+                code[u] = *reinterpret_cast<const uint32_t *>(codes + code_at);
+                held[u] = places[token].scales[is_value][scale_at];
+            }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (!to[u]) break;
-            const uint32_t s = __byte_perm(held[u], 0, 0x1010), z = __byte_perm(held[u], 0, 0x3232), next = code[u] >> 4;
-            uint4 y;                             // byte i of the codes in the low half, its upper code brought down in the high one
-            y.x = Codes<T>::value(__byte_perm(code[u], next, 0x4400), s, z);
-            y.y = Codes<T>::value(__byte_perm(code[u], next, 0x5511), s, z);
-            y.z = Codes<T>::value(__byte_perm(code[u], next, 0x6622), s, z);
-            y.w = Codes<T>::value(__byte_perm(code[u], next, 0x7733), s, z);
-            *to[u] = y;
+            for (int u = 0; u < U; u++) {
+                const int token = token0 + u * rows;
+                if (token >= tokens) break;
+                const uint32_t s = __byte_perm(held[u], 0, 0x1010), z = __byte_perm(held[u], 0, 0x3232), next = code[u] >> 4;
+                uint4 y;                         // byte i of the codes in the low half, its upper code brought down in the high one
+                y.x = Codes<T>::value(__byte_perm(code[u], next, 0x4400), s, z);
+                y.y = Codes<T>::value(__byte_perm(code[u], next, 0x5511), s, z);
+                y.z = Codes<T>::value(__byte_perm(code[u], next, 0x6622), s, z);
+                y.w = Codes<T>::value(__byte_perm(code[u], next, 0x7733), s, z);
+                *reinterpret_cast<uint4 *>(out + token * stride) = y;
+            }
         }
     }
 }
@@ -451,11 +512,10 @@ extern "C" int ortho_b200_read_quantised(const ortho_b200_read_quantised_desc *d
     a.d = *d;
     a.c = *c;
     const int64_t chunks = c->head_dim / 8, items = 2 * c->kv_heads * chunks, sms = device_sm_count(current_device_index());
-    // some 4096 items to a CTA where there are enough of them; where there are few, a token's items over several CTAs
-    const int64_t together = ceil_div(4096, items), fair = ceil_div(d->count, 8 * sms);
-    a.together = (int)(together < fair ? together : fair);
-    if (a.together > kMostRead) a.together = kMostRead;
-    const int64_t ctas = ceil_div(d->count, a.together), most = ceil_div(items * a.together, 1024);
+    // eight CTAs an SM where there are tokens enough, and four items a thread
+    const int64_t rows = items <= 256 ? 256 / items : 1, fair = ceil_div(d->count, 8 * sms), few = 4 * rows < kMostRead ? 4 * rows : kMostRead;
+    a.together = (int)(fair < few ? fair : fair < kMostRead ? fair : kMostRead);
+    const int64_t ctas = ceil_div(d->count, a.together), most = ceil_div(items, 256);
     int64_t y = ceil_div(4 * sms, ctas);
     y = y < 1 ? 1 : y < most ? y : most;
     a.by_token = FastDiv((uint32_t)items);
