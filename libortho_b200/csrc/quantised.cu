@@ -6,6 +6,7 @@
 // arithmetic: FP32 does the work and knows its own error, and what lies within that of a border is taken again in FP64 from the raw values (a key in
 // some 1500 groups, and ties).  A turned key is a c - b s of an 11-bit and a 24-bit factor each, exact in FP64 up to its last sum.
 #include <cfloat>
+#include <type_traits>
 
 #include "quantised.cuh"
 #include "rotary.cuh"
@@ -17,7 +18,7 @@ constexpr int kMostTogether = 4;                 // tokens of a CTA
 struct QuantiseArgs {
     ortho_b200_rotary_append_desc d;
     ortho_b200_quantised_cache c;
-    int turned, items, lanes_log2, together;     // as in rotary.cu; lanes of a head (a power of two)
+    int turned, lanes_log2, together;            // items (two vectors) of a head that turn; lanes of a head, a power of two; tokens of a CTA
     FastDiv by_heads, by_half;
 };
 
@@ -86,260 +87,319 @@ __device__ __forceinline__ Held held_of(double lo, double hi)
     return h;
 }
 
-// Scales and zeros of a warp's heads in FP64: of the groups g0 and g1 that a thread's vectors at e0 and e1 (-1: none) belong to.  src NULL: no head.
-struct HeldTwo { Held of[2]; };
-template <class T, int VEC, bool INTERLEAVED>
-__device__ __noinline__ HeldTwo exact_held(const T *src, int e0, int e1, const float *angles, int rotary, int groups, int g0, int g1, int lanes)
+__device__ __forceinline__ uint32_t exact_code(double x, float s, float z)
 {
-    double least[2] = {INFINITY, INFINITY}, most[2] = {-INFINITY, -INFINITY};
+    const double q = rint((x - (double)z) / (double)s);
+    return s > 0.f && q > 0.0 ? (q < 15.0 ? (uint32_t)q : 15u) : 0u;
+}
+
+// A warp's heads all in FP64, from the raw values to what is stored.  src NULL: no head; e0, e1: where a thread's vectors start (-1: none).
+template <class T, int VEC, bool INTERLEAVED, int GROUPS>
+__device__ __noinline__ void exact_heads(const T *src, int e0, int e1, const float *angles, int rotary, int lanes, unsigned char *codes, uint32_t *scales)
+{
+    double least[GROUPS], most[GROUPS];
 #pragma unroll
+    for (int g = 0; g < GROUPS; g++) { least[g] = INFINITY; most[g] = -INFINITY; }
+#pragma unroll 1
     for (int v = 0; v < 2; v++) {
         const int e = v ? e1 : e0;
-        if (!src || e < 0) break;
+        if (!src || e < 0) continue;
+        double l = INFINITY, m = -INFINITY;
 #pragma unroll 1
         for (int i = 0; i < VEC; i++) {
             const double x = exact_element<T, INTERLEAVED>(src, e + i, angles, rotary);
-            least[v] = x < least[v] ? x : least[v];
-            most[v] = x > most[v] ? x : most[v];
-            if (!(fabs(x) < INFINITY)) most[v] = INFINITY;
+            l = x < l ? x : l;
+            m = x > m ? x : m;
+            if (!(fabs(x) < INFINITY)) m = INFINITY;
         }
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++)
+            if (GROUPS == 1 || e / kQuantGroup == g) { least[g] = l < least[g] ? l : least[g]; most[g] = m > most[g] ? m : most[g]; }
     }
-    HeldTwo r = {};
-    for (int g = 0; g < groups; g++) {
-        double l = INFINITY, m = -INFINITY;
-        if (g0 == g) { l = least[0]; m = most[0]; }
-        if (g1 == g) { l = least[1] < l ? least[1] : l; m = most[1] > m ? most[1] : m; }
+    Held held[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
         for (int o = lanes >> 1; o >= 1; o >>= 1) {
-            const double l2 = __shfl_xor_sync(0xffffffffu, l, o), m2 = __shfl_xor_sync(0xffffffffu, m, o);
-            l = l2 < l ? l2 : l;
-            m = m2 > m ? m2 : m;
+            const double l = __shfl_xor_sync(0xffffffffu, least[g], o), m = __shfl_xor_sync(0xffffffffu, most[g], o);
+            least[g] = l < least[g] ? l : least[g];
+            most[g] = m > most[g] ? m : most[g];
         }
-        const Held h = held_of<T>(l, m);
-        if (g0 == g) r.of[0] = h;
-        if (g1 == g) r.of[1] = h;
+        held[g] = held_of<T>(least[g], most[g]);
     }
-    return r;
+    if (!src) return;
+#pragma unroll 1
+    for (int v = 0; v < 2; v++) {
+        const int e = v ? e1 : e0;
+        if (e < 0) continue;
+        float s = held[0].s, z = held[0].z;
+#pragma unroll
+        for (int g = 1; g < GROUPS; g++)
+            if (e / kQuantGroup == g) { s = held[g].s; z = held[g].z; }
+        uint32_t word = 0;
+#pragma unroll 1
+        for (int i = 0; i < VEC; i++) word |= exact_code(exact_element<T, INTERLEAVED>(src, e + i, angles, rotary), s, z) << (4 * i);
+        if constexpr (VEC == 8) *reinterpret_cast<uint32_t *>(codes + e / 2) = word;
+        else *reinterpret_cast<uint16_t *>(codes + e / 2) = (uint16_t)word;
+    }
+    if ((threadIdx.x & (lanes - 1)) == 0) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) scales[g] = held[g].bits;
+    }
 }
 
-template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 3)
+// Bytes from global to a thread's own place in shared memory
+template <int BYTES> __device__ __forceinline__ void copy_own(uint32_t dst, const void *src)
+{
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+constexpr int kAhead = 4;                   // rows of a thread that are under way
+
+// A row is a head of a token; a warp has 32 / L of them at a time, L lanes each, a lane two vectors of VEC values.  The rows to come are copied ahead into a place of
+// their thread's own in shared memory, so that neither registers nor barriers are spent on them and unsure values are read again from there.
+template <class T, int VEC, bool INTERLEAVED, int GROUPS>
+__global__ void __launch_bounds__(256, 4)
 quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
 {
-    constexpr int U = 1;                    // rows of a segment whose values are in flight together
     constexpr uint32_t kAll = 0xffffffffu;
-    extern __shared__ __align__(16) float angles[];                            // [tokens][rotary]: cosines, then sines
-    struct Places { const T *from[3]; void *to[3]; uint32_t *scales[2]; };     // of a token's queries, keys and values; no place in the cache: NULL
+    extern __shared__ __align__(16) unsigned char smem[];                      // [kAhead][2][256] vectors; [tokens][rotary]: cosines, then sines
+    struct Places { unsigned char *to[3]; uint32_t *scales[3]; };              // of a token's queries, keys and values; no place in the cache: NULL
     __shared__ Places places[kMostTogether];
+    __shared__ int64_t apart[3][2];              // heads in them: in bytes, in pairs
+    float *const angles = reinterpret_cast<float *>(smem + kAhead * 2 * 256 * VEC * 2);
     const auto &d = a.d;
     const auto &c = a.c;
     const int64_t t0 = (int64_t)blockIdx.x * a.together;
     const int tokens = d.tokens - t0 < a.together ? (int)(d.tokens - t0) : a.together;
     const int R = (int)d.rotary, half = R / 2, D = (int)c.head_dim, q_heads = (int)d.q_heads, kv_heads = (int)c.kv_heads, heads = q_heads + 2 * kv_heads, all = tokens * heads;
     const int L = 1 << a.lanes_log2, it = threadIdx.x & (L - 1), seg = (threadIdx.x & 31) >> a.lanes_log2, rows = 256 >> a.lanes_log2, step = (int)gridDim.y * rows;
-    const int groups = (int)c.groups, width = D / groups;
-    const bool some = it < a.items, turns = it < a.turned;
-    int e0, e1;                                  // elements that this thread's two vectors start with
+    const bool turns = it < a.turned;
+    int e0, e1;                                  // elements that this thread's vectors start with; -1: none
     if (!turns) { e0 = R + 2 * (it - a.turned) * VEC; e1 = e0 + VEC; }
     else if (INTERLEAVED) { e0 = 2 * it * VEC; e1 = e0 + VEC; }
     else { e0 = it * VEC; e1 = e0 + half; }
-    const bool second = some && e1 < D;
-    const int g0 = groups == 1 ? 0 : e0 / kQuantGroup, g1 = groups == 1 ? 0 : e1 / kQuantGroup;
+    if (e0 >= D) e0 = -1;
+    if (e1 >= D) e1 = -1;
+    // 0: queries, 1: keys, 2: values; and the head among them
+    auto kind_of = [&](int h, int &own) {
+        const int kind = (h >= q_heads) + (h >= q_heads + kv_heads);
+        own = h - (kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + kv_heads);
+        return kind;
+    };
+    auto source = [&](int token, int h) {
+        int own;
+        const int kind = kind_of(h, own);
+        const int64_t by_token = kind == 0 ? d.q_token_stride : kind == 1 ? d.k_token_stride : d.v_token_stride;
+        const int64_t by_head = kind == 0 ? d.q_head_stride : kind == 1 ? d.k_head_stride : d.v_head_stride;
+        return (const T *)(kind == 0 ? d.q : kind == 1 ? d.k : d.v) + (uint32_t)(t0 + token) * by_token + (uint32_t)own * by_head;
+    };
+    const int first = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2) + seg;
+    auto place = [&](int stage, int v) { return smem + ((stage * 2 + v) * 256 + threadIdx.x) * (VEC * 2); };
+    auto issue = [&](int j, int stage) {
+        if (j < all && e0 >= 0) {
+            const int token = (int)a.by_heads.quotient(j);
+            const T *const src = source(token, j - token * heads);
+            copy_own<VEC * 2>(shared_addr(place(stage, 0)), src + e0);
+            if (e1 >= 0) copy_own<VEC * 2>(shared_addr(place(stage, 1)), src + e1);
+        }
+        copy_commit();
+    };
     griddep_wait();
     griddep_launch();
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; i++) issue(first + i * step, i);
     if ((int)threadIdx.x < tokens) {
         const int64_t t = t0 + threadIdx.x, slot = d.slots[t];
         const bool kept = slot >= 0 && slot < c.pages * c.page_size;
-        const int64_t page = kept ? slot / c.page_size : 0, place = slot - page * c.page_size;
+        const int64_t page = !kept ? 0 : slot <= 0x7FFFFFFF ? (int64_t)((uint32_t)slot / (uint32_t)c.page_size) : slot / c.page_size, in = slot - page * c.page_size;
         Places &p = places[threadIdx.x];
-        p.from[0] = (const T *)d.q + t * d.q_token_stride;
-        p.from[1] = (const T *)d.k + t * d.k_token_stride;
-        p.from[2] = (const T *)d.v + t * d.v_token_stride;
-        p.to[0] = (T *)d.q_out + t * d.out_token_stride;
-        p.to[1] = kept ? (unsigned char *)c.k + page * c.k_page_stride + place * c.k_slot_stride : nullptr;
-        p.to[2] = kept ? (unsigned char *)c.v + page * c.v_page_stride + place * c.v_slot_stride : nullptr;
-        p.scales[0] = kept ? (uint32_t *)c.k_scales + page * c.ks_page_stride + place * c.ks_slot_stride : nullptr;
-        p.scales[1] = kept ? (uint32_t *)c.v_scales + page * c.vs_page_stride + place * c.vs_slot_stride : nullptr;
+        p.to[0] = (unsigned char *)((T *)d.q_out + t * d.out_token_stride);
+        p.scales[0] = nullptr;
+        p.to[1] = kept ? (unsigned char *)c.k + page * c.k_page_stride + in * c.k_slot_stride : nullptr;
+        p.to[2] = kept ? (unsigned char *)c.v + page * c.v_page_stride + in * c.v_slot_stride : nullptr;
+        p.scales[1] = kept ? (uint32_t *)c.k_scales + page * c.ks_page_stride + in * c.ks_slot_stride : nullptr;
+        p.scales[2] = kept ? (uint32_t *)c.v_scales + page * c.vs_page_stride + in * c.vs_slot_stride : nullptr;
+    }
+    if (threadIdx.x == 0) {
+        apart[0][0] = d.out_head_stride * 2;
+        apart[1][0] = c.k_head_stride;
+        apart[2][0] = c.v_head_stride;
+        apart[1][1] = c.ks_head_stride;
+        apart[2][1] = c.vs_head_stride;
     }
     angles_of(d, a.by_half, t0, tokens, angles);
     __syncthreads();
+
+    int stage = 0;
     // (a warp's segments go round the loop together: they meet in shuffles)
-    for (int j0 = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2); j0 < all; j0 += U * step) {
-        Raw<VEC> r0[U], r1[U];
-        // 0: queries, 1: keys, 2: values; and the head among them
-        auto kind_of = [&](int h, int &own) {
-            const int kind = (h >= q_heads) + (h >= q_heads + kv_heads);
-            own = h - (kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + kv_heads);
-            return kind;
-        };
-        auto source = [&](int token, int kind, int own) { return places[token].from[kind] + own * (kind == 0 ? d.q_head_stride : kind == 1 ? d.k_head_stride : d.v_head_stride); };
+    for (int j = first; j - seg < all; j += step, stage = stage == kAhead - 1 ? 0 : stage + 1) {
+        issue(j + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
+        copy_wait<kAhead - 1>();
+        const int token = j < all ? (int)a.by_heads.quotient(j) : 0;
+        int own;
+        const int kind = kind_of(j - token * heads, own);
+        const bool mine = j < all && e0 >= 0, is_value = kind == 2;
+        const float *const angle = angles + token * R;
+        unsigned char *const base = places[token].to[kind], *const to = base + (uint32_t)own * apart[kind][0];
+        const bool kept = mine && kind != 0 && base;
+        float x[2][VEC];
+        {
+            Raw<VEC> r;
+            r.load(place(stage, 0));
+            r.template to<T>(x[0]);
+            r.load(place(stage, 1));             // (what lies there, where there is no second vector, is not used)
+            r.template to<T>(x[1]);
+        }
+        if (turns && !is_value) {
+            const float *const at = angle + it * VEC;
+            float cs[VEC], sn[VEC];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int j = j0 + u * step + seg;
-            if (j >= all || !some) continue;
-            const int token = (int)a.by_heads.quotient(j);
-            int own;
-            const int kind = kind_of(j - token * heads, own);
-            const T *const src = source(token, kind, own);
-            r0[u].load(src + e0);
-            if (second) r1[u].load(src + e1);
+            for (int i = 0; i < VEC; i += 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(at + i), z = *reinterpret_cast<const float4 *>(at + half + i);
+                cs[i] = y.x; cs[i + 1] = y.y; cs[i + 2] = y.z; cs[i + 3] = y.w;
+                sn[i] = z.x; sn[i + 1] = z.y; sn[i + 2] = z.z; sn[i + 3] = z.w;
+            }
+            if (INTERLEAVED) {
+#pragma unroll
+                for (int i = 0; i + 1 < VEC; i += 2) {
+                    turn_pair(x[0][i], x[0][i + 1], cs[i / 2], sn[i / 2]);
+                    turn_pair(x[1][i], x[1][i + 1], cs[(VEC + i) / 2], sn[(VEC + i) / 2]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) turn_pair(x[0][i], x[1][i], cs[i], sn[i]);
+            }
+        }
+        if (mine && kind == 0) {
+            T *const dst = (T *)to;
+            Raw<VEC> r;
+            r.template from<T>(x[0]);
+            r.store(dst + e0);
+            r.template from<T>(x[1]);
+            if (e1 >= 0) r.store(dst + e1);
+        }
+        if (!__any_sync(kAll, kept)) continue;
+        // ---- least and largest value of each group, and the largest size in the head
+        float lo[GROUPS], hi[GROUPS], size = 0.f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) { lo[g] = INFINITY; hi[g] = -INFINITY; }
+        if (kept) {
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const int e = v ? e1 : e0;
+                float l = least_of(x[v][0], x[v][1], x[v][2]), m = most_of(x[v][0], x[v][1], x[v][2]);
+#pragma unroll
+                for (int i = 3; i + 1 < VEC; i += 2) { l = least_of(l, x[v][i], x[v][i + 1]); m = most_of(m, x[v][i], x[v][i + 1]); }
+                l = least_of(l, x[v][VEC - 1]);
+                m = most_of(m, x[v][VEC - 1]);
+                if (e < 0) { l = INFINITY; m = -INFINITY; }
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++)
+                    if (GROUPS == 1 || e / kQuantGroup == g) { lo[g] = least_of(lo[g], l); hi[g] = most_of(hi[g], m); }
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (j0 + u * step >= all) break;     // (the whole warp)
-            const int j = j0 + u * step + seg, token = j < all ? (int)a.by_heads.quotient(j) : 0;
-            int own;
-            const int kind = kind_of(j - token * heads, own);
-            const float *const angle = angles + token * R;
-            const bool mine = j < all && some;
-            float x0[VEC], x1[VEC];
-            if (mine) {
-                r0[u].template to<T>(x0);
-                if (second) r1[u].template to<T>(x1);
-                if (turns && kind != 2) {
-                    float cs[VEC], sn[VEC];
-                    const float *const at = angle + it * VEC;
+        for (int o = 16; o >= 1; o >>= 1)
+            if (o < L) {
 #pragma unroll
-                    for (int i = 0; i < VEC; i += 4) {
-                        const float4 x = *reinterpret_cast<const float4 *>(at + i), y = *reinterpret_cast<const float4 *>(at + half + i);
-                        cs[i] = x.x; cs[i + 1] = x.y; cs[i + 2] = x.z; cs[i + 3] = x.w;
-                        sn[i] = y.x; sn[i + 1] = y.y; sn[i + 2] = y.z; sn[i + 3] = y.w;
-                    }
-                    if (INTERLEAVED) {
-#pragma unroll
-                        for (int i = 0; i + 1 < VEC; i += 2) {
-                            turn_pair(x0[i], x0[i + 1], cs[i / 2], sn[i / 2]);
-                            turn_pair(x1[i], x1[i + 1], cs[(VEC + i) / 2], sn[(VEC + i) / 2]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < VEC; i++) turn_pair(x0[i], x1[i], cs[i], sn[i]);
-                    }
+                for (int g = 0; g < GROUPS; g++) {
+                    lo[g] = least_of(lo[g], __shfl_xor_sync(kAll, lo[g], o));
+                    hi[g] = most_of(hi[g], __shfl_xor_sync(kAll, hi[g], o));
                 }
             }
-            void *const to = places[token].to[kind];
-            if (mine && kind == 0) {
-                r0[u].template from<T>(x0);
-                T *const dst = (T *)to + own * d.out_head_stride;
-                r0[u].store(dst + e0);
-                if (second) {
-                    r1[u].template from<T>(x1);
-                    r1[u].store(dst + e1);
-                }
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) size = most_of(size, -lo[g], hi[g]);
+        // A turned value a c - b s is off by at most 2^-24 (|b s| + |x|), and both are at most sqrt(c c + s s) |(a, b)| = |(x, y)| <= 2 size
+        const float tol = is_value || R == 0 ? 0.f : 0x1p-22f * size;
+        Held held[GROUPS];
+        bool sure = true;
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) sure = held_of<T>(lo[g], hi[g], tol, held[g]) && sure;
+        uint32_t *const scales = places[token].scales[kind] + (uint32_t)own * apart[kind][1];
+        if (!__all_sync(kAll, sure || !kept)) {
+            exact_heads<T, VEC, INTERLEAVED, GROUPS>(kept ? source(token, j - token * heads) : nullptr, e0, e1, angle, is_value ? 0 : R, L, to, scales);
+            continue;
+        }
+        if (!kept) continue;
+        // ---- codes: 15 times a saturated (x - zero) / (15 scale), and how far that is from a whole number.  Off by 15 2^-21.5 for the inverse and the sums' roundings, by
+        // 2^-24 of the zero's own quotient, and for a key by tol: what is that near a half is taken again.
+        float by[GROUPS], less[GROUPS], limit[GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            const float s = held[g].s, z = held[g].z, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
+            by[g] = inverse * (1.f / 15.f);
+            less[g] = -z * by[g];
+            // (quotients that are no normal numbers of FP32: all of them again)
+            limit[g] = s > 0.f && !(s > 0x1p-100f && s < 0x1p100f) ? -1.f : 0.5f - (0x1p-17f + 0x1p-23f * fabsf(z * inverse) + tol * inverse);
+        }
+        uint32_t word[2], unsure = 0;
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            const int e = v ? e1 : e0;
+            float b = by[0], l = less[0], most = limit[0];
+#pragma unroll
+            for (int g = 1; g < GROUPS; g++)
+                if (e / kQuantGroup == g) { b = by[g]; l = less[g]; most = limit[g]; }
+            uint32_t sum = 0;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                const float t = __saturatef(__fmaf_rn(x[v][i], b, l)), m = __fmaf_rn(t, 15.f, 12582912.f);        // (1.5 2^23: the sum's last bits are the code)
+                if (!(fabsf(__fmaf_rn(t, 15.f, -(m - 12582912.f))) < most)) unsure |= 1u << (v * VEC + i);
+                sum += __float_as_uint(m) << (4 * i);
             }
-            const bool kept = mine && kind != 0 && to;
-            if (!__any_sync(kAll, kept)) continue;
-            // ---- least and largest value of the groups of this thread's vectors, and largest size in the head
-            float least[2] = {INFINITY, INFINITY}, most[2] = {-INFINITY, -INFINITY};
-            if (kept) {
-                least[0] = most[0] = x0[0];
+            if (v && e < 0) unsure &= (1u << VEC) - 1;
+            word[v] = sum - 0x4B400000u * (VEC == 8 ? 0x11111111u : 0x1111u);
+        }
+        while (unsure) {
+            const int n = __ffs(unsure) - 1, v = n / VEC, i = n % VEC, e = (v ? e1 : e0) + i;
+            unsure &= unsure - 1;
+            float s = held[0].s, z = held[0].z;
 #pragma unroll
-                for (int i = 1; i + 1 < VEC; i += 2) { least[0] = least_of(least[0], x0[i], x0[i + 1]); most[0] = most_of(most[0], x0[i], x0[i + 1]); }
-                least[0] = least_of(least[0], x0[VEC - 1]);
-                most[0] = most_of(most[0], x0[VEC - 1]);
-                if (second) {
-                    least[1] = most[1] = x1[0];
-#pragma unroll
-                    for (int i = 1; i + 1 < VEC; i += 2) { least[1] = least_of(least[1], x1[i], x1[i + 1]); most[1] = most_of(most[1], x1[i], x1[i + 1]); }
-                    least[1] = least_of(least[1], x1[VEC - 1]);
-                    most[1] = most_of(most[1], x1[VEC - 1]);
-                }
-            }
-            float lo[2], hi[2], size;
-            auto over_lanes = [&](float &l, float &m) {
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1)
-                    if (o < L) {
-                        l = least_of(l, __shfl_xor_sync(kAll, l, o));
-                        m = most_of(m, __shfl_xor_sync(kAll, m, o));
-                    }
-            };
-            if (groups == 1) {
-                lo[0] = least_of(least[0], least[1]);
-                hi[0] = most_of(most[0], most[1]);
-                over_lanes(lo[0], hi[0]);
-                lo[1] = lo[0];
-                hi[1] = hi[0];
-                size = most_of(-lo[0], hi[0]);
+            for (int g = 1; g < GROUPS; g++)
+                if (e / kQuantGroup == g) { s = held[g].s; z = held[g].z; }
+            const T *const raws = reinterpret_cast<const T *>(place(stage, v));
+            const float raw = Half<T>::to_float(raws[i]), y = raw - z;
+            uint32_t code;
+            if (is_value && s > 0.f && fabsf(y) <= FLT_MAX) {
+                // A value: what is left behind a code is exact, and half a scale is a tie unless x - zero was rounded
+                const float m = fminf(fmaxf(y * __fdividef(1.f, s), 0.f), 15.f) + 12582912.f, left = __fmaf_rn(-(m - 12582912.f), s, y);
+                const float lost = (raw - (y + z)) + ((y + z) - y - z);                           // raw = z + y + lost
+                const float over = fabsf(left) == 0.5f * s ? (left > 0.f ? lost : -lost) : fabsf(left) - 0.5f * s;
+                code = __float_as_uint(m) & 15u;
+                if (over > 0.f || (over == 0.f && (code & 1u))) code = (uint32_t)min(max((int)code + (left > 0.f ? 1 : -1), 0), 15);
             } else {
-                size = 0.f;
-                for (int g = 0; g < groups; g++) {
-                    float l = least_of(g0 == g ? least[0] : INFINITY, g1 == g ? least[1] : INFINITY), m = most_of(g0 == g ? most[0] : -INFINITY, g1 == g ? most[1] : -INFINITY);
-                    over_lanes(l, m);
-                    if (g0 == g) { lo[0] = l; hi[0] = m; }
-                    if (g1 == g) { lo[1] = l; hi[1] = m; }
-                    size = most_of(size, -l, m);
+                double exact = (double)raw;
+                if (turns && !is_value) {        // the other element of the pair, and which of the two this one is
+                    const bool upper = INTERLEAVED ? i & 1 : v;
+                    const double other = (double)Half<T>::to_float(INTERLEAVED ? raws[i ^ 1] : reinterpret_cast<const T *>(place(stage, v ^ 1))[i]);
+                    const int pair = it * VEC + (INTERLEAVED ? (v * VEC + i) / 2 : i);
+                    const double co = (double)angle[pair], si = (double)angle[half + pair];
+                    exact = upper ? exact * co + other * si : exact * co - other * si;
                 }
-                if (!second) { lo[1] = lo[0]; hi[1] = hi[0]; }
+                code = exact_code(exact, s, z);
             }
-            // A turned value a c - b s is off by at most 2^-24 (|b s| + |x|), and both are at most sqrt(c c + s s) |(a, b)| = |(x, y)| <= 2 size
-            const float tol = kind == 2 || R == 0 ? 0.f : 0x1p-22f * size;
-            Held held[2] = {};
-            bool sure = true;
-            if (kept) {
-                sure = held_of<T>(lo[0], hi[0], tol, held[0]);
-                held[1] = held[0];
-                if (g1 != g0) sure = held_of<T>(lo[1], hi[1], tol, held[1]) && sure;
-            }
-            if (!__all_sync(kAll, sure)) {       // the same in FP64, for the whole warp
-                const HeldTwo exact = exact_held<T, VEC, INTERLEAVED>(kept ? source(token, kind, own) : nullptr, e0, second ? e1 : -1, angle, kind == 2 ? 0 : R, groups, g0, g1, L);
-                if (kept) { held[0] = exact.of[0]; held[1] = exact.of[1]; }
-            }
-            if (!kept) continue;
-            // ---- codes: 15 times a saturated (x - zero) / (15 scale), and how far that is from a whole number.  Off by 15 2^-21.5 for the inverse and the sums' roundings, by
-            // 2^-24 of the zero's own quotient, and for a key by tol: what is that near a half is taken again.
-            uint32_t word[2], unsure = 0;
+            const uint32_t keep = ~(15u << (4 * i)), put = code << (4 * i);
+            if (v) word[1] = (word[1] & keep) | put;
+            else word[0] = (word[0] & keep) | put;
+        }
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                if (v && !second) break;
-                const float s = held[v].s, z = held[v].z, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f, by = inverse * (1.f / 15.f), less = -z * by;
-                // (quotients that are no normal numbers of FP32: all of them again)
-                const float limit = s > 0.f && !(s > 0x1p-100f && s < 0x1p100f) ? -1.f : 0.5f - (0x1p-17f + 0x1p-23f * fabsf(z * inverse) + tol * inverse);
-                uint32_t sum = 0;
+        for (int v = 0; v < 2; v++) {
+            const int e = v ? e1 : e0;
+            if (e >= 0) {
+                if constexpr (VEC == 8) *reinterpret_cast<uint32_t *>(to + e / 2) = word[v];
+                else *reinterpret_cast<uint16_t *>(to + e / 2) = (uint16_t)word[v];
+            }
+        }
+        if (it == 0) {
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const float t = __saturatef(__fmaf_rn(v ? x1[i] : x0[i], by, less)), m = __fmaf_rn(t, 15.f, 12582912.f);      // (1.5 2^23: the sum's last bits are the code)
-                    if (!(fabsf(__fmaf_rn(t, 15.f, -(m - 12582912.f))) < limit)) unsure |= 1u << (v * VEC + i);
-                    sum += __float_as_uint(m) << (4 * i);
-                }
-                word[v] = sum - 0x4B400000u * (VEC == 8 ? 0x11111111u : 0x1111u);
-            }
-            while (unsure) {
-                const int n = __ffs(unsure) - 1, v = n >= VEC, i = n - v * VEC, e = (v ? e1 : e0) + i;
-                unsure &= unsure - 1;
-                const float s = v ? held[1].s : held[0].s, z = v ? held[1].z : held[0].z;
-                const T *const src = source(token, kind, own);
-                uint32_t code;
-                const float raw = Half<T>::to_float(src[e]), x = raw - z;
-                if (kind == 2 && s > 0.f && fabsf(x) <= FLT_MAX) {
-                    // A value: what is left behind a code is exact, and half a scale is a tie unless x - zero was rounded
-                    const float m = fminf(fmaxf(x * __fdividef(1.f, s), 0.f), 15.f) + 12582912.f, left = __fmaf_rn(-(m - 12582912.f), s, x);
-                    const float lost = (raw - (x + z)) + ((x + z) - x - z);                       // raw = z + x + lost
-                    const float over = fabsf(left) == 0.5f * s ? (left > 0.f ? lost : -lost) : fabsf(left) - 0.5f * s;
-                    code = __float_as_uint(m) & 15u;
-                    if (over > 0.f || (over == 0.f && (code & 1u))) code = (uint32_t)min(max((int)code + (left > 0.f ? 1 : -1), 0), 15);
-                } else {
-                    const double exact = exact_element<T, INTERLEAVED>(src, e, angle, kind == 2 ? 0 : R), y = rint((exact - (double)z) / (double)s);
-                    code = s > 0.f && y > 0.0 ? (y < 15.0 ? (uint32_t)y : 15u) : 0u;
-                }
-                const uint32_t keep = ~(15u << (4 * i)), put = code << (4 * i);
-                if (v) word[1] = (word[1] & keep) | put;
-                else word[0] = (word[0] & keep) | put;
-            }
-            unsigned char *const codes = (unsigned char *)to + own * (kind == 2 ? c.v_head_stride : c.k_head_stride);
-            uint32_t *const scales = places[token].scales[kind - 1] + own * (kind == 2 ? c.vs_head_stride : c.ks_head_stride);
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-                if (v && !second) break;
-                const int e = v ? e1 : e0;
-                if constexpr (VEC == 8) *reinterpret_cast<uint32_t *>(codes + e / 2) = word[v];
-                else *reinterpret_cast<uint16_t *>(codes + e / 2) = (uint16_t)word[v];
-                if (e % width == 0) scales[v ? g1 : g0] = held[v].bits;
-            }
+            for (int g = 0; g < GROUPS; g++) scales[g] = held[g].bits;
         }
     }
+    copy_wait<0>();
 }
 
-template <class T, int VEC>
+template <class T, int VEC, int GROUPS>
 static int launch_quantise(QuantiseArgs &a, cudaStream_t stream)
 {
     const int64_t heads = a.d.q_heads + 2 * a.c.kv_heads, rows = 256 >> a.lanes_log2, sms = device_sm_count(current_device_index());
@@ -349,9 +409,20 @@ static int launch_quantise(QuantiseArgs &a, cudaStream_t stream)
     int64_t y = ceil_div(2 * sms, ctas);
     y = y < 1 ? 1 : y < most ? y : most;
     const dim3 grid((unsigned)ctas, (unsigned)y);
-    const size_t smem = (size_t)(a.together * a.d.rotary * 4);
-    return a.d.interleaved ? launch_dependent(quantise_append_kernel<T, VEC, true>, grid, 256, smem, stream, a)
-                           : launch_dependent(quantise_append_kernel<T, VEC, false>, grid, 256, smem, stream, a);
+    const size_t smem = (size_t)(kAhead * 2 * 256 * VEC * 2 + a.together * a.d.rotary * 4);
+    return a.d.interleaved ? launch_dependent(quantise_append_kernel<T, VEC, true, GROUPS>, grid, 256, smem, stream, a)
+                           : launch_dependent(quantise_append_kernel<T, VEC, false, GROUPS>, grid, 256, smem, stream, a);
+}
+
+template <class T, int VEC>
+static int launch_quantise_of(QuantiseArgs &a, cudaStream_t stream)
+{
+    switch (a.c.groups) {
+    case 1: return launch_quantise<T, VEC, 1>(a, stream);
+    case 2: return launch_quantise<T, VEC, 2>(a, stream);
+    case 3: return launch_quantise<T, VEC, 3>(a, stream);
+    default: return launch_quantise<T, VEC, 4>(a, stream);
+    }
 }
 
 // ---- reading back: value = round16(zero + scale code), one multiply-add in the type itself ------------------------------------------------------
@@ -485,13 +556,13 @@ extern "C" int ortho_b200_rotary_append_quantised(const ortho_b200_rotary_append
     a.d = *d;
     a.c = *c;
     a.turned = (int)(d->rotary / 2 / vec);
-    a.items = a.turned + (int)ceil_div(d->head_dim - d->rotary, 2 * vec);
-    for (a.lanes_log2 = 0; 1 << a.lanes_log2 < a.items; a.lanes_log2++) {}     // (32 items at most)
+    const int64_t items = a.turned + ceil_div(d->head_dim - d->rotary, 2 * vec);
+    for (a.lanes_log2 = 0; 1 << a.lanes_log2 < items; a.lanes_log2++) {}       // (32 items at most)
     a.by_heads = FastDiv((uint32_t)(d->q_heads + 2 * d->kv_heads));
     a.by_half = FastDiv((uint32_t)(d->rotary ? d->rotary / 2 : 1));
     const cudaStream_t s = (cudaStream_t)stream;
-    if (d->type == ORTHO_B200_TYPE_F16) return vec == 8 ? launch_quantise<__half, 8>(a, s) : launch_quantise<__half, 4>(a, s);
-    return vec == 8 ? launch_quantise<__nv_bfloat16, 8>(a, s) : launch_quantise<__nv_bfloat16, 4>(a, s);
+    if (d->type == ORTHO_B200_TYPE_F16) return vec == 8 ? launch_quantise_of<__half, 8>(a, s) : launch_quantise_of<__half, 4>(a, s);
+    return vec == 8 ? launch_quantise_of<__nv_bfloat16, 8>(a, s) : launch_quantise_of<__nv_bfloat16, 4>(a, s);
 }
 
 extern "C" int ortho_b200_read_quantised(const ortho_b200_read_quantised_desc *d, const ortho_b200_quantised_cache *c, void *stream)
