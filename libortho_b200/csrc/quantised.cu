@@ -5,9 +5,6 @@
 // Rounding to 4 bits turns a difference in the last place of FP32 into a whole step wherever x lies next to a border, so the codes are those of exact
 // arithmetic: FP32 does the work and knows its own error, and what lies within that of a border is taken again in FP64 from the raw values (a key in
 // some 1500 groups, and ties).  A turned key is a c - b s of an 11-bit and a 24-bit factor each, exact in FP64 up to its last sum.
-#include <cfloat>
-#include <type_traits>
-
 #include "quantised.cuh"
 #include "rotary.cuh"
 
@@ -19,17 +16,17 @@ struct QuantiseArgs {
     ortho_b200_rotary_append_desc d;
     ortho_b200_quantised_cache c;
     int turned, lanes_log2, together;            // items (two vectors) of a head that turn; lanes of a head, a power of two; tokens of a CTA
-    FastDiv by_heads, by_half;
+    FastDiv by_half;
 };
 
 template <class T> struct QuantType;
 template <> struct QuantType<__half> {
-    static constexpr float safe = 30000.f;                                     // below: neither a value nor zero + 15 scale comes near the type's end
+    static constexpr float safe = 30000.f;                                     // below: neither a value nor zero + 15 scale comes near the type's end, nor a quotient FP32's
     static constexpr double beyond = 65520.0;                                  // rounds to infinity
     static __device__ __forceinline__ __half from_double(double v) { return __double2half(v); }
 };
 template <> struct QuantType<__nv_bfloat16> {
-    static constexpr float safe = 1e38f;
+    static constexpr float safe = 1e28f;
     static constexpr double beyond = 3.3961775292304957e38;
     static __device__ __forceinline__ __nv_bfloat16 from_double(double v) { return __double2bfloat16(v); }
 };
@@ -41,23 +38,11 @@ __device__ __forceinline__ float most_of(float a, float b) { float r; asm("max.N
 __device__ __forceinline__ float least_of(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 __device__ __forceinline__ float most_of(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
 
-// Element e of a head in FP64, turned or not
-template <class T, bool INTERLEAVED>
-__device__ __forceinline__ double exact_element(const T *src, int e, const float *angles, int rotary)
-{
-    if (e >= rotary) return (double)Half<T>::to_float(src[e]);
-    const int half = rotary / 2, pair = INTERLEAVED ? e >> 1 : e < half ? e : e - half;
-    const bool upper = INTERLEAVED ? e & 1 : e >= half;
-    const double a = (double)Half<T>::to_float(src[INTERLEAVED ? 2 * pair : pair]), b = (double)Half<T>::to_float(src[INTERLEAVED ? 2 * pair + 1 : pair + half]);
-    const double c = (double)angles[pair], s = (double)angles[half + pair];
-    return upper ? b * c + a * s : a * c - b * s;
-}
-
 // A group's scale and zero; `bits`: as they are stored.  A group that stands for NaN has scale 0 here, so that its codes come out as 0.
 struct Held { float s, z; uint32_t bits; };
 constexpr uint32_t kNoNumber = 0x7FFFu;
 
-// From the least and largest of values that are each off by up to `tol`; false where that, or an end of the type, could change a bit
+// From the least and largest of values that are each off by up to `tol` and are all below QuantType::safe; false where that could change a bit
 template <class T>
 __device__ __forceinline__ bool held_of(float lo, float hi, float tol, Held &h)
 {
@@ -66,8 +51,7 @@ __device__ __forceinline__ bool held_of(float lo, float hi, float tol, Held &h)
     const float2 f = Half<T>::unpack(h.bits);
     h.s = f.x;
     h.z = f.y;
-    return Half<T>::pack(q - tq, lo - tol) == Half<T>::pack(q + tq, lo + tol) && fmaxf(fabsf(lo), fabsf(hi)) < QuantType<T>::safe
-        && (q > 1e-30f || (lo == hi && tol == 0.f));
+    return Half<T>::pack(q - tq, lo - tol) == Half<T>::pack(q + tq, lo + tol) && (q > 1e-28f || (lo == hi && tol == 0.f));
 }
 template <class T>
 __device__ __forceinline__ Held held_of(double lo, double hi)
@@ -87,66 +71,6 @@ __device__ __forceinline__ Held held_of(double lo, double hi)
     return h;
 }
 
-__device__ __forceinline__ uint32_t exact_code(double x, float s, float z)
-{
-    const double q = rint((x - (double)z) / (double)s);
-    return s > 0.f && q > 0.0 ? (q < 15.0 ? (uint32_t)q : 15u) : 0u;
-}
-
-// A warp's heads all in FP64, from the raw values to what is stored.  src NULL: no head; e0, e1: where a thread's vectors start (-1: none).
-template <class T, int VEC, bool INTERLEAVED, int GROUPS>
-__device__ __noinline__ void exact_heads(const T *src, int e0, int e1, const float *angles, int rotary, int lanes, unsigned char *codes, uint32_t *scales)
-{
-    double least[GROUPS], most[GROUPS];
-#pragma unroll
-    for (int g = 0; g < GROUPS; g++) { least[g] = INFINITY; most[g] = -INFINITY; }
-#pragma unroll 1
-    for (int v = 0; v < 2; v++) {
-        const int e = v ? e1 : e0;
-        if (!src || e < 0) continue;
-        double l = INFINITY, m = -INFINITY;
-#pragma unroll 1
-        for (int i = 0; i < VEC; i++) {
-            const double x = exact_element<T, INTERLEAVED>(src, e + i, angles, rotary);
-            l = x < l ? x : l;
-            m = x > m ? x : m;
-            if (!(fabs(x) < INFINITY)) m = INFINITY;
-        }
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++)
-            if (GROUPS == 1 || e / kQuantGroup == g) { least[g] = l < least[g] ? l : least[g]; most[g] = m > most[g] ? m : most[g]; }
-    }
-    Held held[GROUPS];
-#pragma unroll
-    for (int g = 0; g < GROUPS; g++) {
-        for (int o = lanes >> 1; o >= 1; o >>= 1) {
-            const double l = __shfl_xor_sync(0xffffffffu, least[g], o), m = __shfl_xor_sync(0xffffffffu, most[g], o);
-            least[g] = l < least[g] ? l : least[g];
-            most[g] = m > most[g] ? m : most[g];
-        }
-        held[g] = held_of<T>(least[g], most[g]);
-    }
-    if (!src) return;
-#pragma unroll 1
-    for (int v = 0; v < 2; v++) {
-        const int e = v ? e1 : e0;
-        if (e < 0) continue;
-        float s = held[0].s, z = held[0].z;
-#pragma unroll
-        for (int g = 1; g < GROUPS; g++)
-            if (e / kQuantGroup == g) { s = held[g].s; z = held[g].z; }
-        uint32_t word = 0;
-#pragma unroll 1
-        for (int i = 0; i < VEC; i++) word |= exact_code(exact_element<T, INTERLEAVED>(src, e + i, angles, rotary), s, z) << (4 * i);
-        if constexpr (VEC == 8) *reinterpret_cast<uint32_t *>(codes + e / 2) = word;
-        else *reinterpret_cast<uint16_t *>(codes + e / 2) = (uint16_t)word;
-    }
-    if ((threadIdx.x & (lanes - 1)) == 0) {
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) scales[g] = held[g].bits;
-    }
-}
-
 // Bytes from global to a thread's own place in shared memory
 template <int BYTES> __device__ __forceinline__ void copy_own(uint32_t dst, const void *src)
 {
@@ -158,8 +82,8 @@ constexpr int kAhead = 4;                   // rows of a thread that are under w
 
 // A row is a head of a token; a warp has 32 / L of them at a time, L lanes each, a lane two vectors of VEC values.  The rows to come are copied ahead into a place of
 // their thread's own in shared memory, so that neither registers nor barriers are spent on them and unsure values are read again from there.
-template <class T, int VEC, bool INTERLEAVED, int GROUPS>
-__global__ void __launch_bounds__(256, 4)
+template <class T, int VEC, bool INTERLEAVED, bool GROUPED>
+__global__ void __launch_bounds__(256, 3)
 quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
 {
     constexpr uint32_t kAll = 0xffffffffu;
@@ -172,7 +96,7 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
     const auto &c = a.c;
     const int64_t t0 = (int64_t)blockIdx.x * a.together;
     const int tokens = d.tokens - t0 < a.together ? (int)(d.tokens - t0) : a.together;
-    const int R = (int)d.rotary, half = R / 2, D = (int)c.head_dim, q_heads = (int)d.q_heads, kv_heads = (int)c.kv_heads, heads = q_heads + 2 * kv_heads, all = tokens * heads;
+    const int R = (int)d.rotary, half = R / 2, D = (int)c.head_dim, q_heads = (int)d.q_heads, kv_heads = (int)c.kv_heads, heads = q_heads + 2 * kv_heads;
     const int L = 1 << a.lanes_log2, it = threadIdx.x & (L - 1), seg = (threadIdx.x & 31) >> a.lanes_log2, rows = 256 >> a.lanes_log2, step = (int)gridDim.y * rows;
     const bool turns = it < a.turned;
     int e0, e1;                                  // elements that this thread's vectors start with; -1: none
@@ -181,34 +105,38 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
     else { e0 = it * VEC; e1 = e0 + half; }
     if (e0 >= D) e0 = -1;
     if (e1 >= D) e1 = -1;
-    // 0: queries, 1: keys, 2: values; and the head among them
+    const int groups = (int)c.groups, width = D / groups, g0 = GROUPED ? e0 / kQuantGroup : 0, g1 = GROUPED ? e1 / kQuantGroup : 0;
+    // A segment has a head of one token after the other, then its next head; kinds 0 to 2 are queries, keys and values
+    const int head0 = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2);                // the warp's first
     auto kind_of = [&](int h, int &own) {
         const int kind = (h >= q_heads) + (h >= q_heads + kv_heads);
         own = h - (kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + kv_heads);
         return kind;
     };
-    auto source = [&](int token, int h) {
-        int own;
-        const int kind = kind_of(h, own);
-        const int64_t by_token = kind == 0 ? d.q_token_stride : kind == 1 ? d.k_token_stride : d.v_token_stride;
-        const int64_t by_head = kind == 0 ? d.q_head_stride : kind == 1 ? d.k_head_stride : d.v_head_stride;
-        return (const T *)(kind == 0 ? d.q : kind == 1 ? d.k : d.v) + (uint32_t)(t0 + token) * by_token + (uint32_t)own * by_head;
-    };
-    const int first = (int)blockIdx.y * rows + ((int)threadIdx.x >> 5) * (32 >> a.lanes_log2) + seg;
     auto place = [&](int stage, int v) { return smem + ((stage * 2 + v) * 256 + threadIdx.x) * (VEC * 2); };
-    auto issue = [&](int j, int stage) {
-        if (j < all && e0 >= 0) {
-            const int token = (int)a.by_heads.quotient(j);
-            const T *const src = source(token, j - token * heads);
-            copy_own<VEC * 2>(shared_addr(place(stage, 0)), src + e0);
-            if (e1 >= 0) copy_own<VEC * 2>(shared_addr(place(stage, 1)), src + e1);
+    int next_head = head0 + seg, next_token = 0;                               // of the row that is copied next
+    const T *next = nullptr;
+    int64_t next_step = 0;
+    auto issue = [&](int stage) {
+        if (next_head < heads && e0 >= 0) {
+            if (next_token == 0) {
+                int own;
+                const int kind = kind_of(next_head, own);
+                next_step = kind == 0 ? d.q_token_stride : kind == 1 ? d.k_token_stride : d.v_token_stride;
+                next = (const T *)(kind == 0 ? d.q : kind == 1 ? d.k : d.v) + t0 * next_step
+                     + (uint32_t)own * (kind == 0 ? d.q_head_stride : kind == 1 ? d.k_head_stride : d.v_head_stride);
+            }
+            copy_own<VEC * 2>(shared_addr(place(stage, 0)), next + e0);
+            if (e1 >= 0) copy_own<VEC * 2>(shared_addr(place(stage, 1)), next + e1);
+            next += next_step;
         }
+        if (++next_token == tokens) { next_token = 0; next_head += step; }
         copy_commit();
     };
     griddep_wait();
     griddep_launch();
 #pragma unroll
-    for (int i = 0; i < kAhead - 1; i++) issue(first + i * step, i);
+    for (int i = 0; i < kAhead - 1; i++) issue(i);
     if ((int)threadIdx.x < tokens) {
         const int64_t t = t0 + threadIdx.x, slot = d.slots[t];
         const bool kept = slot >= 0 && slot < c.pages * c.page_size;
@@ -231,17 +159,24 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
     angles_of(d, a.by_half, t0, tokens, angles);
     __syncthreads();
 
-    int stage = 0;
+    int stage = 0, token = tokens - 1, head = head0 + seg - step, kind = 0;
+    int64_t code_at = 0, scale_at = 0;
     // (a warp's segments go round the loop together: they meet in shuffles)
-    for (int j = first; j - seg < all; j += step, stage = stage == kAhead - 1 ? 0 : stage + 1) {
-        issue(j + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
+    for (;; stage = stage == kAhead - 1 ? 0 : stage + 1) {
+        if (++token == tokens) {
+            token = 0;
+            head += step;
+            if (head - seg >= heads) break;
+            int own;
+            kind = kind_of(head, own);
+            code_at = (uint32_t)own * apart[kind][0];
+            scale_at = (uint32_t)own * apart[kind][1];
+        }
+        issue(stage == 0 ? kAhead - 1 : stage - 1);
         copy_wait<kAhead - 1>();
-        const int token = j < all ? (int)a.by_heads.quotient(j) : 0;
-        int own;
-        const int kind = kind_of(j - token * heads, own);
-        const bool mine = j < all && e0 >= 0, is_value = kind == 2;
+        const bool mine = head < heads && e0 >= 0, is_value = kind == 2;
         const float *const angle = angles + token * R;
-        unsigned char *const base = places[token].to[kind], *const to = base + (uint32_t)own * apart[kind][0];
+        unsigned char *const base = places[token].to[kind], *const to = base + code_at;
         const bool kept = mine && kind != 0 && base;
         float x[2][VEC];
         {
@@ -280,88 +215,122 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
             if (e1 >= 0) r.store(dst + e1);
         }
         if (!__any_sync(kAll, kept)) continue;
-        // ---- least and largest value of each group, and the largest size in the head
-        float lo[GROUPS], hi[GROUPS], size = 0.f;
+        // ---- least and largest value of this thread's vectors, then of their groups, and the largest size in the head
+        float lo[2], hi[2], size;
 #pragma unroll
-        for (int g = 0; g < GROUPS; g++) { lo[g] = INFINITY; hi[g] = -INFINITY; }
-        if (kept) {
+        for (int v = 0; v < 2; v++) {
+            float l = least_of(x[v][0], x[v][1], x[v][2]), m = most_of(x[v][0], x[v][1], x[v][2]);
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const int e = v ? e1 : e0;
-                float l = least_of(x[v][0], x[v][1], x[v][2]), m = most_of(x[v][0], x[v][1], x[v][2]);
-#pragma unroll
-                for (int i = 3; i + 1 < VEC; i += 2) { l = least_of(l, x[v][i], x[v][i + 1]); m = most_of(m, x[v][i], x[v][i + 1]); }
-                l = least_of(l, x[v][VEC - 1]);
-                m = most_of(m, x[v][VEC - 1]);
-                if (e < 0) { l = INFINITY; m = -INFINITY; }
-#pragma unroll
-                for (int g = 0; g < GROUPS; g++)
-                    if (GROUPS == 1 || e / kQuantGroup == g) { lo[g] = least_of(lo[g], l); hi[g] = most_of(hi[g], m); }
-            }
+            for (int i = 3; i + 1 < VEC; i += 2) { l = least_of(l, x[v][i], x[v][i + 1]); m = most_of(m, x[v][i], x[v][i + 1]); }
+            const bool some = kept && (v ? e1 : e0) >= 0;
+            lo[v] = some ? least_of(l, x[v][VEC - 1]) : INFINITY;
+            hi[v] = some ? most_of(m, x[v][VEC - 1]) : -INFINITY;
         }
+        auto over_lanes = [&](float &l, float &m) {
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1)
-            if (o < L) {
-#pragma unroll
-                for (int g = 0; g < GROUPS; g++) {
-                    lo[g] = least_of(lo[g], __shfl_xor_sync(kAll, lo[g], o));
-                    hi[g] = most_of(hi[g], __shfl_xor_sync(kAll, hi[g], o));
+            for (int o = 16; o >= 1; o >>= 1)
+                if (o < L) {
+                    l = least_of(l, __shfl_xor_sync(kAll, l, o));
+                    m = most_of(m, __shfl_xor_sync(kAll, m, o));
                 }
+        };
+        if constexpr (GROUPED) {
+            float own_lo[2] = {lo[0], lo[1]}, own_hi[2] = {hi[0], hi[1]};
+            size = 0.f;
+            for (int g = 0; g < groups; g++) {
+                float l = least_of(g0 == g ? own_lo[0] : INFINITY, g1 == g ? own_lo[1] : INFINITY), m = most_of(g0 == g ? own_hi[0] : -INFINITY, g1 == g ? own_hi[1] : -INFINITY);
+                over_lanes(l, m);
+                if (g0 == g) { lo[0] = l; hi[0] = m; }
+                if (g1 == g) { lo[1] = l; hi[1] = m; }
+                size = most_of(size, -l, m);
             }
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) size = most_of(size, -lo[g], hi[g]);
+        } else {
+            lo[0] = least_of(lo[0], lo[1]);
+            hi[0] = most_of(hi[0], hi[1]);
+            over_lanes(lo[0], hi[0]);
+            lo[1] = lo[0];
+            hi[1] = hi[0];
+            size = most_of(-lo[0], hi[0]);
+        }
         // A turned value a c - b s is off by at most 2^-24 (|b s| + |x|), and both are at most sqrt(c c + s s) |(a, b)| = |(x, y)| <= 2 size
         const float tol = is_value || R == 0 ? 0.f : 0x1p-22f * size;
-        Held held[GROUPS];
-        bool sure = true;
+        Held held[2];
+        bool ends = false, sure = held_of<T>(lo[0], hi[0], tol, held[0]) && size < QuantType<T>::safe;
+        if constexpr (GROUPED) sure = held_of<T>(lo[1], hi[1], tol, held[1]) && sure;
+        else held[1] = held[0];
+        // A value in FP64: of vector v, number i
+        auto exact = [&](int v, int i) {
+            const T *const raws = reinterpret_cast<const T *>(place(stage, v));
+            const double raw = (double)Half<T>::to_float(raws[i]);
+            if (!turns || is_value) return raw;
+            const double other = (double)Half<T>::to_float(INTERLEAVED ? raws[i ^ 1] : reinterpret_cast<const T *>(place(stage, v ^ 1))[i]);
+            const int pair = it * VEC + (INTERLEAVED ? (v * VEC + i) / 2 : i);
+            const double co = (double)angle[pair], si = (double)angle[half + pair];
+            return (INTERLEAVED ? i & 1 : v) ? raw * co + other * si : raw * co - other * si;
+        };
+        if (!__all_sync(kAll, sure || !kept)) {  // least and largest values once more in FP64, the warp together: of those that may be
+            uint32_t may = 0;
 #pragma unroll
-        for (int g = 0; g < GROUPS; g++) sure = held_of<T>(lo[g], hi[g], tol, held[g]) && sure;
-        uint32_t *const scales = places[token].scales[kind] + (uint32_t)own * apart[kind][1];
-        if (!__all_sync(kAll, sure || !kept)) {
-            exact_heads<T, VEC, INTERLEAVED, GROUPS>(kept ? source(token, j - token * heads) : nullptr, e0, e1, angle, is_value ? 0 : R, L, to, scales);
-            continue;
+            for (int v = 0; v < 2; v++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++)
+                    if (kept && (v ? e1 : e0) >= 0 && !(x[v][i] > lo[v] + 2.f * tol && x[v][i] < hi[v] - 2.f * tol)) may |= 1u << (v * VEC + i);
+#pragma unroll 1
+            for (int g = 0; g < (GROUPED ? groups : 1); g++) {
+                uint32_t now = may & ((g0 == g ? (1u << VEC) - 1 : 0u) | (g1 == g ? ((1u << VEC) - 1) << VEC : 0u));
+                double l = INFINITY, m = -INFINITY;
+                while (now) {
+                    const int n = __ffs(now) - 1;
+                    now &= now - 1;
+                    const double y = exact(n / VEC, n % VEC);
+                    l = y < l ? y : l;
+                    m = y > m ? y : m;
+                    if (!(fabs(y) < INFINITY)) m = INFINITY;
+                }
+                __syncwarp();
+                for (int o = L >> 1; o >= 1; o >>= 1) {
+                    const double l2 = __shfl_xor_sync(kAll, l, o), m2 = __shfl_xor_sync(kAll, m, o);
+                    l = l2 < l ? l2 : l;
+                    m = m2 > m ? m2 : m;
+                }
+                const Held h = held_of<T>(l, m);
+                if (g0 == g) held[0] = h;
+                if (g1 == g) held[1] = h;
+                // quotients near the ends of FP32: all codes in FP64
+                ends = ends || (h.s > 0.f && !(h.s > 0x1p-100f && size < QuantType<T>::safe));
+            }
         }
         if (!kept) continue;
         // ---- codes: 15 times a saturated (x - zero) / (15 scale), and how far that is from a whole number.  Off by 15 2^-21.5 for the inverse and the sums' roundings, by
         // 2^-24 of the zero's own quotient, and for a key by tol: what is that near a half is taken again.
-        float by[GROUPS], less[GROUPS], limit[GROUPS];
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) {
-            const float s = held[g].s, z = held[g].z, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
-            by[g] = inverse * (1.f / 15.f);
-            less[g] = -z * by[g];
-            // (quotients that are no normal numbers of FP32: all of them again)
-            limit[g] = s > 0.f && !(s > 0x1p-100f && s < 0x1p100f) ? -1.f : 0.5f - (0x1p-17f + 0x1p-23f * fabsf(z * inverse) + tol * inverse);
-        }
         uint32_t word[2], unsure = 0;
+        float by, less, limit;
 #pragma unroll
         for (int v = 0; v < 2; v++) {
-            const int e = v ? e1 : e0;
-            float b = by[0], l = less[0], most = limit[0];
-#pragma unroll
-            for (int g = 1; g < GROUPS; g++)
-                if (e / kQuantGroup == g) { b = by[g]; l = less[g]; most = limit[g]; }
+            if (GROUPED || v == 0) {
+                const float s = held[v].s, z = held[v].z, inverse = s > 0.f ? __fdividef(1.f, s) : 0.f;
+                by = inverse * (1.f / 15.f);
+                less = -z * by;
+                limit = ends ? -1.f : (0.5f - 0x1p-17f) - (0x1p-23f * fabsf(z) + tol) * inverse;
+                if (s == 0.f) limit = 1.f;       // (code 0)
+            }
             uint32_t sum = 0;
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                const float t = __saturatef(__fmaf_rn(x[v][i], b, l)), m = __fmaf_rn(t, 15.f, 12582912.f);        // (1.5 2^23: the sum's last bits are the code)
-                if (!(fabsf(__fmaf_rn(t, 15.f, -(m - 12582912.f))) < most)) unsure |= 1u << (v * VEC + i);
+                const float t = __saturatef(__fmaf_rn(x[v][i], by, less)), m = __fmaf_rn(t, 15.f, 12582912.f);        // (1.5 2^23: the sum's last bits are the code)
+                if (!(fabsf(__fmaf_rn(t, 15.f, -(m - 12582912.f))) < limit)) unsure |= 1u << (v * VEC + i);
                 sum += __float_as_uint(m) << (4 * i);
             }
-            if (v && e < 0) unsure &= (1u << VEC) - 1;
             word[v] = sum - 0x4B400000u * (VEC == 8 ? 0x11111111u : 0x1111u);
         }
+        if (e1 < 0) unsure &= (1u << VEC) - 1;
         while (unsure) {
-            const int n = __ffs(unsure) - 1, v = n / VEC, i = n % VEC, e = (v ? e1 : e0) + i;
+            const int n = __ffs(unsure) - 1, v = n / VEC, i = n % VEC;
             unsure &= unsure - 1;
-            float s = held[0].s, z = held[0].z;
-#pragma unroll
-            for (int g = 1; g < GROUPS; g++)
-                if (e / kQuantGroup == g) { s = held[g].s; z = held[g].z; }
-            const T *const raws = reinterpret_cast<const T *>(place(stage, v));
-            const float raw = Half<T>::to_float(raws[i]), y = raw - z;
+            const float s = v ? held[1].s : held[0].s, z = v ? held[1].z : held[0].z;
+            const float raw = Half<T>::to_float(reinterpret_cast<const T *>(place(stage, v))[i]), y = raw - z;
             uint32_t code;
-            if (is_value && s > 0.f && fabsf(y) <= FLT_MAX) {
+            if (is_value && !ends) {
                 // A value: what is left behind a code is exact, and half a scale is a tie unless x - zero was rounded
                 const float m = fminf(fmaxf(y * __fdividef(1.f, s), 0.f), 15.f) + 12582912.f, left = __fmaf_rn(-(m - 12582912.f), s, y);
                 const float lost = (raw - (y + z)) + ((y + z) - y - z);                           // raw = z + y + lost
@@ -369,15 +338,8 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
                 code = __float_as_uint(m) & 15u;
                 if (over > 0.f || (over == 0.f && (code & 1u))) code = (uint32_t)min(max((int)code + (left > 0.f ? 1 : -1), 0), 15);
             } else {
-                double exact = (double)raw;
-                if (turns && !is_value) {        // the other element of the pair, and which of the two this one is
-                    const bool upper = INTERLEAVED ? i & 1 : v;
-                    const double other = (double)Half<T>::to_float(INTERLEAVED ? raws[i ^ 1] : reinterpret_cast<const T *>(place(stage, v ^ 1))[i]);
-                    const int pair = it * VEC + (INTERLEAVED ? (v * VEC + i) / 2 : i);
-                    const double co = (double)angle[pair], si = (double)angle[half + pair];
-                    exact = upper ? exact * co + other * si : exact * co - other * si;
-                }
-                code = exact_code(exact, s, z);
+                const double q = rint((exact(v, i) - (double)z) / (double)s);
+                code = q > 0.0 ? (q < 15.0 ? (uint32_t)q : 15u) : 0u;
             }
             const uint32_t keep = ~(15u << (4 * i)), put = code << (4 * i);
             if (v) word[1] = (word[1] & keep) | put;
@@ -390,39 +352,31 @@ quantise_append_kernel(const __grid_constant__ QuantiseArgs a)
                 if constexpr (VEC == 8) *reinterpret_cast<uint32_t *>(to + e / 2) = word[v];
                 else *reinterpret_cast<uint16_t *>(to + e / 2) = (uint16_t)word[v];
             }
-        }
-        if (it == 0) {
-#pragma unroll
-            for (int g = 0; g < GROUPS; g++) scales[g] = held[g].bits;
+            if (e >= 0 && e % width == 0) (places[token].scales[kind] + scale_at)[v ? g1 : g0] = held[v].bits;
         }
     }
     copy_wait<0>();
 }
 
-template <class T, int VEC, int GROUPS>
+template <class T, int VEC, bool GROUPED>
 static int launch_quantise(QuantiseArgs &a, cudaStream_t stream)
 {
     const int64_t heads = a.d.q_heads + 2 * a.c.kv_heads, rows = 256 >> a.lanes_log2, sms = device_sm_count(current_device_index());
     // as rotary_append_kernel does it: four tokens of a CTA where there are many, the heads of one over several CTAs where there are few
     a.together = a.d.tokens >= 2 * kMostTogether * sms ? kMostTogether : 1;
-    const int64_t ctas = ceil_div(a.d.tokens, a.together), most = ceil_div(heads * a.together, rows);
+    const int64_t ctas = ceil_div(a.d.tokens, a.together), most = ceil_div(heads, rows);
     int64_t y = ceil_div(2 * sms, ctas);
     y = y < 1 ? 1 : y < most ? y : most;
     const dim3 grid((unsigned)ctas, (unsigned)y);
     const size_t smem = (size_t)(kAhead * 2 * 256 * VEC * 2 + a.together * a.d.rotary * 4);
-    return a.d.interleaved ? launch_dependent(quantise_append_kernel<T, VEC, true, GROUPS>, grid, 256, smem, stream, a)
-                           : launch_dependent(quantise_append_kernel<T, VEC, false, GROUPS>, grid, 256, smem, stream, a);
+    return a.d.interleaved ? launch_dependent(quantise_append_kernel<T, VEC, true, GROUPED>, grid, 256, smem, stream, a)
+                           : launch_dependent(quantise_append_kernel<T, VEC, false, GROUPED>, grid, 256, smem, stream, a);
 }
 
 template <class T, int VEC>
 static int launch_quantise_of(QuantiseArgs &a, cudaStream_t stream)
 {
-    switch (a.c.groups) {
-    case 1: return launch_quantise<T, VEC, 1>(a, stream);
-    case 2: return launch_quantise<T, VEC, 2>(a, stream);
-    case 3: return launch_quantise<T, VEC, 3>(a, stream);
-    default: return launch_quantise<T, VEC, 4>(a, stream);
-    }
+    return a.c.groups > 1 ? launch_quantise<T, VEC, true>(a, stream) : launch_quantise<T, VEC, false>(a, stream);
 }
 
 // ---- reading back: value = round16(zero + scale code), one multiply-add in the type itself ------------------------------------------------------
@@ -558,7 +512,6 @@ extern "C" int ortho_b200_rotary_append_quantised(const ortho_b200_rotary_append
     a.turned = (int)(d->rotary / 2 / vec);
     const int64_t items = a.turned + ceil_div(d->head_dim - d->rotary, 2 * vec);
     for (a.lanes_log2 = 0; 1 << a.lanes_log2 < items; a.lanes_log2++) {}       // (32 items at most)
-    a.by_heads = FastDiv((uint32_t)(d->q_heads + 2 * d->kv_heads));
     a.by_half = FastDiv((uint32_t)(d->rotary ? d->rotary / 2 : 1));
     const cudaStream_t s = (cudaStream_t)stream;
     if (d->type == ORTHO_B200_TYPE_F16) return vec == 8 ? launch_quantise_of<__half, 8>(a, s) : launch_quantise_of<__half, 4>(a, s);
