@@ -64,13 +64,21 @@ __device__ __forceinline__ void copy4_async(uint32_t dst, const void *src, bool 
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-// Codes at bits 4 to 7 and 20 to 23 as 64 + code
-__device__ __forceinline__ uint32_t codes_64(uint32_t w) { return (w & 0x00F000F0u) | 0x54005400u; }
-// Codes at bits 0 to 3 and 16 to 19 (LOW), or 4 to 7 and 20 to 23, less 8
-template <bool LOW> __device__ __forceinline__ uint32_t codes_centred(uint32_t w)
+// (w & mask) | exponent in one instruction (the compiler makes two of it: neither constant fits it beside the other)
+__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t exponent)
 {
-    const uint32_t b = LOW ? (w & 0x000F000Fu) | 0x64006400u : (w & 0x00F000F0u) | 0x54005400u, off = LOW ? 0x64086408u : 0x54805480u;      // 1024 + 8, 64 + 8
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&off));
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(exponent));
+    return r;
+}
+// A pair of codes as FP16, at bits 0 to 3 and 16 to 19 (LOW) or 4 to 7 and 20 to 23, plus OFFSET.  They are joined with the exponent of 1024 or of 64.
+template <bool LOW, int OFFSET> __device__ __forceinline__ uint32_t codes(uint32_t w)
+{
+    const uint32_t b = LOW ? masked(w, 0x000F000Fu, 0x64006400u) : masked(w, 0x00F000F0u, 0x54005400u);
+    if (!LOW && OFFSET == 64) return b;
+    constexpr uint32_t kLess = OFFSET == 64 ? 0x63806380u : LOW ? 0x64086408u : 0x54805480u;      // 1024 - 64; 1024 + 8 and 64 + 8
+    static_assert(OFFSET == 64 || OFFSET == -8, "the constants above");
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 template <class T> __device__ __forceinline__ float2 scale_and_zero(uint32_t w) { return Half<T>::unpack(w); }
@@ -136,6 +144,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 {
     using Shape = QuantisedShape<DP, NT, GROUPED>;
     using Type = AttnType<__half>;
+    // p vs in FP16 is off by up to 2^-12, an eighth of the rounding of a BF16 output and as much as that of an FP16 one, which therefore gets the rest too
+    constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
     constexpr uint32_t kAll = 0xffffffffu;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -255,7 +265,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 
         uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
         float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
-        float o[2 * J][NT][4], top[NT][2], sum[NT][2], zeros[NT][G][2];
+        float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
+        float most[NT][2], base[NT][2];          // scores above `most` move the reference: the largest by then + kSlack, and what is taken off scores, the largest - lift
         float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
         int stage = 0, q_at = -1;
         bool started_here = true;                // the request's first unit is this CTA's
@@ -285,7 +296,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
                     }
-                    top[t][0] = top[t][1] = -INFINITY;
+                    most[t][0] = most[t][1] = -INFINITY;
+                    base[t][0] = base[t][1] = 0.f;
                     sum[t][0] = sum[t][1] = 0.f;
 #pragma unroll
                     for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
@@ -307,24 +319,23 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 // rows (keys) r and r + 8 of the tile, columns (queries) 2 t4 and the next
                 const uint32_t k_row = keys + (16 * h + r) * Shape::kPitch + t4 * 4;
 #pragma unroll
-                for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
                 for (int g = 0; g < G; g++) {
-                    float x[NT][4], odd[NT][4];
+                    float x[NT][4];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) x[t][0] = x[t][1] = x[t][2] = x[t][3] = odd[t][0] = odd[t][1] = odd[t][2] = odd[t][3] = 0.f;
+                    for (int t = 0; t < NT; t++) x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
 #pragma unroll
                     for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
                         const uint32_t w0 = load_shared(k_row + j * 16), w1 = load_shared(k_row + 8 * Shape::kPitch + j * 16);
-                        const uint32_t lower[4] = {codes_64(w0 << 4), codes_64(w1 << 4), codes_64(w0), codes_64(w1)};
-                        const uint32_t upper[4] = {codes_64(w0 >> 4), codes_64(w1 >> 4), codes_64(w0 >> 8), codes_64(w1 >> 8)};
+                        const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+                        const uint32_t lower[4] = {codes<true, 64>(w0), codes<true, 64>(w1), codes<false, 64>(w0), codes<false, 64>(w1)};
+                        const uint32_t upper[4] = {codes<true, 64>(v0), codes<true, 64>(v1), codes<false, 64>(v0), codes<false, 64>(v1)};
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             uint4 b;
                             if constexpr (Shape::kKeepQ) b = q[t][j];
                             else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
                             Half<__half>::mma(x[t], lower, b.x, b.y);
-                            Half<__half>::mma(NT <= 2 ? odd[t] : x[t], upper, b.z, b.w);           // (two chains of products where there are few)
+                            Half<__half>::mma(x[t], upper, b.z, b.w);
                         }
                     }
                     const float2 h0 = scale_and_zero<T>(load_shared(scales + ((16 * h + r) * G + g) * 4)), h1 = scale_and_zero<T>(load_shared(scales + ((16 * h + r + 8) * G + g) * 4));
@@ -333,12 +344,12 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            s[t][e] += h0.x * (NT <= 2 ? x[t][e] + odd[t][e] : x[t][e]) + z0 * q_sum[t][g][e];
-                            s[t][e + 2] += h1.x * (NT <= 2 ? x[t][e + 2] + odd[t][e + 2] : x[t][e + 2]) + z1 * q_sum[t][g][e];
+                            const float y0 = h0.x * x[t][e] + z0 * q_sum[t][g][e], y1 = h1.x * x[t][e + 2] + z1 * q_sum[t][g][e];
+                            s[t][e] = g ? s[t][e] + y0 : y0;
+                            s[t][e + 2] = g ? s[t][e + 2] + y1 : y1;
                         }
                 }
                 float2 v0[G], v1[G];             // scales and zeros of the two keys' values
-                const bool on0 = (ok >> (16 * h + r)) & 1, on1 = (ok >> (16 * h + r + 8)) & 1;
                 bool grows = false;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
@@ -350,19 +361,34 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        s[t][e] = on0 ? s[t][e] * factor[t][e] : -INFINITY;
-                        s[t][e + 2] = on1 ? s[t][e + 2] * factor[t][e] : -INFINITY;
-                        grows = grows || fmaxf(s[t][e], s[t][e + 2]) > top[t][e] + kSlack;
+                        s[t][e] *= factor[t][e];
+                        s[t][e + 2] *= factor[t][e];
+                    }
+                if ((ok >> (16 * h) & 0xFFFFu) != 0xFFFFu) {                   // keys that are not there
+                    const bool on0 = (ok >> (16 * h + r)) & 1, on1 = (ok >> (16 * h + r + 8)) & 1;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            s[t][e] = on0 ? s[t][e] : -INFINITY;
+                            s[t][e + 2] = on1 ? s[t][e + 2] : -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        grows = grows || fmaxf(s[t][e], s[t][e + 2]) > most[t][e];
                     }
                 if (__any_sync(kAll, grows)) {
-                    float most = largest;
+                    float biggest = largest;
 #pragma unroll
-                    for (int g = 0; g < G; g++) most = fmaxf(most, fmaxf(v0[g].x, v1[g].x));
-                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 4));
-                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 8));
-                    most = fmaxf(most, __shfl_xor_sync(kAll, most, 16));
+                    for (int g = 0; g < G; g++) biggest = fmaxf(biggest, fmaxf(v0[g].x, v1[g].x));
+                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 4));
+                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 8));
+                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 16));
                     // the power of two at or above it, between 2^-100 and 2^126
-                    const uint32_t up = min(max((__float_as_uint(most) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
+                    const uint32_t up = min(max((__float_as_uint(biggest) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
                     const float was = largest;
                     largest = __uint_as_float(up);
                     to_one = __uint_as_float((254u << 23) - up);
@@ -375,9 +401,12 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
-                            m = fmaxf(m, top[t][e]);
-                            keep[e] = m == -INFINITY ? 1.f : exp2_approx(top[t][e] - m);
-                            top[t][e] = m;
+                            keep[e] = 1.f;
+                            if (m > most[t][e] - kSlack) {                     // (above the reference, that is; or the first number)
+                                keep[e] = most[t][e] == -INFINITY ? 0.f : exp2_approx(base[t][e] - (m - Type::lift));
+                                most[t][e] = m + kSlack;
+                                base[t][e] = m - Type::lift;
+                            }
                             sum[t][e] *= keep[e];
 #pragma unroll
                             for (int g = 0; g < G; g++) zeros[t][g][e] *= keep[e];
@@ -394,9 +423,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float base = (top[t][e] == -INFINITY ? 0.f : top[t][e]) - Type::lift;
-                        p[t][e] = exp2_approx(s[t][e] - base);
-                        p[t][e + 2] = exp2_approx(s[t][e + 2] - base);
+                        p[t][e] = exp2_approx(s[t][e] - base[t][e]);
+                        p[t][e + 2] = exp2_approx(s[t][e + 2] - base[t][e]);
                         sum[t][e] += p[t][e] + p[t][e + 2];
                     }
                 // a lane's pairs of keys are 2 t4 and 2 t4 + 8 with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
@@ -413,14 +441,16 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         for (int i = 0; i < 2; i++) {
                             const float y0 = p[t][2 * i] * (i ? f1 : f0), y1 = p[t][2 * i + 1] * (i ? f1 : f0);
                             const uint32_t up = pack_half2(y0, y1);
-                            const float2 f = Half<__half>::unpack(up);
                             hi[t][i] = transpose8x8(up);
-                            lo[t][i] = transpose8x8(pack_half2(y0 - f.x, y1 - f.y));
+                            if constexpr (kParts == 2) {
+                                const float2 f = Half<__half>::unpack(up);
+                                lo[t][i] = transpose8x8(pack_half2(y0 - f.x, y1 - f.y));
+                            }
                         }
                     }
                     auto products = [&](int at, const uint32_t (&v)[2][4]) {   // two tiles of 16 elements
 #pragma unroll
-                        for (int part = 0; part < 2; part++)
+                        for (int part = 0; part < kParts; part++)
 #pragma unroll
                             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -428,8 +458,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     };
                     auto unpacked = [&](int at, uint32_t x, uint32_t y) {      // four codes each of a pair of keys, and of the pair 8 behind
                         const uint32_t x8 = x >> 8, y8 = y >> 8;
-                        const uint32_t v[2][4] = {{codes_centred<true>(x), codes_centred<false>(x), codes_centred<true>(y), codes_centred<false>(y)},
-                                                  {codes_centred<true>(x8), codes_centred<false>(x8), codes_centred<true>(y8), codes_centred<false>(y8)}};
+                        const uint32_t v[2][4] = {{codes<true, -8>(x), codes<false, -8>(x), codes<true, -8>(y), codes<false, -8>(y)},
+                                                  {codes<true, -8>(x8), codes<false, -8>(x8), codes<true, -8>(y8), codes<false, -8>(y8)}};
                         products(at, v);
                     };
 #pragma unroll
@@ -468,7 +498,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float l = over_keys(sum[t][e]);
-                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(top[t][e] + AttnType<T>::lift, l * kDown);
+                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(most[t][e] == -INFINITY ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
 #pragma unroll
                         for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
                     }

@@ -44,7 +44,8 @@ def held(cache, scales):
 def attention(q, k_cache, v_cache, k_scales, v_scales, table, lengths, scale, window=0, rows=None):
     """(out, lse, bound of out before its rounding, bound of lse).  A score is made of D products of a query and 64 + code <= 79, a scale, and a sum of queries times zero - 64 scales:
     D + 16 roundings of at most 2^-24 of these terms' sizes.  Weights are off by that, and by 2^-18 for the exponential, the two parts and the sums over keys of a warp; the outputs'
-    products are of at most 8 scales, and of zero + 8 scales."""
+    products are of at most 8 scales, and of zero + 8 scales.  BF16 outputs are made of one part, FP16: a weight times a scale is off by half its last place more, 2^-12."""
+    part = 2.0 ** -12 if q.dtype == torch.bfloat16 else 0.0
     B, H, D = q.shape
     P, heads, G = k_cache.shape[1], k_cache.shape[2], k_scales.shape[3]
     out = torch.zeros(B, H, D, dtype=torch.float64, device=q.device)
@@ -71,6 +72,6 @@ def attention(q, k_cache, v_cache, k_scales, v_scales, table, lengths, scale, wi
             sizes = (8 * vs[..., 0] + (vs[..., 1] + 8 * vs[..., 0]).abs()).repeat_interleave(D // G, -1)
             p = torch.softmax(s, 0)
             out[b, hs], lse[b, hs] = p.T @ v, torch.logsumexp(s, 0)
-            bound[b, hs] = (2 * off.unsqueeze(1) + len(keys) * E32) * (p.T @ sizes)
+            bound[b, hs] = (2 * off.unsqueeze(1) + len(keys) * E32 + part) * (p.T @ sizes)
             lse_bound[b, hs] = off + (len(keys) + 8) * E32 + 4 * E32 * lse[b, hs].abs()
     return out, lse, bound, lse_bound
