@@ -53,13 +53,7 @@ struct QuantisedShape {
     static constexpr int kClusterPerSm = kClusterBytes <= kFour && kPerSm >= 4 ? 4 : kClusterBytes <= kThree && kPerSm >= 3 ? 3 : kClusterBytes <= kTwo && kPerSm >= 2 ? 2 : kClusterBytes <= kOne ? 1 : 0;
 };
 
-__device__ __forceinline__ uint32_t load_shared(uint32_t addr) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory"); return v; }
-__device__ __forceinline__ uint4 load_shared16(uint32_t addr)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
+__device__ __forceinline__ uint32_t word_at(const unsigned char *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ void copy4_async(uint32_t dst, const void *src, bool on)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
@@ -81,7 +75,6 @@ template <bool LOW, int OFFSET> __device__ __forceinline__ uint32_t codes(uint32
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-template <class T> __device__ __forceinline__ float2 scale_and_zero(uint32_t w) { return Half<T>::unpack(w); }
 
 // Eight elements of a query, in memory's order, as the products take them: (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ uint4 as_codes_lie(uint4 w)
@@ -92,12 +85,12 @@ __device__ __forceinline__ uint4 as_codes_lie(uint4 w)
 // One query's operands: `row` is its place in shared memory, thread t of four has the words 4 j + t.  f: what the products are to be multiplied by;
 // sums: of its elements, per group.
 template <class T, int DP, int GROUPS>
-__device__ __forceinline__ void query_operands(uint32_t row, int t, uint4 (&w)[DP / 32], float &f, float (&sums)[GROUPS])
+__device__ __forceinline__ void query_operands(const unsigned char *row, int t, uint4 (&w)[DP / 32], float &f, float (&sums)[GROUPS])
 {
     constexpr int J = DP / 32, PER = J / GROUPS;
     f = 1.f;
 #pragma unroll
-    for (int j = 0; j < J; j++) w[j] = load_shared16(row + (4 * j + t) * 16);
+    for (int j = 0; j < J; j++) w[j] = *reinterpret_cast<const uint4 *>(row + (4 * j + t) * 16);
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         uint32_t most = 0;
 #pragma unroll
@@ -147,7 +140,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
     // p vs in FP16 is off by up to 2^-12, an eighth of the rounding of a BF16 output and as much as that of an FP16 one, which therefore gets the rest too
     constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
-    constexpr uint32_t kAll = 0xffffffffu;
+    constexpr int TILES = NT * DP <= 128 ? 2 : 1;                              // of 16 keys that are worked on together, as registers allow
+    constexpr uint32_t kAll = 0xffffffffu, kHere = TILES == 2 ? kAll : 0xFFFFu;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs &a = args.a;
     const auto &d = a.d;
@@ -175,13 +169,14 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     } else {
         // What the copies of a unit need; a lane has a key of the warp's 32, and looks its page up well ahead of its use
-        struct Ticket { int64_t b; int inner, page, place; bool valid, queries; };
+        struct Ticket { int b, inner, page, place; bool valid, queries; };
         Walk<kQUnitKeys> ahead = now;            // the unit of the next ticket
         bool more_tickets = true;
+        const int32_t *pages = d.block_table + ahead.s.row * d.table_stride;
         auto ticket = [&]() {
             Ticket t;
             t.valid = more_tickets;
-            t.b = ahead.b;
+            t.b = (int)ahead.b;
             t.inner = ahead.inner;
             t.queries = CLUSTER ? ahead.unit == rank : ahead.unit == 0 || (ahead.b == now.b && ahead.inner == now.inner && ahead.unit == now.unit);
             t.page = -1;
@@ -190,32 +185,46 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
             if (more_tickets && key < ahead.s.n) {
                 const int col = (int)a.by_page.quotient((uint32_t)key);
                 t.place = key - col * (int)d.page_size;
-                t.page = d.block_table[ahead.s.row * d.table_stride + col];
+                t.page = pages[col];
             }
             if (more_tickets) {
                 more_tickets = ahead.template more<CLUSTER>(ranks);
-                if (more_tickets) ahead.template step<CLUSTER>(d, inners, ranks);
+                if (more_tickets) {
+                    ahead.template step<CLUSTER>(d, inners, ranks);
+                    if (!CLUSTER && ahead.unit == 0) pages = d.block_table + ahead.s.row * d.table_stride;
+                }
             }
             return t;
         };
         int fresh_q = 0;                         // items issued so far: place in the ring of queries
+        int inner_at = -1, head = 0, group = 0;  // the head group that is copied, and its head's first codes and scales
+        const unsigned char *k = nullptr, *v = nullptr;
+        const uint32_t *ks = nullptr, *vs = nullptr;
         const bool alike = c.k_page_stride == c.v_page_stride && c.k_slot_stride == c.v_slot_stride;
+        const bool alike_s = c.ks_page_stride == c.vs_page_stride && c.ks_slot_stride == c.vs_slot_stride;
         auto issue = [&](const Ticket &t, int stage) {
             if (t.valid) {
-                const int head = t.inner / a.groups, group = t.inner - head * a.groups, place = t.place, page = t.page < d.pages ? t.page : -1;
-                const uint32_t ok = __ballot_sync(kAll, page >= 0);
+                if (t.inner != inner_at) {
+                    inner_at = t.inner;
+                    head = t.inner / a.groups;
+                    group = t.inner - head * a.groups;
+                    k = (const unsigned char *)c.k + head * c.k_head_stride;
+                    v = (const unsigned char *)c.v + head * c.v_head_stride;
+                    ks = (const uint32_t *)c.k_scales + head * c.ks_head_stride;
+                    vs = (const uint32_t *)c.v_scales + head * c.vs_head_stride;
+                }
+                const bool is_there = t.page >= 0 && t.page < d.pages;
+                const uint32_t page = is_there ? t.page : 0, place = is_there ? t.place : 0, ok = __ballot_sync(kAll, is_there);
                 if (lane == 0) seen[stage] = ok;
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
-                const unsigned char *const k = (const unsigned char *)c.k + head * c.k_head_stride, *const v = (const unsigned char *)c.v + head * c.v_head_stride;
                 // a lane's own key's place in the caches; the lanes that copy a row get it from there
-                const int64_t k_mine = page >= 0 ? page * c.k_page_stride + place * c.k_slot_stride : 0;
-                const int64_t v_mine = alike || page < 0 ? k_mine : page * c.v_page_stride + place * c.v_slot_stride;
+                const int64_t k_mine = page * c.k_page_stride + place * c.k_slot_stride, v_mine = alike ? k_mine : page * c.v_page_stride + place * c.v_slot_stride;
                 {
-                    const int64_t ks = page >= 0 ? page * c.ks_page_stride + place * c.ks_slot_stride : 0, vs = page >= 0 ? page * c.vs_page_stride + place * c.vs_slot_stride : 0;
+                    const int64_t ks_mine = page * c.ks_page_stride + place * c.ks_slot_stride, vs_mine = alike_s ? ks_mine : page * c.vs_page_stride + place * c.vs_slot_stride;
 #pragma unroll
                     for (int g = 0; g < G; g++) {
-                        copy4_async(dst + 2 * Shape::kCodes + (lane * G + g) * 4, (const uint32_t *)c.k_scales + ks + head * c.ks_head_stride + g, page >= 0);
-                        copy4_async(dst + 2 * Shape::kCodes + Shape::kScales + (lane * G + g) * 4, (const uint32_t *)c.v_scales + vs + head * c.vs_head_stride + g, page >= 0);
+                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8, ks + ks_mine + g, is_there);
+                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8 + 4, vs + vs_mine + g, is_there);
                     }
                 }
                 if (args.wide) {
@@ -245,7 +254,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     for (int at = tid; at < NT * DP; at += kAttnThreads) {
                         const int row = at / (DP / 8), chunk = at % (DP / 8);
                         const bool on = row < heads && chunk * 8 < D;
-                        copy16_async(qdst + row * Shape::kQPitch + chunk * 16, (const T *)d.q + t.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
+                        copy16_async(qdst + row * Shape::kQPitch + chunk * 16, (const T *)d.q + (int64_t)t.b * d.q_token_stride + (on ? (h0 + row) * d.q_head_stride + chunk * 8 : 0), on);
                     }
                     if (++fresh_q == S) fresh_q = 0;
                 }
@@ -277,7 +286,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 started_here = now.unit == 0;
                 if (++q_at == S) q_at = 0;
                 __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
-                const uint32_t src = shared_addr(q_ring + q_at * Shape::kQ) + r * Shape::kQPitch;
+                const unsigned char *const src = q_ring + q_at * Shape::kQ + r * Shape::kQPitch;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     uint4 w[J];
@@ -309,81 +318,98 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 if constexpr (!Shape::kKeepQ) __syncthreads();
             }
             const uint32_t ok = seen[stage];
-            const uint32_t keys = shared_addr(ring + stage * Shape::kStage), values = keys + Shape::kCodes, scales = values + Shape::kCodes;
+            const unsigned char *const keys = ring + stage * Shape::kStage, *const values = keys + Shape::kCodes, *const scales = values + Shape::kCodes;
             issue(pending, stage == 0 ? S - 1 : stage - 1);
             pending = ticket();
 #pragma unroll
-            for (int h = 0; h < 2; h++) {        // 16 keys
-                if (!(ok >> (16 * h) & 0xFFFFu)) continue;
-                float s[NT][4];
-                // rows (keys) r and r + 8 of the tile, columns (queries) 2 t4 and the next
-                const uint32_t k_row = keys + (16 * h + r) * Shape::kPitch + t4 * 4;
+            for (int h0 = 0; h0 < 2; h0 += TILES) {
+                const uint32_t there = ok >> (16 * h0) & kHere;
+                if (!there) continue;
+                // ---- scores of a tile of 16 keys, or of two: rows (keys) r and r + 8 of a tile, columns (queries) 2 t4 and the next
+                float s[TILES][NT][4];
+                float2 kv[TILES][2][G][2];           // scales and zeros: of key r or r + 8 of a tile, of the key and of the value
+#pragma unroll
+                for (int h = 0; h < TILES; h++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int g = 0; g < G; g++) {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(scales + ((16 * (h0 + h) + 8 * i + r) * G + g) * 8);
+                            kv[h][i][g][0] = Half<T>::unpack(w.x);
+                            kv[h][i][g][1] = Half<T>::unpack(w.y);
+                        }
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    float x[NT][4];
+                    float x[TILES][NT][4];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
+                    for (int h = 0; h < TILES; h++)
+#pragma unroll
+                        for (int t = 0; t < NT; t++) x[h][t][0] = x[h][t][1] = x[h][t][2] = x[h][t][3] = 0.f;
 #pragma unroll
                     for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
-                        const uint32_t w0 = load_shared(k_row + j * 16), w1 = load_shared(k_row + 8 * Shape::kPitch + j * 16);
-                        const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-                        const uint32_t lower[4] = {codes<true, 64>(w0), codes<true, 64>(w1), codes<false, 64>(w0), codes<false, 64>(w1)};
-                        const uint32_t upper[4] = {codes<true, 64>(v0), codes<true, 64>(v1), codes<false, 64>(v0), codes<false, 64>(v1)};
 #pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            uint4 b;
-                            if constexpr (Shape::kKeepQ) b = q[t][j];
-                            else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
-                            Half<__half>::mma(x[t], lower, b.x, b.y);
-                            Half<__half>::mma(x[t], upper, b.z, b.w);
+                        for (int h = 0; h < TILES; h++) {
+                            const unsigned char *const at = keys + (16 * (h0 + h) + r) * Shape::kPitch + t4 * 4 + j * 16;
+                            const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch), v0 = w0 >> 8, v1 = w1 >> 8;
+                            const uint32_t lower[4] = {codes<true, 64>(w0), codes<true, 64>(w1), codes<false, 64>(w0), codes<false, 64>(w1)};
+                            const uint32_t upper[4] = {codes<true, 64>(v0), codes<true, 64>(v1), codes<false, 64>(v0), codes<false, 64>(v1)};
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                uint4 b;
+                                if constexpr (Shape::kKeepQ) b = q[t][j];
+                                else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
+                                Half<__half>::mma(x[h][t], lower, b.x, b.y);
+                                Half<__half>::mma(x[h][t], upper, b.z, b.w);
+                            }
                         }
                     }
-                    const float2 h0 = scale_and_zero<T>(load_shared(scales + ((16 * h + r) * G + g) * 4)), h1 = scale_and_zero<T>(load_shared(scales + ((16 * h + r + 8) * G + g) * 4));
-                    const float z0 = h0.y - 64.f * h0.x, z1 = h1.y - 64.f * h1.x;
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                    for (int h = 0; h < TILES; h++) {
+                        const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
+                        const float z0 = a0.y - 64.f * a0.x, z1 = a1.y - 64.f * a1.x;
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float y0 = h0.x * x[t][e] + z0 * q_sum[t][g][e], y1 = h1.x * x[t][e + 2] + z1 * q_sum[t][g][e];
-                            s[t][e] = g ? s[t][e] + y0 : y0;
-                            s[t][e + 2] = g ? s[t][e + 2] + y1 : y1;
-                        }
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
+                                s[h][t][e] = g ? s[h][t][e] + y0 : y0;
+                                s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
+                            }
+                    }
                 }
-                float2 v0[G], v1[G];             // scales and zeros of the two keys' values
                 bool grows = false;
+                auto greatest = [](const float (&s)[TILES][NT][4], int t, int e) {
+                    float m = fmaxf(s[0][t][e], s[0][t][e + 2]);
+                    if constexpr (TILES == 2) m = fmaxf(m, fmaxf(s[TILES - 1][t][e], s[TILES - 1][t][e + 2]));
+                    return m;
+                };
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    v0[g] = scale_and_zero<T>(load_shared(scales + Shape::kScales + ((16 * h + r) * G + g) * 4));
-                    v1[g] = scale_and_zero<T>(load_shared(scales + Shape::kScales + ((16 * h + r + 8) * G + g) * 4));
-                    grows = grows || fmaxf(v0[g].x, v1[g].x) > largest;
-                }
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        s[t][e] *= factor[t][e];
-                        s[t][e + 2] *= factor[t][e];
-                    }
-                if ((ok >> (16 * h) & 0xFFFFu) != 0xFFFFu) {                   // keys that are not there
-                    const bool on0 = (ok >> (16 * h + r)) & 1, on1 = (ok >> (16 * h + r + 8)) & 1;
+                for (int h = 0; h < TILES; h++)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            s[t][e] = on0 ? s[t][e] : -INFINITY;
-                            s[t][e + 2] = on1 ? s[t][e + 2] : -INFINITY;
-                        }
+                        for (int e = 0; e < 4; e++) s[h][t][e] *= factor[t][e & 1];
+                if (there != kHere) {            // keys that are not there
+#pragma unroll
+                    for (int h = 0; h < TILES; h++) {
+                        const bool on0 = (there >> (16 * h + r)) & 1, on1 = (there >> (16 * h + r + 8)) & 1;
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[h][t][e] = (e < 2 ? on0 : on1) ? s[h][t][e] : -INFINITY;
+                    }
                 }
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        grows = grows || fmaxf(s[t][e], s[t][e + 2]) > most[t][e];
-                    }
-                if (__any_sync(kAll, grows)) {
-                    float biggest = largest;
+                    for (int e = 0; e < 2; e++) grows = grows || greatest(s, t, e) > most[t][e];
+                float scale_here = 0.f;
 #pragma unroll
-                    for (int g = 0; g < G; g++) biggest = fmaxf(biggest, fmaxf(v0[g].x, v1[g].x));
+                for (int h = 0; h < TILES; h++)
+#pragma unroll
+                    for (int g = 0; g < G; g++) scale_here = fmaxf(scale_here, fmaxf(kv[h][0][g][1].x, kv[h][1][g][1].x));
+                if (__any_sync(kAll, grows || scale_here > largest)) {
+                    float biggest = fmaxf(largest, scale_here);
                     biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 4));
                     biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 8));
                     biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 16));
@@ -397,7 +423,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         float keep[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            float m = fmaxf(s[t][e], s[t][e + 2]);
+                            float m = greatest(s, t, e);
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
@@ -418,61 +444,68 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         }
                     }
                 }
-                float p[NT][4];
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int h = 0; h < TILES; h++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        p[t][e] = exp2_approx(s[t][e] - base[t][e]);
-                        p[t][e + 2] = exp2_approx(s[t][e + 2] - base[t][e]);
-                        sum[t][e] += p[t][e] + p[t][e + 2];
-                    }
-                // a lane's pairs of keys are 2 t4 and 2 t4 + 8 with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
-                const uint32_t v_row = values + (16 * h + 2 * t4) * Shape::kPitch + r * 4;
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            s[h][t][e] = exp2_approx(s[h][t][e] - base[t][e]);
+                            s[h][t][e + 2] = exp2_approx(s[h][t][e + 2] - base[t][e]);
+                            sum[t][e] += s[h][t][e] + s[h][t][e + 2];
+                        }
+                // ---- values: a lane's pairs of keys are 2 t4 and 2 t4 + 8 of a tile with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    uint32_t hi[NT][2], lo[NT][2];
-                    const float f0 = v0[g].x * to_one, f1 = v1[g].x * to_one, z0 = v0[g].y + 8.f * v0[g].x, z1 = v1[g].y + 8.f * v1[g].x;
+                    uint32_t hi[TILES][NT][2], lo[TILES][NT][2];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        zeros[t][g][0] += p[t][0] * z0 + p[t][2] * z1;
-                        zeros[t][g][1] += p[t][1] * z0 + p[t][3] * z1;
+                    for (int h = 0; h < TILES; h++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const float y0 = p[t][2 * i] * (i ? f1 : f0), y1 = p[t][2 * i + 1] * (i ? f1 : f0);
-                            const uint32_t up = pack_half2(y0, y1);
-                            hi[t][i] = transpose8x8(up);
-                            if constexpr (kParts == 2) {
-                                const float2 f = Half<__half>::unpack(up);
-                                lo[t][i] = transpose8x8(pack_half2(y0 - f.x, y1 - f.y));
+                            const float2 b = kv[h][i][g][1];
+                            const float f = b.x * to_one, z = b.y + 8.f * b.x;
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                const float p0 = s[h][t][2 * i], p1 = s[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
+                                zeros[t][g][0] += p0 * z;
+                                zeros[t][g][1] += p1 * z;
+                                const uint32_t up = pack_half2(y0, y1);
+                                hi[h][t][i] = transpose8x8(up);
+                                if constexpr (kParts == 2) {
+                                    const float2 w = Half<__half>::unpack(up);
+                                    lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
+                                }
                             }
                         }
-                    }
-                    auto products = [&](int at, const uint32_t (&v)[2][4]) {   // two tiles of 16 elements
+                    // two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind
+                    auto products = [&](int h, int at, uint32_t x, uint32_t y) {
+                        const uint32_t x8 = x >> 8, y8 = y >> 8;
+                        const uint32_t w[2][4] = {{codes<true, -8>(x), codes<false, -8>(x), codes<true, -8>(y), codes<false, -8>(y)},
+                                                  {codes<true, -8>(x8), codes<false, -8>(x8), codes<true, -8>(y8), codes<false, -8>(y8)}};
 #pragma unroll
                         for (int part = 0; part < kParts; part++)
 #pragma unroll
                             for (int i = 0; i < 2; i++)
 #pragma unroll
-                                for (int t = 0; t < NT; t++) Half<__half>::mma(o[at + i][t], v[i], part ? lo[t][0] : hi[t][0], part ? lo[t][1] : hi[t][1]);
-                    };
-                    auto unpacked = [&](int at, uint32_t x, uint32_t y) {      // four codes each of a pair of keys, and of the pair 8 behind
-                        const uint32_t x8 = x >> 8, y8 = y >> 8;
-                        const uint32_t v[2][4] = {{codes<true, -8>(x), codes<false, -8>(x), codes<true, -8>(y), codes<false, -8>(y)},
-                                                  {codes<true, -8>(x8), codes<false, -8>(x8), codes<true, -8>(y8), codes<false, -8>(y8)}};
-                        products(at, v);
+                                for (int t = 0; t < NT; t++) Half<__half>::mma(o[at + i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
                     };
 #pragma unroll
-                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++) {
-                        const uint32_t at = v_row + ch * 32;
-                        const uint32_t w0 = load_shared(at), w1 = load_shared(at + Shape::kPitch), w2 = load_shared(at + 8 * Shape::kPitch), w3 = load_shared(at + 9 * Shape::kPitch);
-                        unpacked(4 * ch, __byte_perm(w0, w1, 0x5410), __byte_perm(w2, w3, 0x5410));
-                        unpacked(4 * ch + 2, __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x7632));
-                    }
+                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++)
+#pragma unroll
+                        for (int h = 0; h < TILES; h++) {
+                            const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + r * 4 + ch * 32;
+                            const uint32_t w0 = word_at(at), w1 = word_at(at + Shape::kPitch), w2 = word_at(at + 8 * Shape::kPitch), w3 = word_at(at + 9 * Shape::kPitch);
+                            products(h, 4 * ch, __byte_perm(w0, w1, 0x5410), __byte_perm(w2, w3, 0x5410));
+                            products(h, 4 * ch + 2, __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x7632));
+                        }
                     if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
-                        const uint32_t at = values + (16 * h + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4, half = r & 1 ? 0x7632 : 0x5410;
-                        const uint32_t w0 = load_shared(at), w1 = load_shared(at + Shape::kPitch), w2 = load_shared(at + 8 * Shape::kPitch), w3 = load_shared(at + 9 * Shape::kPitch);
-                        unpacked(4 * CH, __byte_perm(w0, w1, half), __byte_perm(w2, w3, half));
+#pragma unroll
+                        for (int h = 0; h < TILES; h++) {
+                            const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4;
+                            const uint32_t half = r & 1 ? 0x7632 : 0x5410;
+                            const uint32_t w0 = word_at(at), w1 = word_at(at + Shape::kPitch), w2 = word_at(at + 8 * Shape::kPitch), w3 = word_at(at + 9 * Shape::kPitch);
+                            products(h, 4 * CH, __byte_perm(w0, w1, half), __byte_perm(w2, w3, half));
+                        }
                     }
                 }
             }
