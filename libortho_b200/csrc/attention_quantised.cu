@@ -93,6 +93,10 @@ extern "C" int ortho_b200_paged_attention_quantised(const ortho_b200_paged_atten
     args.c = *c;
     args.wide = c->head_dim % 32 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) == 0;
     for (int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride}) args.wide = args.wide && s % 16 == 0;
+    args.wide = args.wide && c->pages * c->k_page_stride < (1LL << 36) && c->pages * c->v_page_stride < (1LL << 36) && c->page_size * c->k_slot_stride < (1LL << 36) && c->page_size * c->v_slot_stride < (1LL << 36)
+             && c->pages * c->k_page_stride + c->page_size * c->k_slot_stride < (1LL << 36) && c->pages * c->v_page_stride + c->page_size * c->v_slot_stride < (1LL << 36);
+    args.k_page = (uint32_t)(c->k_page_stride / 16); args.k_slot = (uint32_t)(c->k_slot_stride / 16);
+    args.v_page = (uint32_t)(c->v_page_stride / 16); args.v_slot = (uint32_t)(c->v_slot_stride / 16);
     AttentionArgs &a = args.a;
     a.d = *d;
     a.d.pages = c->pages;

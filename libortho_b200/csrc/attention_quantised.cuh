@@ -24,9 +24,11 @@ namespace ob {
 struct QuantisedAttentionArgs {
     AttentionArgs a;                             // (d.kv_heads, head_dim, pages, page_size are the cache's; the other fields of a cache are not read)
     ortho_b200_quantised_cache c;
-    int wide;                                    // rows of the cache are whole 16-byte pieces
+    int wide;                                    // rows of the cache are whole 16-byte pieces, fewer than 2^32 of them; and strides in such pieces
+    uint32_t k_page, k_slot, v_page, v_slot;
 };
 
+constexpr float kNone = -1e30f;
 constexpr int kQWarpKeys = 32, kQUnitKeys = kQWarpKeys * kAttnWarps;
 
 template <int DP, int NT, bool GROUPED>
@@ -44,7 +46,7 @@ struct QuantisedShape {
     static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
     static constexpr int kFour = 57088, kThree = 76458, kTwo = 115712, kOne = 232448;
     static constexpr int kRegs = NT * DP;                                      // a measure of the sums that a thread holds
-    static constexpr int kWanted = kRegs <= 128 ? 4 : kRegs <= 192 ? 3 : kRegs <= 256 ? 2 : 1;
+    static constexpr int kWanted = kRegs <= 64 ? 4 : kRegs <= 192 ? 3 : kRegs <= 256 ? 2 : 1;
     static constexpr int kRoom = kWanted == 4 && bytes(2) <= kFour ? kFour : kWanted >= 3 && bytes(2) <= kThree ? kThree : kWanted >= 2 && bytes(2) <= kTwo ? kTwo : kOne;
     static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2, kBytes = bytes(kStages);
     static constexpr int kPerSm = kRoom == kFour ? 4 : kRoom == kThree ? 3 : kRoom == kTwo ? 2 : 1;
@@ -217,8 +219,6 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 const uint32_t page = is_there ? t.page : 0, place = is_there ? t.place : 0, ok = __ballot_sync(kAll, is_there);
                 if (lane == 0) seen[stage] = ok;
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
-                // a lane's own key's place in the caches; the lanes that copy a row get it from there
-                const int64_t k_mine = page * c.k_page_stride + place * c.k_slot_stride, v_mine = alike ? k_mine : page * c.v_page_stride + place * c.v_slot_stride;
                 {
                     const int64_t ks_mine = page * c.ks_page_stride + place * c.ks_slot_stride, vs_mine = alike_s ? ks_mine : page * c.vs_page_stride + place * c.vs_slot_stride;
 #pragma unroll
@@ -227,20 +227,23 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8 + 4, vs + vs_mine + g, is_there);
                     }
                 }
-                if (args.wide) {
+                // a lane's own key's place in the caches; the lanes that copy a row get it from there
+                if (args.wide) {                 // in pieces of 16 bytes, which 32 bits number
+                    const uint32_t k_mine = page * args.k_page + place * args.k_slot, v_mine = alike ? k_mine : page * args.v_page + place * args.v_slot;
 #pragma unroll
                     for (int i = 0; i < Shape::kPieces; i++) {
                         const int at = i * 32 + lane, row = at / Shape::kPieces, piece = at % Shape::kPieces;
-                        const int64_t k_at = __shfl_sync(kAll, k_mine, row), v_at = alike ? k_at : __shfl_sync(kAll, v_mine, row);
+                        const uint32_t k_at = __shfl_sync(kAll, k_mine, row), v_at = alike ? k_at : __shfl_sync(kAll, v_mine, row);
                         const bool on = (ok >> row & 1) && piece * 32 < D;     // (else zeros; the address is that of the first page)
                         const int e = piece * 32 < D ? piece * 16 : 0;
-                        copy16_async(dst + row * Shape::kPitch + piece * 16, k + k_at + e, on);
-                        copy16_async(dst + Shape::kCodes + row * Shape::kPitch + piece * 16, v + v_at + e, on);
+                        copy16_async(dst + row * Shape::kPitch + piece * 16, k + e + (uint64_t)k_at * 16, on);
+                        copy16_async(dst + Shape::kCodes + row * Shape::kPitch + piece * 16, v + e + (uint64_t)v_at * 16, on);
                     }
                 } else {
+                    const int64_t k_mine = page * c.k_page_stride + place * c.k_slot_stride, v_mine = page * c.v_page_stride + place * c.v_slot_stride;
                     for (int at = lane; at < kQWarpKeys * (DP / 8); at += 32) {
                         const int row = at / (DP / 8), word = at % (DP / 8);
-                        const int64_t k_at = __shfl_sync(kAll, k_mine, row), v_at = alike ? k_at : __shfl_sync(kAll, v_mine, row);
+                        const int64_t k_at = __shfl_sync(kAll, k_mine, row), v_at = __shfl_sync(kAll, v_mine, row);
                         const bool on = (ok >> row & 1) && word * 8 < D;
                         const int e = word * 8 < D ? word * 4 : 0;
                         copy4_async(dst + row * Shape::kPitch + word * 4, k + k_at + e, on);
@@ -275,7 +278,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
         float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
-        float most[NT][2], base[NT][2];          // scores above `most` move the reference: the largest by then + kSlack, and what is taken off scores, the largest - lift
+        float base[NT][2];                       // what is taken off scores, the largest by the time - lift; kNone before the first
         float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
         int stage = 0, q_at = -1;
         bool started_here = true;                // the request's first unit is this CTA's
@@ -305,8 +308,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
                     }
-                    most[t][0] = most[t][1] = -INFINITY;
-                    base[t][0] = base[t][1] = 0.f;
+                    base[t][0] = base[t][1] = kNone;
                     sum[t][0] = sum[t][1] = 0.f;
 #pragma unroll
                     for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
@@ -377,32 +379,29 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             }
                     }
                 }
-                bool grows = false;
+                // from here on relative to the reference, which moves where one is kSlack above it (and at the first number: kNone lies far below)
                 auto greatest = [](const float (&s)[TILES][NT][4], int t, int e) {
                     float m = fmaxf(s[0][t][e], s[0][t][e + 2]);
                     if constexpr (TILES == 2) m = fmaxf(m, fmaxf(s[TILES - 1][t][e], s[TILES - 1][t][e + 2]));
                     return m;
                 };
+                float p[TILES][NT][4];
+                bool grows = false;
 #pragma unroll
-                for (int h = 0; h < TILES; h++)
+                for (int t = 0; t < NT; t++) {
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                    for (int h = 0; h < TILES; h++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[h][t][e] *= factor[t][e & 1];
-                if (there != kHere) {            // keys that are not there
+                        for (int e = 0; e < 4; e++) p[h][t][e] = __fmaf_rn(s[h][t][e], factor[t][e & 1], -base[t][e & 1]);
 #pragma unroll
-                    for (int h = 0; h < TILES; h++) {
+                    for (int h = 0; there != kHere && h < TILES; h++) {        // (keys that are not there)
                         const bool on0 = (there >> (16 * h + r)) & 1, on1 = (there >> (16 * h + r + 8)) & 1;
 #pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) s[h][t][e] = (e < 2 ? on0 : on1) ? s[h][t][e] : -INFINITY;
+                        for (int e = 0; e < 4; e++) p[h][t][e] = (e < 2 ? on0 : on1) ? p[h][t][e] : -INFINITY;
                     }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) grows = grows || greatest(p, t, e) > Type::lift + kSlack;
                 }
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) grows = grows || greatest(s, t, e) > most[t][e];
                 float scale_here = 0.f;
 #pragma unroll
                 for (int h = 0; h < TILES; h++)
@@ -423,15 +422,22 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         float keep[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            float m = greatest(s, t, e);
+                            float m = -INFINITY;
+                            auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? s[h][t][e + 2 * i] * factor[t][e] : -INFINITY; };
+#pragma unroll
+                            for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
-                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 16));
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 16)) - Type::lift;
                             keep[e] = 1.f;
-                            if (m > most[t][e] - kSlack) {                     // (above the reference, that is; or the first number)
-                                keep[e] = most[t][e] == -INFINITY ? 0.f : exp2_approx(base[t][e] - (m - Type::lift));
-                                most[t][e] = m + kSlack;
-                                base[t][e] = m - Type::lift;
+                            if (m > base[t][e]) {
+                                keep[e] = exp2_approx(base[t][e] - m);
+                                base[t][e] = m;
+                            }
+#pragma unroll
+                            for (int h = 0; h < TILES; h++) {
+                                p[h][t][e] = score(h, 0) - base[t][e];
+                                p[h][t][e + 2] = score(h, 1) - base[t][e];
                             }
                             sum[t][e] *= keep[e];
 #pragma unroll
@@ -450,9 +456,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            s[h][t][e] = exp2_approx(s[h][t][e] - base[t][e]);
-                            s[h][t][e + 2] = exp2_approx(s[h][t][e + 2] - base[t][e]);
-                            sum[t][e] += s[h][t][e] + s[h][t][e + 2];
+                            p[h][t][e] = exp2_approx(p[h][t][e]);
+                            p[h][t][e + 2] = exp2_approx(p[h][t][e + 2]);
+                            sum[t][e] += p[h][t][e] + p[h][t][e + 2];
                         }
                 // ---- values: a lane's pairs of keys are 2 t4 and 2 t4 + 8 of a tile with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
 #pragma unroll
@@ -466,7 +472,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             const float f = b.x * to_one, z = b.y + 8.f * b.x;
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
-                                const float p0 = s[h][t][2 * i], p1 = s[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
+                                const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
                                 zeros[t][g][0] += p0 * z;
                                 zeros[t][g][1] += p1 * z;
                                 const uint32_t up = pack_half2(y0, y1);
@@ -531,7 +537,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float l = over_keys(sum[t][e]);
-                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(most[t][e] == -INFINITY ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
+                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
 #pragma unroll
                         for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
                     }
