@@ -46,7 +46,7 @@ struct QuantisedShape {
     static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
     static constexpr int kFour = 57088, kThree = 76458, kTwo = 115712, kOne = 232448;
     static constexpr int kRegs = NT * DP;                                      // a measure of the sums that a thread holds
-    static constexpr int kWanted = kRegs <= 64 ? 4 : kRegs <= 192 ? 3 : kRegs <= 256 ? 2 : 1;
+    static constexpr int kWanted = kRegs <= 64 ? 4 : kRegs <= 192 ? 3 : 2;
     static constexpr int kRoom = kWanted == 4 && bytes(2) <= kFour ? kFour : kWanted >= 3 && bytes(2) <= kThree ? kThree : kWanted >= 2 && bytes(2) <= kTwo ? kTwo : kOne;
     static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2, kBytes = bytes(kStages);
     static constexpr int kPerSm = kRoom == kFour ? 4 : kRoom == kThree ? 3 : kRoom == kTwo ? 2 : 1;
@@ -60,21 +60,13 @@ __device__ __forceinline__ void copy4_async(uint32_t dst, const void *src, bool 
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-// (w & mask) | exponent in one instruction (the compiler makes two of it: neither constant fits it beside the other)
-__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t mask, uint32_t exponent)
+// A pair of codes as FP16 numbers, at bits 0 to 3 and 16 to 19 (LOW) or 4 to 7 and 20 to 23: subnormal numbers, code 2^-24 and code 2^-20.  CENTRED: less 8.
+template <bool LOW, bool CENTRED> __device__ __forceinline__ uint32_t codes(uint32_t w)
 {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(exponent));
-    return r;
-}
-// A pair of codes as FP16, at bits 0 to 3 and 16 to 19 (LOW) or 4 to 7 and 20 to 23, plus OFFSET.  They are joined with the exponent of 1024 or of 64.
-template <bool LOW, int OFFSET> __device__ __forceinline__ uint32_t codes(uint32_t w)
-{
-    const uint32_t b = LOW ? masked(w, 0x000F000Fu, 0x64006400u) : masked(w, 0x00F000F0u, 0x54005400u);
-    if (!LOW && OFFSET == 64) return b;
-    constexpr uint32_t kLess = OFFSET == 64 ? 0x63806380u : LOW ? 0x64086408u : 0x54805480u;      // 1024 - 64; 1024 + 8 and 64 + 8
-    static_assert(OFFSET == 64 || OFFSET == -8, "the constants above");
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
+    const uint32_t b = LOW ? w & 0x000F000Fu : w & 0x00F000F0u;
+    if (!CENTRED) return b;
+    constexpr uint32_t kLess = LOW ? 0x80088008u : 0x80808080u;
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
@@ -90,30 +82,27 @@ template <class T, int DP, int GROUPS>
 __device__ __forceinline__ void query_operands(const unsigned char *row, int t, uint4 (&w)[DP / 32], float &f, float (&sums)[GROUPS])
 {
     constexpr int J = DP / 32, PER = J / GROUPS;
-    f = 1.f;
 #pragma unroll
     for (int j = 0; j < J; j++) w[j] = *reinterpret_cast<const uint4 *>(row + (4 * j + t) * 16);
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        uint32_t most = 0;
+    uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            most = __vmaxu2(__vmaxu2(__vmaxu2(w[j].x & 0x7FFF7FFFu, w[j].y & 0x7FFF7FFFu), __vmaxu2(w[j].z & 0x7FFF7FFFu, w[j].w & 0x7FFF7FFFu)), most);
-        }
-        most = max(most & 0xFFFFu, most >> 16);
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // exponent e of the largest: elements times 2^(8 - e).  (Infinity and NaN stay what they are; of rows below 2^-100 nothing is lost that FP32 shows.)
-        const int e = min(max((int)(most >> 7), 27), 254);
-        const float by = __uint_as_float((uint32_t)(262 - e) << 23);
-        f = __uint_as_float((uint32_t)(e - 8) << 23);
+    for (int j = 0; j < J; j++)
+        most = __vmaxu2(__vmaxu2(__vmaxu2(w[j].x & 0x7FFF7FFFu, w[j].y & 0x7FFF7FFFu), __vmaxu2(w[j].z & 0x7FFF7FFFu, w[j].w & 0x7FFF7FFFu)), most);
+    most = max(most & 0xFFFFu, most >> 16);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // e: FP32's exponent of the largest, of zero the least; elements times 2^(8 - e).  (Infinity and NaN stay what they are; of rows below 2^-100 nothing is lost that FP32 shows.)
+    const float size = Half<T>::unpack(most).x;
+    const int e = min(max((int)(__float_as_uint(size) >> 23), 27), 254);
+    const float by = __uint_as_float((uint32_t)(262 - e) << 23);
+    f = __uint_as_float((uint32_t)(e - 8) << 23);
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            uint32_t *const x = reinterpret_cast<uint32_t *>(&w[j]);
+    for (int j = 0; j < J; j++) {
+        uint32_t *const x = reinterpret_cast<uint32_t *>(&w[j]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 v = Half<T>::unpack(x[i]);
-                x[i] = Half<__half>::pack(v.x * by, v.y * by);
-            }
+        for (int i = 0; i < 4; i++) {
+            const float2 v = Half<T>::unpack(x[i]);
+            x[i] = Half<__half>::pack(v.x * by, v.y * by);
         }
     }
 #pragma unroll
@@ -130,7 +119,13 @@ __device__ __forceinline__ void query_operands(const unsigned char *row, int t, 
         sums[g] = s;
     }
 #pragma unroll
-    for (int j = 0; j < J; j++) w[j] = as_codes_lie(w[j]);
+    for (int j = 0; j < J; j++) {
+        w[j] = as_codes_lie(w[j]);
+        // what meets codes 2^-20 is a sixteenth
+        const __half2 sixteenth = __float2half2_rn(0.0625f), y = __hmul2(*reinterpret_cast<const __half2 *>(&w[j].y), sixteenth), z = __hmul2(*reinterpret_cast<const __half2 *>(&w[j].w), sixteenth);
+        w[j].y = *reinterpret_cast<const uint32_t *>(&y);
+        w[j].w = *reinterpret_cast<const uint32_t *>(&z);
+    }
 }
 
 template <class T, int DP, int NT, bool GROUPED, bool CLUSTER>
@@ -142,6 +137,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
     // p vs in FP16 is off by up to 2^-12, an eighth of the rounding of a BF16 output and as much as that of an FP16 one, which therefore gets the rest too
     constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
+    // Codes less 8 are added up as they come.  With one column of queries it takes less to add up the codes themselves, over 32 keys at a time.
+    constexpr bool CENTRED = NT > 1;
     constexpr int TILES = NT * DP <= 128 ? 2 : 1;                              // of 16 keys that are worked on together, as registers allow
     constexpr uint32_t kAll = 0xffffffffu, kHere = TILES == 2 ? kAll : 0xFFFFu;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -338,6 +335,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         for (int g = 0; g < G; g++) {
                             const uint2 w = *reinterpret_cast<const uint2 *>(scales + ((16 * (h0 + h) + 8 * i + r) * G + g) * 8);
                             kv[h][i][g][0] = Half<T>::unpack(w.x);
+                            kv[h][i][g][0].x *= 0x1p24f;                       // (of the codes' 2^-24)
                             kv[h][i][g][1] = Half<T>::unpack(w.y);
                         }
 #pragma unroll
@@ -353,8 +351,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         for (int h = 0; h < TILES; h++) {
                             const unsigned char *const at = keys + (16 * (h0 + h) + r) * Shape::kPitch + t4 * 4 + j * 16;
                             const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch), v0 = w0 >> 8, v1 = w1 >> 8;
-                            const uint32_t lower[4] = {codes<true, 64>(w0), codes<true, 64>(w1), codes<false, 64>(w0), codes<false, 64>(w1)};
-                            const uint32_t upper[4] = {codes<true, 64>(v0), codes<true, 64>(v1), codes<false, 64>(v0), codes<false, 64>(v1)};
+                            const uint32_t lower[4] = {codes<true, false>(w0), codes<true, false>(w1), codes<false, false>(w0), codes<false, false>(w1)};
+                            const uint32_t upper[4] = {codes<true, false>(v0), codes<true, false>(v1), codes<false, false>(v0), codes<false, false>(v1)};
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 uint4 b;
@@ -368,12 +366,11 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int h = 0; h < TILES; h++) {
                         const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
-                        const float z0 = a0.y - 64.f * a0.x, z1 = a1.y - 64.f * a1.x;
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
-                                const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
+                                const float y0 = a0.x * x[h][t][e] + a0.y * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + a1.y * q_sum[t][g][e];
                                 s[h][t][e] = g ? s[h][t][e] + y0 : y0;
                                 s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
                             }
@@ -469,7 +466,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             const float2 b = kv[h][i][g][1];
-                            const float f = b.x * to_one, z = b.y + 8.f * b.x;
+                            const float f = b.x * to_one, z = CENTRED ? b.y + 8.f * b.x : b.y;
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
@@ -483,35 +480,57 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 }
                             }
                         }
-                    // two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind
-                    auto products = [&](int h, int at, uint32_t x, uint32_t y) {
-                        const uint32_t x8 = x >> 8, y8 = y >> 8;
-                        const uint32_t w[2][4] = {{codes<true, -8>(x), codes<false, -8>(x), codes<true, -8>(y), codes<false, -8>(y)},
-                                                  {codes<true, -8>(x8), codes<false, -8>(x8), codes<true, -8>(y8), codes<false, -8>(y8)}};
+                    // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; n times TILES such pairs, that of tile h from pair(h, x, y)
+                    auto products = [&](int at, auto pair) {
+                        float sums[2][NT][4];
 #pragma unroll
-                        for (int part = 0; part < kParts; part++)
+                        for (int h = 0; h < TILES; h++) {
+                            uint32_t x, y;
+                            pair(h, x, y);
+                            const uint32_t x8 = x >> 8, y8 = y >> 8;
+                            const uint32_t w[2][4] = {{codes<true, CENTRED>(x), codes<false, CENTRED>(x), codes<true, CENTRED>(y), codes<false, CENTRED>(y)},
+                                                      {codes<true, CENTRED>(x8), codes<false, CENTRED>(x8), codes<true, CENTRED>(y8), codes<false, CENTRED>(y8)}};
+#pragma unroll
+                            for (int part = 0; part < kParts; part++)
+#pragma unroll
+                                for (int i = 0; i < 2; i++)
+#pragma unroll
+                                    for (int t = 0; t < NT; t++) {
+                                        if (!CENTRED && h == 0 && part == 0) sums[i][t][0] = sums[i][t][1] = sums[i][t][2] = sums[i][t][3] = 0.f;
+                                        Half<__half>::mma(CENTRED ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                                    }
+                        }
+                        if (!CENTRED) {
 #pragma unroll
                             for (int i = 0; i < 2; i++)
 #pragma unroll
-                                for (int t = 0; t < NT; t++) Half<__half>::mma(o[at + i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                                for (int t = 0; t < NT; t++)
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) o[at + i][t][e] += sums[i][t][e];
+                        }
                     };
 #pragma unroll
-                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++)
+                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++) {
+                        uint32_t w[TILES][4];
 #pragma unroll
                         for (int h = 0; h < TILES; h++) {
                             const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + r * 4 + ch * 32;
-                            const uint32_t w0 = word_at(at), w1 = word_at(at + Shape::kPitch), w2 = word_at(at + 8 * Shape::kPitch), w3 = word_at(at + 9 * Shape::kPitch);
-                            products(h, 4 * ch, __byte_perm(w0, w1, 0x5410), __byte_perm(w2, w3, 0x5410));
-                            products(h, 4 * ch + 2, __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x7632));
+                            w[h][0] = word_at(at); w[h][1] = word_at(at + Shape::kPitch); w[h][2] = word_at(at + 8 * Shape::kPitch); w[h][3] = word_at(at + 9 * Shape::kPitch);
                         }
-                    if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
 #pragma unroll
-                        for (int h = 0; h < TILES; h++) {
+                        for (int half = 0; half < 2; half++)
+                            products(4 * ch + 2 * half, [&](int h, uint32_t &x, uint32_t &y) {
+                                x = __byte_perm(w[h][0], w[h][1], half ? 0x7632 : 0x5410);
+                                y = __byte_perm(w[h][2], w[h][3], half ? 0x7632 : 0x5410);
+                            });
+                    }
+                    if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
+                        products(4 * CH, [&](int h, uint32_t &x, uint32_t &y) {
                             const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4;
                             const uint32_t half = r & 1 ? 0x7632 : 0x5410;
-                            const uint32_t w0 = word_at(at), w1 = word_at(at + Shape::kPitch), w2 = word_at(at + 8 * Shape::kPitch), w3 = word_at(at + 9 * Shape::kPitch);
-                            products(h, 4 * CH, __byte_perm(w0, w1, half), __byte_perm(w2, w3, half));
-                        }
+                            x = __byte_perm(word_at(at), word_at(at + Shape::kPitch), half);
+                            y = __byte_perm(word_at(at + 8 * Shape::kPitch), word_at(at + 9 * Shape::kPitch), half);
+                        });
                     }
                 }
             }
@@ -544,7 +563,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 float *const fold = reinterpret_cast<float *>(ring + stage * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
                 const float *const folds = reinterpret_cast<const float *>(smem + stage * Shape::kStage);
                 constexpr int WARP_FLOATS = S * Shape::kStage / 4;
-                const float times = largest * kDown;
+                const float times = largest * (kDown * 0x1p24f), times16 = times * 0.0625f;       // of codes 2^-24 and 2^-20
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     __syncwarp();                // the warp has read its values
@@ -555,7 +574,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const float z = zeros[t][GROUPED ? i / 4 : 0][e];
-                            *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times + z);
+                            *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times16 + z);
                         }
                     }
                     __syncthreads();
