@@ -93,10 +93,16 @@ extern "C" int ortho_b200_paged_attention_quantised(const ortho_b200_paged_atten
     args.c = *c;
     args.wide = c->head_dim % 32 == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) == 0;
     for (int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride}) args.wide = args.wide && s % 16 == 0;
-    args.wide = args.wide && c->pages * c->k_page_stride < (1LL << 36) && c->pages * c->v_page_stride < (1LL << 36) && c->page_size * c->k_slot_stride < (1LL << 36) && c->page_size * c->v_slot_stride < (1LL << 36)
-             && c->pages * c->k_page_stride + c->page_size * c->k_slot_stride < (1LL << 36) && c->pages * c->v_page_stride + c->page_size * c->v_slot_stride < (1LL << 36);
-    args.k_page = (uint32_t)(c->k_page_stride / 16); args.k_slot = (uint32_t)(c->k_slot_stride / 16);
-    args.v_page = (uint32_t)(c->v_page_stride / 16); args.v_slot = (uint32_t)(c->v_slot_stride / 16);
+    // places of a page and a slot in pieces of 16 bytes, and in scales, as 32 bits: the largest of them is the last page's and slot's
+    auto number = [&](int64_t page_stride, int64_t slot_stride, int64_t unit, uint32_t &page, uint32_t &slot) {
+        if (page_stride < 0 || slot_stride < 0 || page_stride > (1LL << 40) || slot_stride > (1LL << 40) || (c->pages * (page_stride / unit) + c->page_size * (slot_stride / unit)) >= (1LL << 32)) args.wide = 0;
+        page = (uint32_t)(page_stride / unit);
+        slot = (uint32_t)(slot_stride / unit);
+    };
+    number(c->k_page_stride, c->k_slot_stride, 16, args.k_page, args.k_slot);
+    number(c->v_page_stride, c->v_slot_stride, 16, args.v_page, args.v_slot);
+    number(c->ks_page_stride, c->ks_slot_stride, 1, args.ks_page, args.ks_slot);
+    number(c->vs_page_stride, c->vs_slot_stride, 1, args.vs_page, args.vs_slot);
     AttentionArgs &a = args.a;
     a.d = *d;
     a.d.pages = c->pages;

@@ -25,7 +25,7 @@ struct QuantisedAttentionArgs {
     AttentionArgs a;                             // (d.kv_heads, head_dim, pages, page_size are the cache's; the other fields of a cache are not read)
     ortho_b200_quantised_cache c;
     int wide;                                    // rows of the cache are whole 16-byte pieces, fewer than 2^32 of them; and strides in such pieces
-    uint32_t k_page, k_slot, v_page, v_slot;
+    uint32_t k_page, k_slot, v_page, v_slot, ks_page, ks_slot, vs_page, vs_slot;
 };
 
 constexpr float kNone = -1e30f;
@@ -43,7 +43,7 @@ struct QuantisedShape {
     static_assert(8 * kFoldPitch * 4 <= kStage, "room for 8 queries");
     static constexpr bool kKeepQ = NT * DP <= 256;                             // query operands stay in registers
     static constexpr int kOperands = kKeepQ ? 0 : NT * DP / 32 * 512;
-    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8 + kAttnWarps * stages * 4 + 64; }
+    static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8; }
     static constexpr int kFour = 57088, kThree = 76458, kTwo = 115712, kOne = 232448;
     static constexpr int kRegs = NT * DP;                                      // a measure of the sums that a thread holds
     static constexpr int kWanted = kRegs <= 64 ? 4 : kRegs <= 192 ? 3 : 2;
@@ -150,7 +150,6 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
     unsigned char *const q_ring = smem + kAttnWarps * S * Shape::kStage;
     unsigned char *const operands = q_ring + S * Shape::kQ;                    // (of queries that do not stay in registers) [NT][J][32] x 16 bytes
     float2 *const sums = reinterpret_cast<float2 *>(operands + Shape::kOperands);
-    uint32_t *const seen = reinterpret_cast<uint32_t *>(sums + kAttnWarps * NT * 8) + warp * S;
     const int inners = (int)d.kv_heads * a.groups, cta = blockIdx.x;
     float2 *const arrived_sums = reinterpret_cast<float2 *>(smem + (Shape::kBytes + 15) / 16 * 16);           // [ranks][rows]
     float4 *const arrived = reinterpret_cast<float4 *>(arrived_sums + Shape::kMostRanks * NT * 8);            // [ranks][this CTA's share]
@@ -167,30 +166,48 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         others_started();
         if (!CLUSTER && tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     } else {
+        // A CTA goes through its units in runs: those of one item that follow one another (in a cluster, every `ranks`-th of the item's)
+        const int stride = CLUSTER ? ranks * kQUnitKeys : kQUnitKeys;
+        auto run_of = [&](const Walk<kQUnitKeys> &w) {
+            const int units = w.s.units - w.unit;
+            return CLUSTER ? (units + ranks - 1) / ranks : w.left < units ? (int)w.left : units;
+        };
+        auto next_item = [&](Walk<kQUnitKeys> &w, int run) {                   // behind a run; false where there is none
+            if (CLUSTER || w.unit + run < w.s.units) return false;
+            w.left -= run + 1;
+            if (w.left < 1) return false;
+            w.unit = 0;
+            if (++w.inner == inners) {
+                w.inner = 0;
+                do w.b++, w.s = w.b < d.batch ? span_of<kQUnitKeys>(d, w.b) : Span{0, 0, 1, 0}; while (w.s.units == 0);
+            }
+            return true;
+        };
         // What the copies of a unit need; a lane has a key of the warp's 32, and looks its page up well ahead of its use
         struct Ticket { int b, inner, page, place; bool valid, queries; };
-        Walk<kQUnitKeys> ahead = now;            // the unit of the next ticket
-        bool more_tickets = true;
+        Walk<kQUnitKeys> ahead = now;            // the run that the next ticket is of; what is left of it, this lane's next key, and the end of the keys
+        bool more_tickets = true, first_of_run = true;
+        int ahead_run = run_of(ahead), ahead_left = ahead_run, key = ahead.s.from + ahead.unit * kQUnitKeys + warp * kQWarpKeys + lane, end = ahead.s.n;
         const int32_t *pages = d.block_table + ahead.s.row * d.table_stride;
         auto ticket = [&]() {
-            Ticket t;
-            t.valid = more_tickets;
-            t.b = (int)ahead.b;
-            t.inner = ahead.inner;
-            t.queries = CLUSTER ? ahead.unit == rank : ahead.unit == 0 || (ahead.b == now.b && ahead.inner == now.inner && ahead.unit == now.unit);
-            t.page = -1;
-            t.place = 0;
-            const int key = ahead.s.from + ahead.unit * kQUnitKeys + warp * kQWarpKeys + lane;
-            if (more_tickets && key < ahead.s.n) {
-                const int col = (int)a.by_page.quotient((uint32_t)key);
-                t.place = key - col * (int)d.page_size;
-                t.page = pages[col];
-            }
+            Ticket t = {(int)ahead.b, ahead.inner, -1, 0, more_tickets, first_of_run};
             if (more_tickets) {
-                more_tickets = ahead.template more<CLUSTER>(ranks);
-                if (more_tickets) {
-                    ahead.template step<CLUSTER>(d, inners, ranks);
-                    if (!CLUSTER && ahead.unit == 0) pages = d.block_table + ahead.s.row * d.table_stride;
+                if (key < end) {
+                    const int col = (int)a.by_page.quotient((uint32_t)key);
+                    t.place = key - col * (int)d.page_size;
+                    t.page = pages[col];
+                }
+                first_of_run = false;
+                key += stride;
+                if (--ahead_left == 0) {
+                    more_tickets = next_item(ahead, ahead_run);
+                    if (more_tickets) {
+                        first_of_run = true;
+                        ahead_run = ahead_left = run_of(ahead);
+                        key = ahead.s.from + warp * kQWarpKeys + lane;
+                        end = ahead.s.n;
+                        pages = d.block_table + ahead.s.row * d.table_stride;
+                    }
                 }
             }
             return t;
@@ -201,7 +218,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         const uint32_t *ks = nullptr, *vs = nullptr;
         const bool alike = c.k_page_stride == c.v_page_stride && c.k_slot_stride == c.v_slot_stride;
         const bool alike_s = c.ks_page_stride == c.vs_page_stride && c.ks_slot_stride == c.vs_slot_stride;
-        auto issue = [&](const Ticket &t, int stage) {
+        auto issue = [&](const Ticket &t, int stage) {                         // -> which of the warp's keys are there
+            uint32_t ok = 0;
             if (t.valid) {
                 if (t.inner != inner_at) {
                     inner_at = t.inner;
@@ -213,19 +231,20 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     vs = (const uint32_t *)c.v_scales + head * c.vs_head_stride;
                 }
                 const bool is_there = t.page >= 0 && t.page < d.pages;
-                const uint32_t page = is_there ? t.page : 0, place = is_there ? t.place : 0, ok = __ballot_sync(kAll, is_there);
-                if (lane == 0) seen[stage] = ok;
+                const uint32_t page = is_there ? t.page : 0, place = is_there ? t.place : 0;
+                ok = __ballot_sync(kAll, is_there);
                 const uint32_t dst = shared_addr(ring + stage * Shape::kStage);
-                {
-                    const int64_t ks_mine = page * c.ks_page_stride + place * c.ks_slot_stride, vs_mine = alike_s ? ks_mine : page * c.vs_page_stride + place * c.vs_slot_stride;
+                auto copy_scales = [&](const uint32_t *k_from, const uint32_t *v_from) {
 #pragma unroll
                     for (int g = 0; g < G; g++) {
-                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8, ks + ks_mine + g, is_there);
-                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8 + 4, vs + vs_mine + g, is_there);
+                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8, k_from + g, is_there);
+                        copy4_async(dst + 2 * Shape::kCodes + lane * G * 8 + g * 8 + 4, v_from + g, is_there);
                     }
-                }
+                };
                 // a lane's own key's place in the caches; the lanes that copy a row get it from there
-                if (args.wide) {                 // in pieces of 16 bytes, which 32 bits number
+                if (args.wide) {                 // in pieces of 16 bytes, and in scales with their zeros, which 32 bits number
+                    const uint32_t ks_mine = page * args.ks_page + place * args.ks_slot, vs_mine = alike_s ? ks_mine : page * args.vs_page + place * args.vs_slot;
+                    copy_scales(ks + ks_mine, vs + vs_mine);
                     const uint32_t k_mine = page * args.k_page + place * args.k_slot, v_mine = alike ? k_mine : page * args.v_page + place * args.v_slot;
 #pragma unroll
                     for (int i = 0; i < Shape::kPieces; i++) {
@@ -237,6 +256,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         copy16_async(dst + Shape::kCodes + row * Shape::kPitch + piece * 16, v + e + (uint64_t)v_at * 16, on);
                     }
                 } else {
+                    copy_scales(ks + page * c.ks_page_stride + place * c.ks_slot_stride, vs + page * c.vs_page_stride + place * c.vs_slot_stride);
                     const int64_t k_mine = page * c.k_page_stride + place * c.k_slot_stride, v_mine = page * c.v_page_stride + place * c.v_slot_stride;
                     for (int at = lane; at < kQWarpKeys * (DP / 8); at += 32) {
                         const int row = at / (DP / 8), word = at % (DP / 8);
@@ -260,15 +280,17 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 }
             }
             copy_commit();
+            return ok;
         };
         Ticket pending;
+        uint32_t oks[S - 1];                     // of the units that are under way
         {
             Ticket first[S - 1];
 #pragma unroll
             for (int i = 0; i < S - 1; i++) first[i] = ticket();
             pending = ticket();
 #pragma unroll
-            for (int i = 0; i < S - 1; i++) issue(first[i], i);
+            for (int i = 0; i < S - 1; i++) oks[i] = issue(first[i], i);
         }
         others_started();
 
@@ -278,12 +300,13 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         float base[NT][2];                       // what is taken off scores, the largest by the time - lift; kNone before the first
         float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
         int stage = 0, q_at = -1;
-        bool started_here = true;                // the request's first unit is this CTA's
-        for (bool first_one = true, more = true; more; first_one = false) {
+        for (bool more = true; more;) {
+          const bool started_here = now.unit == 0;                             // the item's first unit is this CTA's
+          const int run = run_of(now);
+          for (int u = 0; u < run; u++) {
             copy_wait<S - 2>();
             __syncwarp();
-            if (first_one || (!CLUSTER && now.unit == 0)) {
-                started_here = now.unit == 0;
+            if (u == 0) {
                 if (++q_at == S) q_at = 0;
                 __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
                 const unsigned char *const src = q_ring + q_at * Shape::kQ + r * Shape::kQPitch;
@@ -316,9 +339,11 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                 }
                 if constexpr (!Shape::kKeepQ) __syncthreads();
             }
-            const uint32_t ok = seen[stage];
+            const uint32_t ok = oks[0];
             const unsigned char *const keys = ring + stage * Shape::kStage, *const values = keys + Shape::kCodes, *const scales = values + Shape::kCodes;
-            issue(pending, stage == 0 ? S - 1 : stage - 1);
+#pragma unroll
+            for (int i = 0; i + 1 < S - 1; i++) oks[i] = oks[i + 1];
+            oks[S - 2] = issue(pending, stage == 0 ? S - 1 : stage - 1);
             pending = ticket();
 #pragma unroll
             for (int h0 = 0; h0 < 2; h0 += TILES) {
@@ -534,9 +559,10 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     }
                 }
             }
-            const bool last = now.last();
-            more = now.template more<CLUSTER>(ranks);
-            if (CLUSTER ? !more : last || !more) {
+            if (++stage == S) stage = 0;
+          }
+            const bool last = now.unit + run == now.s.units;
+            {
                 // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
                 // issued behind the barrier above.  What was 2^lift and `largest` times too large is brought back here.
                 const int head = now.inner / a.groups, group = now.inner - head * a.groups;
@@ -560,8 +586,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
                     }
-                float *const fold = reinterpret_cast<float *>(ring + stage * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
-                const float *const folds = reinterpret_cast<const float *>(smem + stage * Shape::kStage);
+                const int used = stage == 0 ? S - 1 : stage - 1;
+                float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
+                const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
                 constexpr int WARP_FLOATS = S * Shape::kStage / 4;
                 const float times = largest * (kDown * 0x1p24f), times16 = times * 0.0625f;       // of codes 2^-24 and 2^-20
 #pragma unroll
@@ -580,13 +607,13 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     __syncthreads();
                     add_warps<T, DP, NT, CLUSTER, WARP_FLOATS, Shape::kFoldPitch>(a, folds, sums, t, now.b, h0, heads, whole, slot, rank, ranks, arrived_sums, arrived);
                 }
+                const Walk<kQUnitKeys> was = now;
+                more = next_item(now, run);
                 if constexpr (!CLUSTER) {
-                    if (!more && tid == 0) a.cut[cta] = make_int4((int)now.b, now.inner, (int)((item_at + now.s.units) / per), started_here && !last ? 1 : 0);
-                    item_at += now.s.units + 1;
+                    if (!more && tid == 0) a.cut[cta] = make_int4((int)was.b, was.inner, (int)((item_at + was.s.units) / per), started_here && !last ? 1 : 0);
+                    item_at += was.s.units + 1;
                 }
             }
-            if (++stage == S) stage = 0;
-            if (more) now.template step<CLUSTER>(d, inners, ranks);
         }
         copy_wait<0>();
     }
