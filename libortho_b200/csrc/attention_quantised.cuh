@@ -369,7 +369,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int h = 0; h < TILES; h++)
 #pragma unroll
-                        for (int t = 0; t < NT; t++) x[h][t][0] = x[h][t][1] = x[h][t][2] = x[h][t][3] = 0.f;
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[h][t][e] = q_sum[t][g][e & 1] * -0x1p-21f;      // (8 off every code)
 #pragma unroll
                     for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
 #pragma unroll
@@ -391,11 +393,12 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int h = 0; h < TILES; h++) {
                         const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
+                        const float z0 = a0.y + 0x1p-21f * a0.x, z1 = a1.y + 0x1p-21f * a1.x;
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
-                                const float y0 = a0.x * x[h][t][e] + a0.y * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + a1.y * q_sum[t][g][e];
+                                const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
                                 s[h][t][e] = g ? s[h][t][e] + y0 : y0;
                                 s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
                             }
@@ -491,7 +494,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             const float2 b = kv[h][i][g][1];
-                            const float f = b.x * to_one, z = CENTRED ? b.y + 8.f * b.x : b.y;
+                            const float f = b.x * to_one, z = b.y + 8.f * b.x;
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
@@ -505,7 +508,20 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 }
                             }
                         }
-                    // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; n times TILES such pairs, that of tile h from pair(h, x, y)
+                    // 8 off every code: a product of the weights with -8 in the codes' units (rows r and r + 8 are of codes 2^-24 and 2^-20), where sums start from
+                    float start[NT][4];
+                    if (!CENTRED) {
+                        const uint32_t eights[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            start[t][0] = start[t][1] = start[t][2] = start[t][3] = 0.f;
+#pragma unroll
+                            for (int h = 0; h < TILES; h++)
+#pragma unroll
+                                for (int part = 0; part < kParts; part++) Half<__half>::mma(start[t], eights, part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                        }
+                    }
+                    // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; those of tile h from pair(h, x, y)
                     auto products = [&](int at, auto pair) {
                         float sums[2][NT][4];
 #pragma unroll
@@ -521,7 +537,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 for (int i = 0; i < 2; i++)
 #pragma unroll
                                     for (int t = 0; t < NT; t++) {
-                                        if (!CENTRED && h == 0 && part == 0) sums[i][t][0] = sums[i][t][1] = sums[i][t][2] = sums[i][t][3] = 0.f;
+                                        if (!CENTRED && h == 0 && part == 0) { sums[i][t][0] = start[t][0]; sums[i][t][1] = start[t][1]; sums[i][t][2] = start[t][2]; sums[i][t][3] = start[t][3]; }
                                         Half<__half>::mma(CENTRED ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
                                     }
                         }
