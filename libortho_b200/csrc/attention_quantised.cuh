@@ -297,7 +297,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
         float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
-        float base[NT][2];                       // what is taken off scores, the largest by the time - lift; kNone before the first
+        float base[NT][2];                       // what is taken off scores: the largest by the time, rounded up to a whole number, - lift; kNone before the first
         float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
         int stage = 0, q_at = -1;
         for (bool more = true; more;) {
@@ -453,7 +453,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
                             m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
-                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 16)) - Type::lift;
+                            m = ceilf(fmaxf(m, __shfl_xor_sync(kAll, m, 16))) - Type::lift;
                             keep[e] = 1.f;
                             if (m > base[t][e]) {
                                 keep[e] = exp2_approx(base[t][e] - m);

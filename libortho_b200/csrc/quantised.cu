@@ -388,7 +388,7 @@ struct ReadArgs {
     int together;
     FastDiv by_token, by_chunk, by_group;        // items of a token, chunks of a head, chunks of a group
 };
-constexpr int kMostRead = 32;
+constexpr int kMostRead = 16;
 
 // Two codes, one from each of the 16-bit halves of w, as numbers of the type: 1024 + code in FP16 and 128 + code in BF16, less that
 template <class T> struct Codes;
@@ -465,7 +465,7 @@ read_quantised_kernel(const __grid_constant__ ReadArgs a)
                 y.y = Codes<T>::value(__byte_perm(code[u], next, 0x5511), s, z);
                 y.z = Codes<T>::value(__byte_perm(code[u], next, 0x6622), s, z);
                 y.w = Codes<T>::value(__byte_perm(code[u], next, 0x7733), s, z);
-                *reinterpret_cast<uint4 *>(out + token * stride) = y;
+                __stcs(reinterpret_cast<uint4 *>(out + token * stride), y);
             }
         }
     }
