@@ -223,7 +223,11 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
     const at::Tensor k = heads(k_arg, "k", nullptr), v = heads(v_arg, "v", &k);
     TORCH_CHECK_VALUE(v.size(1) == k.size(1), "k and v must have the same heads");
     std::conditional_t<QUANTISED, QuantisedCache, Cache> c;
-    if constexpr (QUANTISED) c = quantised_cache_of(caches, type, k);
+    if constexpr (QUANTISED) {
+        c = quantised_cache_of(caches, type, k);
+        for (const at::Tensor *t : {&c.k, &c.v, &c.ks, &c.vs})
+            for (int i = 0; i < 3; i++) TORCH_CHECK_VALUE(t->stride(i) != 0 || t->size(i) <= 1, "a cache that is written must not be expanded");
+    }
     else c = cache_of(caches[0], caches[1], type, k);
     const int64_t T = k.size(0);
     TORCH_CHECK_VALUE(c.heads == k.size(1) && c.D == k.size(2), "k and v must have the caches' heads and head_dim");
@@ -328,6 +332,7 @@ PyObject *read_quantised(PyObject *, PyObject *const *a, Py_ssize_t n)
                               && out[i].stride(0) % 8 == 0 && out[i].stride(1) % 8 == 0,
                               names[i], " must be [tokens, kv_heads, head_dim] with a contiguous last dimension, 16-byte alignment and strides that are multiples of 8");
         }
+        TORCH_CHECK_VALUE(T == 0 || out[0].const_data_ptr() != out[1].const_data_ptr(), "out must be two tensors");
     } else {
         for (int i = 0; i < 2; i++) out[i] = at::empty({T, c.heads, c.D}, scales.options().memory_format(at::MemoryFormat::Contiguous));
     }

@@ -96,7 +96,7 @@ class PagedCache:
 
 
 class QuantisedCache:
-    """Keys and values of one layer in 4 bits: ``PagedCache`` in three tenths of its room.
+    """Keys and values of one layer in 4 bits: what ``PagedCache`` holds, in a good quarter of its room.
 
     Each token's head, or every ``group`` = 64 elements of one, has a scale and a zero of its own.  ``read(slots)`` gives tokens back in ``dtype``.  A page lies head by
     head, so that attention reads whole lines of memory."""

@@ -261,5 +261,8 @@ def test_refusals():
     refused(ValueError, "out", out=q[:1])
     refused(ValueError, "aligned", out=torch.zeros(12, 4, 66, dtype=F16, device=DEV)[:, :, 1:65])
     refused(ValueError, "slots", slots=slots[:3])
+    refused(ValueError, "expanded", v_scales=cache[3][:1].expand(4, -1, -1, -1, -1))
     refused(TypeError, "pair", _C_ops.read_quantised, out=q)
+    one = torch.zeros(12, 2, 64, dtype=F16, device=DEV)
+    refused(ValueError, "two tensors", _C_ops.read_quantised, out=(one, one))
     refused(ValueError, r"out\[1\]", _C_ops.read_quantised, out=(torch.zeros(12, 2, 64, dtype=F16, device=DEV), torch.zeros(12, 2, 65, dtype=F16, device=DEV)))
