@@ -1,17 +1,25 @@
 // Attention of one new token per row over a paged cache held in 4 bits (quantised.cuh; one source for both 16-bit types):
 //
-//     s_j = scale sum_g (ks_jg sum_i q_i c_ji + kz_jg sum_i q_i),     out_i = sum_j p_j (vs_jg (d_ji - 8) + vz_jg + 8 vs_jg) / sum_j p_j,     p_j = exp(s_j - max)
+//     s_j = scale sum_g (ks_jg sum_i q_i (c_ji - 8) + (kz_jg + 8 ks_jg) sum_i q_i),
+//     out_i = sum_j p_j (vs_jg (d_ji - 8) + vz_jg + 8 vs_jg) / sum_j p_j,     p_j = exp(s_j - max)
 //
-// with codes c and d of keys and values, scales and zeros of their groups g.  The division of the work, the ring of asynchronous copies per warp and the joining are those of
-// attention.cuh; here the bytes are a quarter, so what bounds it is the warps' instructions: unpacking, about one a code and 32 lanes.
-// Codes enter the products as whole numbers, and scales and zeros are applied to what 64 elements or 16 keys have in common:
-//   * S^T = K Q^T: a lane reads 8 codes of a key as one word; the halves of the word, masked and joined with an exponent, are four operands of 64 + c
-//     in FP16 (c in the upper bits of the mantissa).  Elements are taken in the order in which a word has them, the queries likewise; the 64 comes off with
-//     the zero's term, ks q.c + (kz - 64 ks) sum q.  A sum of 64 q loses at most 2^-23 of itself, some 2^-19 of a typical q.c.
-//   * O^T += V^T P^T: a pair of keys' words are joined by halves, then unpacked to d - 8 exactly: codes around zero keep the sums as small as the outputs
-//     of a long average are, where 0 to 15 against a zero at the other end would lose two digits.  p vs enters as two FP16 parts, brought into
-//     range by a power of two of the warp's largest scale; p (vz + 8 vs) is summed in FP32 per query.
-// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element near 2^8.
+// with codes c and d of keys and values, scales and zeros of their groups g.  The division of the work and the joining are those of attention.cuh; a unit is 128 keys, 32 a
+// warp.  The bytes are a quarter, so what bounds it is the warps' instructions (some 350 for 16 keys of 128 elements and up to 8 queries, 80 of them unpacking).
+// Codes enter the products as whole numbers, and scales and zeros are applied to what a group's elements or 16 keys have in common:
+//   * A code in the low bits of a 16-bit half is itself a subnormal FP16 number, code 2^-24, or code 2^-20 four bits higher; tensor cores take these exactly.  So
+//     a word of 8 codes becomes four operands by a shift and four masks.  Elements are taken in the order in which a word has them, the queries
+//     likewise, and a sixteenth of those that meet codes 2^-20.
+//   * S^T = K Q^T starts from -8 sum q and O^T += V^T P^T from a product of the weights with -8: codes around zero keep sums as small as the averages of many keys are
+//     (131072 keys: error against 64 bits 2.2e-4, that of the output's rounding; with codes from zero 7.1e-4).  With more than 8 queries the 8 comes off the values' codes
+//     instead, which costs less there.
+//   * p vs enters as FP16, brought into range by a power of two of the warp's largest scale, with its rest as a second part where the output is FP16;
+//     p (vz + 8 vs) is summed in FP32 per query.
+// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element near 2^8.  The tensor core cuts products off 2^-23 below the
+// largest of a step, so that a score is off by some 2^-21 of its terms' sizes: 2e-6 where scores are about 1.
+// Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 87 = 3.3 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 20;
+// 100 of up to 8000 with scales for every 64 elements: 48; 1 x 1000 keys of 32 heads: 7.2.  Of the 87, unpacking and products of the values are 25, of the keys 13, copies 13,
+// and a unit's bookkeeping, scales and exponentials the rest.  Tried, against what the kernel took then: four CTAs an SM with 128 registers 93 (88), two 107 (99); a pair of
+// lanes for the rows of a pair of keys, which saves exchanges of addresses but touches four times the lines a copy, 99 (91); tiles of 16 keys one by one 94 (91).
 #pragma once
 
 #include <type_traits>
