@@ -309,334 +309,335 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
         int stage = 0, q_at = -1;
         for (bool more = true; more;) {
-          const bool started_here = now.unit == 0;                             // the item's first unit is this CTA's
-          const int run = run_of(now);
-          for (int u = 0; u < run; u++) {
-            copy_wait<S - 2>();
-            __syncwarp();
-            if (u == 0) {
-                if (++q_at == S) q_at = 0;
-                __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
-                const unsigned char *const src = q_ring + q_at * Shape::kQ + r * Shape::kQPitch;
+            const bool started_here = now.unit == 0;                             // the item's first unit is this CTA's
+            const int run = run_of(now);
+            for (int u = 0; u < run; u++) {
+                copy_wait<S - 2>();
+                __syncwarp();
+                if (u == 0) {
+                    if (++q_at == S) q_at = 0;
+                    __syncthreads();                 // every warp's part of the queries is there, and the sums of the item before are read
+                    const unsigned char *const src = q_ring + q_at * Shape::kQ + r * Shape::kQPitch;
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    uint4 w[J];
-                    float f, s[G];
-                    query_operands<T, DP, G>(src + t * 8 * Shape::kQPitch, t4, w, f, s);
-                    if constexpr (Shape::kKeepQ) {
+                    for (int t = 0; t < NT; t++) {
+                        uint4 w[J];
+                        float f, s[G];
+                        query_operands<T, DP, G>(src + t * 8 * Shape::kQPitch, t4, w, f, s);
+                        if constexpr (Shape::kKeepQ) {
 #pragma unroll
-                        for (int j = 0; j < J; j++) q[t][j] = w[j];
-                    } else if (t % kAttnWarps == warp) {
+                            for (int j = 0; j < J; j++) q[t][j] = w[j];
+                        } else if (t % kAttnWarps == warp) {
 #pragma unroll
-                        for (int j = 0; j < J; j++) reinterpret_cast<uint4 *>(operands)[(t * J + j) * 32 + lane] = w[j];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * a.scale_log2;
-#pragma unroll
-                        for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
-                    }
-                    base[t][0] = base[t][1] = kNone;
-                    sum[t][0] = sum[t][1] = 0.f;
-#pragma unroll
-                    for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 2 * J; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
-                }
-                if constexpr (!Shape::kKeepQ) __syncthreads();
-            }
-            const uint32_t ok = oks[0];
-            const unsigned char *const keys = ring + stage * Shape::kStage, *const values = keys + Shape::kCodes, *const scales = values + Shape::kCodes;
-#pragma unroll
-            for (int i = 0; i + 1 < S - 1; i++) oks[i] = oks[i + 1];
-            oks[S - 2] = issue(pending, stage == 0 ? S - 1 : stage - 1);
-            pending = ticket();
-#pragma unroll
-            for (int h0 = 0; h0 < 2; h0 += TILES) {
-                const uint32_t there = ok >> (16 * h0) & kHere;
-                if (!there) continue;
-                // ---- scores of a tile of 16 keys, or of two: rows (keys) r and r + 8 of a tile, columns (queries) 2 t4 and the next
-                float s[TILES][NT][4];
-                float2 kv[TILES][2][G][2];           // scales and zeros: of key r or r + 8 of a tile, of the key and of the value
-#pragma unroll
-                for (int h = 0; h < TILES; h++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int g = 0; g < G; g++) {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(scales + ((16 * (h0 + h) + 8 * i + r) * G + g) * 8);
-                            kv[h][i][g][0] = Half<T>::unpack(w.x);
-                            kv[h][i][g][0].x *= 0x1p24f;                       // (of the codes' 2^-24)
-                            kv[h][i][g][1] = Half<T>::unpack(w.y);
+                            for (int j = 0; j < J; j++) reinterpret_cast<uint4 *>(operands)[(t * J + j) * 32 + lane] = w[j];
                         }
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    float x[TILES][NT][4];
+                        for (int e = 0; e < 2; e++) {
+                            factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * a.scale_log2;
+#pragma unroll
+                            for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
+                        }
+                        base[t][0] = base[t][1] = kNone;
+                        sum[t][0] = sum[t][1] = 0.f;
+#pragma unroll
+                        for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 2 * J; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
+                    }
+                    if constexpr (!Shape::kKeepQ) __syncthreads();
+                }
+                const uint32_t ok = oks[0];
+                const unsigned char *const keys = ring + stage * Shape::kStage, *const values = keys + Shape::kCodes, *const scales = values + Shape::kCodes;
+#pragma unroll
+                for (int i = 0; i + 1 < S - 1; i++) oks[i] = oks[i + 1];
+                oks[S - 2] = issue(pending, stage == 0 ? S - 1 : stage - 1);
+                pending = ticket();
+#pragma unroll
+                for (int h0 = 0; h0 < 2; h0 += TILES) {
+                    const uint32_t there = ok >> (16 * h0) & kHere;
+                    if (!there) continue;
+                    // ---- scores of a tile of 16 keys, or of two: rows (keys) r and r + 8 of a tile, columns (queries) 2 t4 and the next
+                    float s[TILES][NT][4];
+                    float2 kv[TILES][2][G][2];           // scales and zeros: of key r or r + 8 of a tile, of the key and of the value
 #pragma unroll
                     for (int h = 0; h < TILES; h++)
 #pragma unroll
-                        for (int t = 0; t < NT; t++)
+                        for (int i = 0; i < 2; i++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) x[h][t][e] = q_sum[t][g][e & 1] * -0x1p-21f;      // (8 off every code)
+                            for (int g = 0; g < G; g++) {
+                                const uint2 w = *reinterpret_cast<const uint2 *>(scales + ((16 * (h0 + h) + 8 * i + r) * G + g) * 8);
+                                kv[h][i][g][0] = Half<T>::unpack(w.x);
+                                kv[h][i][g][0].x *= 0x1p24f;                       // (of the codes' 2^-24)
+                                kv[h][i][g][1] = Half<T>::unpack(w.y);
+                            }
 #pragma unroll
-                    for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
+                    for (int g = 0; g < G; g++) {
+                        float x[TILES][NT][4];
+#pragma unroll
+                        for (int h = 0; h < TILES; h++)
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) x[h][t][e] = q_sum[t][g][e & 1] * -0x1p-21f;      // (8 off every code)
+#pragma unroll
+                        for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
+#pragma unroll
+                            for (int h = 0; h < TILES; h++) {
+                                const unsigned char *const at = keys + (16 * (h0 + h) + r) * Shape::kPitch + t4 * 4 + j * 16;
+                                const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch), v0 = w0 >> 8, v1 = w1 >> 8;
+                                const uint32_t lower[4] = {codes<true, false>(w0), codes<true, false>(w1), codes<false, false>(w0), codes<false, false>(w1)};
+                                const uint32_t upper[4] = {codes<true, false>(v0), codes<true, false>(v1), codes<false, false>(v0), codes<false, false>(v1)};
+#pragma unroll
+                                for (int t = 0; t < NT; t++) {
+                                    uint4 b;
+                                    if constexpr (Shape::kKeepQ) b = q[t][j];
+                                    else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
+                                    Half<__half>::mma(x[h][t], lower, b.x, b.y);
+                                    Half<__half>::mma(x[h][t], upper, b.z, b.w);
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int h = 0; h < TILES; h++) {
-                            const unsigned char *const at = keys + (16 * (h0 + h) + r) * Shape::kPitch + t4 * 4 + j * 16;
-                            const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch), v0 = w0 >> 8, v1 = w1 >> 8;
-                            const uint32_t lower[4] = {codes<true, false>(w0), codes<true, false>(w1), codes<false, false>(w0), codes<false, false>(w1)};
-                            const uint32_t upper[4] = {codes<true, false>(v0), codes<true, false>(v1), codes<false, false>(v0), codes<false, false>(v1)};
+                            const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
+                            const float z0 = a0.y + 0x1p-21f * a0.x, z1 = a1.y + 0x1p-21f * a1.x;
 #pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                uint4 b;
-                                if constexpr (Shape::kKeepQ) b = q[t][j];
-                                else b = reinterpret_cast<const uint4 *>(operands)[(t * J + j) * 32 + lane];
-                                Half<__half>::mma(x[h][t], lower, b.x, b.y);
-                                Half<__half>::mma(x[h][t], upper, b.z, b.w);
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++) {
+                                    const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
+                                    s[h][t][e] = g ? s[h][t][e] + y0 : y0;
+                                    s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
+                                }
+                        }
+                    }
+                    // from here on relative to the reference, which moves where one is kSlack above it (and at the first number: kNone lies far below)
+                    auto greatest = [](const float (&s)[TILES][NT][4], int t, int e) {
+                        float m = fmaxf(s[0][t][e], s[0][t][e + 2]);
+                        if constexpr (TILES == 2) m = fmaxf(m, fmaxf(s[TILES - 1][t][e], s[TILES - 1][t][e + 2]));
+                        return m;
+                    };
+                    float p[TILES][NT][4];
+                    bool grows = false;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+#pragma unroll
+                        for (int h = 0; h < TILES; h++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) p[h][t][e] = __fmaf_rn(s[h][t][e], factor[t][e & 1], -base[t][e & 1]);
+#pragma unroll
+                        if (there != kHere) {        // keys that are not there
+#pragma unroll
+                            for (int h = 0; h < TILES; h++) {
+                                const bool on0 = (there >> (16 * h + r)) & 1, on1 = (there >> (16 * h + r + 8)) & 1;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) p[h][t][e] = (e < 2 ? on0 : on1) ? p[h][t][e] : -INFINITY;
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; e++) grows = grows || greatest(p, t, e) > Type::lift + kSlack;
+                    }
+                    float scale_here = 0.f;
+#pragma unroll
+                    for (int h = 0; h < TILES; h++)
+#pragma unroll
+                        for (int g = 0; g < G; g++) scale_here = fmaxf(scale_here, fmaxf(kv[h][0][g][1].x, kv[h][1][g][1].x));
+                    if (__any_sync(kAll, grows || scale_here > largest)) {
+                        float biggest = fmaxf(largest, scale_here);
+                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 4));
+                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 8));
+                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 16));
+                        // the power of two at or above it, between 2^-100 and 2^126
+                        const uint32_t up = min(max((__float_as_uint(biggest) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
+                        const float was = largest;
+                        largest = __uint_as_float(up);
+                        to_one = __uint_as_float((254u << 23) - up);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            float keep[2];
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                float m = -INFINITY;
+                                auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? s[h][t][e + 2 * i] * factor[t][e] : -INFINITY; };
+#pragma unroll
+                                for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
+                                m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
+                                m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
+                                m = ceilf(fmaxf(m, __shfl_xor_sync(kAll, m, 16))) - Type::lift;
+                                keep[e] = 1.f;
+                                if (m > base[t][e]) {
+                                    keep[e] = exp2_approx(base[t][e] - m);
+                                    base[t][e] = m;
+                                }
+#pragma unroll
+                                for (int h = 0; h < TILES; h++) {
+                                    p[h][t][e] = score(h, 0) - base[t][e];
+                                    p[h][t][e + 2] = score(h, 1) - base[t][e];
+                                }
+                                sum[t][e] *= keep[e];
+#pragma unroll
+                                for (int g = 0; g < G; g++) zeros[t][g][e] *= keep[e];
+                                keep[e] *= was * to_one;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2 * J; i++) {
+                                o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1]; o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
                             }
                         }
                     }
 #pragma unroll
-                    for (int h = 0; h < TILES; h++) {
-                        const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
-                        const float z0 = a0.y + 0x1p-21f * a0.x, z1 = a1.y + 0x1p-21f * a1.x;
+                    for (int h = 0; h < TILES; h++)
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
-                                const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
-                                s[h][t][e] = g ? s[h][t][e] + y0 : y0;
-                                s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
+                                p[h][t][e] = exp2_approx(p[h][t][e]);
+                                p[h][t][e + 2] = exp2_approx(p[h][t][e + 2]);
+                                sum[t][e] += p[h][t][e] + p[h][t][e + 2];
                             }
-                    }
-                }
-                // from here on relative to the reference, which moves where one is kSlack above it (and at the first number: kNone lies far below)
-                auto greatest = [](const float (&s)[TILES][NT][4], int t, int e) {
-                    float m = fmaxf(s[0][t][e], s[0][t][e + 2]);
-                    if constexpr (TILES == 2) m = fmaxf(m, fmaxf(s[TILES - 1][t][e], s[TILES - 1][t][e + 2]));
-                    return m;
-                };
-                float p[TILES][NT][4];
-                bool grows = false;
+                    // ---- values: a lane's pairs of keys are 2 t4 and 2 t4 + 8 of a tile with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
+                    for (int g = 0; g < G; g++) {
+                        uint32_t hi[TILES][NT][2], lo[TILES][NT][2];
 #pragma unroll
-                    for (int h = 0; h < TILES; h++)
+                        for (int h = 0; h < TILES; h++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) p[h][t][e] = __fmaf_rn(s[h][t][e], factor[t][e & 1], -base[t][e & 1]);
+                            for (int i = 0; i < 2; i++) {
+                                const float2 b = kv[h][i][g][1];
+                                const float f = b.x * to_one, z = b.y + 8.f * b.x;
 #pragma unroll
-                    for (int h = 0; there != kHere && h < TILES; h++) {        // (keys that are not there)
-                        const bool on0 = (there >> (16 * h + r)) & 1, on1 = (there >> (16 * h + r + 8)) & 1;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) p[h][t][e] = (e < 2 ? on0 : on1) ? p[h][t][e] : -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; e++) grows = grows || greatest(p, t, e) > Type::lift + kSlack;
-                }
-                float scale_here = 0.f;
-#pragma unroll
-                for (int h = 0; h < TILES; h++)
-#pragma unroll
-                    for (int g = 0; g < G; g++) scale_here = fmaxf(scale_here, fmaxf(kv[h][0][g][1].x, kv[h][1][g][1].x));
-                if (__any_sync(kAll, grows || scale_here > largest)) {
-                    float biggest = fmaxf(largest, scale_here);
-                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 4));
-                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 8));
-                    biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 16));
-                    // the power of two at or above it, between 2^-100 and 2^126
-                    const uint32_t up = min(max((__float_as_uint(biggest) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
-                    const float was = largest;
-                    largest = __uint_as_float(up);
-                    to_one = __uint_as_float((254u << 23) - up);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        float keep[2];
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float m = -INFINITY;
-                            auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? s[h][t][e + 2 * i] * factor[t][e] : -INFINITY; };
-#pragma unroll
-                            for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
-                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
-                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
-                            m = ceilf(fmaxf(m, __shfl_xor_sync(kAll, m, 16))) - Type::lift;
-                            keep[e] = 1.f;
-                            if (m > base[t][e]) {
-                                keep[e] = exp2_approx(base[t][e] - m);
-                                base[t][e] = m;
-                            }
-#pragma unroll
-                            for (int h = 0; h < TILES; h++) {
-                                p[h][t][e] = score(h, 0) - base[t][e];
-                                p[h][t][e + 2] = score(h, 1) - base[t][e];
-                            }
-                            sum[t][e] *= keep[e];
-#pragma unroll
-                            for (int g = 0; g < G; g++) zeros[t][g][e] *= keep[e];
-                            keep[e] *= was * to_one;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 2 * J; i++) {
-                            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1]; o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
-                        }
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < TILES; h++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            p[h][t][e] = exp2_approx(p[h][t][e]);
-                            p[h][t][e + 2] = exp2_approx(p[h][t][e + 2]);
-                            sum[t][e] += p[h][t][e] + p[h][t][e + 2];
-                        }
-                // ---- values: a lane's pairs of keys are 2 t4 and 2 t4 + 8 of a tile with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    uint32_t hi[TILES][NT][2], lo[TILES][NT][2];
-#pragma unroll
-                    for (int h = 0; h < TILES; h++)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const float2 b = kv[h][i][g][1];
-                            const float f = b.x * to_one, z = b.y + 8.f * b.x;
-#pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
-                                zeros[t][g][0] += p0 * z;
-                                zeros[t][g][1] += p1 * z;
-                                const uint32_t up = pack_half2(y0, y1);
-                                hi[h][t][i] = transpose8x8(up);
-                                if constexpr (kParts == 2) {
-                                    const float2 w = Half<__half>::unpack(up);
-                                    lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
+                                for (int t = 0; t < NT; t++) {
+                                    const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
+                                    zeros[t][g][0] += p0 * z;
+                                    zeros[t][g][1] += p1 * z;
+                                    const uint32_t up = pack_half2(y0, y1);
+                                    hi[h][t][i] = transpose8x8(up);
+                                    if constexpr (kParts == 2) {
+                                        const float2 w = Half<__half>::unpack(up);
+                                        lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
+                                    }
                                 }
                             }
+                        // 8 off every code: a product of the weights with -8 in the codes' units (rows r and r + 8 are of codes 2^-24 and 2^-20), where sums start from
+                        float start[NT][4];
+                        if (!CENTRED) {
+                            const uint32_t eights[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                start[t][0] = start[t][1] = start[t][2] = start[t][3] = 0.f;
+#pragma unroll
+                                for (int h = 0; h < TILES; h++)
+#pragma unroll
+                                    for (int part = 0; part < kParts; part++) Half<__half>::mma(start[t], eights, part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                            }
                         }
-                    // 8 off every code: a product of the weights with -8 in the codes' units (rows r and r + 8 are of codes 2^-24 and 2^-20), where sums start from
-                    float start[NT][4];
-                    if (!CENTRED) {
-                        const uint32_t eights[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
+                        // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; those of tile h from pair(h, x, y)
+                        auto products = [&](int at, auto pair) {
+                            float sums[2][NT][4];
 #pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            start[t][0] = start[t][1] = start[t][2] = start[t][3] = 0.f;
+                            for (int h = 0; h < TILES; h++) {
+                                uint32_t x, y;
+                                pair(h, x, y);
+                                const uint32_t x8 = x >> 8, y8 = y >> 8;
+                                const uint32_t w[2][4] = {{codes<true, CENTRED>(x), codes<false, CENTRED>(x), codes<true, CENTRED>(y), codes<false, CENTRED>(y)},
+                                                          {codes<true, CENTRED>(x8), codes<false, CENTRED>(x8), codes<true, CENTRED>(y8), codes<false, CENTRED>(y8)}};
 #pragma unroll
-                            for (int h = 0; h < TILES; h++)
+                                for (int part = 0; part < kParts; part++)
 #pragma unroll
-                                for (int part = 0; part < kParts; part++) Half<__half>::mma(start[t], eights, part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
-                        }
-                    }
-                    // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; those of tile h from pair(h, x, y)
-                    auto products = [&](int at, auto pair) {
-                        float sums[2][NT][4];
+                                    for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int h = 0; h < TILES; h++) {
-                            uint32_t x, y;
-                            pair(h, x, y);
-                            const uint32_t x8 = x >> 8, y8 = y >> 8;
-                            const uint32_t w[2][4] = {{codes<true, CENTRED>(x), codes<false, CENTRED>(x), codes<true, CENTRED>(y), codes<false, CENTRED>(y)},
-                                                      {codes<true, CENTRED>(x8), codes<false, CENTRED>(x8), codes<true, CENTRED>(y8), codes<false, CENTRED>(y8)}};
-#pragma unroll
-                            for (int part = 0; part < kParts; part++)
+                                        for (int t = 0; t < NT; t++) {
+                                            if (!CENTRED && h == 0 && part == 0) { sums[i][t][0] = start[t][0]; sums[i][t][1] = start[t][1]; sums[i][t][2] = start[t][2]; sums[i][t][3] = start[t][3]; }
+                                            Half<__half>::mma(CENTRED ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                                        }
+                            }
+                            if (!CENTRED) {
 #pragma unroll
                                 for (int i = 0; i < 2; i++)
 #pragma unroll
-                                    for (int t = 0; t < NT; t++) {
-                                        if (!CENTRED && h == 0 && part == 0) { sums[i][t][0] = start[t][0]; sums[i][t][1] = start[t][1]; sums[i][t][2] = start[t][2]; sums[i][t][3] = start[t][3]; }
-                                        Half<__half>::mma(CENTRED ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
-                                    }
+                                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                                        for (int e = 0; e < 4; e++) o[at + i][t][e] += sums[i][t][e];
+                            }
+                        };
+#pragma unroll
+                        for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++) {
+                            uint32_t w[TILES][4];
+#pragma unroll
+                            for (int h = 0; h < TILES; h++) {
+                                const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + r * 4 + ch * 32;
+                                w[h][0] = word_at(at); w[h][1] = word_at(at + Shape::kPitch); w[h][2] = word_at(at + 8 * Shape::kPitch); w[h][3] = word_at(at + 9 * Shape::kPitch);
+                            }
+#pragma unroll
+                            for (int half = 0; half < 2; half++)
+                                products(4 * ch + 2 * half, [&](int h, uint32_t &x, uint32_t &y) {
+                                    x = __byte_perm(w[h][0], w[h][1], half ? 0x7632 : 0x5410);
+                                    y = __byte_perm(w[h][2], w[h][3], half ? 0x7632 : 0x5410);
+                                });
                         }
-                        if (!CENTRED) {
-#pragma unroll
-                            for (int i = 0; i < 2; i++)
-#pragma unroll
-                                for (int t = 0; t < NT; t++)
-#pragma unroll
-                                    for (int e = 0; e < 4; e++) o[at + i][t][e] += sums[i][t][e];
-                        }
-                    };
-#pragma unroll
-                    for (int ch = GROUPED ? g : 0; ch < (GROUPED ? g + 1 : CH); ch++) {
-                        uint32_t w[TILES][4];
-#pragma unroll
-                        for (int h = 0; h < TILES; h++) {
-                            const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + r * 4 + ch * 32;
-                            w[h][0] = word_at(at); w[h][1] = word_at(at + Shape::kPitch); w[h][2] = word_at(at + 8 * Shape::kPitch); w[h][3] = word_at(at + 9 * Shape::kPitch);
-                        }
-#pragma unroll
-                        for (int half = 0; half < 2; half++)
-                            products(4 * ch + 2 * half, [&](int h, uint32_t &x, uint32_t &y) {
-                                x = __byte_perm(w[h][0], w[h][1], half ? 0x7632 : 0x5410);
-                                y = __byte_perm(w[h][2], w[h][3], half ? 0x7632 : 0x5410);
+                        if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
+                            products(4 * CH, [&](int h, uint32_t &x, uint32_t &y) {
+                                const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4;
+                                const uint32_t half = r & 1 ? 0x7632 : 0x5410;
+                                x = __byte_perm(word_at(at), word_at(at + Shape::kPitch), half);
+                                y = __byte_perm(word_at(at + 8 * Shape::kPitch), word_at(at + 9 * Shape::kPitch), half);
                             });
-                    }
-                    if constexpr (HALF) {        // the last 32 elements: 4 r to 4 r + 3
-                        products(4 * CH, [&](int h, uint32_t &x, uint32_t &y) {
-                            const unsigned char *const at = values + (16 * (h0 + h) + 2 * t4) * Shape::kPitch + CH * 32 + (r >> 1) * 4;
-                            const uint32_t half = r & 1 ? 0x7632 : 0x5410;
-                            x = __byte_perm(word_at(at), word_at(at + Shape::kPitch), half);
-                            y = __byte_perm(word_at(at + 8 * Shape::kPitch), word_at(at + 9 * Shape::kPitch), half);
-                        });
+                        }
                     }
                 }
+                if (++stage == S) stage = 0;
             }
-            if (++stage == S) stage = 0;
-          }
             const bool last = now.unit + run == now.s.units;
-            {
-                // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
-                // issued behind the barrier above.  What was 2^lift and `largest` times too large is brought back here.
-                const int head = now.inner / a.groups, group = now.inner - head * a.groups;
-                const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
-                const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
-                const bool whole = started_here && last;
-                const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
-                constexpr float kDown = 1.f / 256.f;
-                static_assert(Type::lift == 8.f, "the power of two above");
-                auto over_keys = [](float x) {
-                    x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    x += __shfl_xor_sync(0xffffffffu, x, 8);
-                    return x + __shfl_xor_sync(0xffffffffu, x, 16);
-                };
+            // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
+            // issued behind the barrier above.  What was 2^lift and `largest` times too large is brought back here.
+            const int head = now.inner / a.groups, group = now.inner - head * a.groups;
+            const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
+            const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
+            const bool whole = started_here && last;
+            const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
+            constexpr float kDown = 1.f / 256.f;
+            static_assert(Type::lift == 8.f, "the power of two above");
+            auto over_keys = [](float x) {
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                return x + __shfl_xor_sync(0xffffffffu, x, 16);
+            };
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float l = over_keys(sum[t][e]);
+                    if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
+#pragma unroll
+                    for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
+                }
+            const int used = stage == 0 ? S - 1 : stage - 1;
+            float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
+            const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
+            constexpr int WARP_FLOATS = S * Shape::kStage / 4;
+            const float times = largest * (kDown * 0x1p24f), times16 = times * 0.0625f;       // of codes 2^-24 and 2^-20
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                __syncwarp();                // the warp has read its values
+                if (t) __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 2 * J; i++) {
+                    const int el = i < 4 * CH ? (i / 4) * 64 + 8 * r + 2 * (i % 4) : CH * 64 + 4 * r + 2 * (i % 4);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float l = over_keys(sum[t][e]);
-                        if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
-#pragma unroll
-                        for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
+                        const float z = zeros[t][GROUPED ? i / 4 : 0][e];
+                        *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times16 + z);
                     }
-                const int used = stage == 0 ? S - 1 : stage - 1;
-                float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
-                const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
-                constexpr int WARP_FLOATS = S * Shape::kStage / 4;
-                const float times = largest * (kDown * 0x1p24f), times16 = times * 0.0625f;       // of codes 2^-24 and 2^-20
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    __syncwarp();                // the warp has read its values
-                    if (t) __syncthreads();
-#pragma unroll
-                    for (int i = 0; i < 2 * J; i++) {
-                        const int el = i < 4 * CH ? (i / 4) * 64 + 8 * r + 2 * (i % 4) : CH * 64 + 4 * r + 2 * (i % 4);
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float z = zeros[t][GROUPED ? i / 4 : 0][e];
-                            *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times16 + z);
-                        }
-                    }
-                    __syncthreads();
-                    add_warps<T, DP, NT, CLUSTER, WARP_FLOATS, Shape::kFoldPitch>(a, folds, sums, t, now.b, h0, heads, whole, slot, rank, ranks, arrived_sums, arrived);
                 }
-                const Walk<kQUnitKeys> was = now;
-                more = next_item(now, run);
-                if constexpr (!CLUSTER) {
-                    if (!more && tid == 0) a.cut[cta] = make_int4((int)was.b, was.inner, (int)((item_at + was.s.units) / per), started_here && !last ? 1 : 0);
-                    item_at += was.s.units + 1;
-                }
+                __syncthreads();
+                add_warps<T, DP, NT, CLUSTER, WARP_FLOATS, Shape::kFoldPitch>(a, folds, sums, t, now.b, h0, heads, whole, slot, rank, ranks, arrived_sums, arrived);
+            }
+            const Walk<kQUnitKeys> was = now;
+            more = next_item(now, run);
+            if constexpr (!CLUSTER) {
+                if (!more && tid == 0) a.cut[cta] = make_int4((int)was.b, was.inner, (int)((item_at + was.s.units) / per), started_here && !last ? 1 : 0);
+                item_at += was.s.units + 1;
             }
         }
         copy_wait<0>();

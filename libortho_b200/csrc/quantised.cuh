@@ -1,4 +1,4 @@
-// The paged cache held in 4 bits (include/ortho_b200.h has the format): checks of its record, and the unpacking of codes.
+// The paged cache held in 4 bits (include/ortho_b200.h has the format): the checks of its record.
 #pragma once
 
 #include "launch.cuh"
