@@ -12,8 +12,8 @@
 //   * S^T = K Q^T starts from -8 sum q and O^T += V^T P^T from a product of the weights with -8: codes around zero keep sums as small as the averages of many keys are
 //     (131072 keys: error against 64 bits 2.2e-4, that of the output's rounding; with codes from zero 7.1e-4).  With more than 8 queries the 8 comes off the values' codes
 //     instead, which costs less there.
-//   * p vs enters as FP16, brought into range by a power of two of the warp's largest scale, with its rest as a second part where the output is FP16;
-//     p (vz + 8 vs) is summed in FP32 per query.
+//   * p vs enters as FP16, with its rest as a second part where the output is FP16.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
+//     kept from item to item, would let a key that weighs nothing, or another request, push the others' into FP16's subnormal numbers.  p (vz + 8 vs) is summed in FP32 per query.
 // FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element near 2^8.  The tensor core cuts products off 2^-23 below the
 // largest of a step, so that a score is off by some 2^-21 of its terms' sizes: 2e-6 where scores are about 1.
 // Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 87 = 3.3 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 20;
@@ -77,6 +77,9 @@ template <bool LOW, bool CENTRED> __device__ __forceinline__ uint32_t codes(uint
     const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
+
+// 2^8 / x of a power of two between 2^-118 and 2^126
+__device__ __forceinline__ float two_to_8_over(float x) { return __uint_as_float((262u << 23) - __float_as_uint(x)); }
 
 // Eight elements of a query, in memory's order, as the products take them: (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ uint4 as_codes_lie(uint4 w)
@@ -148,6 +151,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
     // Codes less 8 are added up as they come.  With one column of queries it takes less to add up the codes themselves, over 32 keys at a time.
     constexpr bool CENTRED = NT > 1;
     constexpr int TILES = NT * DP <= 128 ? 2 : 1;                              // of 16 keys that are worked on together, as registers allow
+    // Scales and zeros of values times kSmall, so that FP32 holds their sums with weights of up to 2^15
+    constexpr float kSmall = std::is_same<T, __half>::value ? 1.f : 0x1p-16f, kMostWeight = 32768.f;
+    static_assert(Type::lift + kSlack == 15.f, "log2 of kMostWeight");
     constexpr uint32_t kAll = 0xffffffffu, kHere = TILES == 2 ? kAll : 0xFFFFu;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs &a = args.a;
@@ -306,7 +312,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
         float base[NT][2];                       // what is taken off scores: the largest by the time, rounded up to a whole number, - lift; kNone before the first
-        float largest = 0.f, to_one = 1.f;       // a power of two that no value's scale has been above, and its inverse
+        float down[NT][2];                       // a power of two that brings the item's largest weight times scale by the time to 2^7 .. 2^15
         int stage = 0, q_at = -1;
         for (bool more = true; more;) {
             const bool started_here = now.unit == 0;                             // the item's first unit is this CTA's
@@ -337,6 +343,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
                         }
                         base[t][0] = base[t][1] = kNone;
+                        down[t][0] = down[t][1] = 1.f;
                         sum[t][0] = sum[t][1] = 0.f;
 #pragma unroll
                         for (int g = 0; g < G; g++) zeros[t][g][0] = zeros[t][g][1] = 0.f;
@@ -412,14 +419,19 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 }
                         }
                     }
-                    // from here on relative to the reference, which moves where one is kSlack above it (and at the first number: kNone lies far below)
-                    auto greatest = [](const float (&s)[TILES][NT][4], int t, int e) {
-                        float m = fmaxf(s[0][t][e], s[0][t][e + 2]);
-                        if constexpr (TILES == 2) m = fmaxf(m, fmaxf(s[TILES - 1][t][e], s[TILES - 1][t][e + 2]));
+                    // Weights relative to the reference, which moves where one is kSlack above it (and at the first number: kNone lies far below).  A weight times the value's scale has a
+                    // reference of its own, because the products take it in FP16: what counts is how large it is beside the item's other keys.
+                    float p[TILES][NT][4], most_scale = 0.f;
+                    bool grows = false;
+                    auto value_scale = [&](int h, int i) {
+                        float m = fabsf(kv[h][i][0][1].x);
+#pragma unroll
+                        for (int g = 1; g < G; g++) m = fmaxf(m, fabsf(kv[h][i][g][1].x));
                         return m;
                     };
-                    float p[TILES][NT][4];
-                    bool grows = false;
+#pragma unroll
+                    for (int h = 0; h < TILES; h++) most_scale = fmaxf(most_scale, fmaxf(value_scale(h, 0), value_scale(h, 1)));
+                    most_scale *= kSmall;
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -436,23 +448,22 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 2; e++) grows = grows || greatest(p, t, e) > Type::lift + kSlack;
+                        for (int h = 0; h < TILES; h++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) p[h][t][e] = exp2_approx(p[h][t][e]);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float m = fmaxf(p[0][t][e], p[0][t][e + 2]);
+                            if constexpr (TILES == 2) m = fmaxf(m, fmaxf(p[TILES - 1][t][e], p[TILES - 1][t][e + 2]));
+                            grows = grows || m > kMostWeight || m * down[t][e] * most_scale > kMostWeight;
+                        }
                     }
-                    float scale_here = 0.f;
-#pragma unroll
-                    for (int h = 0; h < TILES; h++)
-#pragma unroll
-                        for (int g = 0; g < G; g++) scale_here = fmaxf(scale_here, fmaxf(kv[h][0][g][1].x, kv[h][1][g][1].x));
-                    if (__any_sync(kAll, grows || scale_here > largest)) {
-                        float biggest = fmaxf(largest, scale_here);
-                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 4));
-                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 8));
-                        biggest = fmaxf(biggest, __shfl_xor_sync(kAll, biggest, 16));
-                        // the power of two at or above it, between 2^-100 and 2^126
-                        const uint32_t up = min(max((__float_as_uint(biggest) + 0x7FFFFFu) & 0x7F800000u, 27u << 23), 253u << 23);
-                        const float was = largest;
-                        largest = __uint_as_float(up);
-                        to_one = __uint_as_float((254u << 23) - up);
+                    if (__any_sync(kAll, grows)) {
+                        auto over_rows = [](float m) {
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
+                            return fmaxf(m, __shfl_xor_sync(kAll, m, 16));
+                        };
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             float keep[2];
@@ -462,23 +473,28 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? s[h][t][e + 2 * i] * factor[t][e] : -INFINITY; };
 #pragma unroll
                                 for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
-                                m = fmaxf(m, __shfl_xor_sync(kAll, m, 4));
-                                m = fmaxf(m, __shfl_xor_sync(kAll, m, 8));
-                                m = ceilf(fmaxf(m, __shfl_xor_sync(kAll, m, 16))) - Type::lift;
+                                m = ceilf(over_rows(m)) - Type::lift;
                                 keep[e] = 1.f;
                                 if (m > base[t][e]) {
                                     keep[e] = exp2_approx(base[t][e] - m);
                                     base[t][e] = m;
                                 }
+                                m = 0.f;
 #pragma unroll
-                                for (int h = 0; h < TILES; h++) {
-                                    p[h][t][e] = score(h, 0) - base[t][e];
-                                    p[h][t][e + 2] = score(h, 1) - base[t][e];
-                                }
+                                for (int h = 0; h < TILES; h++)
+#pragma unroll
+                                    for (int i = 0; i < 2; i++) {
+                                        p[h][t][e + 2 * i] = exp2_approx(score(h, i) - base[t][e]);
+                                        m = fmaxf(m, p[h][t][e + 2 * i] * (value_scale(h, i) * kSmall));
+                                    }
                                 sum[t][e] *= keep[e];
 #pragma unroll
                                 for (int g = 0; g < G; g++) zeros[t][g][e] *= keep[e];
-                                keep[e] *= was * to_one;
+                                // the power of two at or above the largest weight times scale, between 2^-100 and 2^126: this goes to 2^8
+                                keep[e] *= two_to_8_over(down[t][e]);
+                                const uint32_t up = (__float_as_uint(fmaxf(over_rows(m), keep[e])) + 0x7FFFFFu) & 0x7F800000u;
+                                down[t][e] = two_to_8_over(__uint_as_float(min(max(up, 27u << 23), 253u << 23)));
+                                keep[e] *= down[t][e] * (1.f / 256.f);
                             }
 #pragma unroll
                             for (int i = 0; i < 2 * J; i++) {
@@ -491,11 +507,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                p[h][t][e] = exp2_approx(p[h][t][e]);
-                                p[h][t][e + 2] = exp2_approx(p[h][t][e + 2]);
-                                sum[t][e] += p[h][t][e] + p[h][t][e + 2];
-                            }
+                            for (int e = 0; e < 2; e++) sum[t][e] += p[h][t][e] + p[h][t][e + 2];
                     // ---- values: a lane's pairs of keys are 2 t4 and 2 t4 + 8 of a tile with the next ones each; it has the elements 8 r to 8 r + 7 of a chunk of 64
 #pragma unroll
                     for (int g = 0; g < G; g++) {
@@ -504,11 +516,10 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         for (int h = 0; h < TILES; h++)
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
-                                const float2 b = kv[h][i][g][1];
-                                const float f = b.x * to_one, z = b.y + 8.f * b.x;
+                                const float f = kv[h][i][g][1].x * kSmall, z = kv[h][i][g][1].y * kSmall + 8.f * f;
 #pragma unroll
                                 for (int t = 0; t < NT; t++) {
-                                    const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * f, y1 = p1 * f;
+                                    const float p0 = p[h][t][2 * i], p1 = p[h][t][2 * i + 1], y0 = p0 * down[t][0] * f, y1 = p1 * down[t][1] * f;
                                     zeros[t][g][0] += p0 * z;
                                     zeros[t][g][1] += p1 * z;
                                     const uint32_t up = pack_half2(y0, y1);
@@ -590,7 +601,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
             }
             const bool last = now.unit + run == now.s.units;
             // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
-            // issued behind the barrier above.  What was 2^lift and `largest` times too large is brought back here.
+            // issued behind the barrier above.  What 2^lift and `down` have made of the sums is undone here.
             const int head = now.inner / a.groups, group = now.inner - head * a.groups;
             const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
             const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
@@ -610,13 +621,13 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     const float l = over_keys(sum[t][e]);
                     if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
 #pragma unroll
-                    for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * kDown;
+                    for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * (kDown / kSmall);
                 }
             const int used = stage == 0 ? S - 1 : stage - 1;
             float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
             const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
             constexpr int WARP_FLOATS = S * Shape::kStage / 4;
-            const float times = largest * (kDown * 0x1p24f), times16 = times * 0.0625f;       // of codes 2^-24 and 2^-20
+            constexpr float kUp = kDown * 0x1p24f / kSmall, kUp16 = kUp * 0.0625f;              // of codes 2^-24 and 2^-20
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 __syncwarp();                // the warp has read its values
@@ -626,8 +637,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                     const int el = i < 4 * CH ? (i / 4) * 64 + 8 * r + 2 * (i % 4) : CH * 64 + 4 * r + 2 * (i % 4);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float z = zeros[t][GROUPED ? i / 4 : 0][e];
-                        *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * times + z, o[i][t][e + 2] * times16 + z);
+                        const float z = zeros[t][GROUPED ? i / 4 : 0][e], times = two_to_8_over(down[t][e]) * (1.f / 256.f);
+                        *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * kUp * times + z, o[i][t][e + 2] * kUp16 * times + z);
                     }
                 }
                 __syncthreads();
