@@ -14,7 +14,7 @@
 //     instead, which costs less there.
 //   * p vs enters as FP16, with its rest as a second part where the output is FP16.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
 //     kept from item to item, would let a key that weighs nothing, or another request, push the others' into FP16's subnormal numbers.  p (vz + 8 vs) is summed in FP32 per query.
-// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element near 2^8.  The tensor core cuts products off 2^-23 below the
+// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element to 2^14.  The tensor core cuts products off 2^-23 below the
 // largest of a step, so that a score is off by some 2^-21 of its terms' sizes: 2e-6 where scores are about 1.
 // Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 87 = 3.3 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 20;
 // 100 of up to 8000 with scales for every 64 elements: 48; 1 x 1000 keys of 32 heads: 7.2.  Of the 87, unpacking and products of the values are 25, of the keys 13, copies 13,
@@ -78,6 +78,9 @@ template <bool LOW, bool CENTRED> __device__ __forceinline__ uint32_t codes(uint
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
+// a b + c with FP32's subnormal numbers, which scores of very small keys pass through
+__device__ __forceinline__ float mul_add(float a, float b, float c) { float r; asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
 // 2^8 / x of a power of two between 2^-118 and 2^126
 __device__ __forceinline__ float two_to_8_over(float x) { return __uint_as_float((262u << 23) - __float_as_uint(x)); }
 
@@ -102,11 +105,11 @@ __device__ __forceinline__ void query_operands(const unsigned char *row, int t, 
     most = max(most & 0xFFFFu, most >> 16);
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    // e: FP32's exponent of the largest, of zero the least; elements times 2^(8 - e).  (Infinity and NaN stay what they are; of rows below 2^-100 nothing is lost that FP32 shows.)
+    // e: FP32's exponent of the largest, of zero the least; elements times 2^(14 - e).  (Infinity and NaN stay what they are; of rows below 2^-100 nothing is lost that FP32 shows.)
     const float size = Half<T>::unpack(most).x;
     const int e = min(max((int)(__float_as_uint(size) >> 23), 27), 254);
-    const float by = __uint_as_float((uint32_t)(262 - e) << 23);
-    f = __uint_as_float((uint32_t)(e - 8) << 23);
+    const float by = __uint_as_float((uint32_t)(268 - e) << 23);
+    f = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
     for (int j = 0; j < J; j++) {
         uint32_t *const x = reinterpret_cast<uint32_t *>(&w[j]);
@@ -309,7 +312,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         others_started();
 
         uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
-        float factor[NT][2], q_sum[NT][G][2];    // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements
+        // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements.  Scores are in units of the codes' 2^-24 up to `factor`: FP32 holds them for keys of any size.
+        float factor[NT][2], q_sum[NT][G][2];
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
         float base[NT][2];                       // what is taken off scores: the largest by the time, rounded up to a whole number, - lift; kNone before the first
         float down[NT][2];                       // a power of two that brings the item's largest weight times scale by the time to 2^7 .. 2^15
@@ -338,9 +342,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         }
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * a.scale_log2;
+                            factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * (a.scale_log2 * 0x1p24f);
 #pragma unroll
-                            for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4);
+                            for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4) * 0x1p-24f;
                         }
                         base[t][0] = base[t][1] = kNone;
                         down[t][0] = down[t][1] = 1.f;
@@ -375,7 +379,6 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             for (int g = 0; g < G; g++) {
                                 const uint2 w = *reinterpret_cast<const uint2 *>(scales + ((16 * (h0 + h) + 8 * i + r) * G + g) * 8);
                                 kv[h][i][g][0] = Half<T>::unpack(w.x);
-                                kv[h][i][g][0].x *= 0x1p24f;                       // (of the codes' 2^-24)
                                 kv[h][i][g][1] = Half<T>::unpack(w.y);
                             }
 #pragma unroll
@@ -386,7 +389,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                             for (int t = 0; t < NT; t++)
 #pragma unroll
-                                for (int e = 0; e < 4; e++) x[h][t][e] = q_sum[t][g][e & 1] * -0x1p-21f;      // (8 off every code)
+                                for (int e = 0; e < 4; e++) x[h][t][e] = q_sum[t][g][e & 1] * -8.f;           // (8 off every code)
 #pragma unroll
                         for (int j = g * (J / G); j < (g + 1) * (J / G); j++) {
 #pragma unroll
@@ -408,14 +411,13 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int h = 0; h < TILES; h++) {
                             const float2 a0 = kv[h][0][g][0], a1 = kv[h][1][g][0];
-                            const float z0 = a0.y + 0x1p-21f * a0.x, z1 = a1.y + 0x1p-21f * a1.x;
+                            const float z0 = mul_add(8.f, a0.x, a0.y), z1 = mul_add(8.f, a1.x, a1.y);
 #pragma unroll
                             for (int t = 0; t < NT; t++)
 #pragma unroll
                                 for (int e = 0; e < 2; e++) {
-                                    const float y0 = a0.x * x[h][t][e] + z0 * q_sum[t][g][e], y1 = a1.x * x[h][t][e + 2] + z1 * q_sum[t][g][e];
-                                    s[h][t][e] = g ? s[h][t][e] + y0 : y0;
-                                    s[h][t][e + 2] = g ? s[h][t][e + 2] + y1 : y1;
+                                    s[h][t][e] = mul_add(a0.x, x[h][t][e], mul_add(z0, q_sum[t][g][e], g ? s[h][t][e] : 0.f));
+                                    s[h][t][e + 2] = mul_add(a1.x, x[h][t][e + 2], mul_add(z1, q_sum[t][g][e], g ? s[h][t][e + 2] : 0.f));
                                 }
                         }
                     }
@@ -437,7 +439,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                         for (int h = 0; h < TILES; h++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) p[h][t][e] = __fmaf_rn(s[h][t][e], factor[t][e & 1], -base[t][e & 1]);
+                            for (int e = 0; e < 4; e++) p[h][t][e] = mul_add(s[h][t][e], factor[t][e & 1], -base[t][e & 1]);
 #pragma unroll
                         if (there != kHere) {        // keys that are not there
 #pragma unroll
@@ -470,7 +472,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                             for (int e = 0; e < 2; e++) {
                                 float m = -INFINITY;
-                                auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? s[h][t][e + 2 * i] * factor[t][e] : -INFINITY; };
+                                auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? mul_add(s[h][t][e + 2 * i], factor[t][e], 0.f) : -INFINITY; };
 #pragma unroll
                                 for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
                                 m = ceilf(over_rows(m)) - Type::lift;

@@ -86,3 +86,21 @@ def test_scales_that_rise_and_fall_along_a_request(D, groups, G, dtype, far):
             ks[held] = 0
             ks[held, :, 0, :, 1] = (-against * 0.6931471805599453 * ramp).view(100, 16, 1).to(dtype)
             near(_C_ops.paged_attention_quantised(q, k, v, ks, vs, table, n), plain(q, k, v, ks, vs, table, n))
+
+
+@pytest.mark.parametrize("D,groups,G", [(64, 1, 4), (128, 2, 4), (128, 1, 12), (96, 1, 24), (256, 1, 4)])
+def test_sizes_near_the_ends_of_a_type(D, groups, G):
+    """Keys of 2^112 with queries of 2^-112, and the other way round; values of 2^112 and 2^-90: beside ordinary requests, which give the same bits without them."""
+    lengths = [300 if b % 3 else (b * 7919) % 200 + 1 for b in range(60)]
+    q, k, v, ks, vs, table, n = make(lengths, 2 * G, 2, D, 64, BF16, groups, seed=D)
+    table = widened(table, 96)
+    want = _C_ops.paged_attention_quantised(q, k, v, ks, vs, table, n)
+    for b in range(0, 60, 2):
+        pages, far = table[b, :-(-lengths[b] // 64)].long(), 112 if b % 4 else -112
+        times(ks, pages, 2.0 ** far)
+        q[b] = (q[b].double() * 2.0 ** -far).to(BF16)
+        times(vs, pages, 2.0 ** (112 if b % 8 < 4 else -90))
+    got = _C_ops.paged_attention_quantised(q, k, v, ks, vs, table, n)
+    assert torch.equal(got[1::2], want[1::2])
+    pick = list(range(12)) + [56, 57, 58, 59]
+    near(got[pick], plain(q[pick], k, v, ks, vs, table[pick], n[pick]))
