@@ -12,7 +12,7 @@
 //   * S^T = K Q^T starts from -8 sum q and O^T += V^T P^T from a product of the weights with -8: codes around zero keep sums as small as the averages of many keys are
 //     (131072 keys: error against 64 bits 2.2e-4, that of the output's rounding; with codes from zero 7.1e-4).  With more than 8 queries the 8 comes off the values' codes
 //     instead, which costs less there.
-//   * p vs enters as FP16, with its rest as a second part where the output is FP16.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
+//   * p vs enters as FP16, with its rest as a second part.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
 //     kept from item to item, would let a key that weighs nothing, or another request, push the others' into FP16's subnormal numbers.  p (vz + 8 vs) is summed in FP32 per query.
 // FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element to 2^14.  The tensor core cuts products off 2^-23 below the
 // largest of a step, so that a score is off by some 2^-21 of its terms' sizes: 2e-6 where scores are about 1.
@@ -148,8 +148,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 {
     using Shape = QuantisedShape<DP, NT, GROUPED>;
     using Type = AttnType<__half>;
-    // p vs in FP16 is off by up to 2^-12, an eighth of the rounding of a BF16 output and as much as that of an FP16 one, which therefore gets the rest too
-    constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;
+    // p vs in FP16 is off by up to 2^-11: as much as an FP16 output's rounding, and enough to round one BF16 output in twelve otherwise.  So the rest goes in too.
+    constexpr int kParts = 2;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
     // Codes less 8 are added up as they come.  With one column of queries it takes less to add up the codes themselves, over 32 keys at a time.
     constexpr bool CENTRED = NT > 1;
@@ -526,10 +526,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                     zeros[t][g][1] += p1 * z;
                                     const uint32_t up = pack_half2(y0, y1);
                                     hi[h][t][i] = transpose8x8(up);
-                                    if constexpr (kParts == 2) {
-                                        const float2 w = Half<__half>::unpack(up);
-                                        lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
-                                    }
+                                    const float2 w = Half<__half>::unpack(up);
+                                    lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
                                 }
                             }
                         // 8 off every code: a product of the weights with -8 in the codes' units (rows r and r + 8 are of codes 2^-24 and 2^-20), where sums start from
