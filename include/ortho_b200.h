@@ -460,7 +460,7 @@ typedef struct ortho_b200_read_quantised_desc {
 ORTHO_B200_API int ortho_b200_read_quantised(const ortho_b200_read_quantised_desc *d, const ortho_b200_quantised_cache *cache, void *stream);
 
 /* ortho_b200_paged_attention over a cache held in 4 bits; the record's fields of a cache (k_cache to head_dim's, pages, strides) are not read but kv_heads
- * and head_dim, which are the cache's.  Codes enter the matrix products as the whole numbers they are, scales and zeros in FP32, a query
+ * and head_dim, which are the cache's.  Codes enter the matrix products as whole numbers, scales and zeros in FP32, a query
  * in FP16 that was brought into range by a power of two; a probability times a scale enters as two FP16 parts, which hold it to 2^-21 of itself or
  * 2^-32 of the largest of the query's row.  Scales are not negative.  workspace: ortho_b200_paged_attention_quantised_workspace_bytes(d, cache) bytes, 256-byte aligned. */
 ORTHO_B200_API int64_t ortho_b200_paged_attention_quantised_workspace_bytes(const ortho_b200_paged_attention_desc *d, const ortho_b200_quantised_cache *cache);

@@ -6,16 +6,18 @@
 // with codes c and d of keys and values, scales and zeros of their groups g.  The division of the work and the joining are those of attention.cuh; a unit is 128 keys, 32 a
 // warp.  The bytes are a quarter, so what bounds it is the warps' instructions (some 350 for 16 keys of 128 elements and up to 8 queries, 80 of them unpacking).
 // Codes enter the products as whole numbers, and scales and zeros are applied to what a group's elements or 16 keys have in common:
-//   * A code in the low bits of a 16-bit half is itself a subnormal FP16 number, code 2^-24, or code 2^-20 four bits higher; tensor cores take these exactly.  So
-//     a word of 8 codes becomes four operands by a shift and four masks.  Elements are taken in the order in which a word has them, the queries
-//     likewise, and a sixteenth of those that meet codes 2^-20.
-//   * S^T = K Q^T starts from -8 sum q and O^T += V^T P^T from a product of the weights with -8: codes around zero keep sums as small as the averages of many keys are
-//     (131072 keys: error against 64 bits 2.2e-4, that of the output's rounding; with codes from zero 7.1e-4).  With more than 8 queries the 8 comes off the values' codes
-//     instead, which costs less there.
+//   * A code in the low bits of a 16-bit half is itself a subnormal FP16 number.  The tensor core aligns a product by its factors' exponents, which of a subnormal number is that of the
+//     smallest normal one, 2^-14, and cuts what lies 2^-25 below the largest product or sum of a step, towards zero (measured with single products).  A code at bits 0 to 3 therefore
+//     leaves a factor only 15 bits below the step's largest one.
+//   * Keys: codes at bits 2 to 5 and 6 to 9, code 2^-22 and code 2^-18, a shift for two of them and a mask each; a query's small elements keep their digits, lse of a few keys
+//     is off by 1.5e-7 (1.3e-6 at bits 0 to 3 and 4 to 7, with a shift less a word; 9e-8 as the values below, 3 us of 91 more).  Elements are taken in the order in which a word has them, the
+//     queries likewise, and a sixteenth of those that meet codes 2^-18.  S^T = K Q^T starts from -8 sum q: codes around zero keep sums small.
+//   * Values: codes less 8 as normal numbers, an FP16 multiply-add each.  Weights differ by orders of magnitude, and what small ones lost beside large ones as
+//     subnormal factors had one sign: 1.1e-4 of an average over 131072 keys, 28 % of FP16 outputs rounded otherwise than the exact ones (now 0.9 %; 90.7 us against 88.5).
+//     Up to 8 queries: FP32 adds up sums of 32 keys.  More: they stay in the tensor core's, where every step of 16 keys may take 2^-23 off them.
 //   * p vs enters as FP16, with its rest as a second part.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
 //     kept from item to item, would let a key that weighs nothing, or another request, push the others' into FP16's subnormal numbers.  p (vz + 8 vs) is summed in FP32 per query.
-// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element to 2^14.  The tensor core cuts products off 2^-23 below the
-// largest of a step, so that a score is off by some 2^-21 of its terms' sizes: 2e-6 where scores are about 1.
+// FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element to 2^14.
 // Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 87 = 3.3 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 20;
 // 100 of up to 8000 with scales for every 64 elements: 48; 1 x 1000 keys of 32 heads: 7.2.  Of the 87, unpacking and products of the values are 25, of the keys 13, copies 13,
 // and a unit's bookkeeping, scales and exponentials the rest.  Tried, against what the kernel took then: four CTAs an SM with 128 registers 93 (88), two 107 (99); a pair of
@@ -68,13 +70,14 @@ __device__ __forceinline__ void copy4_async(uint32_t dst, const void *src, bool 
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-// A pair of codes as FP16 numbers, at bits 0 to 3 and 16 to 19 (LOW) or 4 to 7 and 20 to 23: subnormal numbers, code 2^-24 and code 2^-20.  CENTRED: less 8.
-template <bool LOW, bool CENTRED> __device__ __forceinline__ uint32_t codes(uint32_t w)
+// Four codes of a 16-bit half as FP16 numbers; w: the codes of two keys or elements, one in each half.
+// As they lie, at bits 2 to 5 or 6 to 9 once w is shifted: subnormal numbers, code 2^-22 (even NUMBER) and code 2^-18
+template <int NUMBER> __device__ __forceinline__ uint32_t codes(uint32_t w) { return (NUMBER < 2 ? w << 2 : w >> 6) & (NUMBER % 2 ? 0x03C003C0u : 0x003C003Cu); }
+// As normal numbers around zero, (code - 8) 2^-9
+template <int NUMBER> __device__ __forceinline__ uint32_t centred_codes(uint32_t w)
 {
-    const uint32_t b = LOW ? w & 0x000F000Fu : w & 0x00F000F0u;
-    if (!CENTRED) return b;
-    constexpr uint32_t kLess = LOW ? 0x80088008u : 0x80808080u;
-    const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&kLess));
+    const uint32_t b = (NUMBER < 2 ? w : w >> 8) & (NUMBER % 2 ? 0x00F000F0u : 0x000F000Fu), by = NUMBER % 2 ? 0x68006800u : 0x78007800u, less = 0xA400A400u;
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&b), *reinterpret_cast<const __half2 *>(&by), *reinterpret_cast<const __half2 *>(&less));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
@@ -135,7 +138,7 @@ __device__ __forceinline__ void query_operands(const unsigned char *row, int t, 
 #pragma unroll
     for (int j = 0; j < J; j++) {
         w[j] = as_codes_lie(w[j]);
-        // what meets codes 2^-20 is a sixteenth
+        // what meets codes 2^-18 is a sixteenth
         const __half2 sixteenth = __float2half2_rn(0.0625f), y = __hmul2(*reinterpret_cast<const __half2 *>(&w[j].y), sixteenth), z = __hmul2(*reinterpret_cast<const __half2 *>(&w[j].w), sixteenth);
         w[j].y = *reinterpret_cast<const uint32_t *>(&y);
         w[j].w = *reinterpret_cast<const uint32_t *>(&z);
@@ -151,8 +154,8 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
     // p vs in FP16 is off by up to 2^-11: as much as an FP16 output's rounding, and enough to round one BF16 output in twelve otherwise.  So the rest goes in too.
     constexpr int kParts = 2;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
-    // Codes less 8 are added up as they come.  With one column of queries it takes less to add up the codes themselves, over 32 keys at a time.
-    constexpr bool CENTRED = NT > 1;
+    // The tensor core cuts its sums towards zero: where registers allow it they are of 32 keys, and FP32 adds them up.
+    constexpr bool APART = NT == 1;
     constexpr int TILES = NT * DP <= 128 ? 2 : 1;                              // of 16 keys that are worked on together, as registers allow
     // Scales and zeros of values times kSmall, so that FP32 holds their sums with weights of up to 2^15
     constexpr float kSmall = std::is_same<T, __half>::value ? 1.f : 0x1p-16f, kMostWeight = 32768.f;
@@ -312,7 +315,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         others_started();
 
         uint4 q[Shape::kKeepQ ? NT : 1][Shape::kKeepQ ? J : 1];
-        // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements.  Scores are in units of the codes' 2^-24 up to `factor`: FP32 holds them for keys of any size.
+        // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements.  Scores are in units of the codes' 2^-22 up to `factor`: FP32 holds them for keys of any size.
         float factor[NT][2], q_sum[NT][G][2];
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
         float base[NT][2];                       // what is taken off scores: the largest by the time, rounded up to a whole number, - lift; kNone before the first
@@ -342,9 +345,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         }
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * (a.scale_log2 * 0x1p24f);
+                            factor[t][e] = __shfl_sync(kAll, f, t4 * 8 + e * 4) * (a.scale_log2 * 0x1p22f);
 #pragma unroll
-                            for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4) * 0x1p-24f;
+                            for (int g = 0; g < G; g++) q_sum[t][g][e] = __shfl_sync(kAll, s[g], t4 * 8 + e * 4) * 0x1p-22f;
                         }
                         base[t][0] = base[t][1] = kNone;
                         down[t][0] = down[t][1] = 1.f;
@@ -395,9 +398,9 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                             for (int h = 0; h < TILES; h++) {
                                 const unsigned char *const at = keys + (16 * (h0 + h) + r) * Shape::kPitch + t4 * 4 + j * 16;
-                                const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch), v0 = w0 >> 8, v1 = w1 >> 8;
-                                const uint32_t lower[4] = {codes<true, false>(w0), codes<true, false>(w1), codes<false, false>(w0), codes<false, false>(w1)};
-                                const uint32_t upper[4] = {codes<true, false>(v0), codes<true, false>(v1), codes<false, false>(v0), codes<false, false>(v1)};
+                                const uint32_t w0 = word_at(at), w1 = word_at(at + 8 * Shape::kPitch);
+                                const uint32_t lower[4] = {codes<0>(w0), codes<0>(w1), codes<1>(w0), codes<1>(w1)};
+                                const uint32_t upper[4] = {codes<2>(w0), codes<2>(w1), codes<3>(w0), codes<3>(w1)};
 #pragma unroll
                                 for (int t = 0; t < NT; t++) {
                                     uint4 b;
@@ -530,19 +533,6 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                     lo[h][t][i] = transpose8x8(pack_half2(y0 - w.x, y1 - w.y));
                                 }
                             }
-                        // 8 off every code: a product of the weights with -8 in the codes' units (rows r and r + 8 are of codes 2^-24 and 2^-20), where sums start from
-                        float start[NT][4];
-                        if (!CENTRED) {
-                            const uint32_t eights[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
-#pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                start[t][0] = start[t][1] = start[t][2] = start[t][3] = 0.f;
-#pragma unroll
-                                for (int h = 0; h < TILES; h++)
-#pragma unroll
-                                    for (int part = 0; part < kParts; part++) Half<__half>::mma(start[t], eights, part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
-                            }
-                        }
                         // Two tiles of 16 elements, from four codes each of a pair of keys and of the pair 8 behind; those of tile h from pair(h, x, y)
                         auto products = [&](int at, auto pair) {
                             float sums[2][NT][4];
@@ -550,20 +540,19 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                             for (int h = 0; h < TILES; h++) {
                                 uint32_t x, y;
                                 pair(h, x, y);
-                                const uint32_t x8 = x >> 8, y8 = y >> 8;
-                                const uint32_t w[2][4] = {{codes<true, CENTRED>(x), codes<false, CENTRED>(x), codes<true, CENTRED>(y), codes<false, CENTRED>(y)},
-                                                          {codes<true, CENTRED>(x8), codes<false, CENTRED>(x8), codes<true, CENTRED>(y8), codes<false, CENTRED>(y8)}};
+                                const uint32_t w[2][4] = {{centred_codes<0>(x), centred_codes<1>(x), centred_codes<0>(y), centred_codes<1>(y)},
+                                                          {centred_codes<2>(x), centred_codes<3>(x), centred_codes<2>(y), centred_codes<3>(y)}};
 #pragma unroll
                                 for (int part = 0; part < kParts; part++)
 #pragma unroll
                                     for (int i = 0; i < 2; i++)
 #pragma unroll
                                         for (int t = 0; t < NT; t++) {
-                                            if (!CENTRED && h == 0 && part == 0) { sums[i][t][0] = start[t][0]; sums[i][t][1] = start[t][1]; sums[i][t][2] = start[t][2]; sums[i][t][3] = start[t][3]; }
-                                            Half<__half>::mma(CENTRED ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
+                                            if (APART && h == 0 && part == 0) { sums[i][t][0] = sums[i][t][1] = sums[i][t][2] = sums[i][t][3] = 0.f; }
+                                            Half<__half>::mma(!APART ? o[at + i][t] : sums[i][t], w[i], part ? lo[h][t][0] : hi[h][t][0], part ? lo[h][t][1] : hi[h][t][1]);
                                         }
                             }
-                            if (!CENTRED) {
+                            if (APART) {
 #pragma unroll
                                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -627,7 +616,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
             float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
             const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
             constexpr int WARP_FLOATS = S * Shape::kStage / 4;
-            constexpr float kUp = kDown * 0x1p24f / kSmall, kUp16 = kUp * 0.0625f;              // of codes 2^-24 and 2^-20
+            constexpr float kUp = kDown * 0x1p9f / kSmall;                                      // (of the codes' unit)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 __syncwarp();                // the warp has read its values
@@ -638,7 +627,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float z = zeros[t][GROUPED ? i / 4 : 0][e], times = two_to_8_over(down[t][e]) * (1.f / 256.f);
-                        *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * kUp * times + z, o[i][t][e + 2] * kUp16 * times + z);
+                        *reinterpret_cast<float2 *>(fold + e * Shape::kFoldPitch + el) = make_float2(o[i][t][e] * kUp * times + z, o[i][t][e + 2] * kUp * times + z);
                     }
                 }
                 __syncthreads();
