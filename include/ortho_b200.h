@@ -446,11 +446,13 @@ typedef struct ortho_b200_quantised_cache {
  * 0 where the scale is 0; all of it as in exact arithmetic on the turned key (the codes do not depend on how FP32 rounds).  Where zero + 15 scale would
  * round to infinity the scale is the next smaller number of the type.  A group with a value that is not finite, or whose zero is not in
  * the type, gets the scale NaN: it stands for NaN.  Values below FP32's normal numbers count as zero.  rotary: a multiple of 8; q, k and v
- * 8-byte aligned with strides that are multiples of 4. */
+ * 8-byte aligned with strides that are multiples of 4.  No two tokens have one slot; q_out and the cache are not expanded (a stride of 0 over several entries is refused), keys
+ * lie apart from values; q_out is q's memory or lies apart from it. */
 ORTHO_B200_API int ortho_b200_rotary_append_quantised(const ortho_b200_rotary_append_desc *d, const ortho_b200_quantised_cache *cache, void *stream);
 
 /* What a cache held in 4 bits stands for, in the model's type, rounded once: token i of the outputs is the cache's token at slots[i], zeros where that
- * lies outside the cache.  k_out and v_out [count, kv_heads, head_dim] 16-byte aligned, strides multiples of 8. */
+ * lies outside the cache.  k_out and v_out [count, kv_heads, head_dim] 16-byte aligned, strides multiples of 8;
+ * they lie apart and are not expanded. */
 typedef struct ortho_b200_read_quantised_desc {
     const int64_t *slots;               /* [count] */
     void *k_out, *v_out;

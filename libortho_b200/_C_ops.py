@@ -504,14 +504,15 @@ def rotary_append_quantised(q: Optional[torch.Tensor], k: torch.Tensor, v: torch
 
     Of a group's elements ``zero`` is the least and ``scale`` a 15th of the range, both rounded to the type; codes are ``(x - zero) / scale`` rounded, ties to
     even, within 0 to 15, as in exact arithmetic.  A group with an element that is not finite in the type reads back as NaN.  No two tokens of a call may have
-    one slot.  rotary_dim: a multiple of 8.  The other arguments and the turned queries are those of ``rotary_append``."""
+    one slot.  rotary_dim: a multiple of 8.  The other arguments and the turned queries are those of ``rotary_append``; ``out`` may be ``q`` or
+    lie apart from it."""
     return _lib.fast().rotary_append_quantised(q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, table, sections, interleaved, out)
 
 
 def read_quantised(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, slots: torch.Tensor,
                    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values [tokens, kv_heads, head_dim] of the tokens at ``slots`` (int64), in the model's type, rounded once; zeros where a slot lies outside the
-    cache.  ``out``: two tensors to write into."""
+    cache.  ``out``: two tensors to write into, which lie apart and have a place for every element."""
     return _lib.fast().read_quantised(k_cache, v_cache, k_scales, v_scales, slots, out)
 
 
@@ -519,7 +520,8 @@ def paged_attention_quantised(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
                               block_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None, window: int = 0,
                               rows: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``paged_attention`` over a cache held in 4 bits: scores, softmax and sums are of what the codes, scales and zeros stand for, in FP32."""
+    """``paged_attention`` over a cache held in 4 bits: scores, softmax and sums are of what the codes, scales and zeros stand for, in FP32.
+    ``out`` may be ``q`` or lie apart from it."""
     return _lib.fast().paged_attention_quantised(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, scale, window, rows, out, lse)
 
 

@@ -19,7 +19,7 @@ static int check_attention_quantised(const ortho_b200_paged_attention_desc *d, c
     if (((uintptr_t)d->q | (uintptr_t)d->out) & 15u) return ORTHO_B200_ERR_ALIGN;
     for (int64_t s : {d->q_token_stride, d->q_head_stride, d->out_token_stride, d->out_head_stride})
         if (s % 8) return ORTHO_B200_ERR_ALIGN;
-    return ORTHO_B200_OK;
+    return expanded(d->batch, d->out_token_stride) || expanded(d->q_heads, d->out_head_stride) ? ORTHO_B200_ERR_SHAPE : ORTHO_B200_OK;
 }
 
 template <int DP, int NT, bool GROUPED> static void take(AttnPlan &p)

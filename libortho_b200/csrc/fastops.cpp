@@ -9,6 +9,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/torch.h>
 
+#include <algorithm>
 #include <limits>
 
 #include "../../include/ortho_b200.h"
@@ -95,6 +96,42 @@ at::Tensor scratch(int64_t bytes, const at::Tensor &like)
     return at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(like.device()));
 }
 bool given(PyObject *o) { return o != Py_None; }
+
+// A [tokens, heads, elements] tensor of 16-bit values as rows of elements; strides of a dimension that has one entry do not count
+struct Rows { int64_t at, T, H, D, token, head; };
+Rows rows_of(const at::Tensor &t)
+{
+    return {(int64_t)((uintptr_t)t.const_data_ptr() / 2), t.size(0), t.size(1), t.size(2), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
+}
+// Whether two rows of a share memory, or (b another tensor) one of a and one of b; true also where a and b lie in one piece of memory with different strides
+bool rows_meet(const Rows &a, const Rows *b = nullptr)
+{
+    if (a.T < 1 || a.H < 1 || a.D < 1) return false;
+    int64_t apart = 0;
+    if (b) {
+        auto behind = [](const Rows &r) { return r.at + (r.T - 1) * r.token + (r.H - 1) * r.head + r.D; };
+        if (behind(a) <= b->at || behind(*b) <= a.at) return false;
+        if ((a.T > 1 && a.token != b->token) || (a.H > 1 && a.head != b->head)) return true;
+        apart = b->at - a.at;
+    } else if ((a.H == 1 || a.head >= a.D) && (a.T == 1 || a.token >= (a.H - 1) * a.head + a.D)) return false;
+    // rows that are h heads and t tokens apart; the t nearest to a whole one
+    for (int64_t h = b ? 1 - a.H : 0; h < a.H; h++) {
+        const int64_t gap = apart + h * a.head, near = a.token ? -gap / a.token : 0;
+        for (int64_t i = -1; i <= 1; i++) {
+            const int64_t t = std::min(std::max(near + i, 1 - a.T), a.T - 1), far = gap + t * a.token;
+            if (far < a.D && far > -a.D && (b || h || t)) return true;
+        }
+    }
+    return false;
+}
+// out, over which q may lie as it is or not at all
+void fits_beside(const at::Tensor &out, const at::Tensor &q)
+{
+    const Rows o = rows_of(out), r = rows_of(q);
+    TORCH_CHECK_VALUE(!rows_meet(o), "out must not be expanded or overlap itself");
+    TORCH_CHECK_VALUE((o.at == r.at && o.token == r.token && o.head == r.head) || !rows_meet(o, &r), "out must be q's memory or lie apart from it");
+}
+bool strides_are_multiples(const at::Tensor &t, int64_t of) { return t.stride(0) % of == 0 && t.stride(1) % of == 0; }
 
 struct Cache { at::Tensor k, v; int64_t pages, page_size, heads, D; };
 Cache cache_of(PyObject *k, PyObject *v, at::ScalarType type, const at::Tensor &like)
@@ -213,7 +250,7 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
     PyObject *const q_arg = caches[-3], *const k_arg = caches[-2], *const v_arg = caches[-1];
     const auto type = half_type(tensor(k_arg, "k"), "k");
     // (codes are made of vectors of four values at least)
-    auto fits = [](const at::Tensor &t) { return ((uintptr_t)t.const_data_ptr() & 7u) == 0 && t.stride(0) % 4 == 0 && t.stride(1) % 4 == 0; };
+    auto fits = [](const at::Tensor &t) { return ((uintptr_t)t.const_data_ptr() & 7u) == 0 && strides_are_multiples(t, 4); };
     auto heads = [&](PyObject *o, const char *name, const at::Tensor *like) {
         at::Tensor t = input(o, name, type, like);
         three_dims(t, name, like ? like->size(0) : -1, like ? like->size(2) : -1);
@@ -227,6 +264,7 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
         c = quantised_cache_of(caches, type, k);
         for (const at::Tensor *t : {&c.k, &c.v, &c.ks, &c.vs})
             for (int i = 0; i < 3; i++) TORCH_CHECK_VALUE(t->stride(i) != 0 || t->size(i) <= 1, "a cache that is written must not be expanded");
+        TORCH_CHECK_VALUE(c.pages == 0 || (c.k.const_data_ptr() != c.v.const_data_ptr() && c.ks.const_data_ptr() != c.vs.const_data_ptr()), "keys and values must be two tensors");
     }
     else c = cache_of(caches[0], caches[1], type, k);
     const int64_t T = k.size(0);
@@ -275,11 +313,13 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
             out = output(a[10], "out", type, k);
             TORCH_CHECK_VALUE(out.sizes() == q.sizes() && (out.stride(2) == 1 || out.size(2) <= 1), "out must have q's shape and a contiguous last dimension");
             TORCH_CHECK_VALUE(!QUANTISED || fits(out), "out must be 8-byte aligned, with strides that are multiples of 4");
+            if (QUANTISED) fits_beside(out, q);
         } else {
             out = at::empty(q.sizes(), q.options());
         }
         d.q = ptr<void>(q); d.q_out = ptr<void>(out); d.q_heads = q.size(1);
-        d.q_token_stride = q.stride(0); d.q_head_stride = q.stride(1); d.out_token_stride = out.stride(0); d.out_head_stride = out.stride(1);
+        const Rows from = rows_of(q), to = rows_of(out);
+        d.q_token_stride = from.token; d.q_head_stride = from.head; d.out_token_stride = to.token; d.out_head_stride = to.head;
     } else {
         TORCH_CHECK_VALUE(!given(a[10]), "out is for q");
     }
@@ -287,7 +327,8 @@ PyObject *rotary_append(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (truth < 0) throw python_error();
     d.k = ptr<void>(k); d.v = ptr<void>(v); d.slots = ptr<int64_t>(slots);
     d.tokens = T; d.kv_heads = c.heads; d.head_dim = c.D; d.pages = c.pages; d.page_size = c.page_size;
-    d.k_token_stride = k.stride(0); d.k_head_stride = k.stride(1); d.v_token_stride = v.stride(0); d.v_head_stride = v.stride(1);
+    const Rows k_rows = rows_of(k), v_rows = rows_of(v);
+    d.k_token_stride = k_rows.token; d.k_head_stride = k_rows.head; d.v_token_stride = v_rows.token; d.v_head_stride = v_rows.head;
     if (!QUANTISED) {
         d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v);
         d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_cache_head_stride = c.k.stride(2);
@@ -329,17 +370,20 @@ PyObject *read_quantised(PyObject *, PyObject *const *a, Py_ssize_t n)
         for (int i = 0; i < 2; i++) {
             out[i] = output(PyTuple_GET_ITEM(a[5], i), names[i], type, scales);
             TORCH_CHECK_VALUE(out[i].dim() == 3 && out[i].size(0) == T && out[i].size(1) == c.heads && out[i].size(2) == c.D && out[i].stride(2) == 1 && aligned(out[i])
-                              && out[i].stride(0) % 8 == 0 && out[i].stride(1) % 8 == 0,
+                              && strides_are_multiples(out[i], 8),
                               names[i], " must be [tokens, kv_heads, head_dim] with a contiguous last dimension, 16-byte alignment and strides that are multiples of 8");
         }
-        TORCH_CHECK_VALUE(T == 0 || out[0].const_data_ptr() != out[1].const_data_ptr(), "out must be two tensors");
+        const Rows k = rows_of(out[0]), v = rows_of(out[1]);
+        TORCH_CHECK_VALUE(!rows_meet(k, &v), "out must be two tensors that lie apart");
+        for (int i = 0; i < 2; i++) TORCH_CHECK_VALUE(!rows_meet(i ? v : k), names[i], " must not be expanded or overlap itself");
     } else {
         for (int i = 0; i < 2; i++) out[i] = at::empty({T, c.heads, c.D}, scales.options().memory_format(at::MemoryFormat::Contiguous));
     }
     ortho_b200_read_quantised_desc d;
     memset(&d, 0, sizeof(d));
     d.slots = ptr<int64_t>(slots); d.k_out = ptr<void>(out[0]); d.v_out = ptr<void>(out[1]); d.count = T; d.type = type_number(type);
-    d.k_token_stride = out[0].stride(0); d.k_head_stride = out[0].stride(1); d.v_token_stride = out[1].stride(0); d.v_head_stride = out[1].stride(1);
+    const Rows to[2] = {rows_of(out[0]), rows_of(out[1])};
+    d.k_token_stride = to[0].token; d.k_head_stride = to[0].head; d.v_token_stride = to[1].token; d.v_head_stride = to[1].head;
     void *stream = current_stream(scales);
     int st;
     Py_BEGIN_ALLOW_THREADS
@@ -387,12 +431,13 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     const int64_t window = integer(a[6], "window", 0);
     const c10::cuda::CUDAGuard guard(q.device());
-    if (q.stride(2) != 1 || !aligned(q) || q.stride(0) % 8 || q.stride(1) % 8) q = q.clone(at::MemoryFormat::Contiguous);
+    if (q.stride(2) != 1 || !aligned(q) || !strides_are_multiples(q, 8)) q = q.clone(at::MemoryFormat::Contiguous);
     at::Tensor out;
     if (given(a[8])) {
         out = output(a[8], "out", type, q);
-        TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.stride(2) == 1 && aligned(out) && out.stride(0) % 8 == 0 && out.stride(1) % 8 == 0,
+        TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.stride(2) == 1 && aligned(out) && strides_are_multiples(out, 8),
                           "out must have q's shape, a contiguous last dimension, 16-byte alignment and strides that are multiples of 8");
+        if (QUANTISED) fits_beside(out, q);
     } else {
         out = at::empty(q.sizes(), q.options());
     }
@@ -407,7 +452,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     d.block_table = ptr<int32_t>(table); d.lengths = ptr<int32_t>(lengths); d.row_of = rows.defined() ? ptr<int32_t>(rows) : nullptr;
     d.batch = B; d.q_heads = H; d.kv_heads = c.heads; d.head_dim = D; d.rows = table.size(0); d.width = table.size(1); d.table_stride = table.stride(0);
     d.pages = c.pages; d.page_size = c.page_size; d.window = window;
-    d.q_token_stride = q.stride(0); d.q_head_stride = q.stride(1); d.out_token_stride = out.stride(0); d.out_head_stride = out.stride(1);
+    const Rows from = rows_of(q), to = rows_of(out);
+    d.q_token_stride = from.token; d.q_head_stride = from.head; d.out_token_stride = to.token; d.out_head_stride = to.head;
     if (!QUANTISED) {
         d.k_cache = ptr<void>(c.k); d.v_cache = ptr<void>(c.v);
         d.k_page_stride = c.k.stride(0); d.k_slot_stride = c.k.stride(1); d.k_head_stride = c.k.stride(2);

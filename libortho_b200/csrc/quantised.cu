@@ -509,6 +509,9 @@ extern "C" int ortho_b200_rotary_append_quantised(const ortho_b200_rotary_append
         if ((uintptr_t)p & 7u) return ORTHO_B200_ERR_ALIGN;
         if ((uintptr_t)p & 15u) vec = 4;
     }
+    if (d->q_heads && (expanded(d->tokens, d->out_token_stride) || expanded(d->q_heads, d->out_head_stride))) return ORTHO_B200_ERR_SHAPE;
+    st = check_written(*c);
+    if (st) return st;
     st = check_device();
     if (st) return st;
     QuantiseArgs a;
@@ -535,6 +538,8 @@ extern "C" int ortho_b200_read_quantised(const ortho_b200_read_quantised_desc *d
     if (((uintptr_t)d->k_out | (uintptr_t)d->v_out) & 15u) return ORTHO_B200_ERR_ALIGN;
     for (int64_t s : {d->k_token_stride, d->k_head_stride, d->v_token_stride, d->v_head_stride})
         if (s % 8) return ORTHO_B200_ERR_ALIGN;
+    if (d->k_out == d->v_out || expanded(d->count, d->k_token_stride) || expanded(d->count, d->v_token_stride) || expanded(c->kv_heads, d->k_head_stride)
+        || expanded(c->kv_heads, d->v_head_stride)) return ORTHO_B200_ERR_SHAPE;
     st = check_device();
     if (st) return st;
     ReadArgs a;

@@ -19,4 +19,18 @@ inline int check_quantised(const ortho_b200_quantised_cache *c)
     return ORTHO_B200_OK;
 }
 
+// Entries of a dimension that is written would lie in one place
+inline bool expanded(int64_t entries, int64_t stride) { return entries > 1 && stride == 0; }
+
+// A cache that is written: no two tokens or heads in one place, keys apart from values
+inline int check_written(const ortho_b200_quantised_cache &c)
+{
+    if (c.pages == 0) return ORTHO_B200_OK;
+    if (c.k == c.v || c.k_scales == c.v_scales) return ORTHO_B200_ERR_SHAPE;
+    for (int64_t s : {c.k_page_stride, c.v_page_stride, c.ks_page_stride, c.vs_page_stride}) if (expanded(c.pages, s)) return ORTHO_B200_ERR_SHAPE;
+    for (int64_t s : {c.k_slot_stride, c.v_slot_stride, c.ks_slot_stride, c.vs_slot_stride}) if (expanded(c.page_size, s)) return ORTHO_B200_ERR_SHAPE;
+    for (int64_t s : {c.k_head_stride, c.v_head_stride, c.ks_head_stride, c.vs_head_stride}) if (expanded(c.kv_heads, s)) return ORTHO_B200_ERR_SHAPE;
+    return ORTHO_B200_OK;
+}
+
 }  // namespace ob
