@@ -131,7 +131,12 @@ void fits_beside(const at::Tensor &out, const at::Tensor &q)
     TORCH_CHECK_VALUE(!rows_meet(o), "out must not be expanded or overlap itself");
     TORCH_CHECK_VALUE((o.at == r.at && o.token == r.token && o.head == r.head) || !rows_meet(o, &r), "out must be q's memory or lie apart from it");
 }
-bool strides_are_multiples(const at::Tensor &t, int64_t of) { return t.stride(0) % of == 0 && t.stride(1) % of == 0; }
+// strides of a written or read tensor that count
+bool strides_are_multiples(const at::Tensor &t, int64_t of)
+{
+    const Rows r = rows_of(t);
+    return r.token % of == 0 && r.head % of == 0;
+}
 
 struct Cache { at::Tensor k, v; int64_t pages, page_size, heads, D; };
 Cache cache_of(PyObject *k, PyObject *v, at::ScalarType type, const at::Tensor &like)

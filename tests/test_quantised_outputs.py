@@ -1,4 +1,4 @@
-"""Where the operators of a cache held in 4 bits write: memory that several of their threads would write at once is refused."""
+"""Where the operators of a cache held in 4 bits write: memory that several of their threads would write at once is refused, strides that do not count are not looked at."""
 import ctypes
 
 import pytest
@@ -90,6 +90,10 @@ def test_read_writes_into_views(filled):
         got = _C_ops.read_quantised(*tensors(c), slots, out=(a, b))
         assert got[0] is a and got[1] is b and torch.equal(a, want[0]) and torch.equal(b, want[1])
         assert int((one != 0).sum()) == int((want[0] != 0).sum() + (want[1] != 0).sum())
+    # a single token: its stride does not count
+    a, b = (rows(1, 2, 64, 133) for _ in range(2))
+    _C_ops.read_quantised(*tensors(c), slots[:1], out=(a, b))
+    assert torch.equal(a, want[0][:1]) and torch.equal(b, want[1][:1])
 
 
 @pytest.mark.gpu
@@ -112,6 +116,11 @@ def test_append_and_attention_outputs(filled):
             with pytest.raises(ValueError, match="q's memory"):
                 call(fused.as_strided((20, 4, 64), (256, 64, 1), at), mine)
         assert torch.equal(call(mine, mine), right)                            # in place
+        single = rows(1, 4, 64, 131)
+        assert torch.equal(call(single, n=1), right[:1])
+        heads = rows(20, 1, 64, 72, 51)
+        if call is append:
+            assert torch.equal(append(heads, q[:, :1]), want[:, :1])
     with pytest.raises(ValueError, match="two tensors"):
         _C_ops.rotary_append_quantised(None, k, v, c.k, c.k, c.k_scales, c.v_scales, slots)
     with pytest.raises(ValueError, match="two tensors"):
