@@ -95,6 +95,13 @@ class PagedCache:
         return _C.paged_attention(q, self.k, self.v, block_table, lengths, scale=scale, window=window, rows=rows)
 
 
+class _Plain(PagedCache):
+    """The methods of ``PagedCache`` on another object's ``k`` and ``v``."""
+
+    def __init__(self, cache):
+        self.k, self.v = cache.k, cache.v
+
+
 class QuantisedCache:
     """Keys and values of one layer in 4 bits: what ``PagedCache`` holds, in a good quarter of its room.
 
@@ -159,7 +166,8 @@ class PagedAttentionBlock(nn.Module):
                 positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` [tokens, in_features]: the step's new tokens, request after request, as ``step`` lists them.
         ``positions``: rotary positions where they are not those in the request, [tokens] or [axes, tokens].  Every token sees its
-        request up to itself and reads its keys for itself: meant for decoding and short prompts.  Places behind the step's
+        request up to itself and reads its keys for itself: meant for decoding and short prompts.  A ``cache`` of another kind is asked for ``append`` and
+        ``attention``; one that only has tensors ``k`` and ``v`` is taken as a ``PagedCache``'s.  Places behind the step's
         last token give what an empty attention gives."""
         T, D = x.shape[0], self.head_dim
         qkv = self.qkv(x)
@@ -167,9 +175,10 @@ class PagedAttentionBlock(nn.Module):
             qkv = self.qkv_adapters(x, qkv, ids, out=qkv)
         heads = qkv.view(T, self.q_heads + 2 * self.kv_heads, D)
         q, k, v = heads.split((self.q_heads, self.kv_heads, self.kv_heads), dim=1)
-        q = cache.append(q, k, v, step.slots, step.positions if positions is None else positions, self.table,
-                         sections=self.sections, interleaved=self.interleaved)
-        o = cache.attention(q, pool.block_table, step.positions + 1, window=self.window, rows=step.requests)
+        kind = cache if hasattr(cache, "append") and hasattr(cache, "attention") else _Plain(cache)
+        q = kind.append(q, k, v, step.slots, step.positions if positions is None else positions, self.table,
+                        sections=self.sections, interleaved=self.interleaved)
+        o = kind.attention(q, pool.block_table, step.positions + 1, window=self.window, rows=step.requests)
         o = o.view(T, self.q_heads * D)
         y = self.proj(o)
         if self.proj_adapters is not None and ids is not None:
