@@ -50,6 +50,10 @@ static AttnPlan plan_attention_quantised(const ortho_b200_paged_attention_desc &
     }
     OB_QUANTISED_DIMS(OB_CASE)
 #undef OB_CASE
+    // Clusters or the even cut, as for a 16-bit cache and with the same reckoning.  A unit is 128 keys here instead of 64 and costs about as much (bound by instructions, not bytes), so joining
+    // costs as many of them.  Measured, clusters / cut, us: 64 + 2 x 8 heads of 128, 1 request of 1000 / 8000 / 16000 keys 6.7 / 14.2 / 22.8, 10.0 / 17.4 / 21.1; 4 of 1000 / 8000 / 16000
+    // 7.9 / 21.3 / 36.5, 12.8 / 23.4 / 35.1; 32 of 100 / 1000 / 4000 8.5 / 22.1 / 66.0, 12.5 / 25.6 / 56.0, of up to 1000 / 4000 log-spread 17.4 / 48.6, 15.6 / 20.7; 128 of 100 23.1, 22.8;
+    // 32 + 2 x 2 heads of 256, 1 of 1000 / 8000 10.5 / 25.2, 13.7 / 20.3.
     const int64_t sms = device_sm_count(current_device_index()), width = d.width * c.page_size;
     const int64_t keys = d.window > 0 && d.window < width ? d.window : width;
     const int64_t units = ceil_div(keys, kQUnitKeys), items = d.batch * d.kv_heads * p.groups;      // of one item at most; all items

@@ -55,8 +55,10 @@ struct QuantisedShape {
     static constexpr int kOperands = kKeepQ ? 0 : NT * DP / 32 * 512;
     static constexpr int bytes(int stages) { return stages * (kAttnWarps * kStage + kQ) + kOperands + kAttnWarps * NT * 8 * 8; }
     static constexpr int kFour = 57088, kThree = 76458, kTwo = 115712, kOne = 232448;
-    static constexpr int kRegs = NT * DP;                                      // a measure of the sums that a thread holds
-    static constexpr int kWanted = kRegs <= 64 ? 4 : kRegs <= 192 ? 3 : 2;
+    // CTAs an SM, by the registers that NT * DP sums and up to 16 queries' operands leave: four have 128 of them, three 168, two 255.  Measured, 60 requests of up to 8000 keys, log-spread, 8
+    // key-value heads, us.  Four / three: heads of 64, 8 queries or fewer 25.9 / 25.8, 16 queries 51.5 / 38.7; of 96 32.4 / 29.5, of 128 37.0 / 33.4.  Three / two: of 192 46.2 / 46.9;
+    // of 96, 16 queries 57.9 / 48.6; of 128, 12 queries 59.4 / 51.8, of 64, 24 queries 90.7 / 65.7.
+    static constexpr int kWanted = NT * DP <= 64 ? 4 : NT * DP <= (NT == 1 ? 192 : 128) ? 3 : 2;
     static constexpr int kRoom = kWanted == 4 && bytes(2) <= kFour ? kFour : kWanted >= 3 && bytes(2) <= kThree ? kThree : kWanted >= 2 && bytes(2) <= kTwo ? kTwo : kOne;
     static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2, kBytes = bytes(kStages);
     static constexpr int kPerSm = kRoom == kFour ? 4 : kRoom == kThree ? 3 : kRoom == kTwo ? 2 : 1;
