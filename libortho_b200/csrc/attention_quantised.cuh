@@ -152,16 +152,15 @@ __global__ void __launch_bounds__(kAttnThreads, QuantisedShape<DP, NT, GROUPED>:
 paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs args)
 {
     using Shape = QuantisedShape<DP, NT, GROUPED>;
-    using Type = AttnType<__half>;
     // p vs in FP16 is off by up to 2^-11: as much as an FP16 output's rounding, and enough to round one BF16 output in twelve otherwise.  So the rest goes in too.
     constexpr int kParts = 2;
     constexpr int S = Shape::kStages, J = DP / 32, G = Shape::kGroups, CH = DP / 64, HALF = DP / 32 % 2;      // pieces of 32 elements, groups, chunks of 64 and a half one
     // The tensor core cuts its sums towards zero: where registers allow it they are of 32 keys, and FP32 adds them up.
     constexpr bool APART = NT == 1;
     constexpr int TILES = NT * DP <= 128 ? 2 : 1;                              // of 16 keys that are worked on together, as registers allow
-    // Scales and zeros of values times kSmall, so that FP32 holds their sums with weights of up to 2^15
-    constexpr float kSmall = std::is_same<T, __half>::value ? 1.f : 0x1p-16f, kMostWeight = 32768.f;
-    static_assert(Type::lift + kSlack == 15.f, "log2 of kMostWeight");
+    // Scales and zeros of values times kSmall, so that FP32 holds their sums with weights of up to 2^kSlack; what weights, and weights times scales in FP16, stay below
+    constexpr float kSmall = std::is_same<T, __half>::value ? 1.f : 0x1p-16f, kMostWeight = 128.f, kMostProduct = 32768.f;
+    static_assert(kSlack == 7.f, "log2 of kMostWeight");
     constexpr uint32_t kAll = 0xffffffffu, kHere = TILES == 2 ? kAll : 0xFFFFu;
     extern __shared__ __align__(128) unsigned char smem[];
     const AttentionArgs &a = args.a;
@@ -320,7 +319,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
         // of queries 2 (lane % 4) and the next: scale, power of two and log2 e; sums of elements.  Scores are in units of the codes' 2^-22 up to `factor`: FP32 holds them for keys of any size.
         float factor[NT][2], q_sum[NT][G][2];
         float o[2 * J][NT][4], sum[NT][2], zeros[NT][G][2];
-        float base[NT][2];                       // what is taken off scores: the largest by the time, rounded up to a whole number, - lift; kNone before the first
+        float base[NT][2];                       // what is taken off scores: the largest by the time, which weighs exactly one; kNone before the first
         float down[NT][2];                       // a power of two that brings the item's largest weight times scale by the time to 2^7 .. 2^15
         int stage = 0, q_at = -1;
         for (bool more = true; more;) {
@@ -462,7 +461,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                         for (int e = 0; e < 2; e++) {
                             float m = fmaxf(p[0][t][e], p[0][t][e + 2]);
                             if constexpr (TILES == 2) m = fmaxf(m, fmaxf(p[TILES - 1][t][e], p[TILES - 1][t][e + 2]));
-                            grows = grows || m > kMostWeight || m * down[t][e] * most_scale > kMostWeight;
+                            grows = grows || m > kMostWeight || m * down[t][e] * most_scale > kMostProduct;
                         }
                     }
                     if (__any_sync(kAll, grows)) {
@@ -480,7 +479,7 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
                                 auto score = [&](int h, int i) { return (there >> (16 * h + r + 8 * i)) & 1 ? mul_add(s[h][t][e + 2 * i], factor[t][e], 0.f) : -INFINITY; };
 #pragma unroll
                                 for (int h = 0; h < TILES; h++) m = fmaxf(m, fmaxf(score(h, 0), score(h, 1)));
-                                m = ceilf(over_rows(m)) - Type::lift;
+                                m = over_rows(m);
                                 keep[e] = 1.f;
                                 if (m > base[t][e]) {
                                     keep[e] = exp2_approx(base[t][e] - m);
@@ -592,14 +591,12 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
             }
             const bool last = now.unit + run == now.s.units;
             // ---- the four warps' sums over their keys of this item become one.  They pass through the stage that was just used: its next copies are
-            // issued behind the barrier above.  What 2^lift and `down` have made of the sums is undone here.
+            // issued behind the barrier above.  What `down` has made of the sums is undone here.
             const int head = now.inner / a.groups, group = now.inner - head * a.groups;
             const int64_t h0 = head * (d.q_heads / d.kv_heads) + group * a.per_group;
             const int heads = min(a.per_group, (int)(d.q_heads / d.kv_heads) - group * a.per_group);
             const bool whole = started_here && last;
             const int64_t slot = 2 * (int64_t)cta + (started_here ? 1 : 0);
-            constexpr float kDown = 1.f / 256.f;
-            static_assert(Type::lift == 8.f, "the power of two above");
             auto over_keys = [](float x) {
                 x += __shfl_xor_sync(0xffffffffu, x, 4);
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
@@ -610,15 +607,15 @@ paged_attention_quantised_kernel(const __grid_constant__ QuantisedAttentionArgs 
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const float l = over_keys(sum[t][e]);
-                    if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + (Type::lift + AttnType<T>::lift), l * kDown);
+                    if (lane < 4) sums[warp * NT * 8 + t * 8 + 2 * lane + e] = make_float2(base[t][e] == kNone ? -INFINITY : base[t][e] + AttnType<T>::lift, l);
 #pragma unroll
-                    for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * (kDown / kSmall);
+                    for (int g = 0; g < G; g++) zeros[t][g][e] = over_keys(zeros[t][g][e]) * (1.f / kSmall);
                 }
             const int used = stage == 0 ? S - 1 : stage - 1;
             float *const fold = reinterpret_cast<float *>(ring + used * Shape::kStage) + 2 * t4 * Shape::kFoldPitch;
             const float *const folds = reinterpret_cast<const float *>(smem + used * Shape::kStage);
             constexpr int WARP_FLOATS = S * Shape::kStage / 4;
-            constexpr float kUp = kDown * 0x1p9f / kSmall;                                      // (of the codes' unit)
+            constexpr float kUp = 0x1p9f / kSmall;                                              // (of the codes' unit)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 __syncwarp();                // the warp has read its values

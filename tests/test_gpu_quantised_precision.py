@@ -56,6 +56,18 @@ def test_outputs_are_rounded_as_the_exact_ones(lengths, Hq, Hkv, D, groups, std,
         plain_ops.within(lse, want_lse, lse_bound(q, cache[2], want_lse, max(lengths)), "lse")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Hq,Hkv,D,groups", [(8, 2, 64, 1), (24, 2, 96, 1), (8, 8, 128, 2), (48, 2, 128, 1), (16, 1, 256, 4)])
+def test_a_key_alone_gives_its_value(Hq, Hkv, D, groups, dtype):
+    """One key weighs one: zero + scale code, rounded once, with ties (one value in dozens) to even."""
+    for B, columns in ((3, 1), (200, 40)):
+        q, *cache, table, n = make([1] * B, Hq, Hkv, D, 16, dtype, groups, seed=D)
+        got = _C_ops.paged_attention_quantised(q, *cache, widened(table, columns), n)
+        want = quantised_ops.held(cache[1][table[:, 0].long(), 0], cache[3][table[:, 0].long(), 0]).repeat_interleave(Hq // Hkv, 1)
+        assert torch.equal(got.double(), quantised_ops.nearest(want, dtype))
+
+
 def test_the_bound_sees_weights_of_few_digits():
     """Weights rounded to 11 bits in the plain form: too many outputs are rounded otherwise."""
     g = torch.Generator().manual_seed(0)
