@@ -4,7 +4,7 @@
 //     out_i = sum_j p_j (vs_jg (d_ji - 8) + vz_jg + 8 vs_jg) / sum_j p_j,     p_j = exp(s_j - max)
 //
 // with codes c and d of keys and values, scales and zeros of their groups g.  The division of the work and the joining are those of attention.cuh; a unit is 128 keys, 32 a
-// warp.  The bytes are a quarter, so what bounds it is the warps' instructions (some 350 for 16 keys of 128 elements and up to 8 queries, 80 of them unpacking).
+// warp.  The bytes are a quarter, so what bounds it is the warps' instructions (some 400 for 16 keys of 128 elements and up to 8 queries, 130 of them unpacking).
 // Codes enter the products as whole numbers, and scales and zeros are applied to what a group's elements or 16 keys have in common:
 //   * A code in the low bits of a 16-bit half is itself a subnormal FP16 number.  The tensor core aligns a product by its factors' exponents, which of a subnormal number is that of the
 //     smallest normal one, 2^-14, and cuts what lies 2^-25 below the largest product or sum of a step, towards zero (measured with single products).  A code at bits 0 to 3 therefore
@@ -13,15 +13,16 @@
 //     is off by 1.5e-7 (1.3e-6 at bits 0 to 3 and 4 to 7, with a shift less a word; 9e-8 as the values below, 3 us of 91 more).  Elements are taken in the order in which a word has them, the
 //     queries likewise, and a sixteenth of those that meet codes 2^-18.  S^T = K Q^T starts from -8 sum q: codes around zero keep sums small.
 //   * Values: codes less 8 as normal numbers, an FP16 multiply-add each.  Weights differ by orders of magnitude, and what small ones lost beside large ones as
-//     subnormal factors had one sign: 1.1e-4 of an average over 131072 keys, 28 % of FP16 outputs rounded otherwise than the exact ones (now 0.9 %; 90.7 us against 88.5).
+//     subnormal factors had one sign: 1.1e-4 of an average over 131072 keys, 28 % of FP16 outputs rounded otherwise than those of an FP32 form (now 0.9 %; 90.7 us against 88.5).
 //     Up to 8 queries: FP32 adds up sums of 32 keys.  More: they stay in the tensor core's, where every step of 16 keys may take 2^-23 off them.
 //   * p vs enters as FP16, with its rest as a second part.  A power of two per query brings the largest of its item to 2^7 .. 2^15: one of the scales alone, or one
 //     kept from item to item, would let a key that weighs nothing, or another request, push the others' into FP16's subnormal numbers.  p (vz + 8 vs) is summed in FP32 per query.
 // FP16 serves BF16 models too: a query is multiplied by a power of two that brings its largest element to 2^14.
-// Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 87 = 3.3 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 20;
-// 100 of up to 8000 with scales for every 64 elements: 48; 1 x 1000 keys of 32 heads: 7.2.  Of the 87, unpacking and products of the values are 25, of the keys 13, copies 13,
-// and a unit's bookkeeping, scales and exponentials the rest.  Tried, against what the kernel took then: four CTAs an SM with 128 registers 93 (88), two 107 (99); a pair of
-// lanes for the rows of a pair of keys, which saves exchanges of addresses but touches four times the lines a copy, 99 (91); tiles of 16 keys one by one 94 (91).
+// Measured (GPU time, us): 2 x 131072 keys of 8 heads of 128, 285 MB: 91 = 3.1 TB/s (a 16-bit cache: 166); 32 requests of up to 4096 keys, log-spread: 21;
+// 100 of up to 8000 with scales for every 64 elements: 54; 16 of up to 10000 with 16 queries and heads of 256: 25; 1 x 1000 keys of 32 heads: 7.7.  Warps wait for fixed latencies, 56 % of
+// the issue slots in use; in short runs for instructions, because a unit's are more than the nearest cache holds (heads of 256: three of seven cycles).  Tried, against what the kernel took
+// then: four CTAs an SM with 128 registers 93 (88), two 107 (99); a pair of lanes for the rows of a pair of keys, which saves exchanges of addresses but touches four times the lines a
+// copy, 99 (91); tiles of 16 keys one by one 94 (91); values' codes as subnormal numbers at bits 2 to 5 and 6 to 9, their sums turned round every other time, 96 (91).
 #pragma once
 
 #include <type_traits>
